@@ -148,8 +148,9 @@ def _rows(x):
     """Codes (as floats) and scales of the rows of an fp32 matrix."""
     a = x.abs().amax(1, keepdim=True)
     some = a >= TINY
-    inv = torch.where(some, 127 / torch.where(some, a, 1.0), 0.0)
-    return torch.round(x * inv), torch.where(some, a / 127, 0.0)
+    top = torch.full_like(a, 127.0)  # a tensor: by a number torch multiplies with its reciprocal
+    inv = torch.where(some, top / torch.where(some, a, 1.0), 0.0)
+    return torch.round(x * inv), torch.where(some, a / top, 0.0)
 
 
 def _plain_linear(x, wq, sw, bias):
