@@ -711,6 +711,92 @@ int ksd_layernorm_backward(const float *x, const float *dy, const float *dres, c
                            const float *rstd, const float *weight, int64_t M, int64_t d,
                            float *dx, float *partials, void *stream);
 
+/*
+ * W8A8 with one fp32 scale per token and one per output channel (no reference counterpart; the
+ * group-128 form is ksd_w8a8_gemm_nt).
+ *
+ * ksd_tc_quantize_rows: per row of x (M, K; row stride `stride` elements, any alignment of the
+ * element type), a = max |x|: a < 2^-100 gives scale 0 and codes 0, else scale = a / 127 and
+ * code = rint(x * (127 / a)), each operation rounded to fp32. A row with NaN or inf gets scale NaN
+ * and codes 0.
+ *   codes  (M, K) int8 in rows of ld bytes, ld = K rounded up to 16, zeros past K; 16-byte aligned
+ *   scales (M,) fp32
+ */
+int ksd_tc_quantize_rows(const void *x, int x_dtype, int64_t M, int64_t K, int64_t stride,
+                         int8_t *codes, int64_t ld, float *scales, void *stream);
+/*
+ * ksd_tc_gemm: y[m,n] = ((sum_k a w) * sa[m]) * sw[n] (+ bias[n]) (+ residual[m,n]), in fp32,
+ * rounded once to out_dtype (KSD_F32, KSD_BF16, KSD_F16). The int32 sums are exact for any K (parts
+ * past 131072 steps are joined in 64 bits).
+ *   a     (M, K) int8 in rows of lda bytes, zeros from K to the next multiple of 16; with a_t
+ *         (K, M) instead
+ *   w     (N, K) int8 in rows of ldw bytes; with w_t (K, N) instead. a_t needs w_t
+ *   lda, ldw multiples of 16 that hold a row rounded up to 16 bytes, all of it readable, bases
+ *         16-byte aligned
+ *   sa (M,), sw (N,), bias (N,) fp32 or NULL; residual (M, N) of the output type or NULL
+ *   workspace: ksd_tc_gemm_workspace bytes
+ */
+int ksd_tc_gemm_workspace(int64_t M, int64_t N, int64_t K, int64_t *bytes);
+int ksd_tc_gemm(const int8_t *a, int64_t lda, int a_t, const float *sa, const int8_t *w,
+                int64_t ldw, int w_t, const float *sw, int64_t M, int64_t N, int64_t K,
+                const float *bias, const void *residual, void *y, int out_dtype, void *workspace,
+                int64_t workspace_bytes, void *stream);
+/*
+ * ksd_tc_quantize_grad: the operands of both gradients of that product from dY (M, N):
+ *   q (M, N), e (M,)  row quantization of dY * sw[n]     (dX = e * q . w_codes)
+ *   c (M, N), f (N,)  column quantization of dY * sx[m]  (dW = f * c^T . x_codes)
+ *   db (N,) or NULL   column sums of dY
+ * q and c are in rows of ld bytes (zeros past N), either may be NULL; the rules are those of
+ * ksd_tc_quantize_rows. workspace: ksd_tc_grad_workspace bytes.
+ */
+int ksd_tc_grad_workspace(int64_t M, int64_t N, int64_t *bytes);
+int ksd_tc_quantize_grad(const void *g, int g_dtype, int64_t M, int64_t N, int64_t stride,
+                         const float *sx, const float *sw, int8_t *q, float *e, int8_t *c, float *f,
+                         int64_t ld, float *db, void *workspace, int64_t workspace_bytes,
+                         void *stream);
+
+/*
+ * Embedding lookup with a scale: out[i] = round(scale * table[ids[i]]), a row of zeros for an id
+ * out of range. table (V, d) of row stride `stride` elements; ids int64 (ids_wide) or int32; out
+ * (n, d) dense. Float types KSD_F32, KSD_BF16, KSD_F16 on both sides.
+ */
+int ksd_embedding_lookup(const void *table, int table_dtype, int64_t V, int64_t d, int64_t stride,
+                         const void *ids, int ids_wide, int64_t n, float scale, void *out,
+                         int out_dtype, void *stream);
+/*
+ * Its gradient: out[v] (+)= scale * sum of g[i] over ids[i] = v, positions in order, fp32 sums,
+ * without the id `padding` (-1 for none) and ids out of range. g (n, d) of row stride `stride`; out
+ * (V, d) dense, 16-byte aligned; accumulate = 0 writes all of it, else only the rows of ids that
+ * occur are read and written. The same inputs give the same bits on every call.
+ */
+int ksd_embedding_gradient_workspace(int64_t n, int64_t d, int64_t *bytes);
+int ksd_embedding_gradient(const void *g, int g_dtype, int64_t n, int64_t d, int64_t stride,
+                           const void *ids, int ids_wide, int64_t V, int64_t padding, float scale,
+                           int accumulate, void *out, int out_dtype, void *workspace,
+                           int64_t workspace_bytes, void *stream);
+
+/*
+ * The global norm of many gradients and their clipping (torch.nn.utils.clip_grad_norm_, reference
+ * ksdraft/train/__init__.py:165).
+ *   norm   = (max_kind ? max |g| : sqrt(sum g^2)) / loss_scale, summed in fp64 in a fixed order
+ *   factor = min(1, max_norm / (norm + 1e-6)) / loss_scale (NULL: not formed)
+ * ksd_grad_scale writes out = grad * factor[0] for every tensor (out may be grad; then a factor of
+ * exactly 1 leaves the memory untouched). tensors is a host array; n elements of type dtype
+ * (KSD_F32, KSD_BF16, KSD_F16), dense, at any alignment of the element type.
+ */
+typedef struct {
+  const void *grad;
+  void *out;
+  int64_t n;
+  int32_t dtype;
+  int32_t reserved;
+} KsdClipTensor;
+int ksd_grad_norm_workspace(const KsdClipTensor *tensors, int n, int64_t *bytes);
+int ksd_grad_norm(const KsdClipTensor *tensors, int n, int max_kind, float max_norm,
+                  float loss_scale, float *norm, float *factor, void *workspace,
+                  int64_t workspace_bytes, void *stream);
+int ksd_grad_scale(const KsdClipTensor *tensors, int n, const float *factor, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

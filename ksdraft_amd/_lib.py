@@ -87,6 +87,17 @@ SIGNATURES = {
     "ksd_rosa_credits": [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _INT, _P, _P, _P, _P],
     "ksd_rosa_credit_grads": [_P, _P, _P, _P, _INT, _P, _I64, _I64, _I64,
                               _P, _P, _P, _P, _P],
+    "ksd_tc_quantize_rows": [_P, _INT, _I64, _I64, _I64, _P, _I64, _P, _P],
+    "ksd_tc_gemm_workspace": [_I64, _I64, _I64, _P],
+    "ksd_tc_gemm": [_P, _I64, _INT, _P, _P, _I64, _INT, _P, _I64, _I64, _I64, _P, _P, _P, _INT, _P, _I64, _P],
+    "ksd_tc_grad_workspace": [_I64, _I64, _P],
+    "ksd_tc_quantize_grad": [_P, _INT, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P, _I64, _P, _P, _I64, _P],
+    "ksd_embedding_lookup": [_P, _INT, _I64, _I64, _I64, _P, _INT, _I64, _F, _P, _INT, _P],
+    "ksd_embedding_gradient_workspace": [_I64, _I64, _P],
+    "ksd_embedding_gradient": [_P, _INT, _I64, _I64, _I64, _P, _INT, _I64, _I64, _F, _INT, _P, _INT, _P, _I64, _P],
+    "ksd_grad_norm_workspace": [_P, _INT, _P],
+    "ksd_grad_norm": [_P, _INT, _INT, _F, _F, _P, _P, _P, _I64, _P],
+    "ksd_grad_scale": [_P, _INT, _P, _P],
 }
 
 _lib = None

@@ -1,0 +1,244 @@
+// Global norm of many gradient tensors, and their clipping:
+//
+//   norm = sqrt(sum of all g^2) / loss_scale   (or max |g| / loss_scale)
+//   factor = min(1, max_norm / (norm + 1e-6)) / loss_scale,   g' = g * factor
+//
+// Squares and their sums are fp64: an fp32 gradient's square neither overflows nor underflows there,
+// and at one fma per element the fp64 pipe keeps up with memory. The partial sums of a fixed
+// assignment of chunks to workgroups are added in a fixed order: repeated calls give the same bits.
+#include "ksd_common.h"
+
+#include <algorithm>
+
+namespace ksd {
+namespace clip {
+
+constexpr int kBatch = 96;     // tensors of a launch (their descriptors are its arguments)
+constexpr int kChunk = 16384;  // elements of a chunk
+constexpr int kGrid = 1024;    // workgroups of a launch, at most
+
+struct Tensor {
+  const void *g;
+  void *out;
+  int64_t n;
+  int32_t first, type;  // first chunk; element type
+};
+struct Batch {
+  Tensor t[kBatch];
+  int n, chunks;
+};
+
+__device__ __forceinline__ const Tensor &tensor_of(const Batch &b, int chunk) {
+  int lo = 0, hi = b.n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (b.t[mid].first <= chunk) lo = mid;
+    else hi = mid - 1;
+  }
+  return b.t[lo];
+}
+
+template <int DT>
+__device__ __forceinline__ void load8(const typename Elem<DT>::T *p, float *v) {
+  struct __attribute__((packed, aligned(DT == KSD_F32 ? 4 : 2))) Any { uint4 q; };
+  Raw8<DT> r;
+  r.a = ((const Any *)p)->q;
+  if constexpr (DT == KSD_F32) r.b = ((const Any *)(p + 4))->q;
+  cvt_raw8<DT>(r, true, v);
+}
+
+template <int DT, bool MAX>
+__device__ __forceinline__ void chunk_norm(const Tensor &t, int64_t e0, double &sum, uint32_t &top) {
+  using T = typename Elem<DT>::T;
+  const T *g = (const T *)t.g;
+  const int64_t e1 = min(t.n, e0 + kChunk);
+  for (int64_t e = e0 + threadIdx.x * 8; e < e1; e += 2048) {
+    float v[8];
+    if (e + 8 <= e1) {
+      load8<DT>(g + e, v);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = e + j < e1 ? Elem<DT>::load(g + e + j) : 0.0f;
+    }
+    if constexpr (MAX) {
+      top = max(top, __builtin_bit_cast(uint32_t, abs_max<8>(v)));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum = fma((double)v[j], (double)v[j], sum);
+    }
+  }
+}
+
+template <bool MAX>
+__global__ __launch_bounds__(256) void norm_kernel(const Batch b, double *__restrict__ parts) {
+  double sum = 0.0;
+  uint32_t top = 0;
+  for (int c = blockIdx.x; c < b.chunks; c += gridDim.x) {
+    const Tensor &t = tensor_of(b, c);
+    const int64_t e0 = (int64_t)(c - t.first) * kChunk;
+    if (t.type == KSD_F32) chunk_norm<KSD_F32, MAX>(t, e0, sum, top);
+    else if (t.type == KSD_BF16) chunk_norm<KSD_BF16, MAX>(t, e0, sum, top);
+    else chunk_norm<KSD_F16, MAX>(t, e0, sum, top);
+  }
+  if constexpr (MAX) sum = (double)__builtin_bit_cast(float, top);
+  __shared__ double s[256];
+  s[threadIdx.x] = sum;
+  __syncthreads();
+  for (int o = 128; o > 0; o >>= 1) {
+    if ((int)threadIdx.x < o) {
+      const double x = s[threadIdx.x], y = s[threadIdx.x + o];
+      s[threadIdx.x] = MAX ? (x != x || x > y ? x : y) : x + y;
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) parts[blockIdx.x] = s[0];
+}
+
+template <bool MAX>
+__global__ __launch_bounds__(1024) void fold_kernel(const double *__restrict__ parts, int n, float max_norm, float loss_scale,
+                                                    float *__restrict__ norm, float *__restrict__ factor) {
+  __shared__ double s[1024];
+  double sum = 0.0;
+  for (int i = threadIdx.x; i < n; i += 1024) {
+    const double y = parts[i];
+    sum = MAX ? (sum != sum || sum > y ? sum : y) : sum + y;
+  }
+  s[threadIdx.x] = sum;
+  __syncthreads();
+  for (int o = 512; o > 0; o >>= 1) {
+    if ((int)threadIdx.x < o) {
+      const double x = s[threadIdx.x], y = s[threadIdx.x + o];
+      s[threadIdx.x] = MAX ? (x != x || x > y ? x : y) : x + y;
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) {
+    const float total = (float)((MAX ? s[0] : sqrt(s[0])) / (double)loss_scale);
+    norm[0] = total;
+    if (factor) {
+      float c = max_norm / (total + 1e-6f);
+      c = c > 1.0f ? 1.0f : c;  // a NaN norm stays
+      factor[0] = c / loss_scale;
+    }
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ void chunk_scale(const Tensor &t, int64_t e0, float f) {
+  using T = typename Elem<DT>::T;
+  const T *g = (const T *)t.g;
+  T *o = (T *)t.out;
+  const int64_t e1 = min(t.n, e0 + kChunk);
+  for (int64_t e = e0 + threadIdx.x * 8; e < e1; e += 2048) {
+    float v[8];
+    if (e + 8 <= e1) {
+      load8<DT>(g + e, v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] *= f;
+      struct __attribute__((packed, aligned(DT == KSD_F32 ? 4 : 2))) Any { uint32_t w[4]; };
+      Any *q = (Any *)(o + e);
+      if constexpr (DT == KSD_F32) {
+        Any a, b;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) a.w[j] = __builtin_bit_cast(uint32_t, v[j]), b.w[j] = __builtin_bit_cast(uint32_t, v[4 + j]);
+        q[0] = a, q[1] = b;
+      } else {
+        Any a;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          uint16_t lo, hi;
+          store_out<DT>(&lo, 0, v[2 * k]);
+          store_out<DT>(&hi, 0, v[2 * k + 1]);
+          a.w[k] = lo | (uint32_t)hi << 16;
+        }
+        q[0] = a;
+      }
+    } else {
+      for (int j = 0; j < 8 && e + j < e1; ++j) store_out<DT>(o, e + j, Elem<DT>::load(g + e + j) * f);
+    }
+  }
+}
+
+__global__ __launch_bounds__(256) void scale_kernel(const Batch b, const float *__restrict__ factor) {
+  const float f = factor[0];
+  for (int c = blockIdx.x; c < b.chunks; c += gridDim.x) {
+    const Tensor &t = tensor_of(b, c);
+    if (f == 1.0f && t.g == t.out) continue;  // in place, nothing to change
+    const int64_t e0 = (int64_t)(c - t.first) * kChunk;
+    if (t.type == KSD_F32) chunk_scale<KSD_F32>(t, e0, f);
+    else if (t.type == KSD_BF16) chunk_scale<KSD_BF16>(t, e0, f);
+    else chunk_scale<KSD_F16>(t, e0, f);
+  }
+}
+
+// Calls launch(batch, grid) for batches of the tensors; an error code ends it.
+template <class F>
+static void batches(const KsdClipTensor *t, int n, F launch) {
+  Batch b;
+  b.n = b.chunks = 0;
+  for (int i = 0; i < n; ++i) {
+    if (t[i].n == 0) continue;
+    const int64_t chunks = cdiv(t[i].n, kChunk);
+    if (b.n == kBatch || b.chunks + chunks > 0x7fffffff) {
+      launch(b, std::min(b.chunks, kGrid));
+      b.n = b.chunks = 0;
+    }
+    b.t[b.n++] = Tensor{t[i].grad, t[i].out, t[i].n, b.chunks, t[i].dtype};
+    b.chunks += (int)chunks;
+  }
+  if (b.n) launch(b, std::min(b.chunks, kGrid));
+}
+
+static int check(const KsdClipTensor *t, int n, const char *who, bool out) {
+  if (n < 0 || (n > 0 && !t)) return fail(KSD_EINVAL, "%s: bad tensor list", who);
+  for (int i = 0; i < n; ++i) {
+    if (t[i].n < 0 || t[i].n > (int64_t)kChunk * 0x7fffffff) return fail(KSD_EINVAL, "%s: tensor %d: bad size", who, i);
+    if (t[i].dtype != KSD_F32 && t[i].dtype != KSD_BF16 && t[i].dtype != KSD_F16)
+      return fail(KSD_ETYPE, "%s: tensor %d: unsupported element type %d", who, i, t[i].dtype);
+    if (t[i].n > 0 && (!t[i].grad || (out && !t[i].out))) return fail(KSD_EINVAL, "%s: tensor %d: null pointer", who, i);
+  }
+  return KSD_OK;
+}
+
+}  // namespace clip
+}  // namespace ksd
+
+using namespace ksd;
+
+extern "C" int ksd_grad_norm_workspace(const KsdClipTensor *tensors, int n, int64_t *bytes) {
+  if (!bytes) return fail(KSD_EINVAL, "grad_norm_workspace: null pointer");
+  const int rc = clip::check(tensors, n, "grad_norm_workspace", false);
+  if (rc) return rc;
+  int64_t parts = 0;
+  clip::batches(tensors, n, [&](const clip::Batch &, int grid) { parts += grid; });
+  *bytes = 8 * std::max<int64_t>(parts, 1);
+  return KSD_OK;
+}
+
+extern "C" int ksd_grad_norm(const KsdClipTensor *tensors, int n, int max_kind, float max_norm, float loss_scale, float *norm,
+                             float *factor, void *workspace, int64_t workspace_bytes, void *stream) {
+  int64_t need = 0;
+  const int rc = ksd_grad_norm_workspace(tensors, n, &need);
+  if (rc) return rc;
+  if (!norm || !workspace || workspace_bytes < need) return fail(KSD_EINVAL, "grad_norm: null pointer or short workspace");
+  hipStream_t st = (hipStream_t)stream;
+  double *parts = (double *)workspace;
+  int at = 0;
+  clip::batches(tensors, n, [&](const clip::Batch &b, int grid) {
+    if (max_kind) clip::norm_kernel<true><<<grid, 256, 0, st>>>(b, parts + at);
+    else clip::norm_kernel<false><<<grid, 256, 0, st>>>(b, parts + at);
+    at += grid;
+  });
+  if (max_kind) clip::fold_kernel<true><<<1, 1024, 0, st>>>(parts, at, max_norm, loss_scale, norm, factor);
+  else clip::fold_kernel<false><<<1, 1024, 0, st>>>(parts, at, max_norm, loss_scale, norm, factor);
+  return check_launch("grad_norm");
+}
+
+extern "C" int ksd_grad_scale(const KsdClipTensor *tensors, int n, const float *factor, void *stream) {
+  const int rc = clip::check(tensors, n, "grad_scale", true);
+  if (rc) return rc;
+  if (!factor) return fail(KSD_EINVAL, "grad_scale: null pointer");
+  hipStream_t st = (hipStream_t)stream;
+  clip::batches(tensors, n, [&](const clip::Batch &b, int grid) { clip::scale_kernel<<<grid, 256, 0, st>>>(b, factor); });
+  return check_launch("grad_scale");
+}

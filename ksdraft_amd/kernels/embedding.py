@@ -8,9 +8,14 @@ both the head GEMM and the lookup. ``embedding_gather_int8`` returns the looked-
 dequantized (code * scale, exact in fp32). ``Int8Embedding`` is an nn.Embedding drop-in
 (fp32 master ``weight``) whose backward is the float embedding's: the scatter-add of the
 upstream gradient into the master (straight through the quantization).
+
+``embedding_lookup`` / ``embedding_gradient`` / ``ScaledEmbedding`` are the float table's lookup
+times a scale (nn.Embedding and a multiplication) and its gradient by sorted tokens.
 """
 
 from __future__ import annotations
+
+import ctypes
 
 import torch
 from torch import nn
@@ -136,3 +141,119 @@ class Int8Embedding(nn.Module):
     def forward(self, ids: torch.Tensor) -> torch.Tensor:
         codes, scales = self._codes()
         return _Int8EmbeddingFunction.apply(ids, self.weight, codes, scales, self.group)
+
+
+def _check_ids(ids: torch.Tensor, V: int, check: bool) -> torch.Tensor:
+    if ids.dtype not in (torch.int64, torch.int32):
+        raise TypeError("ids must be integer token indices")
+    flat = ids.reshape(-1).contiguous()
+    if check and flat.numel():  # nn.Embedding raises for such ids (a host sync)
+        bad = (flat < 0) | (flat >= V)
+        if bool(bad.any()):
+            raise IndexError(f"index {int(flat[bad][0])} is out of range for {V} rows")
+    return flat
+
+
+def _dense_rows(t: torch.Tensor) -> torch.Tensor:
+    return t if t.stride(1) == 1 and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]) else t.contiguous()
+
+
+def embedding_lookup(weight: torch.Tensor, ids: torch.Tensor, scale: float = 1.0,
+                     out_dtype: torch.dtype | None = None, check_ids: bool = True) -> torch.Tensor:
+    """round(scale * weight[ids]) in out_dtype (weight's by default): weight (V, d) float, ids (...)
+    int32 or int64 -> (..., d). The product is fp32, rounded once. With check_ids=False (no host
+    sync) an id out of range gives a row of zeros."""
+    dev = _lib.require_gpu(weight, ids)
+    if weight.dim() != 2:
+        raise ValueError("weight must be a 2-D table (V, d)")
+    out_dtype = out_dtype or weight.dtype
+    if weight.dtype not in _OUT or out_dtype not in _OUT:
+        raise TypeError(f"unsupported dtypes {weight.dtype} -> {out_dtype}")
+    V, d = weight.shape
+    flat = _check_ids(ids, V, check_ids)
+    weight = _dense_rows(weight)
+    out = torch.empty((*ids.shape, d), dtype=out_dtype, device=dev)
+    _lib.call("ksd_embedding_lookup", weight.data_ptr(), _OUT[weight.dtype], V, d, weight.stride(0) if V > 1 else d,
+              flat.data_ptr(), int(flat.dtype == torch.int64), flat.numel(), scale, out.data_ptr(), _OUT[out_dtype],
+              _lib.stream_ptr(dev))
+    return out
+
+
+def embedding_gradient(grad: torch.Tensor, ids: torch.Tensor, num_embeddings: int, scale: float = 1.0,
+                       padding_idx: int | None = None, out_dtype: torch.dtype = torch.float32,
+                       out: torch.Tensor | None = None, accumulate: bool = False,
+                       check_ids: bool = True) -> torch.Tensor:
+    """The gradient of embedding_lookup's table: dW[v] = scale * sum of grad[i] over ids[i] == v, in
+    fp32 in the order of the positions, rounded once to out_dtype; the row of padding_idx is 0.
+
+    grad (..., d) float, ids of its leading shape -> (num_embeddings, d). ``out`` (dense) takes the
+    result; with accumulate=True the sums are added to what it holds and only the rows of ids that
+    occur are touched (a tied head's dense gradient). Without atomics: repeated calls give the same
+    bits. With check_ids=False (no host sync) ids out of range are left out."""
+    dev = _lib.require_gpu(grad, ids, out)
+    if grad.shape[:-1] != ids.shape:
+        raise ValueError(f"grad {tuple(grad.shape)} does not match ids {tuple(ids.shape)}")
+    V, d = int(num_embeddings), grad.shape[-1]
+    if out is not None:
+        if out.shape != (V, d) or not out.is_contiguous() or out.data_ptr() % 16:
+            raise ValueError(f"out must be a contiguous ({V}, {d}) tensor on a 16-byte boundary")
+        out_dtype = out.dtype
+    elif accumulate:
+        raise ValueError("accumulate=True adds to out, and none is given")
+    if grad.dtype not in _OUT or out_dtype not in _OUT:
+        raise TypeError(f"unsupported dtypes {grad.dtype} -> {out_dtype}")
+    if padding_idx is not None and not -V <= padding_idx < V:
+        raise ValueError(f"padding_idx {padding_idx} is out of range for {V} rows")
+    pad = -1 if padding_idx is None else padding_idx % V
+    flat = _check_ids(ids, V, check_ids)
+    g = _dense_rows(grad.reshape(-1, d)) if d else grad.reshape(-1, 0)
+    n = flat.numel()
+    if out is None:
+        out = torch.empty((V, d), dtype=out_dtype, device=dev)
+    need = ctypes.c_int64()
+    _lib.call("ksd_embedding_gradient_workspace", n, d, ctypes.byref(need))
+    work = torch.empty(need.value, dtype=torch.int8, device=dev)
+    _lib.call("ksd_embedding_gradient", g.data_ptr(), _OUT[g.dtype], n, d, g.stride(0) if n > 1 else d, flat.data_ptr(),
+              int(flat.dtype == torch.int64), V, pad, scale, int(accumulate), out.data_ptr(), _OUT[out_dtype],
+              work.data_ptr(), need.value, _lib.stream_ptr(dev))
+    return out
+
+
+class _ScaledLookup(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, weight, ids, scale, padding_idx, out_dtype, check_ids):
+        ctx.save_for_backward(ids)
+        ctx.args = (weight.shape[0], scale, padding_idx, weight.dtype)
+        return embedding_lookup(weight, ids, scale, out_dtype, check_ids)
+
+    @staticmethod
+    def backward(ctx, grad):
+        (ids,) = ctx.saved_tensors
+        V, scale, pad, dtype = ctx.args
+        dw = embedding_gradient(grad, ids, V, scale, pad, dtype, check_ids=False)  # checked in the forward
+        return dw, None, None, None, None, None
+
+
+class ScaledEmbedding(nn.Module):
+    """nn.Embedding(V, d) whose rows come out times ``scale`` (a model's sqrt(d), for instance), in
+    ``out_dtype``, with the gradient of embedding_gradient."""
+
+    def __init__(self, num_embeddings: int, embedding_dim: int, scale: float = 1.0, padding_idx: int | None = None,
+                 out_dtype: torch.dtype | None = None, check_ids: bool = True):
+        super().__init__()
+        self.num_embeddings = num_embeddings
+        self.embedding_dim = embedding_dim
+        self.scale = float(scale)
+        self.padding_idx = padding_idx
+        self.out_dtype = out_dtype
+        self.check_ids = check_ids
+        self.weight = nn.Parameter(torch.zeros(num_embeddings, embedding_dim))
+
+    @classmethod
+    def from_float(cls, module: nn.Embedding, scale: float = 1.0, **kwargs) -> "ScaledEmbedding":
+        emb = cls(module.num_embeddings, module.embedding_dim, scale, module.padding_idx, **kwargs)
+        emb.weight = module.weight  # the same master (a tied head keeps its tie)
+        return emb
+
+    def forward(self, ids: torch.Tensor) -> torch.Tensor:
+        return _ScaledLookup.apply(self.weight, ids, self.scale, self.padding_idx, self.out_dtype, self.check_ids)

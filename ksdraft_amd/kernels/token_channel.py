@@ -1,0 +1,289 @@
+"""W8A8 products with one fp32 scale per token and one per output channel.
+
+The group-128 product (``kernels.gemm``) rescales its int32 sums every 128 columns; here the
+scales stand outside the whole reduction:
+
+    y[m, n] = (sum_k xq[m, k] wq[n, k]) * sx[m] * sw[n] + bias[n]
+
+``quantize_rows`` gives the codes of either operand (symmetric, max |row| / 127). Both gradients
+use the forward's codes as they are: a scale along the contracted dimension moves into dY before
+dY is quantized,
+
+    dX = e[m] sum_n q[m, n] wq[n, k],   (q, e) = quantize_rows(dY * sw)
+    dW = f[n] sum_m c[m, n] xq[m, k],   (c, f) = the same per column of dY * sx
+
+``TokenChannelLinear`` is an nn.Linear drop-in on them. There is no CPU path.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+from torch import nn
+
+from .. import _lib
+
+_OUT = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+
+
+def _pitch(n: int) -> int:
+    return -(-n // 16) * 16
+
+
+def _matrix(x: torch.Tensor, name: str) -> torch.Tensor:
+    """A 2-D float tensor with dense rows, as the kernels read it."""
+    if x.dim() != 2:
+        raise ValueError(f"{name} must be 2-D, got {tuple(x.shape)}")
+    if x.dtype not in _OUT:
+        raise TypeError(f"{name}: unsupported dtype {x.dtype}")
+    if x.shape[1] == 0:
+        raise ValueError(f"{name} has no columns")
+    if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
+        x = x.contiguous()
+    return x
+
+
+def _rows(x: torch.Tensor, dev: torch.device):
+    """Codes in a (M, pitch) buffer with zeros past K, and scales."""
+    M, K = x.shape
+    codes = torch.empty((M, _pitch(K)), dtype=torch.int8, device=dev)
+    scales = torch.empty(M, dtype=torch.float32, device=dev)
+    _lib.call("ksd_tc_quantize_rows", x.data_ptr(), _OUT[x.dtype], M, K, x.stride(0) if M > 1 else K,
+              codes.data_ptr(), codes.shape[1], scales.data_ptr(), _lib.stream_ptr(dev))
+    return codes, scales
+
+
+def quantize_rows(x: torch.Tensor):
+    """x (M, K) float -> (codes (M, K) int8, scales (M,) fp32) with x ~ codes * scales[:, None].
+
+    Per row: a = max |x|; scale = a / 127 and code = rint(x * (127 / a)), each operation rounded to
+    fp32; a < 2**-100 gives scale 0 and codes 0, a row with NaN or inf scale NaN and codes 0. The
+    codes are a view of rows padded with zeros to a multiple of 16 bytes, the layout the products
+    read without a copy."""
+    dev = _lib.require_gpu(x)
+    x = _matrix(x, "x")
+    codes, scales = _rows(x, dev)
+    return codes[:, :x.shape[1]], scales
+
+
+def _codes_operand(q: torch.Tensor, name: str, zeros: bool = False):
+    """An int8 matrix as the products read it: (tensor that owns the memory, row pitch). Rows whose
+    pitch is no multiple of 16, or that end before their last 16-byte chunk does, are copied; with
+    ``zeros`` (one operand of a product needs zeros up to its rows' next multiple of 16) also rows
+    of another length, since what follows a caller's rows is not known."""
+    if q.dim() != 2 or q.dtype != torch.int8:
+        raise ValueError(f"{name} must be a 2-D int8 tensor")
+    M, K = q.shape
+    if K == 0:
+        raise ValueError(f"{name} has no columns")
+    ld = q.stride(0) if M > 1 else _pitch(K)
+    end = (q.storage_offset() + max(M - 1, 0) * ld + _pitch(K))
+    if (not (zeros and K % 16) and q.stride(1) == 1 and ld % 16 == 0 and ld >= _pitch(K) and q.data_ptr() % 16 == 0
+            and end <= q.untyped_storage().nbytes()):
+        return q, ld
+    out = torch.zeros((M, _pitch(K)), dtype=torch.int8, device=q.device)
+    out[:, :K] = q
+    return out, _pitch(K)
+
+
+def _vector(t: torch.Tensor | None, n: int, name: str) -> torch.Tensor | None:
+    if t is None:
+        return None
+    if t.dtype != torch.float32 or t.numel() != n:
+        raise ValueError(f"{name} must hold {n} float32 values, got {tuple(t.shape)} {t.dtype}")
+    return t.contiguous()
+
+
+def _gemm(a, lda, a_t, sa, w, ldw, w_t, sw, M, N, K, bias, residual, out_dtype, dev):
+    y = torch.empty((M, N), dtype=out_dtype, device=dev)
+    need = ctypes.c_int64()
+    _lib.call("ksd_tc_gemm_workspace", M, N, K, ctypes.byref(need))
+    work = torch.empty(need.value, dtype=torch.int8, device=dev) if need.value else None
+    _lib.call("ksd_tc_gemm", a.data_ptr(), lda, a_t, _lib.ptr(sa), w.data_ptr(), ldw, w_t, _lib.ptr(sw), M, N, K,
+              _lib.ptr(bias), _lib.ptr(residual), y.data_ptr(), _OUT[out_dtype], _lib.ptr(work), need.value,
+              _lib.stream_ptr(dev))
+    return y
+
+
+def _epilogue(M: int, N: int, bias, residual, out_dtype):
+    if out_dtype not in _OUT:
+        raise TypeError(f"unsupported output dtype {out_dtype}")
+    bias = _vector(bias, N, "bias")
+    if residual is not None:
+        if residual.shape != (M, N) or residual.dtype != out_dtype:
+            raise ValueError(f"residual must be ({M}, {N}) {out_dtype}, got {tuple(residual.shape)} {residual.dtype}")
+        residual = residual.contiguous()
+    return bias, residual
+
+
+def token_channel_gemm(a_codes: torch.Tensor, a_scales: torch.Tensor, w_codes: torch.Tensor, w_scales: torch.Tensor,
+                       bias: torch.Tensor | None = None, residual: torch.Tensor | None = None,
+                       out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """y = (a_codes . w_codes^T) * a_scales[:, None] * w_scales (+ bias) (+ residual), in fp32,
+    rounded once to out_dtype. a_codes (M, K), w_codes (N, K) int8 with |code| <= 127; scales and
+    bias fp32. K must be the same; the int32 sums are exact for any K."""
+    dev = _lib.require_gpu(a_codes, a_scales, w_codes, w_scales, bias, residual)
+    a, lda = _codes_operand(a_codes, "a_codes", zeros=True)
+    w, ldw = _codes_operand(w_codes, "w_codes")
+    (M, K), (N, Kw) = a_codes.shape, w_codes.shape
+    if K != Kw:
+        raise ValueError(f"a_codes has {K} columns, w_codes {Kw}")
+    bias, residual = _epilogue(M, N, bias, residual, out_dtype)
+    return _gemm(a, lda, 0, _vector(a_scales, M, "a_scales"), w, ldw, 0, _vector(w_scales, N, "w_scales"), M, N, K,
+                 bias, residual, out_dtype, dev)
+
+
+def token_channel_linear(x: torch.Tensor, w_codes: torch.Tensor, w_scales: torch.Tensor,
+                         bias: torch.Tensor | None = None, residual: torch.Tensor | None = None,
+                         out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """y = W8A8(x, W) + bias (+ residual): x (..., K) float is quantized per token and multiplied
+    with the stored codes (N, K) of quantize_rows(weight). The output has x's dtype unless
+    out_dtype is given; residual is (..., N) of the output's."""
+    dev = _lib.require_gpu(x, w_codes, w_scales, bias, residual)
+    w, ldw = _codes_operand(w_codes, "w_codes")
+    N, K = w_codes.shape
+    if x.dim() == 0 or x.shape[-1] != K:
+        raise ValueError(f"x has shape {tuple(x.shape)}, w_codes {tuple(w_codes.shape)}")
+    x2 = _matrix(x.reshape(-1, K), "x")
+    M = x2.shape[0]
+    out_dtype = out_dtype or x.dtype
+    bias, residual = _epilogue(M, N, bias, None if residual is None else residual.reshape(-1, N), out_dtype)
+    w_scales = _vector(w_scales, N, "w_scales")
+    codes, scales = _rows(x2, dev)
+    y = _gemm(codes, codes.shape[1], 0, scales, w, ldw, 0, w_scales, M, N, K, bias, residual, out_dtype, dev)
+    return y.reshape(*x.shape[:-1], N)
+
+
+class Saved:
+    """What token_channel_linear_backward needs of a training forward: both operands' codes and
+    scales (a byte per element of x and W instead of x itself)."""
+
+    __slots__ = ("xq", "xs", "wq", "ws", "M", "N", "K", "dtype", "lead", "has_bias")
+
+
+def token_channel_linear_train(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
+                               residual: torch.Tensor | None = None):
+    """The training forward on a float master ``weight`` (N, K): quantizes both operands and returns
+    (y, saved), y as token_channel_linear gives it in x's dtype."""
+    dev = _lib.require_gpu(x, weight, bias, residual)
+    w2 = _matrix(weight, "weight")
+    N, K = w2.shape
+    if x.dim() == 0 or x.shape[-1] != K:
+        raise ValueError(f"x has shape {tuple(x.shape)}, weight {tuple(weight.shape)}")
+    x2 = _matrix(x.reshape(-1, K), "x")
+    s = Saved()
+    s.M, s.N, s.K, s.dtype, s.lead, s.has_bias = x2.shape[0], N, K, x.dtype, x.shape[:-1], bias is not None
+    bias, residual = _epilogue(s.M, N, bias, None if residual is None else residual.reshape(-1, N), x.dtype)
+    s.wq, s.ws = _rows(w2, dev)
+    s.xq, s.xs = _rows(x2, dev)
+    y = _gemm(s.xq, s.xq.shape[1], 0, s.xs, s.wq, s.wq.shape[1], 0, s.ws, s.M, N, K, bias, residual, x.dtype, dev)
+    return y.reshape(*s.lead, N), s
+
+
+def token_channel_linear_backward(grad: torch.Tensor, saved: Saved, need_dx: bool = True, need_dw: bool = True,
+                                  need_db: bool | None = None):
+    """(dx in x's dtype, dw (N, K) fp32, db (N,) fp32) for the upstream gradient of y; what is not
+    needed is None (db by default when the layer has a bias)."""
+    dev = _lib.require_gpu(grad, saved.xq)
+    M, N, K = saved.M, saved.N, saved.K
+    if grad.shape != (*saved.lead, N):
+        raise ValueError(f"grad has shape {tuple(grad.shape)}, the output {(*saved.lead, N)}")
+    g = _matrix(grad.reshape(-1, N), "grad")
+    need_db = saved.has_bias if need_db is None else need_db
+    dx = dw = db = None
+    if M == 0:
+        return (torch.empty((*saved.lead, K), dtype=saved.dtype, device=dev) if need_dx else None,
+                torch.zeros((N, K), device=dev) if need_dw else None,
+                torch.zeros(N, device=dev) if need_db else None)
+    ld = _pitch(N)
+    q = torch.empty((M, ld), dtype=torch.int8, device=dev) if need_dx else None
+    c = torch.empty((M, ld), dtype=torch.int8, device=dev) if need_dw else None
+    db = torch.empty(N, dtype=torch.float32, device=dev) if need_db else None
+    need = ctypes.c_int64()
+    _lib.call("ksd_tc_grad_workspace", M, N, ctypes.byref(need))
+    work = torch.empty(need.value, dtype=torch.int8, device=dev)
+    ef = torch.empty(M + N, dtype=torch.float32, device=dev)
+    e, f = ef[:M], ef[M:]
+    _lib.call("ksd_tc_quantize_grad", g.data_ptr(), _OUT[g.dtype], M, N, g.stride(0) if M > 1 else N,
+              saved.xs.data_ptr(), saved.ws.data_ptr(), _lib.ptr(q), e.data_ptr(), _lib.ptr(c), f.data_ptr(), ld,
+              _lib.ptr(db), work.data_ptr(), need.value, _lib.stream_ptr(dev))
+    if need_dx:
+        dx = _gemm(q, ld, 0, e, saved.wq, saved.wq.shape[1], 1, None, M, K, N, None, None, saved.dtype, dev)
+        dx = dx.reshape(*saved.lead, K)
+    if need_dw:
+        dw = _gemm(c, ld, 1, f, saved.xq, saved.xq.shape[1], 1, None, N, K, M, None, None, torch.float32, dev)
+    return dx, dw, db
+
+
+class _LinearFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual):
+        y, saved = token_channel_linear_train(x, weight, bias, residual)
+        # through save_for_backward, so that they are freed with the graph
+        ctx.save_for_backward(saved.xq, saved.xs, saved.wq, saved.ws)
+        ctx.shape = (saved.M, saved.N, saved.K, saved.dtype, saved.lead, saved.has_bias)
+        ctx.weight_dtype = weight.dtype
+        return y
+
+    @staticmethod
+    def backward(ctx, grad):
+        s = Saved()
+        s.xq, s.xs, s.wq, s.ws = ctx.saved_tensors
+        s.M, s.N, s.K, s.dtype, s.lead, s.has_bias = ctx.shape
+        need = ctx.needs_input_grad
+        if grad.dtype not in _OUT:
+            grad = grad.float()
+        dx, dw, db = token_channel_linear_backward(grad, s, need[0], need[1], need[2])
+        return dx, None if dw is None else dw.to(ctx.weight_dtype), db, grad if need[3] else None
+
+
+class TokenChannelLinear(nn.Module):
+    """nn.Linear with int8 products in both directions, scales per token and per output channel.
+
+    The float master ``weight`` stays authoritative: its codes are rebuilt in every call, unless
+    ``pack()`` has stored them (serving: the master no longer changes); ``unpack()``, training
+    calls, moves and state-dict loads drop stored codes."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True):
+        super().__init__()
+        self.in_features = in_features
+        self.out_features = out_features
+        self.weight = nn.Parameter(torch.zeros(out_features, in_features))
+        self.bias = nn.Parameter(torch.zeros(out_features)) if bias else None
+        self._packed = None
+
+    @classmethod
+    def from_float(cls, module: nn.Linear) -> "TokenChannelLinear":
+        lin = cls(module.in_features, module.out_features, bias=module.bias is not None)
+        lin = lin.to(module.weight.device)
+        with torch.no_grad():
+            lin.weight.copy_(module.weight)
+            if module.bias is not None:
+                lin.bias.copy_(module.bias)
+        return lin
+
+    def pack(self) -> "TokenChannelLinear":
+        """Stores the codes of the master as it is now for calls without gradients."""
+        self._packed = quantize_rows(self.weight.detach())
+        return self
+
+    def unpack(self) -> "TokenChannelLinear":
+        self._packed = None
+        return self
+
+    def _apply(self, fn, *args, **kwargs):
+        self._packed = None
+        return super()._apply(fn, *args, **kwargs)
+
+    def _load_from_state_dict(self, *args, **kwargs):
+        self._packed = None
+        return super()._load_from_state_dict(*args, **kwargs)
+
+    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
+        if torch.is_grad_enabled() and (self.weight.requires_grad or x.requires_grad
+                                        or (residual is not None and residual.requires_grad)):
+            self._packed = None
+            return _LinearFunction.apply(x, self.weight, self.bias, residual)
+        codes, scales = self._packed or quantize_rows(self.weight.detach())
+        return token_channel_linear(x, codes, scales, None if self.bias is None else self.bias.detach(), residual)
