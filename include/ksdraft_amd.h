@@ -730,7 +730,7 @@ int ksd_tc_quantize_rows(const void *x, int x_dtype, int64_t M, int64_t K, int64
  * past 131072 steps are joined in 64 bits).
  *   a     (M, K) int8 in rows of lda bytes, zeros from K to the next multiple of 16; with a_t
  *         (K, M) instead
- *   w     (N, K) int8 in rows of ldw bytes; with w_t (K, N) instead. a_t needs w_t
+ *   w     (N, K) int8 in rows of ldw bytes; with w_t (K, N) instead. a_t needs w_t and fp32 y
  *   lda, ldw multiples of 16 that hold a row rounded up to 16 bytes, all of it readable, bases
  *         16-byte aligned
  *   sa (M,), sw (N,), bias (N,) fp32 or NULL; residual (M, N) of the output type or NULL

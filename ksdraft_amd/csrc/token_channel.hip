@@ -19,6 +19,7 @@
 #include "ksd_common.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace ksd {
 namespace tc {
@@ -304,11 +305,10 @@ struct Prob {
 
 constexpr int BK = 128;
 
+typedef __attribute__((address_space(3))) const v4i lds_v4i;
+typedef __attribute__((address_space(3))) v2i lds_v2i;
 __device__ __forceinline__ uint32_t lds_addr(const void *p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)(p);
-}
-__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, uint32_t off, int8_t *lds) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)lds, 16, off, 0, 0, 0);
 }
 
 // Position of 16-byte chunk c of LDS row r, in bytes. N tiles have rows of 128 bytes (the reduction),
@@ -316,138 +316,396 @@ __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t r, uint32_t off, in
 // the 16 lanes that read one fragment chunk (16 rows of an N tile; 8 rows of a T tile, two such row
 // sets per 32 lanes) hit 16 different 16-byte bank groups.
 template <bool T, int B>
-__device__ __forceinline__ int lds_pos(int r, int c) {
-  if constexpr (!T) return r * BK + ((c ^ ((r >> 1) & 7)) << 4);
-  else if constexpr (B == 256) return r * 256 + ((c ^ ((r & 7) | ((r >> 1) & 8))) << 4);
-  else return r * 128 + ((c ^ (((r >> 1) & 3) | ((r >> 2) & 4))) << 4);
+__device__ __forceinline__ constexpr int lds_swz(int r) {
+  if constexpr (!T) return (r >> 1) & 7;
+  else if constexpr (B == 256) return (r & 7) | ((r >> 1) & 8);
+  else if constexpr (B == 192) return ((r >> 2) & 1) | ((r >> 3) & 2);
+  else return ((r >> 1) & 3) | ((r >> 2) & 4);
 }
-
-// Fills a B x 128 tile: rows [row0, row0 + B) (output index), reduction steps [k0, k0 + 128) of an
-// operand with `rows` output rows and K reduction steps. NW waves; what lies outside reads as zero.
-// PERM: the output index of LDS row p within each block of 16 NJ rows is permuted so that one lane's
-// results are 4 NJ consecutive columns (see the store).
-template <bool T, int B, int NW, int NJ>
-__device__ __forceinline__ void fill(const int8_t *P, int64_t ld, int rows, int K, int row0, int k0, int8_t *lds,
-                                     int wave, int lane) {
-  constexpr int INSTR = B * BK / 1024;  // 1 KB each
-  if constexpr (!T) {
-    const int valid = min(B, rows - row0), kb = (K + 15) & ~15;
-    const __amdgpu_buffer_rsrc_t r = rsrc(P + (int64_t)row0 * ld, (int64_t)valid * ld);
-#pragma unroll
-    for (int i = wave; i < INSTR; i += NW) {
-      const int p = i * 8 + (lane >> 3), c = (lane & 7) ^ ((p >> 1) & 7);
-      int row = p;
-      if constexpr (NJ > 0) {
-        const int b = p / (16 * NJ), o = p % (16 * NJ), j = o >> 4, ii = o & 15;
-        row = b * (16 * NJ) + (ii >> 2) * (4 * NJ) + j * 4 + (ii & 3);
-      }
-      const int k = k0 + c * 16;
-      const uint32_t off = row < valid && k < kb ? (uint32_t)(row * ld + k) : kOob;
-      dma16(r, off, lds + i * 1024);
-    }
-  } else {
-    const int valid = min(BK, K - k0), cb = (rows + 15) & ~15;
-    const __amdgpu_buffer_rsrc_t r = rsrc(P + (int64_t)k0 * ld, (int64_t)max(valid, 0) * ld);
-#pragma unroll
-    for (int i = wave; i < INSTR; i += NW) {
-      constexpr int CPR = B / 16;
-      const int kr = i * (64 / CPR) + lane / CPR, slot = lane % CPR;
-      const int c = slot ^ ((lds_pos<true, B>(kr, 0) >> 4) & (CPR - 1));
-      const int col = row0 + c * 16;
-      const uint32_t off = kr < valid && col < cb ? (uint32_t)(kr * ld + col) : kOob;
-      dma16(r, off, lds + i * 1024);
-    }
-  }
-}
-
-// 16 output rows x 64 reduction steps as an MFMA operand: lane l holds row l % 16, steps
-// 16 (l / 16) .. + 15 of half kk.
 template <bool T, int B>
-__device__ __forceinline__ v4i frag(const int8_t *lds, int row0, int kk, int lane) {
-  if constexpr (!T) {
-    return *(const v4i *)(lds + lds_pos<false, B>(row0 + (lane & 15), kk * 4 + (lane >> 4)));
-  } else {
-    // lanes 2r, 2r + 1 of each 16 address the two halves of step r's 16 bytes; the read leaves lane
-    // c the 8 steps of column c
-    typedef __attribute__((address_space(3))) v2i lds_v2i;
-    const int kr = kk * 64 + (lane >> 4) * 16 + ((lane & 15) >> 1);
-    const v2i lo = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-        (lds_v2i *)(lds + lds_pos<true, B>(kr, row0 >> 4) + (lane & 1) * 8));
-    const v2i hi = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-        (lds_v2i *)(lds + lds_pos<true, B>(kr + 8, row0 >> 4) + (lane & 1) * 8));
-    return (v4i){lo.x, lo.y, hi.x, hi.y};
-  }
+__device__ __forceinline__ constexpr int lds_pos(int r, int c) {
+  return r * (T ? B : BK) + ((c ^ lds_swz<T, B>(r)) << 4);
 }
+
+// The DMA of one operand's B x 128 tile into LDS: 1 KB instructions, lane l of instruction i fills
+// chunk 64 i + l of the tile. PERM > 0: the output index of LDS row p within each block of 16 PERM rows
+// is permuted so that one lane's results are PERM consecutive columns (see the store). What lies
+// outside the operand reads as zero (offsets past the buffer's range).
+template <bool T, int B, int NW, int PERM>
+struct Stage {
+  static constexpr int INSTR = B * BK / 1024, D = INSTR / NW;
+  static_assert(INSTR % NW == 0, "whole instructions per wave");
+  uint32_t off[D];
+  const int8_t *base;
+  int64_t ld;
+  int k0, K, valid, cb;
+
+  __device__ __forceinline__ void start(const int8_t *P, int64_t pitch, int rows, int Kn, int row0, int kfirst, int wave, int lane) {
+    ld = pitch, k0 = kfirst, K = Kn;
+    if constexpr (!T) {
+      valid = min(B, rows - row0);
+      base = P + (int64_t)row0 * ld + kfirst;
+#pragma unroll
+      for (int i = 0; i < D; ++i) {
+        const int p = (wave * D + i) * 8 + (lane >> 3), c = (lane & 7) ^ lds_swz<false, B>(p);
+        int row = p;
+        if constexpr (PERM > 0) {
+          const int b = p / (16 * PERM), o = p % (16 * PERM), j = o >> 4, ii = o & 15;
+          row = b * (16 * PERM) + ii * PERM + j;
+        }
+        off[i] = row < valid ? (uint32_t)(row * (int)ld + c * 16) : kOob;
+      }
+    } else {
+      cb = (rows + 15) & ~15;
+      base = P + (int64_t)kfirst * ld + row0;
+#pragma unroll
+      for (int i = 0; i < D; ++i) {
+        const int L = (wave * D + i) * 64 + lane, r = L / (B / 16), c = (L % (B / 16)) ^ lds_swz<true, B>(r);
+        off[i] = row0 + c * 16 < cb ? (uint32_t)(r * (int)ld + c * 16) : kOob;
+      }
+    }
+  }
+  typedef uint32_t rsrc4 __attribute__((ext_vector_type(4)));
+  rsrc4 rs;
+  bool tail;
+  // before the issues of a step; not live: every load reads as zero
+  __device__ __forceinline__ void open(bool live) {
+    const uint64_t a = (uint64_t)base;
+    const int rows_k = min(BK, K - k0);
+    uint32_t bytes;
+    if constexpr (!T) bytes = (uint32_t)(valid - 1) * (uint32_t)ld + BK;
+    else bytes = (uint32_t)rows_k * (uint32_t)ld;
+    if (!live) bytes = 0;
+    tail = !T && rows_k < BK;
+    rs = (rsrc4){(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)a), (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(a >> 32)),
+                 (uint32_t)__builtin_amdgcn_readfirstlane((int)bytes), (uint32_t)kBufFlags};
+  }
+  __device__ __forceinline__ void issue(int i, uint32_t lds, int wave, int lane) {
+    uint32_t o = off[i];
+    if constexpr (!T) {
+      if (__builtin_expect(tail, 0)) {
+        const int p = (wave * D + i) * 8 + (lane >> 3), c = (lane & 7) ^ lds_swz<false, B>(p);
+        if (k0 + c * 16 >= ((K + 15) & ~15)) o = kOob;
+      }
+    }
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+                 :: "v"(o), "s"(rs), "s"(lds + (uint32_t)(wave * D + i) * 1024) : "memory", "m0");
+  }
+  __device__ __forceinline__ void next() {
+    k0 += BK;
+    base += T ? (int64_t)BK * ld : BK;
+  }
+};
+
+// Reads of 16 output rows x 64 reduction steps as an MFMA operand: lane l holds row l % 16, steps
+// 16 (l / 16) .. + 15 of half kk. The swizzle of an N tile does not depend on the block of 16 rows i and
+// that of a T tile not on kk, so few lane addresses serve all reads and the rest is an immediate.
+template <bool T, int B, int NB>
+struct Reader {
+  uint32_t pos[T ? NB : 2];
+  __device__ __forceinline__ void start(uint32_t lds, int row0, int lane) {
+    if constexpr (!T) {
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) pos[kk] = lds + row0 * BK + lds_pos<false, B>(lane & 15, kk * 4 + (lane >> 4));
+    } else {
+      // lanes 2r, 2r + 1 of each 16 address the two halves of step r's 16 bytes; the read leaves lane
+      // c the 8 steps of column c
+      const int kr = (lane >> 4) * 16 + ((lane & 15) >> 1);
+#pragma unroll
+      for (int i = 0; i < NB; ++i) pos[i] = lds + lds_pos<true, B>(kr, row0 / 16 + i) + (lane & 1) * 8;
+    }
+  }
+  __device__ __forceinline__ void shift(uint32_t by) {
+#pragma unroll
+    for (int i = 0; i < (T ? NB : 2); ++i) pos[i] += by;
+  }
+  __device__ __forceinline__ v4i read(int i, int kk) const {
+    if constexpr (!T) {
+      return *(lds_v4i *)(uintptr_t)(pos[kk] + i * 16 * BK);
+    } else {
+      const v2i lo = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i *)(uintptr_t)(pos[i] + kk * 64 * B));
+      const v2i hi = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_v2i *)(uintptr_t)(pos[i] + kk * 64 * B + 8 * B));
+      return (v4i){lo.x, lo.y, hi.x, hi.y};
+    }
+  }
+};
 
 template <int OUT>
 __device__ __forceinline__ float load_out(const void *p, int64_t i) {
   return Elem<OUT>::load((const typename Elem<OUT>::T *)p + i);
 }
-
-// BM x BN tiles, WM x WN waves; TA, TW: the operand is a T one.
-template <int BM, int BN, int WM, int WN, bool TA, bool TW, int OUT>
-__global__ __launch_bounds__(WM *WN * 64) void gemm_kernel(const Prob p) {
-  constexpr int NW = WM * WN, NI = BM / WM / 16, NJ = BN / WN / 16;
-  constexpr int PERM = TW ? 0 : NJ;
-  __shared__ __attribute__((aligned(16))) int8_t sA[2][BM * BK];
-  __shared__ __attribute__((aligned(16))) int8_t sW[2][BN * BK];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave / WN, wn = wave % WN;
-  const int tn = (p.N + BN - 1) / BN;
-  const int t = blockIdx.x / p.splits, part = blockIdx.x % p.splits;
-  const int m0 = t / tn * BM, n0 = t % tn * BN;
-  const int kt = (p.K + BK - 1) / BK, q0 = part * p.ksteps, q1 = min(kt, q0 + p.ksteps);
-  auto stage = [&](int q) {
-    fill<TA, BM, NW, 0>(p.A, p.lda, p.M, p.K, m0, q * BK, sA[q & 1], wave, lane);
-    fill<TW, BN, NW, PERM>(p.W, p.ldw, p.N, p.K, n0, q * BK, sW[q & 1], wave, lane);
-  };
-  v4i acc[NI][NJ];
+// W (even) consecutive elements at any element alignment
+template <int OUT, int W>
+__device__ __forceinline__ void loadv(const void *p, int64_t i, float *v) {
+  if constexpr (OUT == KSD_F32) {
+    struct __attribute__((packed, aligned(4))) Any { float w[W]; };
+    const Any a = *(const Any *)((const float *)p + i);
 #pragma unroll
-  for (int i = 0; i < NI; ++i)
+    for (int j = 0; j < W; ++j) v[j] = a.w[j];
+  } else {
+    struct __attribute__((packed, aligned(2))) Any { uint32_t w[W / 2]; };
+    const Any a = *(const Any *)((const uint16_t *)p + i);
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) acc[i][j] = (v4i){0, 0, 0, 0};
-  if (q0 < q1) stage(q0);
-  for (int q = q0; q < q1; ++q) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (q + 1 < q1) stage(q + 1);
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      v4i a[NI], w[NJ];
-#pragma unroll
-      for (int i = 0; i < NI; ++i) a[i] = frag<TA, BM>(sA[q & 1], wm * (BM / WM) + i * 16, kk, lane);
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) w[j] = frag<TW, BN>(sW[q & 1], wn * (BN / WN) + j * 16, kk, lane);
-#pragma unroll
-      for (int i = 0; i < NI; ++i)
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[j], a[i], acc[i][j], 0, 0, 0);
+    for (int j = 0; j < W; ++j) {
+      const uint16_t h = (uint16_t)(a.w[j / 2] >> (j % 2 * 16));
+      v[j] = Elem<OUT>::load(&h);
     }
   }
-  // lane l of tile (i, j) holds row l % 16 and 4 consecutive columns
+}
+// Non-temporal: the streamed output does not push the operands' panels out of L2.
+template <int OUT, int W>
+__device__ __forceinline__ void storev(void *p, int64_t i, const float *v) {
+  if constexpr (OUT == KSD_F32) {
+    typedef float vec __attribute__((ext_vector_type(W), aligned(4)));
+    vec a;
 #pragma unroll
-  for (int i = 0; i < NI; ++i) {
-    const int m = m0 + wm * (BM / WM) + i * 16 + (lane & 15);
-    if (m >= p.M) continue;
-    const float sa = p.sa ? p.sa[m] : 1.0f;
+    for (int j = 0; j < W; ++j) a[j] = v[j];
+    __builtin_nontemporal_store(a, (vec *)((float *)p + i));
+  } else {
+    typedef uint32_t vec __attribute__((ext_vector_type(W / 2), aligned(2)));
+    vec a;
 #pragma unroll
-    for (int j = 0; j < NJ; ++j)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int n = n0 + wn * (BN / WN) + (PERM ? (lane >> 4) * 4 * NJ + j * 4 : j * 16 + (lane >> 4) * 4) + r;
-        if (n >= p.N) continue;
-        const int64_t at = (int64_t)m * p.N + n;
-        if (p.splits > 1) {
-          p.parts[(int64_t)part * p.M * p.N + at] = acc[i][j][r];
-          continue;
-        }
-        float y = (float)acc[i][j][r] * sa;
-        if (p.sw) y = y * p.sw[n];
-        if (p.bias) y = y + p.bias[n];
-        if (p.R) y = y + load_out<OUT>(p.R, at);
-        store_out<OUT>(p.Y, at, y);
+    for (int j = 0; j < W / 2; ++j) {
+      if constexpr (OUT == KSD_BF16) {
+        typedef float f32x2 __attribute__((ext_vector_type(2)));
+        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+        a[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){v[2 * j], v[2 * j + 1]}, bf16x2));
+      } else {
+        a[j] = f16_bits(v[2 * j]) | (uint32_t)f16_bits(v[2 * j + 1]) << 16;
       }
+    }
+    __builtin_nontemporal_store(a, (vec *)((uint16_t *)p + i));
   }
+}
+
+__device__ __forceinline__ void wg_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// BM x BN tiles, WM x WN waves; TA, TW: the operand is a T one. Persistent: a workgroup walks its
+// units (tile, part of the reduction); the DMA runs one step of 128 ahead across unit ends.
+// Per step each wave multiplies the first half (64) of the step while it reads the fragments of the
+// second, then one barrier, then the second half while it reads the next step's first.
+template <int BM, int BN, int WM, int WN, bool TA, bool TW, int OUT>
+__global__ __launch_bounds__(WM *WN * 64, WM * WN == 8 ? 1 : 2) void gemm_kernel(const Prob p) {
+  constexpr int NW = WM * WN, NI = BM / WM / 16, NJ = BN / WN / 16;
+  constexpr int PERM = TW ? 0 : NJ;
+  constexpr uint32_t SA = BM * BK, SW = BN * BK;
+  extern __shared__ __attribute__((aligned(1024))) int8_t smem[];  // A slots 0, 1, then W slots 0, 1
+  const uint32_t ldsA = lds_addr(smem), ldsW = ldsA + 2 * SA;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / WN, wn = wave % WN;
+  const int tm = (p.M + BM - 1) / BM, tn = (p.N + BN - 1) / BN, units = tm * tn * p.splits;
+  const int kt = (p.K + BK - 1) / BK;
+
+  // units of this workgroup: those of one XCD (blockIdx % 8) are consecutive, its workgroups
+  // take them in turn
+  int u, u_end, u_step;
+  {
+    const int G = gridDim.x, x = blockIdx.x % 8;
+    const int nx = (G - x + 7) / 8, before = (G / 8) * x + min(x, G % 8);
+    const int lo = (int)((int64_t)units * before / G);
+    u_end = (int)((int64_t)units * (before + nx) / G);
+    u = lo + blockIdx.x / 8;
+    u_step = nx;
+  }
+  if (u >= u_end) return;
+  // unit -> tile: groups of 8 tile rows, column by column
+  auto tile_of = [&](int v, int &m0, int &n0, int &part) __attribute__((always_inline)) {
+    part = v % p.splits;
+    const int t = v / p.splits, per = 8 * tn, g = t / per, gm = min(8, tm - g * 8), r = t - g * per;
+    m0 = (g * 8 + r % gm) * BM;
+    n0 = r / gm * BN;
+  };
+
+  Stage<TA, BM, NW, 0> a;
+  Stage<TW, BN, NW, PERM> w;
+  int is_u = u, is_left = 0;  // issue cursor: unit and its steps left
+  auto is_start = [&]() __attribute__((always_inline)) {
+    int m0, n0, part;
+    tile_of(is_u, m0, n0, part);
+    const int q0 = part * p.ksteps;
+    is_left = min(kt, q0 + p.ksteps) - q0;
+    a.start(p.A, p.lda, p.M, p.K, m0, q0 * BK, wave, lane);
+    w.start(p.W, p.ldw, p.N, p.K, n0, q0 * BK, wave, lane);
+  };
+  auto is_next = [&]() __attribute__((always_inline)) {
+    a.next();
+    w.next();
+    if (__builtin_expect(--is_left == 0, 0)) {
+      is_u += u_step;
+      if (is_u < u_end) is_start();
+      else is_left = 0x7fffffff;
+    }
+  };
+  is_start();
+  auto stage_all = [&](int slot) __attribute__((always_inline)) {
+    a.open(is_u < u_end);
+    w.open(is_u < u_end);
+#pragma unroll
+    for (int i = 0; i < a.D; ++i) a.issue(i, ldsA + slot * SA, wave, lane);
+#pragma unroll
+    for (int i = 0; i < w.D; ++i) w.issue(i, ldsW + slot * SW, wave, lane);
+    is_next();
+  };
+
+  // Lane (g, c) = (lane / 16, lane % 16) holds rows 4 g .. 4 g + 3 of each 16 and, with a permuted W, NJ
+  // consecutive columns from c NJ on: 16 lanes store one contiguous piece of a row. A T operand's columns
+  // are c + 16 j.
+  auto store = [&](const v4i (&acc)[NI][NJ], int v) __attribute__((always_inline)) {
+    int m0, n0, part;
+    tile_of(v, m0, n0, part);
+    const int c = lane & 15;
+    const int nb = n0 + wn * (BN / WN) + (PERM ? c * NJ : c);
+    const int mb = m0 + wm * (BM / WM) + (lane >> 4) * 4;
+    constexpr int NS = PERM ? 1 : 16;  // from one column to the next
+    const bool full = m0 + BM <= p.M && n0 + BN <= p.N;
+    if (p.splits > 1) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      int32_t *const o = p.parts + ((int64_t)part * p.M + mb) * p.N + nb;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          int32_t *const q = o + (int64_t)(i * 16 + r) * p.N;
+          if (full || mb + i * 16 + r < p.M) {
+            if (PERM && (full || nb + NJ <= p.N)) {
+              struct __attribute__((packed, aligned(4))) Any { int32_t w[NJ]; } t;
+#pragma unroll
+              for (int j = 0; j < NJ; ++j) t.w[j] = acc[i][j][r];
+              *(Any *)q = t;
+            } else {
+#pragma unroll
+              for (int j = 0; j < NJ; ++j)
+                if (full || nb + j * NS < p.N) q[j * NS] = acc[i][j][r];
+            }
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      return;
+    }
+    float sw[NJ], bs[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      const int n = min(nb + j * NS, p.N - 1);
+      sw[j] = p.sw ? p.sw[n] : 1.0f;
+      bs[j] = p.bias ? p.bias[n] : 0.0f;
+    }
+    float sa[NI][4];
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sa[i][r] = p.sa ? p.sa[min(mb + i * 16 + r, p.M - 1)] : 1.0f;
+    // This wave's loads have arrived, the DMA of the next step with them: its wait, which would also
+    // wait for the stores below, is left out (`ahead` in the main loop).
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    auto rows = [&](auto full_c) __attribute__((always_inline)) {
+      constexpr bool whole = decltype(full_c)::value;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if (whole || mb + i * 16 + r < p.M) {
+            const int64_t at = (int64_t)(mb + i * 16 + r) * p.N + nb;
+            float y[NJ];
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+              y[j] = ((float)acc[i][j][r] * sa[i][r]) * sw[j];
+              if (p.bias) y[j] += bs[j];
+            }
+            if (PERM && (whole || nb + NJ <= p.N)) {
+              if (p.R) {
+                float t[NJ];
+                loadv<OUT, NJ>(p.R, at, t);
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) y[j] += t[j];
+              }
+              storev<OUT, NJ>(p.Y, at, y);
+            } else {
+#pragma unroll
+              for (int j = 0; j < NJ; ++j)
+                if (whole || nb + j * NS < p.N) {
+                  if (p.R) y[j] += load_out<OUT>(p.R, at + j * NS);
+                  store_out<OUT>(p.Y, at + j * NS, y[j]);
+                }
+            }
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    if (full) rows(std::true_type());
+    else rows(std::false_type());
+  };
+
+  Reader<TA, BM, NI> ra;
+  Reader<TW, BN, NJ> rw;
+  ra.start(ldsA, wm * (BM / WM), lane);
+  rw.start(ldsW, wn * (BN / WN), lane);
+  // half b's products, spread between them the reads of the other half and, with DMA, the loads of a
+  // later step into slot dslot
+  auto half = [&](v4i (&acc)[NI][NJ], v4i (&fa)[2][NI], v4i (&fw)[2][NJ], auto b_c, auto dma_c, int dslot) __attribute__((always_inline)) {
+    constexpr int b = decltype(b_c)::value;
+    constexpr bool dma = decltype(dma_c)::value;
+    constexpr int DA = Stage<TA, BM, NW, 0>::D, DT = DA + Stage<TW, BN, NW, PERM>::D;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) fw[b ^ 1][j] = rw.read(j, b ^ 1);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      fa[b ^ 1][i] = ra.read(i, b ^ 1);
+      if constexpr (dma) {
+#pragma unroll
+        for (int d = i * DT / NI; d < (i + 1) * DT / NI; ++d) {
+          if (d < DA) a.issue(d, ldsA + dslot * SA, wave, lane);
+          else w.issue(d - DA, ldsW + dslot * SW, wave, lane);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fa[b][i], fw[b][j], acc[i][j], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+
+  stage_all(0);
+  stage_all(1);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  wg_barrier();
+  int slot = 0;
+  bool ahead = false;
+  for (; u < u_end; u += u_step) {
+    v4i acc[NI][NJ];
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) acc[i][j] = (v4i){0, 0, 0, 0};
+    v4i fa[2][NI], fw[2][NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) fw[0][j] = rw.read(j, 0);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) fa[0][i] = ra.read(i, 0);
+    const int q0 = (u % p.splits) * p.ksteps;
+    for (int left = min(kt, q0 + p.ksteps) - q0; left > 0; --left) {
+      half(acc, fa, fw, std::integral_constant<int, 0>(), std::false_type(), 0);
+      // the next step's data has arrived, and every wave holds this step's second half
+      if (ahead) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      ahead = false;
+      wg_barrier();
+      ra.shift(slot ? -SA : SA);
+      rw.shift(slot ? -SW : SW);
+      a.open(is_u < u_end);
+      w.open(is_u < u_end);
+      half(acc, fa, fw, std::integral_constant<int, 1>(), std::true_type(), slot);
+      is_next();
+      slot ^= 1;
+    }
+    store(acc, u);
+    ahead = true;
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no DMA into LDS outlives the workgroup
 }
 
 // Joins the parts of a split reduction. Their sum may pass 32 bits (K > 133144): 64-bit integers.
@@ -466,25 +724,70 @@ __global__ __launch_bounds__(256) void combine_kernel(const Prob p) {
   }
 }
 
-constexpr int TM = 128, TN = 128;
 // int32 sums of |a w| <= 127^2 hold 133144 terms
 constexpr int kMaxSteps = 1024;
 
-static void plan(int64_t M, int64_t N, int64_t K, int &splits, int &ksteps) {
-  const int64_t tiles = cdiv(M, TM) * cdiv(N, TN), kt = cdiv(K, BK);
-  int64_t s = 1;
-  if (tiles < 256) s = std::max<int64_t>(1, std::min<int64_t>(512 / tiles, kt / 4));
-  s = std::max(s, cdiv(kt, kMaxSteps));
-  ksteps = (int)cdiv(kt, s);
-  splits = (int)cdiv(kt, ksteps);
+// Tile, parts of the reduction, and steps of a part: the least time by a model of a launch (us): rounds of
+// units over the CUs, a step of 128 and a unit's start and end per tile form, and the combine's traffic.
+// The step times are those measured on 8192 x 8192 x 8192 (256 x 256 500 us, 256 x 192 557, 128 x 128 with
+// two workgroups per CU 719).
+struct Form {
+  int bm, bn, per_cu;
+  float step, unit;
+};
+constexpr Form kForms[3] = {{256, 256, 1, 1.9f, 7.0f}, {256, 192, 1, 1.55f, 6.0f}, {128, 128, 2, 1.4f, 5.0f}};
+
+struct Plan {
+  int form, splits, ksteps;
+};
+static Plan plan(int64_t M, int64_t N, int64_t K) {
+  const int64_t kt = cdiv(K, BK);
+  Plan best{0, 1, (int)kt};
+  float best_t = 1e30f;
+  for (int f = 0; f < 3; ++f) {
+    const Form &c = kForms[f];
+    const int64_t tiles = cdiv(M, c.bm) * cdiv(N, c.bn), slots = 256 * c.per_cu;
+    const int64_t s_min = cdiv(kt, kMaxSteps);
+    const int64_t s_max = std::max(s_min, std::min<int64_t>(cdiv(kt, 4), std::max<int64_t>(1, 2 * slots / tiles)));
+    for (int64_t s = s_min; s <= std::min<int64_t>(s_max, s_min + 64); ++s) {
+      const int64_t ks = cdiv(kt, s), sp = cdiv(kt, ks), units = tiles * sp, rounds = cdiv(units, slots);
+      // a CU that holds one workgroup of two runs it faster
+      const float step = c.per_cu == 2 && units <= 256 ? 0.7f * c.step : c.step;
+      float t = (float)rounds * ((float)ks * step + c.unit);
+      if (sp > 1) t += 4.0f + (float)(M * N) * 8.0f * (float)sp * 1.5e-7f;
+      if (t < best_t) best_t = t, best = Plan{f, (int)sp, (int)ks};
+    }
+  }
+  return best;
+}
+
+template <int BM, int BN, int WM, int WN, bool TA, bool TW, int OUT>
+static void launch_tile(const Prob &p, hipStream_t st) {
+  constexpr int lds = 2 * (BM + BN) * BK;
+  static const hipError_t set = hipFuncSetAttribute((const void *)gemm_kernel<BM, BN, WM, WN, TA, TW, OUT>,
+                                                    hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  (void)set;
+  const int64_t units = cdiv(p.M, BM) * cdiv(p.N, BN) * p.splits;
+  const int64_t cus = cu_count() * (lds <= 80 * 1024 ? 2 : 1);
+  gemm_kernel<BM, BN, WM, WN, TA, TW, OUT><<<(unsigned)std::min(units, cus), WM * WN * 64, lds, st>>>(p);
+}
+
+template <bool TA, bool TW, int OUT>
+static void launch_form(int form, const Prob &p, hipStream_t st) {
+  if (form == 0) launch_tile<256, 256, 2, 4, TA, TW, OUT>(p, st);
+  else if (form == 1) launch_tile<256, 192, 4, 2, TA, TW, OUT>(p, st);
+  else launch_tile<128, 128, 2, 2, TA, TW, OUT>(p, st);
 }
 
 template <int OUT>
-static void launch(const Prob &p, bool ta, bool tw, hipStream_t st) {
-  const unsigned g = (unsigned)(cdiv(p.M, TM) * cdiv(p.N, TN) * p.splits);
-  if (ta && tw) gemm_kernel<TM, TN, 2, 2, true, true, OUT><<<g, 256, 0, st>>>(p);
-  else if (tw) gemm_kernel<TM, TN, 2, 2, false, true, OUT><<<g, 256, 0, st>>>(p);
-  else gemm_kernel<TM, TN, 2, 2, false, false, OUT><<<g, 256, 0, st>>>(p);
+static void launch(int form, const Prob &p, bool ta, bool tw, hipStream_t st) {
+  if (ta) {  // a weight gradient
+    if constexpr (OUT == KSD_F32) launch_form<true, true, OUT>(form, p, st);
+  } else if (tw) {
+    launch_form<false, true, OUT>(form, p, st);
+  } else {
+    launch_form<false, false, OUT>(form, p, st);
+  }
   if (p.splits > 1) combine_kernel<OUT><<<(unsigned)std::min<int64_t>(cdiv((int64_t)p.M * p.N, 256), 8192), 256, 0, st>>>(p);
 }
 
@@ -515,8 +818,7 @@ extern "C" int ksd_tc_quantize_rows(const void *x, int x_dtype, int64_t M, int64
 
 extern "C" int ksd_tc_gemm_workspace(int64_t M, int64_t N, int64_t K, int64_t *bytes) {
   if (M < 0 || N < 0 || K < 1 || !bytes) return fail(KSD_EINVAL, "tc_gemm_workspace: bad arguments");
-  int splits = 1, ksteps = 0;
-  if (M > 0 && N > 0) tc::plan(M, N, K, splits, ksteps);
+  const int splits = M > 0 && N > 0 ? tc::plan(M, N, K).splits : 1;
   *bytes = splits > 1 ? (int64_t)splits * M * N * 4 : 0;
   return KSD_OK;
 }
@@ -528,7 +830,8 @@ extern "C" int ksd_tc_gemm(const int8_t *a, int64_t lda, int a_t, const float *s
     return fail(KSD_EINVAL, "tc_gemm: bad shape (%lld, %lld, %lld)", (long long)M, (long long)N, (long long)K);
   if (out_dtype != KSD_F32 && out_dtype != KSD_BF16 && out_dtype != KSD_F16)
     return fail(KSD_ETYPE, "tc_gemm: unsupported output type %d", out_dtype);
-  if (a_t && !w_t) return fail(KSD_EINVAL, "tc_gemm: a transposed A needs a transposed W");
+  if (a_t && (!w_t || out_dtype != KSD_F32))
+    return fail(KSD_EINVAL, "tc_gemm: a transposed A needs a transposed W and an fp32 output");
   const int64_t ra = a_t ? K : M, ca = a_t ? M : K, rw = w_t ? K : N, cw = w_t ? N : K;
   if (lda % 16 || ldw % 16 || lda < cdiv(ca, 16) * 16 || ldw < cdiv(cw, 16) * 16)
     return fail(KSD_EINVAL, "tc_gemm: row pitches must be multiples of 16 that cover the rows");
@@ -538,16 +841,17 @@ extern "C" int ksd_tc_gemm(const int8_t *a, int64_t lda, int a_t, const float *s
   if (!a || !w || !y) return fail(KSD_EINVAL, "tc_gemm: null pointer");
   if (((uintptr_t)a) % 16 || ((uintptr_t)w) % 16) return fail(KSD_EINVAL, "tc_gemm: codes must be 16-byte aligned");
   tc::Prob p{a, w, sa, sw, bias, residual, y, (int32_t *)workspace, lda, ldw, (int)M, (int)N, (int)K, 1, 0};
-  tc::plan(M, N, K, p.splits, p.ksteps);
+  const tc::Plan pl = tc::plan(M, N, K);
+  p.splits = pl.splits, p.ksteps = pl.ksteps;
   const int64_t need = p.splits > 1 ? (int64_t)p.splits * M * N * 4 : 0;
   if (need > 0 && (!workspace || workspace_bytes < need))
     return fail(KSD_EINVAL, "tc_gemm: workspace of %lld bytes needed", (long long)need);
-  if (!grid_fits(cdiv(M, tc::TM) * cdiv(N, tc::TN) * p.splits, 256)) return fail(KSD_EINVAL, "tc_gemm: shape too large");
+  if (!grid_fits(cdiv(M, 64) * cdiv(N, 64), 256)) return fail(KSD_EINVAL, "tc_gemm: shape too large");
   hipStream_t st = (hipStream_t)stream;
   switch (out_dtype) {
-    case KSD_F32: tc::launch<KSD_F32>(p, a_t, w_t, st); break;
-    case KSD_BF16: tc::launch<KSD_BF16>(p, a_t, w_t, st); break;
-    default: tc::launch<KSD_F16>(p, a_t, w_t, st);
+    case KSD_F32: tc::launch<KSD_F32>(pl.form, p, a_t, w_t, st); break;
+    case KSD_BF16: tc::launch<KSD_BF16>(pl.form, p, a_t, w_t, st); break;
+    default: tc::launch<KSD_F16>(pl.form, p, a_t, w_t, st);
   }
   return check_launch("tc_gemm");
 }
