@@ -756,6 +756,33 @@ int ksd_tc_quantize_grad(const void *g, int g_dtype, int64_t M, int64_t N, int64
                          void *stream);
 
 /*
+ * A layer's calls on those. The float operands have row strides in elements; out_dtype and residual
+ * as for ksd_tc_gemm.
+ * ksd_tc_linear: quantizes x (M, K) and multiplies with stored codes w (N, K) in rows of ldw bytes
+ * with scales sw; up to 32 tokens in one launch (ksd_tc_linear_workspace is then 0).
+ * ksd_tc_linear_train: quantizes x and the float master w into x_codes, w_codes (rows of K rounded up
+ * to 16 bytes) and their scales, then y; workspace as for ksd_tc_gemm of (M, N, K).
+ * ksd_tc_linear_backward: dx (M, K) of dx_dtype, dw (N, K) fp32 and db (N,) fp32 (each may be NULL)
+ * from g = dY and what ksd_tc_linear_train left.
+ */
+int ksd_tc_linear_workspace(int64_t M, int64_t N, int64_t K, int64_t *bytes);
+int ksd_tc_linear(const void *x, int x_dtype, int64_t M, int64_t K, int64_t stride, const int8_t *w,
+                  int64_t ldw, const float *sw, int64_t N, const float *bias, const void *residual,
+                  void *y, int out_dtype, void *workspace, int64_t workspace_bytes, void *stream);
+int ksd_tc_linear_train(const void *x, int x_dtype, int64_t M, int64_t K, int64_t stride,
+                        const void *w, int w_dtype, int64_t N, int64_t w_stride, const float *bias,
+                        const void *residual, int8_t *x_codes, float *x_scales, int8_t *w_codes,
+                        float *w_scales, void *y, int out_dtype, void *workspace,
+                        int64_t workspace_bytes, void *stream);
+int ksd_tc_linear_backward_workspace(int64_t M, int64_t N, int64_t K, int need_dx, int need_dw,
+                                     int64_t *bytes);
+int ksd_tc_linear_backward(const void *g, int g_dtype, int64_t M, int64_t N, int64_t stride,
+                           int64_t K, const int8_t *x_codes, const float *x_scales,
+                           const int8_t *w_codes, const float *w_scales, void *dx, int dx_dtype,
+                           float *dw, float *db, void *workspace, int64_t workspace_bytes,
+                           void *stream);
+
+/*
  * Embedding lookup with a scale: out[i] = round(scale * table[ids[i]]), a row of zeros for an id
  * out of range. table (V, d) of row stride `stride` elements; ids int64 (ids_wide) or int32; out
  * (n, d) dense. Float types KSD_F32, KSD_BF16, KSD_F16 on both sides.

@@ -92,6 +92,12 @@ SIGNATURES = {
     "ksd_tc_gemm": [_P, _I64, _INT, _P, _P, _I64, _INT, _P, _I64, _I64, _I64, _P, _P, _P, _INT, _P, _I64, _P],
     "ksd_tc_grad_workspace": [_I64, _I64, _P],
     "ksd_tc_quantize_grad": [_P, _INT, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P, _I64, _P, _P, _I64, _P],
+    "ksd_tc_linear_workspace": [_I64, _I64, _I64, _P],
+    "ksd_tc_linear": [_P, _INT, _I64, _I64, _I64, _P, _I64, _P, _I64, _P, _P, _P, _INT, _P, _I64, _P],
+    "ksd_tc_linear_train": [_P, _INT, _I64, _I64, _I64, _P, _INT, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _INT, _P,
+                            _I64, _P],
+    "ksd_tc_linear_backward_workspace": [_I64, _I64, _I64, _INT, _INT, _P],
+    "ksd_tc_linear_backward": [_P, _INT, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _P, _INT, _P, _P, _P, _I64, _P],
     "ksd_embedding_lookup": [_P, _INT, _I64, _I64, _I64, _P, _INT, _I64, _F, _P, _INT, _P],
     "ksd_embedding_gradient_workspace": [_I64, _I64, _P],
     "ksd_embedding_gradient": [_P, _INT, _I64, _I64, _I64, _P, _INT, _I64, _I64, _F, _INT, _P, _INT, _P, _I64, _P],

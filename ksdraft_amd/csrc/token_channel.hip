@@ -81,17 +81,22 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
 }
 
 // ------------------------------------------------------------------------------------ rows
+struct Rows {
+  const void *x;
+  int64_t M, K, stride, ld;
+  int8_t *codes;
+  float *scales;
+};
+
 // LANES threads per row (64: four rows per workgroup; 256: one), the first NCH * LANES * 8 elements
 // kept in registers between the maximum and the codes, the rest read again (from cache).
 template <int DT, int LANES, int NCH>
-__global__ __launch_bounds__(256) void quant_rows_kernel(const void *__restrict__ x, int64_t M, int64_t K,
-                                                         int64_t stride, int8_t *__restrict__ codes, int64_t ld,
-                                                         float *__restrict__ scales) {
+__device__ __forceinline__ void quant_rows(const Rows &p, int64_t block) {
   using T = typename Elem<DT>::T;
   const int lane = threadIdx.x % LANES;
-  const int64_t m = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
-  if (LANES == 64 && m >= M) return;
-  const T *row = (const T *)x + m * stride;
+  const int64_t m = block * (256 / LANES) + threadIdx.x / LANES, K = p.K, ld = p.ld;
+  if (LANES == 64 && m >= p.M) return;
+  const T *row = (const T *)p.x + m * p.stride;
   float v[NCH][8];
   uint32_t top = 0;
 #pragma unroll
@@ -121,8 +126,8 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const void *__restrict_
   float scale, inv;
   row_scale(top, scale, inv);
   const bool bad = top >= 0x7f800000u;
-  if (lane == 0) scales[m] = scale;
-  int8_t *out = codes + m * ld;
+  if (lane == 0) p.scales[m] = scale;
+  int8_t *out = p.codes + m * ld;
   auto put = [&](int64_t k, const float *t) {
     uint2 w;
     w.x = bad ? 0 : pack4(t[0] * inv, t[1] * inv, t[2] * inv, t[3] * inv);
@@ -141,153 +146,209 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const void *__restrict_
   }
 }
 
-template <int DT>
-static void launch_rows(const void *x, int64_t M, int64_t K, int64_t stride, int8_t *codes, int64_t ld,
-                        float *scales, hipStream_t st) {
-  if (K <= 512) quant_rows_kernel<DT, 64, 1><<<(unsigned)cdiv(M, 4), 256, 0, st>>>(x, M, K, stride, codes, ld, scales);
-  else if (K <= 1536) quant_rows_kernel<DT, 64, 3><<<(unsigned)cdiv(M, 4), 256, 0, st>>>(x, M, K, stride, codes, ld, scales);
-  else quant_rows_kernel<DT, 256, 4><<<(unsigned)M, 256, 0, st>>>(x, M, K, stride, codes, ld, scales);
+// Workgroups below `blocks0` take the first matrix, the others the second (of type DT1; a layer's weights
+// and its tokens have one row length, so one launch covers both).
+template <int DT0, int DT1, int LANES, int NCH>
+__global__ __launch_bounds__(256) void quant_rows_kernel(const Rows a, const Rows b, unsigned blocks0) {
+  if (blockIdx.x < blocks0) quant_rows<DT0, LANES, NCH>(a, blockIdx.x);
+  else quant_rows<DT1, LANES, NCH>(b, blockIdx.x - blocks0);
+}
+
+template <int DT0, int DT1>
+static void launch_rows(const Rows &a, const Rows &b, hipStream_t st) {
+  const int64_t per = a.K <= 1536 ? 4 : 1, n0 = cdiv(a.M, per), n = n0 + cdiv(b.M, per);
+  if (a.K <= 512) quant_rows_kernel<DT0, DT1, 64, 1><<<(unsigned)n, 256, 0, st>>>(a, b, (unsigned)n0);
+  else if (a.K <= 1536) quant_rows_kernel<DT0, DT1, 64, 3><<<(unsigned)n, 256, 0, st>>>(a, b, (unsigned)n0);
+  else quant_rows_kernel<DT0, DT1, 256, 4><<<(unsigned)n, 256, 0, st>>>(a, b, (unsigned)n0);
+}
+static void launch_rows(const Rows &a, int t, hipStream_t st) {
+  const Rows none{nullptr, 0, a.K, 0, 0, nullptr, nullptr};
+  if (t == KSD_F32) launch_rows<KSD_F32, KSD_F32>(a, none, st);
+  else if (t == KSD_BF16) launch_rows<KSD_BF16, KSD_BF16>(a, none, st);
+  else launch_rows<KSD_F16, KSD_F16>(a, none, st);
 }
 
 // ------------------------------------------------------------------------------- gradient's codes
-// Workgroup (row block, column block) of 64 x 1024 elements of dY: thread t holds columns 4t .. 4t+3
-// over all rows (column maxima of |dY * sx| and column sums), each row's maximum of |dY * sw| goes
-// through the workgroup. Partial results per block, folded by grad_fold_kernel in a fixed order.
-constexpr int GR = 64, GC = 1024;
+// Two reads of dY, bound by memory: the first leaves per row block the column maxima of |dY * sx| and
+// the column sums, per column block the row maxima of |dY * sw|; a fold in a fixed order makes scales of
+// them; the second writes both codes. (8192 x 1536 bf16: MEASURED_STATS us, MEASURED_FOLD us and MEASURED_CODES us.)
+// A wave takes `rows` (a multiple of 16) x 64 V columns: lane l holds columns V l .. V l + V - 1, 16 rows'
+// loads in flight. A row's maximum crosses the lanes through LDS, 16 rows at once.
+template <int DT> constexpr int kVec = DT == KSD_F32 ? 4 : 8;  // 16 bytes
 
 template <int DT>
-__device__ __forceinline__ void load4_tail(const typename Elem<DT>::T *row, int64_t c, int64_t N, float *v) {
-  using T = typename Elem<DT>::T;
-  if (c + 4 <= N) {
-    if constexpr (DT == KSD_F32) {
-      struct __attribute__((packed, aligned(4))) Any { uint4 q; };
-      const uint4 q = ((const Any *)(row + c))->q;
-      v[0] = __builtin_bit_cast(float, q.x), v[1] = __builtin_bit_cast(float, q.y);
-      v[2] = __builtin_bit_cast(float, q.z), v[3] = __builtin_bit_cast(float, q.w);
-    } else {
-      struct __attribute__((packed, aligned(2))) Any { uint2 q; };
-      const uint2 q = ((const Any *)(row + c))->q;
-      const T h[4] = {(T)(q.x & 0xffff), (T)(q.x >> 16), (T)(q.y & 0xffff), (T)(q.y >> 16)};
+__device__ __forceinline__ void load16(const typename Elem<DT>::T *p, float *v) {
+  if constexpr (DT == KSD_F32) {
+    struct __attribute__((packed, aligned(4))) Any { float w[4]; };
+    const Any q = *(const Any *)p;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = Elem<DT>::load(&h[j]);
-    }
+    for (int j = 0; j < 4; ++j) v[j] = q.w[j];
   } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = c + j < N ? Elem<DT>::load(row + c + j) : 0.0f;
+    load8<DT>(p, v);
   }
 }
 
 template <int DT>
-__global__ __launch_bounds__(256) void grad_stats_kernel(const void *__restrict__ g, int64_t M, int64_t N, int64_t stride,
+__global__ __launch_bounds__(256) void grad_stats_kernel(const void *__restrict__ g, int64_t M, int64_t N, int64_t stride, int rows,
                                                          const float *__restrict__ sx, const float *__restrict__ sw,
                                                          uint32_t *__restrict__ row_part, uint32_t *__restrict__ col_part,
                                                          float *__restrict__ sum_part) {
   using T = typename Elem<DT>::T;
-  __shared__ uint32_t rmax[GR][4];
-  const int tid = threadIdx.x;
-  const int64_t cb = blockIdx.x, rb = blockIdx.y, c = cb * GC + tid * 4, m0 = rb * GR;
-  float w[4], sum[4] = {0, 0, 0, 0};
-  uint32_t cm[4] = {0, 0, 0, 0};
+  constexpr int V = kVec<DT>;
+  __shared__ uint32_t rmax_all[4][16][65];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  uint32_t(*const rmax)[65] = rmax_all[wave];
+  const int64_t cb = (int64_t)blockIdx.x * 4 + wave, rb = blockIdx.y, c = (cb * 64 + lane) * V;
+  const int64_t m0 = rb * rows, m1 = min(M, m0 + rows);
+  if (cb * 64 * V >= N) return;
+  const bool cols = (cb + 1) * 64 * V <= N;
+  float w[V], sum[V];
+  uint32_t cm[V];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) w[j] = c + j < N ? sw[c + j] : 0.0f;
-  const int rows = (int)min((int64_t)GR, M - m0);
-#pragma unroll 4
-  for (int r = 0; r < rows; ++r) {
-    float v[4] = {0, 0, 0, 0};
-    if (c < N) load4_tail<DT>((const T *)g + (m0 + r) * stride, c, N, v);
-    const float s = sx[m0 + r];
-    float t[4];
+  for (int j = 0; j < V; ++j) {
+    w[j] = c + j < N ? sw[c + j] : 0.0f;
+    sum[j] = 0.0f;
+    cm[j] = 0;
+  }
+  for (int64_t mb = m0; mb < m1; mb += 16) {
+    float v[16][V], s[16];
+    if (cols && mb + 16 <= m1) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      t[j] = c + j < N ? v[j] * w[j] : 0.0f;
-      sum[j] += v[j];
-      cm[j] = max(cm[j], __builtin_bit_cast(uint32_t, fabsf(v[j] * s)));
+      for (int r = 0; r < 16; ++r) load16<DT>((const T *)g + (mb + r) * stride + c, v[r]);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = sx[mb + r];
+    } else {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[r] = mb + r < m1 ? sx[mb + r] : 0.0f;
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          v[r][j] = c + j < N && mb + r < m1 ? Elem<DT>::load((const T *)g + (mb + r) * stride + c + j) : 0.0f;
+      }
     }
-    const uint32_t top = wave_max(__builtin_bit_cast(uint32_t, abs_max<4>(t)));
-    if ((tid & 63) == 0) rmax[r][tid >> 6] = top;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      float t[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        t[j] = v[r][j] * w[j];
+        sum[j] += v[r][j];
+        cm[j] = max(cm[j], __builtin_bit_cast(uint32_t, fabsf(v[r][j] * s[r])));
+      }
+      rmax[r][lane] = __builtin_bit_cast(uint32_t, abs_max<V>(t));
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    uint32_t top = 0;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) top = max(top, rmax[lane >> 2][(lane & 3) * 16 + k]);
+    top = group_max_u32<4>(top);
+    if ((lane & 3) == 0 && mb + (lane >> 2) < m1) row_part[cb * M + mb + (lane >> 2)] = top;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
+  for (int j = 0; j < V; ++j)
     if (c + j < N) {
       col_part[rb * N + c + j] = cm[j];
       if (sum_part) sum_part[rb * N + c + j] = sum[j];
     }
-  __syncthreads();
-  if (tid < rows)
-    row_part[cb * M + m0 + tid] = max(max(rmax[tid][0], rmax[tid][1]), max(rmax[tid][2], rmax[tid][3]));
 }
 
-// scales, reciprocals and column sums from the partial results; thread i < M is row i, the next N
-// threads are the columns
-__global__ __launch_bounds__(256) void grad_fold_kernel(const uint32_t *__restrict__ row_part, const uint32_t *__restrict__ col_part,
-                                                        const float *__restrict__ sum_part, int64_t M, int64_t N, int ncb, int nrb,
-                                                        float *__restrict__ e, float *__restrict__ einv, float *__restrict__ f,
-                                                        float *__restrict__ finv, float *__restrict__ db) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i < M) {
-    uint32_t top = 0;
-    for (int b = 0; b < ncb; ++b) top = max(top, row_part[(int64_t)b * M + i]);
-    float s, inv;
-    row_scale(top, s, inv);
-    e[i] = s, einv[i] = inv;
-  } else if (i < M + N) {
-    const int64_t n = i - M;
-    uint32_t top = 0;
-    float sum = 0.0f;
-    for (int b = 0; b < nrb; ++b) {
-      top = max(top, col_part[(int64_t)b * N + n]);
-      if (sum_part) sum += sum_part[(int64_t)b * N + n];
+// Scales, reciprocals and column sums from the partial results: workgroup b < ceil(M / 64) folds 64 rows, the
+// others 64 columns each; wave w takes every 16th part, the waves' results meet in wave order.
+__global__ __launch_bounds__(1024) void grad_fold_kernel(const uint32_t *__restrict__ row_part, const uint32_t *__restrict__ col_part,
+                                                         const float *__restrict__ sum_part, int64_t M, int64_t N, int ncb, int nrb,
+                                                         float *__restrict__ e, float *__restrict__ einv, float *__restrict__ f,
+                                                         float *__restrict__ finv, float *__restrict__ db) {
+  __shared__ uint32_t tops[16][64];
+  __shared__ float sums[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t rblocks = (M + 63) / 64;
+  const bool is_row = blockIdx.x < rblocks;
+  const int64_t i = (is_row ? (int64_t)blockIdx.x : (int64_t)blockIdx.x - rblocks) * 64 + lane, L = is_row ? M : N;
+  const uint32_t *part = is_row ? row_part : col_part;
+  const int n = is_row ? ncb : nrb;
+  const bool add = !is_row && db;
+  uint32_t top = 0;
+  float sum = 0.0f;
+  if (i < L) {
+#pragma unroll 4
+    for (int b = wave; b < n; b += 16) {
+      top = max(top, part[(int64_t)b * L + i]);
+      if (add) sum += sum_part[(int64_t)b * L + i];
+    }
+  }
+  tops[wave][lane] = top;
+  sums[wave][lane] = sum;
+  __syncthreads();
+  if (wave == 0 && i < L) {
+    for (int k = 1; k < 16; ++k) {
+      top = max(top, tops[k][lane]);
+      sum += sums[k][lane];
     }
     float s, inv;
     row_scale(top, s, inv);
-    f[n] = s, finv[n] = inv;
-    if (db) db[n] = sum;
+    (is_row ? e : f)[i] = s;
+    (is_row ? einv : finv)[i] = inv;
+    if (add) db[i] = sum;
   }
 }
 
-// Both codes of dY, in its own layout: q (rows, for dX) and c (columns, for dW), rows of ld bytes
-// with zeros past N. A thread holds 8 columns over 8 rows.
+// Both codes of dY, in its own layout: q (rows, for dX) and c (columns, for dW), rows of ld bytes with zeros
+// past N. A thread holds 8 columns over 16 rows, 8 of them in flight. A row or column whose scale is NaN
+// has codes of no meaning: its products are NaN through the scale.
 template <int DT>
 __global__ __launch_bounds__(256) void grad_codes_kernel(const void *__restrict__ g, int64_t M, int64_t N, int64_t stride,
                                                          const float *__restrict__ sx, const float *__restrict__ sw,
                                                          const float *__restrict__ einv, const float *__restrict__ finv,
-                                                         const float *__restrict__ e, const float *__restrict__ f,
                                                          int8_t *__restrict__ q, int8_t *__restrict__ cq, int64_t ld) {
   using T = typename Elem<DT>::T;
   const int64_t c = ((int64_t)blockIdx.x * 64 + (threadIdx.x & 63)) * 8;
-  const int64_t m0 = (int64_t)blockIdx.y * 32 + (threadIdx.x >> 6) * 8;
+  const int64_t m0 = (int64_t)blockIdx.y * 64 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 16;
   if (c >= ld) return;
+  const bool cols = (int64_t)(blockIdx.x + 1) * 512 <= N;
   float w[8], fi[8];
-  bool cbad[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     w[j] = c + j < N ? sw[c + j] : 0.0f;
     fi[j] = c + j < N ? finv[c + j] : 0.0f;
-    cbad[j] = c + j < N && f[c + j] != f[c + j];
   }
 #pragma unroll
-  for (int r = 0; r < 8; ++r) {
-    const int64_t m = m0 + r;
-    if (m >= M) break;
-    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (c < N) load8_tail<DT>((const T *)g + m * stride, c, N, v);
-    if (q) {
-      const float inv = einv[m];
-      const bool bad = e[m] != e[m];
-      float t[8];
+  for (int h = 0; h < 2; ++h) {
+    float v[8][8];
+    if (cols && m0 + h * 8 + 8 <= M) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) t[j] = bad || c + j >= N ? 0.0f : (v[j] * w[j]) * inv;
-      *(uint2 *)(q + m * ld + c) = make_uint2(pack4(t[0], t[1], t[2], t[3]), pack4(t[4], t[5], t[6], t[7]));
+      for (int r = 0; r < 8; ++r) load8<DT>((const T *)g + (m0 + h * 8 + r) * stride + c, v[r]);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          v[r][j] = m0 + h * 8 + r < M && c + j < N ? Elem<DT>::load((const T *)g + (m0 + h * 8 + r) * stride + c + j) : 0.0f;
     }
-    if (cq) {
-      const float s = sx[m];
-      float t[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) t[j] = cbad[j] || c + j >= N ? 0.0f : (v[j] * s) * fi[j];
-      *(uint2 *)(cq + m * ld + c) = make_uint2(pack4(t[0], t[1], t[2], t[3]), pack4(t[4], t[5], t[6], t[7]));
+    for (int r = 0; r < 8; ++r) {
+      const int64_t m = m0 + h * 8 + r;
+      if (m >= M) break;
+      if (q) {
+        const float inv = einv[m];
+        float t[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) t[j] = (v[r][j] * w[j]) * inv;
+        *(uint2 *)(q + m * ld + c) = make_uint2(pack4(t[0], t[1], t[2], t[3]), pack4(t[4], t[5], t[6], t[7]));
+      }
+      if (cq) {
+        const float s = sx[m];
+        float t[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) t[j] = (v[r][j] * s) * fi[j];
+        *(uint2 *)(cq + m * ld + c) = make_uint2(pack4(t[0], t[1], t[2], t[3]), pack4(t[4], t[5], t[6], t[7]));
+      }
     }
   }
 }
+
+// Rows of a stats workgroup: 32, 64 where that still leaves every CU several (the parts halve).
+static int stats_rows(int64_t M, int64_t N) { return M * N >= (int64_t)1 << 25 ? 64 : 32; }
 
 // ------------------------------------------------------------------------------------ product
 // One operand of the product. Plain ("N"): (rows, K) with the reduction contiguous; "T": (K, rows)
@@ -708,20 +769,42 @@ __global__ __launch_bounds__(WM *WN * 64, WM * WN == 8 ? 1 : 2) void gemm_kernel
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no DMA into LDS outlives the workgroup
 }
 
-// Joins the parts of a split reduction. Their sum may pass 32 bits (K > 133144): 64-bit integers.
-template <int OUT>
+// Joins the parts of a split reduction, V columns per thread. Their sum may pass 32 bits (K > 133144):
+// 64-bit integers.
+template <int OUT, int V>
 __global__ __launch_bounds__(256) void combine_kernel(const Prob p) {
-  const int64_t total = (int64_t)p.M * p.N;
-  for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < total; at += (int64_t)gridDim.x * 256) {
-    int64_t s = 0;
-    for (int k = 0; k < p.splits; ++k) s += p.parts[k * total + at];
-    const int64_t m = at / p.N, n = at - m * p.N;
-    float y = (float)s * (p.sa ? p.sa[m] : 1.0f);
-    if (p.sw) y = y * p.sw[n];
-    if (p.bias) y = y + p.bias[n];
-    if (p.R) y = y + load_out<OUT>(p.R, at);
-    store_out<OUT>(p.Y, at, y);
+  const int per = p.N / V;
+  const int64_t total = (int64_t)p.M * p.N, n = (int64_t)p.M * per;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t m = i / per;
+    const int c = (int)(i - m * per) * V;
+    const int64_t at = m * p.N + c;
+    typedef int vec __attribute__((ext_vector_type(V)));
+    int64_t s[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) s[j] = 0;
+#pragma unroll 4
+    for (int k = 0; k < p.splits; ++k) {
+      const vec q = *(const vec *)(p.parts + k * total + at);
+#pragma unroll
+      for (int j = 0; j < V; ++j) s[j] += q[j];
+    }
+    const float sa = p.sa ? p.sa[m] : 1.0f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      float y = (float)s[j] * sa;
+      if (p.sw) y = y * p.sw[c + j];
+      if (p.bias) y = y + p.bias[c + j];
+      if (p.R) y = y + load_out<OUT>(p.R, at + j);
+      store_out<OUT>(p.Y, at + j, y);
+    }
   }
+}
+template <int OUT>
+static void launch_combine(const Prob &p, hipStream_t st) {
+  const unsigned g = (unsigned)std::min<int64_t>(cdiv((int64_t)p.M * p.N, p.N % 4 == 0 ? 1024 : 256), 16384);
+  if (p.N % 4 == 0) combine_kernel<OUT, 4><<<g, 256, 0, st>>>(p);
+  else combine_kernel<OUT, 1><<<g, 256, 0, st>>>(p);
 }
 
 // int32 sums of |a w| <= 127^2 hold 133144 terms
@@ -788,31 +871,198 @@ static void launch(int form, const Prob &p, bool ta, bool tw, hipStream_t st) {
   } else {
     launch_form<false, false, OUT>(form, p, st);
   }
-  if (p.splits > 1) combine_kernel<OUT><<<(unsigned)std::min<int64_t>(cdiv((int64_t)p.M * p.N, 256), 8192), 256, 0, st>>>(p);
+  if (p.splits > 1) launch_combine<OUT>(p, st);
 }
+
+
+// -------------------------------------------------------------------------------------- few rows
+// y for few tokens in one launch: what bounds it is one read of the codes of W (or the launch itself).
+// Every workgroup quantizes the M tokens into LDS (their first W chunks are already on the way) and walks
+// tiles of 16 columns; its 4 waves take every fourth 64 steps of the reduction, W straight into MFMA registers
+// (each byte is used once), and meet in LDS. Measured: MEASURED_FEW.
+struct Few {
+  const void *x;
+  const int8_t *W;
+  const float *sw, *bias;
+  const void *R;
+  void *Y;
+  int64_t stride, ldw;
+  int M, N, K, pitch;  // pitch: bytes of an LDS row of codes, = 16 mod 256 (16 rows on 16 bank groups)
+};
+
+template <int DT, int OUT, int MT>
+__global__ __launch_bounds__(256) void few_rows_kernel(const Few p) {
+  using T = typename Elem<DT>::T;
+  constexpr int U = 6;  // W chunks in flight per wave
+  extern __shared__ __attribute__((aligned(16))) int8_t smem[];  // codes, then 2 x 4 x MT x 256 int32 and M scales
+  int32_t *const part = (int32_t *)(smem + (int64_t)p.M * p.pitch);
+  float *const sx = (float *)(part + 2 * 4 * MT * 256);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c16 = lane & 15, g = lane >> 4;
+  const int nk = (p.K + 63) / 64, kb = (p.K + 15) & ~15, tiles = (p.N + 15) / 16;
+  v4i w[U];
+  auto load = [&](int t, int k0) __attribute__((always_inline)) {
+    const int8_t *row = p.W + (int64_t)min(t * 16 + c16, p.N - 1) * p.ldw;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int k = (k0 + i * 4) * 64 + g * 16;
+      w[i] = *(const v4i *)(row + (k < kb ? k : 0));  // steps past K meet zero codes of x
+    }
+  };
+  int t = blockIdx.x;
+  load(t, wave);
+  for (int m = wave; m < p.M; m += 4) {
+    const T *row = (const T *)p.x + m * p.stride;
+    constexpr int NC = 4;
+    float v[NC][8];
+    uint32_t top = 0;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int k = (c * 64 + lane) * 8;
+      if (k < p.K) {
+        load8_tail<DT>(row, k, p.K, v[c]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[c][j] = 0.0f;
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c) top = max(top, __builtin_bit_cast(uint32_t, abs_max<8>(v[c])));
+    for (int k = (NC * 64 + lane) * 8; k < p.K; k += 512) {
+      float q[8];
+      load8_tail<DT>(row, k, p.K, q);
+      top = max(top, __builtin_bit_cast(uint32_t, abs_max<8>(q)));
+    }
+    top = wave_max(top);
+    float scale, inv;
+    row_scale(top, scale, inv);
+    const bool bad = top >= 0x7f800000u;
+    if (lane == 0) sx[m] = scale;
+    int8_t *out = smem + m * p.pitch;
+    auto put = [&](int k, const float *q) __attribute__((always_inline)) {
+      const uint2 o = make_uint2(bad ? 0 : pack4(q[0] * inv, q[1] * inv, q[2] * inv, q[3] * inv),
+                                 bad ? 0 : pack4(q[4] * inv, q[5] * inv, q[6] * inv, q[7] * inv));
+      *(uint2 *)(out + k) = o;
+    };
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int k = (c * 64 + lane) * 8;
+      if (k < nk * 64) put(k, v[c]);
+    }
+    for (int k = (NC * 64 + lane) * 8; k < nk * 64; k += 512) {
+      float q[8];
+      if (k < p.K) {
+        load8_tail<DT>(row, k, p.K, q);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) q[j] = 0.0f;
+      }
+      put(k, q);
+    }
+  }
+  __syncthreads();
+  const int8_t *arow[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) arow[i] = smem + (int64_t)min(i * 16 + c16, p.M - 1) * p.pitch + g * 16;
+  int par = 0;
+  for (; t < tiles; t += gridDim.x, par ^= 1) {
+    v4i acc[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) acc[i] = (v4i){0, 0, 0, 0};
+    for (int k0 = wave; k0 < nk; k0 += 4 * U) {
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        const int k = k0 + i * 4;
+        if (k < nk) {
+#pragma unroll
+          for (int r = 0; r < MT; ++r)
+            acc[r] = __builtin_amdgcn_mfma_i32_16x16x64_i8(*(const v4i *)(arow[r] + k * 64), w[i], acc[r], 0, 0, 0);
+        }
+      }
+      if (k0 + 4 * U < nk) load(t, k0 + 4 * U);
+      else if (t + (int)gridDim.x < tiles) load(t + gridDim.x, wave);
+    }
+    if (wave >= nk && t + (int)gridDim.x < tiles) load(t + gridDim.x, wave);
+    int32_t *const q = part + (par * 4 + wave) * MT * 256;
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) q[i * 256 + (g * 4 + r) * 16 + c16] = acc[i][r];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      const int m = i * 16 + (tid >> 4), n = t * 16 + (tid & 15);
+      if (m < p.M && n < p.N) {
+        const int32_t *z = part + par * 4 * MT * 256 + i * 256 + tid;
+        const int32_t sum = z[0] + z[MT * 256] + z[2 * MT * 256] + z[3 * MT * 256];
+        float y = ((float)sum * sx[m]) * p.sw[n];
+        const int64_t at = (int64_t)m * p.N + n;
+        if (p.bias) y += p.bias[n];
+        if (p.R) y += load_out<OUT>(p.R, at);
+        store_out<OUT>(p.Y, at, y);
+      }
+    }
+  }
+}
+
+static int few_lds(int64_t M, int64_t K) {
+  const int64_t pitch = cdiv(K, 256) * 256 + 16, mt = cdiv(M, 16);
+  const int64_t b = M * pitch + 2 * 4 * mt * 1024 + 4 * M;
+  return b <= 160 * 1024 ? (int)b : 0;
+}
+// Up to 32 tokens whose codes leave room for two workgroups on a CU. K: int32 sums.
+static bool few_rows(int64_t M, int64_t K) {
+  return M <= 32 && K <= 65536 && few_lds(M, K) > 0 && few_lds(M, K) <= 80 * 1024;
+}
+
+template <int DT, int OUT>
+static void launch_few(const Few &p, hipStream_t st) {
+  const int lds = few_lds(p.M, p.K), mt = (p.M + 15) / 16;
+  const int per_cu = std::min(8, 160 * 1024 / lds);
+  const unsigned grid = (unsigned)std::min<int64_t>(cdiv(p.N, 16), (int64_t)cu_count() * per_cu);
+  if (mt == 1) {
+    static const hipError_t set = hipFuncSetAttribute((const void *)few_rows_kernel<DT, OUT, 1>, hipFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024);
+    (void)set;
+    few_rows_kernel<DT, OUT, 1><<<grid, 256, lds, st>>>(p);
+  } else {
+    static const hipError_t set = hipFuncSetAttribute((const void *)few_rows_kernel<DT, OUT, 2>, hipFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024);
+    (void)set;
+    few_rows_kernel<DT, OUT, 2><<<grid, 256, lds, st>>>(p);
+  }
+}
+template <int DT>
+static void launch_few(int out, const Few &p, hipStream_t st) {
+  if (out == KSD_F32) launch_few<DT, KSD_F32>(p, st);
+  else if (out == KSD_BF16) launch_few<DT, KSD_BF16>(p, st);
+  else launch_few<DT, KSD_F16>(p, st);
+}
+
+static bool float_type(int t) { return t == KSD_F32 || t == KSD_BF16 || t == KSD_F16; }
+static int64_t pad256(int64_t b) { return (b + 255) / 256 * 256; }
+static int64_t pitch16(int64_t n) { return (n + 15) / 16 * 16; }
 
 }  // namespace tc
 }  // namespace ksd
 
 using namespace ksd;
 
+// Checks what every entry asks of a float matrix and its codes.
+static int check_rows(const char *who, const void *x, int t, int64_t M, int64_t K, const int8_t *codes, int64_t ld, const float *scales) {
+  if (M < 0 || K < 1) return fail(KSD_EINVAL, "%s: bad shape (%lld, %lld)", who, (long long)M, (long long)K);
+  if (!tc::float_type(t)) return fail(KSD_ETYPE, "%s: unsupported element type %d", who, t);
+  if (ld != tc::pitch16(K)) return fail(KSD_EINVAL, "%s: pitch %lld must be K rounded up to 16", who, (long long)ld);
+  if (M == 0) return KSD_OK;
+  if (!x || !codes || !scales) return fail(KSD_EINVAL, "%s: null pointer", who);
+  if (((uintptr_t)codes) % 16) return fail(KSD_EINVAL, "%s: codes must be 16-byte aligned", who);
+  if (!grid_fits(M, 256)) return fail(KSD_EINVAL, "%s: too many rows", who);
+  return KSD_OK;
+}
+
 extern "C" int ksd_tc_quantize_rows(const void *x, int x_dtype, int64_t M, int64_t K, int64_t stride, int8_t *codes,
                                     int64_t ld, float *scales, void *stream) {
-  if (M < 0 || K < 1) return fail(KSD_EINVAL, "tc_quantize_rows: bad shape (%lld, %lld)", (long long)M, (long long)K);
-  if (x_dtype != KSD_F32 && x_dtype != KSD_BF16 && x_dtype != KSD_F16)
-    return fail(KSD_ETYPE, "tc_quantize_rows: unsupported element type %d", x_dtype);
-  if (ld < K || ld % 16 != 0 || ld >= K + 16)
-    return fail(KSD_EINVAL, "tc_quantize_rows: pitch %lld must be K rounded up to 16", (long long)ld);
-  if (M == 0) return KSD_OK;
-  if (!x || !codes || !scales) return fail(KSD_EINVAL, "tc_quantize_rows: null pointer");
-  if (((uintptr_t)codes) % 16) return fail(KSD_EINVAL, "tc_quantize_rows: codes must be 16-byte aligned");
-  if (!grid_fits(M, 256)) return fail(KSD_EINVAL, "tc_quantize_rows: too many rows");
-  hipStream_t st = (hipStream_t)stream;
-  switch (x_dtype) {
-    case KSD_F32: tc::launch_rows<KSD_F32>(x, M, K, stride, codes, ld, scales, st); break;
-    case KSD_BF16: tc::launch_rows<KSD_BF16>(x, M, K, stride, codes, ld, scales, st); break;
-    default: tc::launch_rows<KSD_F16>(x, M, K, stride, codes, ld, scales, st);
-  }
+  const int rc = check_rows("tc_quantize_rows", x, x_dtype, M, K, codes, ld, scales);
+  if (rc || M == 0) return rc;
+  tc::launch_rows(tc::Rows{x, M, K, stride, ld, codes, scales}, x_dtype, (hipStream_t)stream);
   return check_launch("tc_quantize_rows");
 }
 
@@ -858,7 +1108,7 @@ extern "C" int ksd_tc_gemm(const int8_t *a, int64_t lda, int a_t, const float *s
 
 extern "C" int ksd_tc_grad_workspace(int64_t M, int64_t N, int64_t *bytes) {
   if (M < 0 || N < 0 || !bytes) return fail(KSD_EINVAL, "tc_grad_workspace: bad arguments");
-  const int64_t ncb = cdiv(N, tc::GC), nrb = cdiv(M, tc::GR);
+  const int64_t ncb = cdiv(N, 256), nrb = cdiv(M, tc::stats_rows(M, N));
   *bytes = 4 * (ncb * M + 2 * nrb * N + M + N);
   return KSD_OK;
 }
@@ -875,17 +1125,18 @@ extern "C" int ksd_tc_quantize_grad(const void *g, int g_dtype, int64_t M, int64
   ksd_tc_grad_workspace(M, N, &need);
   if (!g || !sx || !sw || !e || !f || !workspace || workspace_bytes < need)
     return fail(KSD_EINVAL, "tc_quantize_grad: null pointer or short workspace");
-  const int64_t ncb = cdiv(N, tc::GC), nrb = cdiv(M, tc::GR);
-  if (nrb > 65535 || cdiv(M, 32) > 65535) return fail(KSD_EINVAL, "tc_quantize_grad: too many rows");
+  const int rows = tc::stats_rows(M, N);
+  const int64_t ncb = cdiv(N, g_dtype == KSD_F32 ? 256 : 512), nrb = cdiv(M, rows);
+  if (nrb > 65535) return fail(KSD_EINVAL, "tc_quantize_grad: too many rows");
   uint32_t *row_part = (uint32_t *)workspace, *col_part = row_part + ncb * M;
   float *sum_part = (float *)(col_part + nrb * N), *einv = sum_part + nrb * N, *finv = einv + M;
   hipStream_t st = (hipStream_t)stream;
-  const dim3 gs((unsigned)ncb, (unsigned)nrb), gq((unsigned)cdiv(ld, 512), (unsigned)cdiv(M, 32));
-#define KSD_TC(DT)                                                                                                  \
-  tc::grad_stats_kernel<DT><<<gs, 256, 0, st>>>(g, M, N, stride, sx, sw, row_part, col_part, db ? sum_part : nullptr); \
-  tc::grad_fold_kernel<<<(unsigned)cdiv(M + N, 256), 256, 0, st>>>(row_part, col_part, db ? sum_part : nullptr, M, N, \
-                                                                   (int)ncb, (int)nrb, e, einv, f, finv, db);       \
-  if (q || c) tc::grad_codes_kernel<DT><<<gq, 256, 0, st>>>(g, M, N, stride, sx, sw, einv, finv, e, f, q, c, ld);
+  const dim3 gs((unsigned)cdiv(ncb, 4), (unsigned)nrb), gq((unsigned)cdiv(ld, 512), (unsigned)cdiv(M, 64));
+  const unsigned folds = (unsigned)(cdiv(M, 64) + cdiv(N, 64));
+#define KSD_TC(DT)                                                                                                    \
+  tc::grad_stats_kernel<DT><<<gs, 256, 0, st>>>(g, M, N, stride, rows, sx, sw, row_part, col_part, db ? sum_part : nullptr); \
+  tc::grad_fold_kernel<<<folds, 1024, 0, st>>>(row_part, col_part, sum_part, M, N, (int)ncb, (int)nrb, e, einv, f, finv, db); \
+  if (q || c) tc::grad_codes_kernel<DT><<<gq, 256, 0, st>>>(g, M, N, stride, sx, sw, einv, finv, q, c, ld);
   switch (g_dtype) {
     case KSD_F32: KSD_TC(KSD_F32) break;
     case KSD_BF16: KSD_TC(KSD_BF16) break;
@@ -893,4 +1144,120 @@ extern "C" int ksd_tc_quantize_grad(const void *g, int g_dtype, int64_t M, int64
   }
 #undef KSD_TC
   return check_launch("tc_quantize_grad");
+}
+
+extern "C" int ksd_tc_linear_workspace(int64_t M, int64_t N, int64_t K, int64_t *bytes) {
+  if (M < 0 || N < 0 || K < 1 || !bytes) return fail(KSD_EINVAL, "tc_linear_workspace: bad arguments");
+  if (tc::few_rows(M, K)) {
+    *bytes = 0;
+    return KSD_OK;
+  }
+  const int rc = ksd_tc_gemm_workspace(M, N, K, bytes);
+  *bytes += tc::pad256(M * tc::pitch16(K)) + tc::pad256(4 * M);
+  return rc;
+}
+
+extern "C" int ksd_tc_linear(const void *x, int x_dtype, int64_t M, int64_t K, int64_t stride, const int8_t *w, int64_t ldw,
+                             const float *sw, int64_t N, const float *bias, const void *residual, void *y, int out_dtype,
+                             void *workspace, int64_t workspace_bytes, void *stream) {
+  int64_t need = 0;
+  const int rc = ksd_tc_linear_workspace(M, N, K, &need);
+  if (rc) return rc;
+  if (!tc::float_type(x_dtype) || !tc::float_type(out_dtype)) return fail(KSD_ETYPE, "tc_linear: unsupported element type");
+  if (M == 0 || N == 0) return KSD_OK;
+  if (need > 0 && (!workspace || workspace_bytes < need))
+    return fail(KSD_EINVAL, "tc_linear: workspace of %lld bytes needed", (long long)need);
+  hipStream_t st = (hipStream_t)stream;
+  if (tc::few_rows(M, K)) {
+    if (!x || !w || !sw || !y) return fail(KSD_EINVAL, "tc_linear: null pointer");
+    if (ldw % 16 || ldw < tc::pitch16(K) || ((uintptr_t)w) % 16)
+      return fail(KSD_EINVAL, "tc_linear: the codes' rows must be 16-byte aligned and cover K rounded up to 16");
+    if (N > 0x7fffffff / 2) return fail(KSD_EINVAL, "tc_linear: shape too large");
+    const tc::Few p{x, w, sw, bias, residual, y, stride, ldw, (int)M, (int)N, (int)K, (int)(cdiv(K, 256) * 256 + 16)};
+    if (x_dtype == KSD_F32) tc::launch_few<KSD_F32>(out_dtype, p, st);
+    else if (x_dtype == KSD_BF16) tc::launch_few<KSD_BF16>(out_dtype, p, st);
+    else tc::launch_few<KSD_F16>(out_dtype, p, st);
+    return check_launch("tc_linear");
+  }
+  int8_t *codes = (int8_t *)workspace;
+  const int64_t ld = tc::pitch16(K), cb = tc::pad256(M * ld), sb = tc::pad256(4 * M);
+  float *scales = (float *)(codes + cb);
+  const int rq = ksd_tc_quantize_rows(x, x_dtype, M, K, stride, codes, ld, scales, stream);
+  if (rq) return rq;
+  return ksd_tc_gemm(codes, ld, 0, scales, w, ldw, 0, sw, M, N, K, bias, residual, y, out_dtype, codes + cb + sb,
+                     workspace_bytes - cb - sb, stream);
+}
+
+extern "C" int ksd_tc_linear_train(const void *x, int x_dtype, int64_t M, int64_t K, int64_t stride, const void *w, int w_dtype,
+                                   int64_t N, int64_t w_stride, const float *bias, const void *residual, int8_t *x_codes,
+                                   float *x_scales, int8_t *w_codes, float *w_scales, void *y, int out_dtype, void *workspace,
+                                   int64_t workspace_bytes, void *stream) {
+  const int64_t ld = tc::pitch16(K);
+  int rc = check_rows("tc_linear_train", x, x_dtype, M, K, x_codes, ld, x_scales);
+  if (!rc) rc = check_rows("tc_linear_train", w, w_dtype, N, K, w_codes, ld, w_scales);
+  if (rc) return rc;
+  if (!grid_fits(M + N, 256)) return fail(KSD_EINVAL, "tc_linear_train: too many rows");
+  const tc::Rows a{w, N, K, w_stride, ld, w_codes, w_scales}, b{x, M, K, stride, ld, x_codes, x_scales};
+  hipStream_t st = (hipStream_t)stream;
+  if (M + N > 0) {
+    if (w_dtype != KSD_F32) {
+      if (N > 0) tc::launch_rows(a, w_dtype, st);
+      if (M > 0) tc::launch_rows(b, x_dtype, st);
+    } else if (x_dtype == KSD_F32) {
+      tc::launch_rows<KSD_F32, KSD_F32>(a, b, st);
+    } else if (x_dtype == KSD_BF16) {
+      tc::launch_rows<KSD_F32, KSD_BF16>(a, b, st);
+    } else {
+      tc::launch_rows<KSD_F32, KSD_F16>(a, b, st);
+    }
+  }
+  return ksd_tc_gemm(x_codes, ld, 0, x_scales, w_codes, ld, 0, w_scales, M, N, K, bias, residual, y, out_dtype, workspace,
+                     workspace_bytes, stream);
+}
+
+namespace {
+// the backward's scratch: q, c, scales, then one region that the gradient's statistics and the two
+// products' parts use in turn
+struct BackwardScratch {
+  int64_t q, c, ef, rest, bytes;
+};
+BackwardScratch backward_scratch(int64_t M, int64_t N, int64_t K, bool dx, bool dw) {
+  BackwardScratch s;
+  const int64_t codes = tc::pad256(M * tc::pitch16(N));
+  s.q = 0;
+  s.c = s.q + (dx ? codes : 0);
+  s.ef = s.c + (dw ? codes : 0);
+  s.rest = s.ef + tc::pad256(4 * (M + N));
+  int64_t a = 0, b = 0, c = 0;
+  ksd_tc_grad_workspace(M, N, &a);
+  if (dx) ksd_tc_gemm_workspace(M, K, N, &b);
+  if (dw) ksd_tc_gemm_workspace(N, K, M, &c);
+  s.bytes = s.rest + std::max(a, std::max(b, c));
+  return s;
+}
+}  // namespace
+
+extern "C" int ksd_tc_linear_backward_workspace(int64_t M, int64_t N, int64_t K, int need_dx, int need_dw, int64_t *bytes) {
+  if (M < 1 || N < 1 || K < 1 || !bytes) return fail(KSD_EINVAL, "tc_linear_backward_workspace: bad arguments");
+  *bytes = backward_scratch(M, N, K, need_dx, need_dw).bytes;
+  return KSD_OK;
+}
+
+extern "C" int ksd_tc_linear_backward(const void *g, int g_dtype, int64_t M, int64_t N, int64_t stride, int64_t K,
+                                      const int8_t *x_codes, const float *x_scales, const int8_t *w_codes, const float *w_scales,
+                                      void *dx, int dx_dtype, float *dw, float *db, void *workspace, int64_t workspace_bytes,
+                                      void *stream) {
+  if (M < 1 || N < 1 || K < 1) return fail(KSD_EINVAL, "tc_linear_backward: bad shape");
+  const BackwardScratch s = backward_scratch(M, N, K, dx, dw);
+  if (!workspace || workspace_bytes < s.bytes) return fail(KSD_EINVAL, "tc_linear_backward: workspace of %lld bytes needed", (long long)s.bytes);
+  char *ws = (char *)workspace;
+  int8_t *q = dx ? (int8_t *)(ws + s.q) : nullptr, *c = dw ? (int8_t *)(ws + s.c) : nullptr;
+  float *e = (float *)(ws + s.ef), *f = e + M;
+  const int64_t ld = tc::pitch16(N), ldk = tc::pitch16(K), rest = workspace_bytes - s.rest;
+  int rc = ksd_tc_quantize_grad(g, g_dtype, M, N, stride, x_scales, w_scales, q, e, c, f, ld, db, ws + s.rest, rest, stream);
+  if (!rc && dx)
+    rc = ksd_tc_gemm(q, ld, 0, e, w_codes, ldk, 1, nullptr, M, K, N, nullptr, nullptr, dx, dx_dtype, ws + s.rest, rest, stream);
+  if (!rc && dw)
+    rc = ksd_tc_gemm(c, ld, 1, f, x_codes, ldk, 1, nullptr, N, K, M, nullptr, nullptr, dw, KSD_F32, ws + s.rest, rest, stream);
+  return rc;
 }

@@ -150,9 +150,14 @@ def token_channel_linear(x: torch.Tensor, w_codes: torch.Tensor, w_scales: torch
     out_dtype = out_dtype or x.dtype
     bias, residual = _epilogue(M, N, bias, None if residual is None else residual.reshape(-1, N), out_dtype)
     w_scales = _vector(w_scales, N, "w_scales")
-    codes, scales = _rows(x2, dev)
-    y = _gemm(codes, codes.shape[1], 0, scales, w, ldw, 0, w_scales, M, N, K, bias, residual, out_dtype, dev)
-    return y.reshape(*x.shape[:-1], N)
+    y = torch.empty((*x.shape[:-1], N), dtype=out_dtype, device=dev)
+    need = ctypes.c_int64()
+    _lib.call("ksd_tc_linear_workspace", M, N, K, ctypes.byref(need))
+    work = torch.empty(need.value, dtype=torch.int8, device=dev) if need.value else None
+    _lib.call("ksd_tc_linear", x2.data_ptr(), _OUT[x2.dtype], M, K, x2.stride(0) if M > 1 else K, w.data_ptr(), ldw,
+              w_scales.data_ptr(), N, _lib.ptr(bias), _lib.ptr(residual), y.data_ptr(), _OUT[out_dtype],
+              _lib.ptr(work), need.value, _lib.stream_ptr(dev))
+    return y
 
 
 class Saved:
@@ -175,10 +180,19 @@ def token_channel_linear_train(x: torch.Tensor, weight: torch.Tensor, bias: torc
     s = Saved()
     s.M, s.N, s.K, s.dtype, s.lead, s.has_bias = x2.shape[0], N, K, x.dtype, x.shape[:-1], bias is not None
     bias, residual = _epilogue(s.M, N, bias, None if residual is None else residual.reshape(-1, N), x.dtype)
-    s.wq, s.ws = _rows(w2, dev)
-    s.xq, s.xs = _rows(x2, dev)
-    y = _gemm(s.xq, s.xq.shape[1], 0, s.xs, s.wq, s.wq.shape[1], 0, s.ws, s.M, N, K, bias, residual, x.dtype, dev)
-    return y.reshape(*s.lead, N), s
+    M, ld = s.M, _pitch(K)
+    codes = torch.empty((M + N, ld), dtype=torch.int8, device=dev)
+    scales = torch.empty(M + N, dtype=torch.float32, device=dev)
+    s.xq, s.wq, s.xs, s.ws = codes[:M], codes[M:], scales[:M], scales[M:]
+    y = torch.empty((*s.lead, N), dtype=x.dtype, device=dev)
+    need = ctypes.c_int64()
+    _lib.call("ksd_tc_gemm_workspace", M, N, K, ctypes.byref(need))
+    work = torch.empty(need.value, dtype=torch.int8, device=dev) if need.value else None
+    _lib.call("ksd_tc_linear_train", x2.data_ptr(), _OUT[x2.dtype], M, K, x2.stride(0) if M > 1 else K, w2.data_ptr(),
+              _OUT[w2.dtype], N, w2.stride(0) if N > 1 else K, _lib.ptr(bias), _lib.ptr(residual), s.xq.data_ptr(),
+              s.xs.data_ptr(), s.wq.data_ptr(), s.ws.data_ptr(), y.data_ptr(), _OUT[x.dtype], _lib.ptr(work),
+              need.value, _lib.stream_ptr(dev))
+    return y, s
 
 
 def token_channel_linear_backward(grad: torch.Tensor, saved: Saved, need_dx: bool = True, need_dw: bool = True,
@@ -191,28 +205,19 @@ def token_channel_linear_backward(grad: torch.Tensor, saved: Saved, need_dx: boo
         raise ValueError(f"grad has shape {tuple(grad.shape)}, the output {(*saved.lead, N)}")
     g = _matrix(grad.reshape(-1, N), "grad")
     need_db = saved.has_bias if need_db is None else need_db
-    dx = dw = db = None
     if M == 0:
         return (torch.empty((*saved.lead, K), dtype=saved.dtype, device=dev) if need_dx else None,
                 torch.zeros((N, K), device=dev) if need_dw else None,
                 torch.zeros(N, device=dev) if need_db else None)
-    ld = _pitch(N)
-    q = torch.empty((M, ld), dtype=torch.int8, device=dev) if need_dx else None
-    c = torch.empty((M, ld), dtype=torch.int8, device=dev) if need_dw else None
+    dx = torch.empty((*saved.lead, K), dtype=saved.dtype, device=dev) if need_dx else None
+    dw = torch.empty((N, K), dtype=torch.float32, device=dev) if need_dw else None
     db = torch.empty(N, dtype=torch.float32, device=dev) if need_db else None
     need = ctypes.c_int64()
-    _lib.call("ksd_tc_grad_workspace", M, N, ctypes.byref(need))
+    _lib.call("ksd_tc_linear_backward_workspace", M, N, K, need_dx, need_dw, ctypes.byref(need))
     work = torch.empty(need.value, dtype=torch.int8, device=dev)
-    ef = torch.empty(M + N, dtype=torch.float32, device=dev)
-    e, f = ef[:M], ef[M:]
-    _lib.call("ksd_tc_quantize_grad", g.data_ptr(), _OUT[g.dtype], M, N, g.stride(0) if M > 1 else N,
-              saved.xs.data_ptr(), saved.ws.data_ptr(), _lib.ptr(q), e.data_ptr(), _lib.ptr(c), f.data_ptr(), ld,
-              _lib.ptr(db), work.data_ptr(), need.value, _lib.stream_ptr(dev))
-    if need_dx:
-        dx = _gemm(q, ld, 0, e, saved.wq, saved.wq.shape[1], 1, None, M, K, N, None, None, saved.dtype, dev)
-        dx = dx.reshape(*saved.lead, K)
-    if need_dw:
-        dw = _gemm(c, ld, 1, f, saved.xq, saved.xq.shape[1], 1, None, N, K, M, None, None, torch.float32, dev)
+    _lib.call("ksd_tc_linear_backward", g.data_ptr(), _OUT[g.dtype], M, N, g.stride(0) if M > 1 else N, K,
+              saved.xq.data_ptr(), saved.xs.data_ptr(), saved.wq.data_ptr(), saved.ws.data_ptr(), _lib.ptr(dx),
+              _OUT[saved.dtype], _lib.ptr(dw), _lib.ptr(db), work.data_ptr(), need.value, _lib.stream_ptr(dev))
     return dx, dw, db
 
 

@@ -93,7 +93,7 @@ def test_quantize_rows_edges():
 
 
 SHAPES = [(1, 1, 1), (1, 512, 1536), (3, 5, 7), (4, 1000, 129), (16, 64, 1536), (17, 33, 2048), (64, 130, 597),
-          (129, 127, 16), (130, 257, 1000), (300, 1536, 512), (515, 384, 4099), (1021, 777, 333)]
+          (2, 40, 20011), (32, 50, 2500), (33, 48, 1537), (31, 2000, 100), (129, 127, 16), (130, 257, 1000), (300, 1536, 512), (515, 384, 4099), (1021, 777, 333)]
 
 
 @pytest.mark.gpu
