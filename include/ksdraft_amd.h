@@ -807,22 +807,16 @@ int ksd_embedding_gradient(const void *g, int g_dtype, int64_t n, int64_t d, int
  * ksdraft/train/__init__.py:165).
  *   norm   = (max_kind ? max |g| : sqrt(sum g^2)) / loss_scale, summed in fp64 in a fixed order
  *   factor = min(1, max_norm / (norm + 1e-6)) / loss_scale (NULL: not formed)
- * ksd_grad_scale writes out = grad * factor[0] for every tensor (out may be grad; then a factor of
- * exactly 1 leaves the memory untouched). tensors is a host array; n elements of type dtype
- * (KSD_F32, KSD_BF16, KSD_F16), dense, at any alignment of the element type.
+ * ksd_grad_scale writes outs[i] = grads[i] * factor[0] (an outs[i] may be grads[i]; a factor of exactly
+ * 1 then leaves its memory untouched). grads, outs, sizes (elements) and types (KSD_F32, KSD_BF16,
+ * KSD_F16) are host arrays of n entries; the tensors are dense, at any alignment of the element type.
  */
-typedef struct {
-  const void *grad;
-  void *out;
-  int64_t n;
-  int32_t dtype;
-  int32_t reserved;
-} KsdClipTensor;
-int ksd_grad_norm_workspace(const KsdClipTensor *tensors, int n, int64_t *bytes);
-int ksd_grad_norm(const KsdClipTensor *tensors, int n, int max_kind, float max_norm,
-                  float loss_scale, float *norm, float *factor, void *workspace,
-                  int64_t workspace_bytes, void *stream);
-int ksd_grad_scale(const KsdClipTensor *tensors, int n, const float *factor, void *stream);
+int ksd_grad_norm_workspace(const int64_t *sizes, int n, int64_t *bytes);
+int ksd_grad_norm(const void *const *grads, const int64_t *sizes, const int32_t *types, int n,
+                  int max_kind, float max_norm, float loss_scale, float *norm, float *factor,
+                  void *workspace, int64_t workspace_bytes, void *stream);
+int ksd_grad_scale(const void *const *grads, void *const *outs, const int64_t *sizes,
+                   const int32_t *types, int n, const float *factor, void *stream);
 
 #ifdef __cplusplus
 }

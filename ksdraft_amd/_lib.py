@@ -102,8 +102,8 @@ SIGNATURES = {
     "ksd_embedding_gradient_workspace": [_I64, _I64, _P],
     "ksd_embedding_gradient": [_P, _INT, _I64, _I64, _I64, _P, _INT, _I64, _I64, _F, _INT, _P, _INT, _P, _I64, _P],
     "ksd_grad_norm_workspace": [_P, _INT, _P],
-    "ksd_grad_norm": [_P, _INT, _INT, _F, _F, _P, _P, _P, _I64, _P],
-    "ksd_grad_scale": [_P, _INT, _P, _P],
+    "ksd_grad_norm": [_P, _P, _P, _INT, _INT, _F, _F, _P, _P, _P, _I64, _P],
+    "ksd_grad_scale": [_P, _P, _P, _P, _INT, _P, _P],
 }
 
 _lib = None

@@ -171,31 +171,40 @@ __global__ __launch_bounds__(256) void scale_kernel(const Batch b, const float *
   }
 }
 
-// Calls launch(batch, grid) for batches of the tensors; an error code ends it.
+// Calls launch(batch, grid) for batches of the tensors, from the last to the first with `back`.
+struct List {
+  const void *const *grads;
+  void *const *outs;
+  const int64_t *sizes;
+  const int32_t *types;
+  int n;
+};
 template <class F>
-static void batches(const KsdClipTensor *t, int n, F launch) {
+static void batches(const List &l, bool back, F launch) {
   Batch b;
   b.n = b.chunks = 0;
-  for (int i = 0; i < n; ++i) {
-    if (t[i].n == 0) continue;
-    const int64_t chunks = cdiv(t[i].n, kChunk);
+  for (int k = 0; k < l.n; ++k) {
+    const int i = back ? l.n - 1 - k : k;
+    if (l.sizes[i] == 0) continue;
+    const int64_t chunks = cdiv(l.sizes[i], kChunk);
     if (b.n == kBatch || b.chunks + chunks > 0x7fffffff) {
       launch(b, std::min(b.chunks, kGrid));
       b.n = b.chunks = 0;
     }
-    b.t[b.n++] = Tensor{t[i].grad, t[i].out, t[i].n, b.chunks, t[i].dtype};
+    b.t[b.n++] = Tensor{l.grads[i], l.outs ? l.outs[i] : nullptr, l.sizes[i], b.chunks, l.types[i]};
     b.chunks += (int)chunks;
   }
   if (b.n) launch(b, std::min(b.chunks, kGrid));
 }
 
-static int check(const KsdClipTensor *t, int n, const char *who, bool out) {
-  if (n < 0 || (n > 0 && !t)) return fail(KSD_EINVAL, "%s: bad tensor list", who);
-  for (int i = 0; i < n; ++i) {
-    if (t[i].n < 0 || t[i].n > (int64_t)kChunk * 0x7fffffff) return fail(KSD_EINVAL, "%s: tensor %d: bad size", who, i);
-    if (t[i].dtype != KSD_F32 && t[i].dtype != KSD_BF16 && t[i].dtype != KSD_F16)
-      return fail(KSD_ETYPE, "%s: tensor %d: unsupported element type %d", who, i, t[i].dtype);
-    if (t[i].n > 0 && (!t[i].grad || (out && !t[i].out))) return fail(KSD_EINVAL, "%s: tensor %d: null pointer", who, i);
+static int check(const List &l, const char *who, bool out) {
+  if (l.n < 0 || (l.n > 0 && (!l.grads || !l.sizes || !l.types || (out && !l.outs))))
+    return fail(KSD_EINVAL, "%s: bad tensor list", who);
+  for (int i = 0; i < l.n; ++i) {
+    if (l.sizes[i] < 0 || l.sizes[i] > (int64_t)kChunk * 0x7fffffff) return fail(KSD_EINVAL, "%s: tensor %d: bad size", who, i);
+    if (l.types[i] != KSD_F32 && l.types[i] != KSD_BF16 && l.types[i] != KSD_F16)
+      return fail(KSD_ETYPE, "%s: tensor %d: unsupported element type %d", who, i, l.types[i]);
+    if (l.sizes[i] > 0 && (!l.grads[i] || (out && !l.outs[i]))) return fail(KSD_EINVAL, "%s: tensor %d: null pointer", who, i);
   }
   return KSD_OK;
 }
@@ -205,26 +214,33 @@ static int check(const KsdClipTensor *t, int n, const char *who, bool out) {
 
 using namespace ksd;
 
-extern "C" int ksd_grad_norm_workspace(const KsdClipTensor *tensors, int n, int64_t *bytes) {
-  if (!bytes) return fail(KSD_EINVAL, "grad_norm_workspace: null pointer");
-  const int rc = clip::check(tensors, n, "grad_norm_workspace", false);
-  if (rc) return rc;
-  int64_t parts = 0;
-  clip::batches(tensors, n, [&](const clip::Batch &, int grid) { parts += grid; });
-  *bytes = 8 * std::max<int64_t>(parts, 1);
+extern "C" int ksd_grad_norm_workspace(const int64_t *sizes, int n, int64_t *bytes) {
+  if (!bytes || n < 0 || (n > 0 && !sizes)) return fail(KSD_EINVAL, "grad_norm_workspace: bad arguments");
+  // at most kGrid results per launch and one per chunk
+  int64_t chunks = 0;
+  for (int i = 0; i < n; ++i) {
+    if (sizes[i] < 0) return fail(KSD_EINVAL, "grad_norm_workspace: tensor %d: bad size", i);
+    chunks += cdiv(sizes[i], clip::kChunk);
+  }
+  const int64_t launches = cdiv(n, clip::kBatch) + chunks / 0x7fffffff + 1;
+  *bytes = 8 * std::max<int64_t>(1, std::min(chunks, launches * clip::kGrid));
   return KSD_OK;
 }
 
-extern "C" int ksd_grad_norm(const KsdClipTensor *tensors, int n, int max_kind, float max_norm, float loss_scale, float *norm,
-                             float *factor, void *workspace, int64_t workspace_bytes, void *stream) {
+extern "C" int ksd_grad_norm(const void *const *grads, const int64_t *sizes, const int32_t *types, int n, int max_kind,
+                             float max_norm, float loss_scale, float *norm, float *factor, void *workspace,
+                             int64_t workspace_bytes, void *stream) {
+  const clip::List l{grads, nullptr, sizes, types, n};
+  int rc = clip::check(l, "grad_norm", false);
+  if (rc) return rc;
   int64_t need = 0;
-  const int rc = ksd_grad_norm_workspace(tensors, n, &need);
+  rc = ksd_grad_norm_workspace(sizes, n, &need);
   if (rc) return rc;
   if (!norm || !workspace || workspace_bytes < need) return fail(KSD_EINVAL, "grad_norm: null pointer or short workspace");
   hipStream_t st = (hipStream_t)stream;
   double *parts = (double *)workspace;
   int at = 0;
-  clip::batches(tensors, n, [&](const clip::Batch &b, int grid) {
+  clip::batches(l, false, [&](const clip::Batch &b, int grid) {
     if (max_kind) clip::norm_kernel<true><<<grid, 256, 0, st>>>(b, parts + at);
     else clip::norm_kernel<false><<<grid, 256, 0, st>>>(b, parts + at);
     at += grid;
@@ -234,11 +250,14 @@ extern "C" int ksd_grad_norm(const KsdClipTensor *tensors, int n, int max_kind, 
   return check_launch("grad_norm");
 }
 
-extern "C" int ksd_grad_scale(const KsdClipTensor *tensors, int n, const float *factor, void *stream) {
-  const int rc = clip::check(tensors, n, "grad_scale", true);
+extern "C" int ksd_grad_scale(const void *const *grads, void *const *outs, const int64_t *sizes, const int32_t *types, int n,
+                              const float *factor, void *stream) {
+  const clip::List l{grads, outs, sizes, types, n};
+  const int rc = clip::check(l, "grad_scale", true);
   if (rc) return rc;
   if (!factor) return fail(KSD_EINVAL, "grad_scale: null pointer");
   hipStream_t st = (hipStream_t)stream;
-  clip::batches(tensors, n, [&](const clip::Batch &b, int grid) { clip::scale_kernel<<<grid, 256, 0, st>>>(b, factor); });
+  // backwards: the tensors that the norm has read last are still in the last-level cache
+  clip::batches(l, true, [&](const clip::Batch &b, int grid) { clip::scale_kernel<<<grid, 256, 0, st>>>(b, factor); });
   return check_launch("grad_scale");
 }

@@ -84,13 +84,33 @@ __global__ __launch_bounds__(256) void lookup_kernel(const void *__restrict__ ta
 }
 
 // ------------------------------------------------------------------------------------ sort
-// Least significant digit first, 8 bits a pass, tiles of 2048 keys. Ids that take no part (the
-// padding token, ids out of range) become the key V, which sorts last.
-constexpr int kTile = 2048;
+// Stable, least significant digit first, at most 9 bits a pass. Ids that take no part (the padding
+// token, ids out of range) become the key V, which sorts last. Keys of one digit keep their order:
+// rank = earlier tiles' + earlier waves' + earlier rounds of 64 + lower lanes with that digit, the last
+// from ballots over the digit's bits.
+constexpr int kDigits = 512;
+constexpr int kOne = 8192;   // keys that one workgroup sorts in LDS
 
 __device__ __forceinline__ uint32_t key_of(const void *ids, int wide, int64_t i, int64_t V, int64_t pad) {
   const int64_t id = load_id(ids, wide, i);
   return (uint32_t)(id < 0 || id >= V || id == pad ? V : id);
+}
+
+// Zeros for n bytes at p, 16-byte aligned: workgroup `block` of 256 threads writes one piece of 4 KB, so that
+// the stores walk through memory in launch order. (922 MB: 6.3 to 6.6 TB/s; loops over a smaller grid 4.7 to
+// 6.1, larger pieces 4.2 to 5.6. Non-temporal: 8192 rows' sums after it take 15 us, after ordinary stores,
+// whose dirty lines have to leave first, 28.)
+struct Fill {
+  char *p;
+  int64_t n;
+};
+static int64_t fill_blocks(const Fill &f) { return cdiv(f.n, 4096); }
+__device__ __forceinline__ void fill(const Fill &f, int64_t block) {
+  typedef uint32_t vec __attribute__((ext_vector_type(4)));
+  const int64_t at = (block * 256 + threadIdx.x) * 16;
+  if (at + 16 <= f.n) __builtin_nontemporal_store((vec){0, 0, 0, 0}, (vec *)(f.p + at));
+  else
+    for (int64_t i = at; i < f.n; ++i) f.p[i] = 0;
 }
 
 struct SortArgs {
@@ -99,106 +119,224 @@ struct SortArgs {
   const int32_t *pos;
   uint32_t *out_keys;
   int32_t *out_pos;
-  uint32_t *counts;  // (256, tiles)
+  uint32_t *counts;  // (tiles, kDigits)
   int64_t V, pad;
-  int n, tiles, shift, wide;
+  int n, tiles, shift, bits, wide;
 };
 
 __device__ __forceinline__ uint32_t sort_key(const SortArgs &a, int i) {
   return a.ids ? key_of(a.ids, a.wide, i, a.V, a.pad) : a.keys[i];
 }
 
+// Lanes of the wave that hold digit d too (`in`: lanes that hold a key).
+__device__ __forceinline__ uint64_t same_digit(uint32_t d, int bits, bool in) {
+  uint64_t m = __ballot(in);
+  for (int b = 0; b < bits; ++b) {
+    const uint64_t bal = __ballot((d >> b) & 1);
+    m &= (d >> b) & 1 ? bal : ~bal;
+  }
+  return m;
+}
+
+// Exclusive sum over one value per thread of a workgroup of NT threads (scratch: NT / 64 words).
+template <int NT>
+__device__ __forceinline__ uint32_t exclusive_sum(uint32_t v, uint32_t *scratch) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t s = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t u = (uint32_t)__shfl_up((int)s, o);
+    if (lane >= o) s += u;
+  }
+  if (lane == 63) scratch[wave] = s;
+  __syncthreads();
+  uint32_t before = 0;
+  for (int w = 0; w < wave; ++w) before += scratch[w];
+  __syncthreads();
+  return before + s - v;
+}
+
+// Tiles of 256 R keys, four waves of R rounds. Digit counts of the tiles.
+template <int R>
 __global__ __launch_bounds__(256) void sort_count_kernel(const SortArgs a) {
-  __shared__ uint32_t h[256];
-  const int tid = threadIdx.x, t0 = blockIdx.x * kTile;
-  h[tid] = 0;
+  __shared__ uint32_t h[kDigits];
+  const int tid = threadIdx.x, t0 = blockIdx.x * (256 * R);
+  h[tid] = h[tid + 256] = 0;
   __syncthreads();
-  for (int i = t0 + tid; i < min(a.n, t0 + kTile); i += 256) atomicAdd(&h[(sort_key(a, i) >> a.shift) & 255], 1u);
-  __syncthreads();
-  a.counts[tid * a.tiles + blockIdx.x] = h[tid];
-}
-
-// exclusive sum over `len` counts, one workgroup
-__global__ __launch_bounds__(1024) void sort_scan_kernel(uint32_t *counts, int len) {
-  __shared__ uint32_t part[16];
-  __shared__ uint32_t carry;
-  const int tid = threadIdx.x, lane = tid & 63;
-  if (tid == 0) carry = 0;
-  __syncthreads();
-  for (int b = 0; b < len; b += 1024) {
-    const uint32_t v = b + tid < len ? counts[b + tid] : 0;
-    uint32_t s = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const uint32_t u = (uint32_t)__shfl_up((int)s, o);
-      if (lane >= o) s += u;
-    }
-    if (lane == 63) part[tid >> 6] = s;
-    __syncthreads();
-    uint32_t before = carry;
-    for (int w = 0; w < tid >> 6; ++w) before += part[w];
-    if (b + tid < len) counts[b + tid] = before + s - v;
-    __syncthreads();
-    if (tid == 1023) carry = before + s;
-    __syncthreads();
+  const uint32_t mask = (1u << a.bits) - 1;
+#pragma unroll 4
+  for (int r = 0; r < R; ++r) {
+    const int i = t0 + r * 256 + tid;
+    if (i < a.n) atomicAdd(&h[(sort_key(a, i) >> a.shift) & mask], 1u);
   }
+  __syncthreads();
+  uint32_t *const c = a.counts + (int64_t)blockIdx.x * kDigits;
+  c[tid] = h[tid];
+  c[tid + 256] = h[tid + 256];
 }
 
-// Wave w of a tile takes its keys [512 w, 512 w + 512) in 8 rounds of 64, so keys of one digit keep
-// their order: rank = earlier tiles' (counts) + earlier waves' + earlier rounds' + lower lanes'.
+template <int R>
 __global__ __launch_bounds__(256) void sort_scatter_kernel(const SortArgs a) {
-  __shared__ uint32_t h[4][256];
+  __shared__ uint32_t h[4][kDigits];
+  __shared__ uint32_t scratch[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int base = blockIdx.x * kTile + wave * 512;
-  for (int w = 0; w < 4; ++w) h[w][tid] = 0;
-  __syncthreads();
-  uint32_t key[8];
-  uint64_t same[8];
+  const int base = blockIdx.x * (256 * R) + wave * (64 * R);
+  const uint32_t mask = (1u << a.bits) - 1;
+  const uint64_t below = (1ull << lane) - 1;
+  uint32_t key[R];
+  int32_t pos[R];
 #pragma unroll
-  for (int r = 0; r < 8; ++r) {
+  for (int r = 0; r < R; ++r) {
     const int i = base + r * 64 + lane;
-    const bool in = i < a.n;
-    key[r] = in ? sort_key(a, i) : 0xffffffffu;
-    const uint32_t d = (key[r] >> a.shift) & 255;
-    uint64_t m = __ballot(in);
+    key[r] = i < a.n ? sort_key(a, i) : 0;
+    pos[r] = a.ids || i >= a.n ? i : a.pos[i];
+  }
 #pragma unroll
-    for (int b = 0; b < 8; ++b) {
-      const uint64_t bal = __ballot((d >> b) & 1);
-      m &= (d >> b) & 1 ? bal : ~bal;
-    }
-    same[r] = m;
-    if (in && (m & ((1ull << lane) - 1)) == 0) h[wave][d] += (uint32_t)__popcll(m);
+  for (int w = 0; w < 4; ++w) h[w][tid] = h[w][tid + 256] = 0;
+  // digits 2 tid, 2 tid + 1: keys of earlier tiles, and of all tiles for the digits' starts
+  uint2 earlier = make_uint2(0, 0), all = make_uint2(0, 0);
+#pragma unroll 8
+  for (int t = 0; t < a.tiles; ++t) {
+    const uint2 c = *(const uint2 *)(a.counts + (int64_t)t * kDigits + 2 * tid);
+    all.x += c.x, all.y += c.y;
+    if (t < (int)blockIdx.x) earlier.x += c.x, earlier.y += c.y;
+  }
+  const uint32_t start = exclusive_sum<256>(all.x + all.y, scratch);
+  uint64_t same[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const bool in = base + r * 64 + lane < a.n;
+    const uint32_t d = (key[r] >> a.shift) & mask;
+    same[r] = same_digit(d, a.bits, in);
+    if (in && (same[r] & below) == 0) h[wave][d] += (uint32_t)__popcll(same[r]);
+    __builtin_amdgcn_wave_barrier();
   }
   __syncthreads();
-  {
-    uint32_t at = a.counts[tid * a.tiles + blockIdx.x];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    uint32_t at = start + (e ? all.x + earlier.y : earlier.x);
+#pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const uint32_t c = h[w][tid];
-      h[w][tid] = at;
+      const uint32_t c = h[w][2 * tid + e];
+      h[w][2 * tid + e] = at;
       at += c;
     }
   }
   __syncthreads();
 #pragma unroll
-  for (int r = 0; r < 8; ++r) {
-    const int i = base + r * 64 + lane;
-    const uint32_t d = (key[r] >> a.shift) & 255;
+  for (int r = 0; r < R; ++r) {
+    const bool in = base + r * 64 + lane < a.n;
+    const uint32_t d = (key[r] >> a.shift) & mask;
     uint32_t first = 0;
-    if (i < a.n) {
+    if (in) {
       first = h[wave][d];
-      const uint32_t to = first + (uint32_t)__popcll(same[r] & ((1ull << lane) - 1));
+      const uint32_t to = first + (uint32_t)__popcll(same[r] & below);
       a.out_keys[to] = key[r];
-      a.out_pos[to] = a.ids ? i : a.pos[i];
+      a.out_pos[to] = pos[r];
     }
     __builtin_amdgcn_wave_barrier();
-    if (i < a.n && (same[r] & ((1ull << lane) - 1)) == 0) h[wave][d] = first + (uint32_t)__popcll(same[r]);
+    if (in && (same[r] & below) == 0) h[wave][d] = first + (uint32_t)__popcll(same[r]);
     __builtin_amdgcn_wave_barrier();
   }
 }
 
-// ------------------------------------------------------------------------------------ sums
-constexpr int kRun = 32;  // sorted positions of a chunk
+// Up to kOne keys: one workgroup sorts them, all passes in one launch (NT = 1024 threads: 8192 ids of
+// 150144 in MEASURED_SORT us). With NT = 256 the other workgroups clear `out` meanwhile; that form keeps little
+// in registers and LDS, so that a CU still holds 8 workgroups of the clearing.
+template <int NT>
+__global__ __launch_bounds__(NT) void sort_one_kernel(const SortArgs a, int passes, uint32_t *keys2, int32_t *pos2, const Fill f) {
+  constexpr int NW = NT / 64, R = kOne / NT, U = R < 4 ? R : 4;
+  __shared__ uint32_t h[NW * kDigits];
+  __shared__ uint32_t scratch[NW];
+  if (blockIdx.x > 0) {
+    if constexpr (NT == 256) fill(f, blockIdx.x - 1);
+    return;
+  }
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int per = (a.n + NT - 1) / NT;  // rounds of a wave that hold keys
+  const uint32_t mask = (1u << a.bits) - 1;
+  const uint64_t below = (1ull << lane) - 1;
+  for (int pass = 0; pass < passes; ++pass) {
+    const int shift = pass * a.bits;
+    // the last pass ends in out_keys, out_pos
+    const bool even = (passes - 1 - pass) % 2 == 0;
+    uint32_t *const to_keys = even ? a.out_keys : keys2;
+    int32_t *const to_pos = even ? a.out_pos : pos2;
+    const uint32_t *const from_keys = even ? keys2 : a.out_keys;
+    const int32_t *const from_pos = even ? pos2 : a.out_pos;
+    auto load = [&](int r, uint32_t &key, int32_t &p, bool &in) __attribute__((always_inline)) {
+      const int i = (wave * per + r) * 64 + lane;
+      in = r < per && i < a.n;
+      const int j = in ? i : 0;
+      key = pass == 0 ? key_of(a.ids, a.wide, j, a.V, a.pad) : from_keys[j];
+      p = pass == 0 ? j : from_pos[j];
+    };
+    for (int i = tid; i < NW * kDigits; i += NT) h[i] = 0;
+    __syncthreads();
+    for (int r0 = 0; r0 < per; r0 += U) {
+      uint32_t key[U];
+      int32_t p[U];
+      bool in[U];
+#pragma unroll
+      for (int r = 0; r < U; ++r) load(r0 + r, key[r], p[r], in[r]);
+#pragma unroll
+      for (int r = 0; r < U; ++r) {
+        const uint32_t d = (key[r] >> shift) & mask;
+        const uint64_t same = same_digit(d, a.bits, in[r]);
+        if (in[r] && (same & below) == 0) h[wave * kDigits + d] += (uint32_t)__popcll(same);
+        __builtin_amdgcn_wave_barrier();
+      }
+    }
+    __syncthreads();
+    // digit starts: NT = 256 threads hold two digits each
+    constexpr int E = NT < kDigits ? kDigits / NT : 1;
+    uint32_t all[E], sum = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      all[e] = 0;
+      if (tid * E + e < kDigits)
+        for (int w = 0; w < NW; ++w) all[e] += h[w * kDigits + tid * E + e];
+      sum += all[e];
+    }
+    uint32_t at = exclusive_sum<NT>(sum, scratch);
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (tid * E + e < kDigits)
+        for (int w = 0; w < NW; ++w) {
+          const uint32_t c = h[w * kDigits + tid * E + e];
+          h[w * kDigits + tid * E + e] = at;
+          at += c;
+        }
+    __syncthreads();
+    for (int r0 = 0; r0 < per; r0 += U) {
+      uint32_t key[U];
+      int32_t p[U];
+      bool in[U];
+#pragma unroll
+      for (int r = 0; r < U; ++r) load(r0 + r, key[r], p[r], in[r]);
+#pragma unroll
+      for (int r = 0; r < U; ++r) {
+        const uint32_t d = (key[r] >> shift) & mask;
+        const uint64_t same = same_digit(d, a.bits, in[r]);
+        uint32_t first = 0;
+        if (in[r]) {
+          first = h[wave * kDigits + d];
+          const uint32_t to = first + (uint32_t)__popcll(same & below);
+          to_keys[to] = key[r];
+          to_pos[to] = p[r];
+        }
+        __builtin_amdgcn_wave_barrier();
+        if (in[r] && (same & below) == 0) h[wave * kDigits + d] = first + (uint32_t)__popcll(same);
+        __builtin_amdgcn_wave_barrier();
+      }
+    }
+    // this pass's keys are read by other waves of the workgroup in the next
+    __threadfence_block();
+    __syncthreads();
+  }
+}
 
+// ------------------------------------------------------------------------------------ sums
 struct SumArgs {
   const uint32_t *keys;
   const int32_t *pos;
@@ -206,94 +344,247 @@ struct SumArgs {
   void *out;
   float *parts;  // (2, chunks, d): the piece of the run that a chunk begins in, and the one it ends in
   int64_t d, stride, V;
-  int n, chunks, add;
+  int64_t rows;                     // rows of out that this launch writes where no token occurs
+  int n, chunks, run, slices, add;  // run: sorted positions of a chunk; slices of 64 lanes' columns
+  unsigned sums;                    // workgroups that sum
   float scale;
 };
 
-template <int OUT>
-__device__ __forceinline__ void put_row(const SumArgs &a, uint32_t key, int64_t c, int m, const float *acc) {
-  typename Elem<OUT>::T *o = (typename Elem<OUT>::T *)a.out + (int64_t)key * a.d + c;
-  float v[8];
+// A lane's NV columns (16 bytes) from c on as raw bits, loaded at c0 = min(c, d - NV) so that rows need no
+// branches.
+template <int DT, int NV>
+struct RawCols {
+  using T = typename Elem<DT>::T;
+  uint32_t w[NV * sizeof(T) / 4];
+  __device__ __forceinline__ void load(const T *row, int64_t c0, int64_t d) {
+    constexpr int W = NV * sizeof(T) / 4;
+    if (d >= NV) {
+      struct __attribute__((packed, aligned(sizeof(T)))) Any { uint32_t w[W]; };
+      const Any q = *(const Any *)(row + c0);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = acc[j] * a.scale;
-  if (a.add) {
-    float was[8];
-    load_any<OUT>(o, m, was);
+      for (int j = 0; j < W; ++j) w[j] = q.w[j];
+    } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = was[j] + v[j];
+      for (int j = 0; j < W; ++j) {
+        if constexpr (DT == KSD_F32) w[j] = j < d ? __builtin_bit_cast(uint32_t, row[j]) : 0;
+        else w[j] = (2 * j < d ? row[2 * j] : 0) | (uint32_t)(2 * j + 1 < d ? row[2 * j + 1] : 0) << 16;
+      }
+    }
   }
-  store_any<OUT>(o, m, v);
+  __device__ __forceinline__ float at(int j) const {
+    if constexpr (DT == KSD_F32) {
+      return __builtin_bit_cast(float, w[j]);
+    } else {
+      const uint16_t h = (uint16_t)(w[j / 2] >> (j % 2 * 16));
+      return Elem<DT>::load(&h);
+    }
+  }
+};
+template <int DT, int NV>
+__device__ __forceinline__ void load_cols(const typename Elem<DT>::T *row, int64_t c0, int64_t d, float *v) {
+  RawCols<DT, NV> q;
+  q.load(row, c0, d);
+#pragma unroll
+  for (int j = 0; j < NV; ++j) v[j] = q.at(j);
 }
 
-// Chunk blockIdx.x, columns blockIdx.y * 2048 + 8 tid ..: sums its runs in order. A run that lies in
-// the chunk is finished; the pieces of runs that reach past it go to parts.
+template <int OUT, int NV>
+__device__ __forceinline__ void put_row(const SumArgs &a, uint32_t key, int64_t c, int64_t c0, const float *acc) {
+  typename Elem<OUT>::T *o = (typename Elem<OUT>::T *)a.out + (int64_t)key * a.d;
+  if (c + NV <= a.d) {
+    float v[NV], was[NV];
+    if (a.add) load_cols<OUT, NV>(o, c, a.d, was);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) v[j] = a.add ? was[j] + acc[j] * a.scale : acc[j] * a.scale;
+    if constexpr (OUT == KSD_F32) {
+      struct __attribute__((packed, aligned(4))) Any { float w[NV]; } q;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) q.w[j] = v[j];
+      *(Any *)(o + c) = q;
+    } else {
+      struct __attribute__((packed, aligned(2))) Any { uint16_t w[NV]; } q;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) store_out<OUT>(&q.w[j], 0, v[j]);
+      *(Any *)(o + c) = q;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {  // columns c0 + j, those from c on
+      const int64_t i = c0 + j;
+      if (i >= c && i < a.d) store_out<OUT>(o, i, a.add ? Elem<OUT>::load(o + i) + acc[j] * a.scale : acc[j] * a.scale);
+    }
+  }
+}
+
+template <int NV>
+__device__ __forceinline__ void put_part(float *o, int64_t c, int64_t c0, int64_t d, const float *acc) {
+  if (c + NV <= d) {
+    struct __attribute__((packed, aligned(4))) Any { float w[NV]; } q;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) q.w[j] = acc[j];
+    *(Any *)(o + c) = q;
+  } else {
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if (c0 + j >= c && c0 + j < d) o[c0 + j] = acc[j];
+  }
+}
+
+// Clears the rows [v0, v0 + kGap) of `out` below `rows` whose token does not occur: lane i looks row v0 + i up
+// in the sorted keys.
+constexpr int kGap = 16;
+template <int OUT>
+__device__ __forceinline__ void fill_gaps(const SumArgs &a, int64_t v0) {
+  using T = typename Elem<OUT>::T;
+  const int lane = threadIdx.x & 63;
+  const int64_t v = v0 + (lane & (kGap - 1));
+  int lo = 0, hi = a.n;  // first key >= v
+  while (lo < hi) {
+    const int mid = lo + ((hi - lo) >> 1);
+    if ((int64_t)a.keys[mid] < v) lo = mid + 1;
+    else hi = mid;
+  }
+  const uint64_t there = __ballot(lo < a.n && a.keys[min(lo, a.n - 1)] == (uint32_t)v);
+  typedef uint32_t vec __attribute__((ext_vector_type(4), aligned(2)));
+  constexpr int NV = 16 / sizeof(T);
+  for (int r = threadIdx.x >> 6; r < kGap && v0 + r < a.rows; r += 4) {  // a row per wave
+    if (there >> r & 1) continue;
+    T *o = (T *)a.out + (v0 + r) * a.d;
+#pragma unroll 4
+    for (int64_t c = lane * NV; c < a.d; c += 64 * NV) {
+      if (c + NV <= a.d) {
+        __builtin_nontemporal_store((vec){0, 0, 0, 0}, (vec *)(o + c));
+      } else {
+        for (int64_t j = c; j < a.d; ++j) o[j] = (T)0;
+      }
+    }
+  }
+}
+
+// One wave per chunk and slice of 64 NV columns: sums the chunk's runs in order, 8 rows in flight. A run
+// that lies in the chunk is finished; the pieces of runs that reach past it go to parts. Workgroups past
+// `sums` clear the rows without a token meanwhile, so every row of `out` is written once.
 template <int DT, int OUT>
 __global__ __launch_bounds__(256) void sum_kernel(const SumArgs a) {
   using T = typename Elem<DT>::T;
-  const int64_t c = ((int64_t)blockIdx.y * 256 + threadIdx.x) * 8;
-  if (c >= a.d) return;
-  const int m = (int)min((int64_t)8, a.d - c);
-  const int b = blockIdx.x, s0 = b * kRun, s1 = min(a.n, s0 + kRun);
-  const T *g = (const T *)a.g + c;
+  constexpr int NV = DT == KSD_F32 ? 4 : 8;
+  if (blockIdx.x >= a.sums) {
+    fill_gaps<OUT>(a, (int64_t)(blockIdx.x - a.sums) * kGap);
+    return;
+  }
+  const int64_t id = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int b = (int)(id / a.slices), slice = (int)(id % a.slices);
+  if (b >= a.chunks) return;
+  const int64_t c = ((int64_t)slice * 64 + (threadIdx.x & 63)) * NV, c0 = max((int64_t)0, min(c, a.d - NV));
+  const int s0 = b * a.run, s1 = min(a.n, s0 + a.run);
+  const T *g = (const T *)a.g;
   uint32_t key = a.keys[s0];
   bool whole = b == 0 || a.keys[s0 - 1] != key;  // the run begins in this chunk
-  float acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  auto part = [&](int which) {
-    float *o = a.parts + ((int64_t)which * a.chunks + b) * a.d + c;
-    store_any<KSD_F32>(o, m, acc);
-  };
-  for (int s = s0; s < s1; ++s) {
-    const uint32_t k = a.keys[s];
-    if (k != key) {
-      if (whole) put_row<OUT>(a, key, c, m, acc);
-      else part(0);
+  float acc[NV];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) acc[j] = 0.0f;
-      key = k;
-      whole = true;
+  for (int j = 0; j < NV; ++j) acc[j] = 0.0f;
+  for (int sb = s0; sb < s1; sb += 8) {
+    uint32_t k[8];
+    RawCols<DT, NV> v[8];
+    const T *row[8];
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      const int i = min(sb + r, s1 - 1);
+      k[r] = a.keys[i];
+      row[r] = g + (int64_t)a.pos[i] * a.stride;
     }
-    if (k >= a.V) return;  // ids that take no part sort last
-    float v[8];
-    load_any<DT>(g + (int64_t)a.pos[s] * a.stride, m, v);
+    if (k[0] >= a.V) break;  // ids that take no part sort last
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] += v[j];
+    for (int r = 0; r < 8; ++r) v[r].load(row[r], c0, a.d);
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      if (sb + r >= s1 || k[r] >= a.V) continue;
+      if (k[r] != key) {
+        if (whole) put_row<OUT, NV>(a, key, c, c0, acc);
+        else put_part<NV>(a.parts + (int64_t)b * a.d, c, c0, a.d, acc);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) acc[j] = 0.0f;
+        key = k[r];
+        whole = true;
+      }
+#pragma unroll
+      for (int j = 0; j < NV; ++j) acc[j] += v[r].at(j);
+    }
   }
-  if (!whole) part(0);
-  else if (s1 < a.n && a.keys[s1] == key) part(1);
-  else put_row<OUT>(a, key, c, m, acc);
+  if (key >= a.V) return;
+  if (!whole) put_part<NV>(a.parts + (int64_t)b * a.d, c, c0, a.d, acc);
+  else if (s1 < a.n && a.keys[s1] == key) put_part<NV>(a.parts + ((int64_t)a.chunks + b) * a.d, c, c0, a.d, acc);
+  else put_row<OUT, NV>(a, key, c, c0, acc);
 }
 
-// Joins the pieces of the run that begins in chunk blockIdx.x and reaches past it.
+// Joins the pieces of runs that reach past the chunk they begin in: workgroup x looks at chunks 4 x .. 4 x + 3,
+// 256 columns each. The lanes find a run's last chunk 64 at a time; each of the 4 waves adds an equal share of
+// the pieces in order, the waves' sums are added in order.
 template <int OUT>
 __global__ __launch_bounds__(256) void join_kernel(const SumArgs a) {
-  const int64_t c = ((int64_t)blockIdx.y * 256 + threadIdx.x) * 8;
-  const int b = blockIdx.x, s0 = b * kRun, s1 = s0 + kRun;
-  if (c >= a.d || s1 >= a.n) return;
-  const uint32_t key = a.keys[s1 - 1];
-  if (key >= a.V || a.keys[s1] != key) return;
-  if (a.keys[s0] == key && b > 0 && a.keys[s0 - 1] == key) return;  // it began earlier
-  const int m = (int)min((int64_t)8, a.d - c);
-  float acc[8], v[8];
-  load_any<KSD_F32>(a.parts + ((int64_t)a.chunks + b) * a.d + c, m, acc);
-  for (int q = b + 1; q < a.chunks && a.keys[q * kRun] == key; ++q) {
-    load_any<KSD_F32>(a.parts + (int64_t)q * a.d + c, m, v);
+  __shared__ float part[4][64][4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t key[4];
+  bool begins[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] += v[j];
+  for (int i = 0; i < 4; ++i) {
+    const int b = (int)blockIdx.x * 4 + i, s0 = min(b, a.chunks - 1) * a.run, s1 = min(s0 + a.run, a.n - 1);
+    key[i] = a.keys[s1 - 1 > s0 ? s1 - 1 : s0];
+    begins[i] = b < a.chunks && b * a.run + a.run < a.n && key[i] < a.V && a.keys[s1] == key[i] &&
+                !(a.keys[s0] == key[i] && b > 0 && a.keys[s0 - 1] == key[i]);
   }
-  put_row<OUT>(a, key, c, m, acc);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (!begins[i]) continue;
+    const int b = (int)blockIdx.x * 4 + i;
+    int last = b + 1;  // chunks b + 1 .. last - 1 begin with the key
+    while (true) {
+      const int q = last + lane;
+      const uint64_t hit = __ballot(q < a.chunks && a.keys[(int64_t)min(q, a.chunks - 1) * a.run] == key[i]);
+      const int more = hit == ~0ull ? 64 : __builtin_ctzll(~hit);
+      last += more;
+      if (more < 64) break;
+    }
+    const int m = last - b;  // pieces: the one that b ends in, then the beginnings of b + 1 .. last - 1
+    const int64_t c = ((int64_t)blockIdx.y * 64 + lane) * 4, c0 = max((int64_t)0, min(c, a.d - 4));
+    float acc[4] = {0, 0, 0, 0};
+    const int lo = (int)((int64_t)m * wave / 4), hi = (int)((int64_t)m * (wave + 1) / 4);
+#pragma unroll 8
+    for (int q = lo; q < hi; ++q) {
+      float v[4];
+      load_cols<KSD_F32, 4>(a.parts + (q == 0 ? (int64_t)a.chunks + b : (int64_t)b + q) * a.d, c0, a.d, v);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[j] += v[j];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) part[wave][lane][j] = acc[j];
+    __syncthreads();
+    if (wave == 0) {
+      for (int w = 1; w < 4; ++w)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[j] += part[w][lane][j];
+      put_row<OUT, 4>(a, key[i], c, c0, acc);
+    }
+  }
 }
 
-__global__ __launch_bounds__(256) void fill_kernel(uint4 *p, int64_t n16, char *tail, int ntail) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n16; i += (int64_t)gridDim.x * 256)
-    p[i] = make_uint4(0, 0, 0, 0);
-  if (blockIdx.x == 0 && (int)threadIdx.x < ntail) tail[threadIdx.x] = 0;
-}
+__global__ __launch_bounds__(256) void fill_kernel(const Fill f) { fill(f, blockIdx.x); }
 
-static int passes(int64_t V) {
-  int bits = 1;
-  while (bits < 32 && (V >> bits)) ++bits;
-  return (bits + 7) / 8;
+// Bytes whose clearing takes longer than the one-workgroup sort of NT = 256.
+constexpr int64_t kLongFill = 256 << 20;
+// Rounds of a tile: short tiles spread few keys over the CUs, long ones keep the tiles few whose counts every
+// workgroup adds up.
+static int rounds_of(int64_t n) { return n <= 131072 ? 4 : 16; }
+
+static void digits(int64_t V, int &passes, int &bits) {  // keys are 0 .. V
+  int all = 1;
+  while (all < 32 && (V >> all)) ++all;
+  passes = (all + 8) / 9;
+  bits = (all + passes - 1) / passes;
 }
+// Short chunks where few rows would leave CUs idle.
+static int run_of(int64_t n) { return n <= 16384 ? 16 : 32; }
 
 struct Layout {
   int64_t keys[2], pos[2], counts, parts, bytes;
@@ -307,8 +598,8 @@ static Layout layout(int64_t n, int64_t d) {
     return r;
   };
   for (int i = 0; i < 2; ++i) l.keys[i] = take(n * 4), l.pos[i] = take(n * 4);
-  l.counts = take(cdiv(n, kTile) * 256 * 4);
-  l.parts = take(2 * cdiv(n, kRun) * d * 4);
+  l.counts = take(cdiv(n, 256 * rounds_of(n)) * kDigits * 4);
+  l.parts = take(2 * cdiv(n, run_of(n)) * d * 4);
   l.bytes = at;
   return l;
 }
@@ -321,10 +612,10 @@ static void launch_lookup(int out, unsigned g, const void *t, const void *ids, i
   else lookup_kernel<DT, KSD_F16><<<g, 256, 0, st>>>(t, ids, wide, n, V, d, stride, scale, y);
 }
 template <int DT, int OUT>
-static void launch_sums(const SumArgs &a, hipStream_t st) {
-  const dim3 g((unsigned)a.chunks, (unsigned)cdiv(a.d, 2048));
-  sum_kernel<DT, OUT><<<g, 256, 0, st>>>(a);
-  if (a.chunks > 1) join_kernel<OUT><<<g, 256, 0, st>>>(a);
+static void launch_sums(SumArgs a, hipStream_t st) {
+  a.sums = (unsigned)cdiv((int64_t)a.chunks * a.slices, 4);
+  sum_kernel<DT, OUT><<<a.sums + (unsigned)cdiv(a.rows, kGap), 256, 0, st>>>(a);
+  if (a.chunks > 1) join_kernel<OUT><<<dim3((unsigned)cdiv(a.chunks, 4), (unsigned)cdiv(a.d, 256)), 256, 0, st>>>(a);
 }
 
 static bool float_type(int t) { return t == KSD_F32 || t == KSD_BF16 || t == KSD_F16; }
@@ -365,38 +656,63 @@ extern "C" int ksd_embedding_gradient(const void *g, int g_dtype, int64_t n, int
   if (n < 0 || V < 0 || d < 0 || (n > 0 && stride < d)) return fail(KSD_EINVAL, "embedding_gradient: bad shape");
   if (!emb::float_type(g_dtype) || !emb::float_type(out_dtype))
     return fail(KSD_ETYPE, "embedding_gradient: unsupported element type");
-  if (n > 0x7fffffff - emb::kTile || V > 0x7ffffffe) return fail(KSD_EINVAL, "embedding_gradient: more than 2^31 ids or rows");
+  if (n > 0x7fffffff - 65536 || V > 0x7ffffffe) return fail(KSD_EINVAL, "embedding_gradient: more than 2^31 ids or rows");
   if (V == 0 || d == 0) return KSD_OK;
   if (!out) return fail(KSD_EINVAL, "embedding_gradient: null pointer");
   if (((uintptr_t)out) % 16) return fail(KSD_EINVAL, "embedding_gradient: out must be 16-byte aligned");
-  if (cdiv(d, 2048) > 65535) return fail(KSD_EINVAL, "embedding_gradient: rows too long");
+  if (cdiv(d, 256) > 65535) return fail(KSD_EINVAL, "embedding_gradient: rows too long");
   const emb::Layout l = emb::layout(n, d);
   if (n > 0 && (!g || !ids || !workspace || workspace_bytes < l.bytes))
     return fail(KSD_EINVAL, "embedding_gradient: null pointer or short workspace");
+  const int run = emb::run_of(n), vec = g_dtype == KSD_F32 ? 4 : 8, es = out_dtype == KSD_F32 ? 4 : 2;
+  const int64_t chunks = cdiv(n, run), slices = cdiv(d, 64 * vec);
+  if (!grid_fits(cdiv(chunks * slices, 4) + cdiv(V, emb::kGap), 256)) return fail(KSD_EINVAL, "embedding_gradient: too many ids");
   hipStream_t st = (hipStream_t)stream;
-  if (!accumulate) {
-    const int64_t bytes = V * d * (out_dtype == KSD_F32 ? 4 : 2), n16 = bytes / 16;
-    emb::fill_kernel<<<(unsigned)std::max<int64_t>(1, std::min<int64_t>(cdiv(n16, 256 * 8), 1 << 20)), 256, 0, st>>>(
-        (uint4 *)out, n16, (char *)out + n16 * 16, (int)(bytes % 16));
+  const emb::Fill f{(char *)out, V * d * es};
+  const bool fits = grid_fits(emb::fill_blocks(f) + 1, 256);
+  if (n == 0) {
+    if (accumulate) return KSD_OK;
+    if (!fits) return fail(KSD_EINVAL, "embedding_gradient: table too large");
+    emb::fill_kernel<<<(unsigned)emb::fill_blocks(f), 256, 0, st>>>(f);
+    return check_launch("embedding_gradient");
   }
-  if (n == 0) return check_launch("embedding_gradient");
   char *w = (char *)workspace;
   emb::SortArgs s{};
-  s.counts = (uint32_t *)(w + l.counts);
-  s.V = V, s.pad = padding, s.n = (int)n, s.tiles = (int)cdiv(n, emb::kTile), s.wide = ids_wide;
-  int at = 0;
-  for (int p = 0; p < emb::passes(V); ++p, at ^= 1) {
-    s.ids = p == 0 ? ids : nullptr;
-    s.keys = (uint32_t *)(w + l.keys[at ^ 1]), s.pos = (int32_t *)(w + l.pos[at ^ 1]);
-    s.out_keys = (uint32_t *)(w + l.keys[at]), s.out_pos = (int32_t *)(w + l.pos[at]);
-    s.shift = p * 8;
-    emb::sort_count_kernel<<<s.tiles, 256, 0, st>>>(s);
-    emb::sort_scan_kernel<<<1, 1024, 0, st>>>(s.counts, s.tiles * 256);
-    emb::sort_scatter_kernel<<<s.tiles, 256, 0, st>>>(s);
+  int passes, at = 0;
+  emb::digits(V, passes, s.bits);
+  s.ids = ids, s.V = V, s.pad = padding, s.n = (int)n, s.wide = ids_wide;
+  int64_t rows = accumulate ? 0 : V;  // rows that the sums' launch clears where no token occurs
+  if (n <= emb::kOne) {
+    s.out_keys = (uint32_t *)(w + l.keys[0]), s.out_pos = (int32_t *)(w + l.pos[0]);
+    uint32_t *keys2 = (uint32_t *)(w + l.keys[1]);
+    int32_t *pos2 = (int32_t *)(w + l.pos[1]);
+    if (!accumulate && f.n >= emb::kLongFill && fits) {
+      rows = 0;
+      emb::sort_one_kernel<256><<<(unsigned)(1 + emb::fill_blocks(f)), 256, 0, st>>>(s, passes, keys2, pos2, f);
+    } else {
+      emb::sort_one_kernel<1024><<<1, 1024, 0, st>>>(s, passes, keys2, pos2, f);
+    }
+  } else {
+    const int rounds = emb::rounds_of(n);
+    s.counts = (uint32_t *)(w + l.counts);
+    s.tiles = (int)cdiv(n, 256 * rounds);
+    for (int p = 0; p < passes; ++p, at ^= 1) {
+      if (p > 0) s.ids = nullptr;
+      s.keys = (uint32_t *)(w + l.keys[at ^ 1]), s.pos = (int32_t *)(w + l.pos[at ^ 1]);
+      s.out_keys = (uint32_t *)(w + l.keys[at]), s.out_pos = (int32_t *)(w + l.pos[at]);
+      s.shift = p * s.bits;
+      if (rounds == 4) {
+        emb::sort_count_kernel<4><<<s.tiles, 256, 0, st>>>(s);
+        emb::sort_scatter_kernel<4><<<s.tiles, 256, 0, st>>>(s);
+      } else {
+        emb::sort_count_kernel<16><<<s.tiles, 256, 0, st>>>(s);
+        emb::sort_scatter_kernel<16><<<s.tiles, 256, 0, st>>>(s);
+      }
+    }
+    at ^= 1;  // the last pass's output
   }
-  at ^= 1;  // the last pass's output
-  emb::SumArgs a{(uint32_t *)(w + l.keys[at]), (int32_t *)(w + l.pos[at]), g, out, (float *)(w + l.parts), d, stride, V,
-                 (int)n, (int)cdiv(n, emb::kRun), accumulate, scale};
+  emb::SumArgs a{(uint32_t *)(w + l.keys[at]), (int32_t *)(w + l.pos[at]), g, out, (float *)(w + l.parts), d, stride, V, rows,
+                 (int)n, (int)chunks, run, (int)slices, accumulate, 0, scale};
 #define KSD_SUMS(DT)                                                        \
   if (out_dtype == KSD_F32) emb::launch_sums<DT, KSD_F32>(a, st);           \
   else if (out_dtype == KSD_BF16) emb::launch_sums<DT, KSD_BF16>(a, st);    \

@@ -12,14 +12,15 @@ from __future__ import annotations
 
 import ctypes
 import math
+from array import array
+from operator import attrgetter
 
-import numpy as np
 import torch
 
 from .. import _lib
 
-# KsdClipTensor of the C ABI
-_TENSOR = np.dtype([("grad", "<u8"), ("out", "<u8"), ("n", "<i8"), ("dtype", "<i4"), ("reserved", "<i4")])
+_T = torch.Tensor
+_dtype_of = attrgetter("dtype")
 _CODE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 
 
@@ -32,34 +33,46 @@ def _check(grads, out, norm_type, loss_scale):
         raise ValueError(f"{len(grads)} gradients, {len(out)} outputs")
 
 
-def _table(grads, out):
-    """The tensors' descriptors (a host array) and their device."""
-    dev = _lib.require_gpu(*grads, *(out or ()))
-    rows = []
-    for i, g in enumerate(grads):
-        if g.is_sparse or not g.is_contiguous():
-            raise ValueError(f"gradient {i} is not dense and contiguous")
-        code = _CODE.get(g.dtype)
-        if code is None:
-            raise TypeError(f"gradient {i}: unsupported dtype {g.dtype}")
-        p = g.data_ptr()
-        if out is None:
-            rows.append((p, p, g.numel(), code, 0))
-            continue
-        o = out[i]
-        if o.shape != g.shape or o.dtype != g.dtype or not o.is_contiguous():
-            raise ValueError(f"output {i} must be contiguous {tuple(g.shape)} {g.dtype}")
-        rows.append((p, o.data_ptr(), g.numel(), code, 0))
-    return np.array(rows, dtype=_TENSOR), dev
+class _Table:
+    """The tensors as the C ABI takes them: host arrays of addresses, sizes and types. Built by a few
+    passes in C over the list (a model has hundreds of gradients, and the call's own cost is this)."""
+
+    def __init__(self, grads, out):
+        devices = set(map(_T.get_device, grads))
+        if out is not None:
+            devices |= set(map(_T.get_device, out))
+        if len(devices) > 1 or -1 in devices:
+            _lib.require_gpu(*grads, *(out or ()))
+        if not all(map(_T.is_contiguous, grads)):  # False for sparse tensors too
+            raise ValueError("a gradient is not dense and contiguous")
+        dtypes = list(map(_dtype_of, grads))
+        try:
+            codes = list(map(_CODE.__getitem__, dtypes))
+        except KeyError as e:
+            raise TypeError(f"unsupported gradient dtype {e.args[0]}") from None
+        sizes = list(map(_T.numel, grads))
+        if out is not None and (list(map(_dtype_of, out)) != dtypes or list(map(_T.numel, out)) != sizes
+                                or not all(map(_T.is_contiguous, out))):
+            raise ValueError("outputs must be contiguous and of their gradients' sizes and dtypes")
+        self.n = len(grads)
+        self.dev = grads[0].device
+        self.grads = array("Q", map(_T.data_ptr, grads))
+        self.outs = self.grads if out is None else array("Q", map(_T.data_ptr, out))
+        self.sizes = array("q", sizes)
+        self.types = array("i", codes)
 
 
-def _norm(table, dev, norm_type, max_norm, loss_scale):
+def _at(a: array) -> int:
+    return a.buffer_info()[0]
+
+
+def _norm(t: _Table, norm_type, max_norm, loss_scale):
     need = ctypes.c_int64()
-    _lib.call("ksd_grad_norm_workspace", table.ctypes.data, len(table), ctypes.byref(need))
-    work = torch.empty(need.value, dtype=torch.int8, device=dev)
-    res = torch.empty(2, dtype=torch.float32, device=dev)
-    _lib.call("ksd_grad_norm", table.ctypes.data, len(table), int(norm_type == math.inf), max_norm, loss_scale,
-              res.data_ptr(), res.data_ptr() + 4, work.data_ptr(), need.value, _lib.stream_ptr(dev))
+    _lib.call("ksd_grad_norm_workspace", _at(t.sizes), t.n, ctypes.byref(need))
+    work = torch.empty(need.value, dtype=torch.int8, device=t.dev)
+    res = torch.empty(2, dtype=torch.float32, device=t.dev)
+    _lib.call("ksd_grad_norm", _at(t.grads), _at(t.sizes), _at(t.types), t.n, int(norm_type == math.inf), max_norm,
+              loss_scale, res.data_ptr(), res.data_ptr() + 4, work.data_ptr(), need.value, _lib.stream_ptr(t.dev))
     return res
 
 
@@ -70,22 +83,22 @@ def gradient_norm(grads, max_norm: float = math.inf, norm_type: float = 2.0, los
     _check(grads, None, norm_type, loss_scale)
     if not grads:
         raise ValueError("no gradients")
-    table, dev = _table(grads, None)
-    res = _norm(table, dev, norm_type, max_norm, loss_scale)
+    res = _norm(_Table(grads, None), norm_type, max_norm, loss_scale)
     return res[0], res[1:]
 
 
 def clip_gradients(grads, max_norm: float, norm_type: float = 2.0, out=None, loss_scale: float = 1.0) -> torch.Tensor:
-    """Multiplies every gradient by the factor above, in place or into ``out`` (tensors of the same
-    shapes and dtypes), and returns the norm (0-d, on the device)."""
+    """Multiplies every gradient by the factor above, in place or into ``out`` (contiguous tensors of the
+    same sizes and dtypes), and returns the norm (0-d, on the device)."""
     grads = list(grads)
     out = None if out is None else list(out)
     _check(grads, out, norm_type, loss_scale)
     if not grads:
         raise ValueError("no gradients")
-    table, dev = _table(grads, out)
-    res = _norm(table, dev, norm_type, max_norm, loss_scale)
-    _lib.call("ksd_grad_scale", table.ctypes.data, len(table), res.data_ptr() + 4, _lib.stream_ptr(dev))
+    t = _Table(grads, out)
+    res = _norm(t, norm_type, max_norm, loss_scale)
+    _lib.call("ksd_grad_scale", _at(t.grads), _at(t.outs), _at(t.sizes), _at(t.types), t.n, res.data_ptr() + 4,
+              _lib.stream_ptr(t.dev))
     return res[0]
 
 
