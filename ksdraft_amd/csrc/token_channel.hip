@@ -174,27 +174,32 @@ static void launch_rows(const Rows &a, int t, hipStream_t st) {
 // them; the second writes both codes. (8192 x 1536 bf16: MEASURED_STATS us, MEASURED_FOLD us and MEASURED_CODES us.)
 // A wave takes `rows` (a multiple of 16) x 64 V columns: lane l holds columns V l .. V l + V - 1, 16 rows'
 // loads in flight. A row's maximum crosses the lanes through LDS, 16 rows at once.
-template <int DT> constexpr int kVec = DT == KSD_F32 ? 4 : 8;  // 16 bytes
-
-template <int DT>
-__device__ __forceinline__ void load16(const typename Elem<DT>::T *p, float *v) {
-  if constexpr (DT == KSD_F32) {
+template <int DT, int V>
+__device__ __forceinline__ void load_vec(const typename Elem<DT>::T *p, float *v) {
+  if constexpr (V == 8) {
+    load8<DT>(p, v);
+  } else if constexpr (DT == KSD_F32) {
     struct __attribute__((packed, aligned(4))) Any { float w[4]; };
     const Any q = *(const Any *)p;
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = q.w[j];
   } else {
-    load8<DT>(p, v);
+    struct __attribute__((packed, aligned(2))) Any { uint32_t w[2]; };
+    const Any q = *(const Any *)p;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint16_t h = (uint16_t)(q.w[j / 2] >> (j % 2 * 16));
+      v[j] = Elem<DT>::load(&h);
+    }
   }
 }
 
-template <int DT>
+template <int DT, int V>
 __global__ __launch_bounds__(256) void grad_stats_kernel(const void *__restrict__ g, int64_t M, int64_t N, int64_t stride, int rows,
                                                          const float *__restrict__ sx, const float *__restrict__ sw,
                                                          uint32_t *__restrict__ row_part, uint32_t *__restrict__ col_part,
                                                          float *__restrict__ sum_part) {
   using T = typename Elem<DT>::T;
-  constexpr int V = kVec<DT>;
   __shared__ uint32_t rmax_all[4][16][65];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   uint32_t(*const rmax)[65] = rmax_all[wave];
@@ -214,7 +219,7 @@ __global__ __launch_bounds__(256) void grad_stats_kernel(const void *__restrict_
     float v[16][V], s[16];
     if (cols && mb + 16 <= m1) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) load16<DT>((const T *)g + (mb + r) * stride + c, v[r]);
+      for (int r = 0; r < 16; ++r) load_vec<DT, V>((const T *)g + (mb + r) * stride + c, v[r]);
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = sx[mb + r];
     } else {
@@ -271,7 +276,7 @@ __global__ __launch_bounds__(1024) void grad_fold_kernel(const uint32_t *__restr
   uint32_t top = 0;
   float sum = 0.0f;
   if (i < L) {
-#pragma unroll 4
+#pragma unroll 8
     for (int b = wave; b < n; b += 16) {
       top = max(top, part[(int64_t)b * L + i]);
       if (add) sum += sum_part[(int64_t)b * L + i];
@@ -294,16 +299,16 @@ __global__ __launch_bounds__(1024) void grad_fold_kernel(const uint32_t *__restr
 }
 
 // Both codes of dY, in its own layout: q (rows, for dX) and c (columns, for dW), rows of ld bytes with zeros
-// past N. A thread holds 8 columns over 16 rows, 8 of them in flight. A row or column whose scale is NaN
+// past N. A thread holds 8 columns over 8 H rows, 8 of them in flight. A row or column whose scale is NaN
 // has codes of no meaning: its products are NaN through the scale.
-template <int DT>
+template <int DT, int H>
 __global__ __launch_bounds__(256) void grad_codes_kernel(const void *__restrict__ g, int64_t M, int64_t N, int64_t stride,
                                                          const float *__restrict__ sx, const float *__restrict__ sw,
                                                          const float *__restrict__ einv, const float *__restrict__ finv,
                                                          int8_t *__restrict__ q, int8_t *__restrict__ cq, int64_t ld) {
   using T = typename Elem<DT>::T;
   const int64_t c = ((int64_t)blockIdx.x * 64 + (threadIdx.x & 63)) * 8;
-  const int64_t m0 = (int64_t)blockIdx.y * 64 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 16;
+  const int64_t m0 = (int64_t)blockIdx.y * (32 * H) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * (8 * H);
   if (c >= ld) return;
   const bool cols = (int64_t)(blockIdx.x + 1) * 512 <= N;
   float w[8], fi[8];
@@ -313,7 +318,7 @@ __global__ __launch_bounds__(256) void grad_codes_kernel(const void *__restrict_
     fi[j] = c + j < N ? finv[c + j] : 0.0f;
   }
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
+  for (int h = 0; h < H; ++h) {
     float v[8][8];
     if (cols && m0 + h * 8 + 8 <= M) {
 #pragma unroll
@@ -347,8 +352,10 @@ __global__ __launch_bounds__(256) void grad_codes_kernel(const void *__restrict_
   }
 }
 
-// Rows of a stats workgroup: 32, 64 where that still leaves every CU several (the parts halve).
-static int stats_rows(int64_t M, int64_t N) { return M * N >= (int64_t)1 << 25 ? 64 : 32; }
+// A large dY is read in pieces of 16 bytes, 64 rows to a wave, which halves the partial results; a small one in
+// pieces of 4 elements, 32 rows to a wave (and 8, not 16, in the second read), for more waves.
+static bool large_grad(int64_t M, int64_t N) { return M * N >= (int64_t)1 << 25; }
+static int stats_rows(int64_t M, int64_t N) { return large_grad(M, N) ? 64 : 32; }
 
 // ------------------------------------------------------------------------------------ product
 // One operand of the product. Plain ("N"): (rows, K) with the reduction contiguous; "T": (K, rows)
@@ -362,6 +369,7 @@ struct Prob {
   int32_t *parts;  // splits > 1: (splits, M, N) int32 sums
   int64_t lda, ldw;
   int M, N, K, splits, ksteps;  // ksteps: steps of 128 of one split
+  int nt;                       // non-temporal stores
 };
 
 constexpr int BK = 128;
@@ -380,7 +388,7 @@ template <bool T, int B>
 __device__ __forceinline__ constexpr int lds_swz(int r) {
   if constexpr (!T) return (r >> 1) & 7;
   else if constexpr (B == 256) return (r & 7) | ((r >> 1) & 8);
-  else if constexpr (B == 192) return ((r >> 2) & 1) | ((r >> 3) & 2);
+  else if constexpr (B == 192 || B == 64) return ((r >> 2) & 1) | ((r >> 3) & 2);
   else return ((r >> 1) & 3) | ((r >> 2) & 4);
 }
 template <bool T, int B>
@@ -513,15 +521,17 @@ __device__ __forceinline__ void loadv(const void *p, int64_t i, float *v) {
     }
   }
 }
-// Non-temporal: the streamed output does not push the operands' panels out of L2.
-template <int OUT, int W>
+// nt: non-temporal, so that a streamed output does not push the operands' panels out of L2.
+template <int OUT, int W, bool nt>
 __device__ __forceinline__ void storev(void *p, int64_t i, const float *v) {
   if constexpr (OUT == KSD_F32) {
     typedef float vec __attribute__((ext_vector_type(W), aligned(4)));
     vec a;
 #pragma unroll
     for (int j = 0; j < W; ++j) a[j] = v[j];
-    __builtin_nontemporal_store(a, (vec *)((float *)p + i));
+    vec *const q = (vec *)((float *)p + i);
+    if constexpr (nt) __builtin_nontemporal_store(a, q);
+    else *q = a;
   } else {
     typedef uint32_t vec __attribute__((ext_vector_type(W / 2), aligned(2)));
     vec a;
@@ -535,7 +545,9 @@ __device__ __forceinline__ void storev(void *p, int64_t i, const float *v) {
         a[j] = f16_bits(v[2 * j]) | (uint32_t)f16_bits(v[2 * j + 1]) << 16;
       }
     }
-    __builtin_nontemporal_store(a, (vec *)((uint16_t *)p + i));
+    vec *const q = (vec *)((uint16_t *)p + i);
+    if constexpr (nt) __builtin_nontemporal_store(a, q);
+    else *q = a;
   }
 }
 
@@ -546,16 +558,16 @@ __device__ __forceinline__ void wg_barrier() {
 }
 
 // BM x BN tiles, WM x WN waves; TA, TW: the operand is a T one. Persistent: a workgroup walks its
-// units (tile, part of the reduction); the DMA runs one step of 128 ahead across unit ends.
-// Per step each wave multiplies the first half (64) of the step while it reads the fragments of the
-// second, then one barrier, then the second half while it reads the next step's first.
-template <int BM, int BN, int WM, int WN, bool TA, bool TW, int OUT>
-__global__ __launch_bounds__(WM *WN * 64, WM * WN == 8 ? 1 : 2) void gemm_kernel(const Prob p) {
+// units (tile, part of the reduction) through a ring of S LDS slots of 128 reduction steps each, filled by DMA
+// up to S steps ahead, across unit ends. Per step each wave multiplies the first half (64) of the step while it
+// reads the fragments of the second, then one barrier, then the second half while it reads the next step's first.
+template <int BM, int BN, int WM, int WN, int S, bool TA, bool TW, int OUT>
+__global__ __launch_bounds__(WM *WN * 64, WM *WN == 8 ? 1 : 2) void gemm_kernel(const Prob p) {
   constexpr int NW = WM * WN, NI = BM / WM / 16, NJ = BN / WN / 16;
   constexpr int PERM = TW ? 0 : NJ;
-  constexpr uint32_t SA = BM * BK, SW = BN * BK;
-  extern __shared__ __attribute__((aligned(1024))) int8_t smem[];  // A slots 0, 1, then W slots 0, 1
-  const uint32_t ldsA = lds_addr(smem), ldsW = ldsA + 2 * SA;
+  constexpr uint32_t SA = BM * BK, SLOT = (BM + BN) * BK;
+  extern __shared__ __attribute__((aligned(1024))) int8_t smem[];  // S slots of an A and a W tile
+  const uint32_t lds0 = lds_addr(smem);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WN, wn = wave % WN;
   const int tm = (p.M + BM - 1) / BM, tn = (p.N + BN - 1) / BN, units = tm * tn * p.splits;
@@ -602,45 +614,57 @@ __global__ __launch_bounds__(WM *WN * 64, WM * WN == 8 ? 1 : 2) void gemm_kernel
     }
   };
   is_start();
-  auto stage_all = [&](int slot) __attribute__((always_inline)) {
+  constexpr int DA = Stage<TA, BM, NW, 0>::D, DT = DA + Stage<TW, BN, NW, PERM>::D;
+  auto open = [&]() __attribute__((always_inline)) {
     a.open(is_u < u_end);
     w.open(is_u < u_end);
-#pragma unroll
-    for (int i = 0; i < a.D; ++i) a.issue(i, ldsA + slot * SA, wave, lane);
-#pragma unroll
-    for (int i = 0; i < w.D; ++i) w.issue(i, ldsW + slot * SW, wave, lane);
-    is_next();
+  };
+  auto issue = [&](int d, uint32_t slot) __attribute__((always_inline)) {
+    if (d < DA) a.issue(d, slot, wave, lane);
+    else w.issue(d - DA, slot + SA, wave, lane);
   };
 
-  // Lane (g, c) = (lane / 16, lane % 16) holds rows 4 g .. 4 g + 3 of each 16 and, with a permuted W, NJ
+  // With a permuted W, lane (g, c) = (lane / 16, lane % 16) holds rows 4 g .. 4 g + 3 of each 16 and NJ
   // consecutive columns from c NJ on: 16 lanes store one contiguous piece of a row. A T operand's columns
-  // are c + 16 j.
+  // cannot be permuted: its product is formed transposed, so that a lane holds row c and columns 4 g .. 4 g + 3
+  // of each 16.
   auto store = [&](const v4i (&acc)[NI][NJ], int v) __attribute__((always_inline)) {
     int m0, n0, part;
     tile_of(v, m0, n0, part);
-    const int c = lane & 15;
-    const int nb = n0 + wn * (BN / WN) + (PERM ? c * NJ : c);
-    const int mb = m0 + wm * (BM / WM) + (lane >> 4) * 4;
-    constexpr int NS = PERM ? 1 : 16;  // from one column to the next
+    const int c = lane & 15, g = lane >> 4;
+    constexpr int RR = PERM ? 4 : 1;       // rows of a lane per i
+    constexpr int CW = PERM ? NJ : 4;      // columns of one store
+    constexpr int CN = PERM ? 1 : NJ;      // stores of a row
+    const int nb = n0 + wn * (BN / WN) + (PERM ? c * NJ : g * 4);
+    const int mb = m0 + wm * (BM / WM) + (PERM ? g * 4 : c);
     const bool full = m0 + BM <= p.M && n0 + BN <= p.N;
+    auto at = [&](int i, int r, int q, int j) __attribute__((always_inline)) {
+      return PERM ? acc[i][j][r] : acc[i][q][j];
+    };
+    // This wave's loads have arrived, the DMA of the next step with them: its wait, which would also
+    // wait for the stores below, is left out (`ahead` in the main loop).
     if (p.splits > 1) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       int32_t *const o = p.parts + ((int64_t)part * p.M + mb) * p.N + nb;
+      typedef int vec __attribute__((ext_vector_type(CW), aligned(4)));
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          int32_t *const q = o + (int64_t)(i * 16 + r) * p.N;
+        for (int r = 0; r < RR; ++r) {
           if (full || mb + i * 16 + r < p.M) {
-            if (PERM && (full || nb + NJ <= p.N)) {
-              struct __attribute__((packed, aligned(4))) Any { int32_t w[NJ]; } t;
 #pragma unroll
-              for (int j = 0; j < NJ; ++j) t.w[j] = acc[i][j][r];
-              *(Any *)q = t;
-            } else {
+            for (int q = 0; q < CN; ++q) {
+              int32_t *const z = o + (int64_t)(i * 16 + r) * p.N + q * 16;
+              if (full || nb + q * 16 + CW <= p.N) {
+                vec t;
 #pragma unroll
-              for (int j = 0; j < NJ; ++j)
-                if (full || nb + j * NS < p.N) q[j * NS] = acc[i][j][r];
+                for (int j = 0; j < CW; ++j) t[j] = at(i, r, q, j);
+                *(vec *)z = t;
+              } else {
+#pragma unroll
+                for (int j = 0; j < CW; ++j)
+                  if (nb + q * 16 + j < p.N) z[j] = at(i, r, q, j);
+              }
             }
           }
         }
@@ -648,70 +672,74 @@ __global__ __launch_bounds__(WM *WN * 64, WM * WN == 8 ? 1 : 2) void gemm_kernel
       }
       return;
     }
-    float sw[NJ], bs[NJ];
+    float sw[CN][CW], bs[CN][CW];
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      const int n = min(nb + j * NS, p.N - 1);
-      sw[j] = p.sw ? p.sw[n] : 1.0f;
-      bs[j] = p.bias ? p.bias[n] : 0.0f;
-    }
-    float sa[NI][4];
+    for (int q = 0; q < CN; ++q)
+#pragma unroll
+      for (int j = 0; j < CW; ++j) {
+        const int n = min(nb + q * 16 + j, p.N - 1);
+        sw[q][j] = p.sw ? p.sw[n] : 1.0f;
+        bs[q][j] = p.bias ? p.bias[n] : 0.0f;
+      }
+    float sa[NI][RR];
 #pragma unroll
     for (int i = 0; i < NI; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) sa[i][r] = p.sa ? p.sa[min(mb + i * 16 + r, p.M - 1)] : 1.0f;
-    // This wave's loads have arrived, the DMA of the next step with them: its wait, which would also
-    // wait for the stores below, is left out (`ahead` in the main loop).
+      for (int r = 0; r < RR; ++r) sa[i][r] = p.sa ? p.sa[min(mb + i * 16 + r, p.M - 1)] : 1.0f;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    auto rows = [&](auto full_c) __attribute__((always_inline)) {
-      constexpr bool whole = decltype(full_c)::value;
+    auto rows = [&](auto full_c, auto nt_c) __attribute__((always_inline)) {
+      constexpr bool whole = decltype(full_c)::value, nt = decltype(nt_c)::value;
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
+        for (int r = 0; r < RR; ++r) {
           if (whole || mb + i * 16 + r < p.M) {
-            const int64_t at = (int64_t)(mb + i * 16 + r) * p.N + nb;
-            float y[NJ];
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) {
-              y[j] = ((float)acc[i][j][r] * sa[i][r]) * sw[j];
-              if (p.bias) y[j] += bs[j];
-            }
-            if (PERM && (whole || nb + NJ <= p.N)) {
-              if (p.R) {
-                float t[NJ];
-                loadv<OUT, NJ>(p.R, at, t);
+            for (int q = 0; q < CN; ++q) {
+              const int64_t to = (int64_t)(mb + i * 16 + r) * p.N + nb + q * 16;
+              float y[CW];
 #pragma unroll
-                for (int j = 0; j < NJ; ++j) y[j] += t[j];
+              for (int j = 0; j < CW; ++j) {
+                y[j] = (float)at(i, r, q, j) * sa[i][r];
+                if (!TW || p.sw) y[j] *= sw[q][j];
+                if (p.bias) y[j] += bs[q][j];
               }
-              storev<OUT, NJ>(p.Y, at, y);
-            } else {
+              if (whole || nb + q * 16 + CW <= p.N) {
+                if (p.R) {
+                  float t[CW];
+                  loadv<OUT, CW>(p.R, to, t);
 #pragma unroll
-              for (int j = 0; j < NJ; ++j)
-                if (whole || nb + j * NS < p.N) {
-                  if (p.R) y[j] += load_out<OUT>(p.R, at + j * NS);
-                  store_out<OUT>(p.Y, at + j * NS, y[j]);
+                  for (int j = 0; j < CW; ++j) y[j] += t[j];
                 }
+                storev<OUT, CW, nt>(p.Y, to, y);
+              } else {
+#pragma unroll
+                for (int j = 0; j < CW; ++j)
+                  if (nb + q * 16 + j < p.N) {
+                    if (p.R) y[j] += load_out<OUT>(p.R, to + j);
+                    store_out<OUT>(p.Y, to + j, y[j]);
+                  }
+              }
             }
           }
         }
         __builtin_amdgcn_sched_barrier(0);
       }
     };
-    if (full) rows(std::true_type());
-    else rows(std::false_type());
+    if (!full) rows(std::false_type(), std::false_type());
+    else if (p.nt) rows(std::true_type(), std::true_type());
+    else rows(std::true_type(), std::false_type());
   };
 
   Reader<TA, BM, NI> ra;
   Reader<TW, BN, NJ> rw;
-  ra.start(ldsA, wm * (BM / WM), lane);
-  rw.start(ldsW, wn * (BN / WN), lane);
+  ra.start(lds0, wm * (BM / WM), lane);
+  rw.start(lds0 + SA, wn * (BN / WN), lane);
   // half b's products, spread between them the reads of the other half and, with DMA, the loads of a
-  // later step into slot dslot
-  auto half = [&](v4i (&acc)[NI][NJ], v4i (&fa)[2][NI], v4i (&fw)[2][NJ], auto b_c, auto dma_c, int dslot) __attribute__((always_inline)) {
+  // later step into `slot`
+  auto half = [&](v4i (&acc)[NI][NJ], v4i (&fa)[2][NI], v4i (&fw)[2][NJ], auto b_c, uint32_t slot) __attribute__((always_inline)) {
     constexpr int b = decltype(b_c)::value;
-    constexpr bool dma = decltype(dma_c)::value;
-    constexpr int DA = Stage<TA, BM, NW, 0>::D, DT = DA + Stage<TW, BN, NW, PERM>::D;
+    constexpr bool dma = b == 1;
 #pragma unroll
     for (int j = 0; j < NJ; ++j) fw[b ^ 1][j] = rw.read(j, b ^ 1);
 #pragma unroll
@@ -719,23 +747,27 @@ __global__ __launch_bounds__(WM *WN * 64, WM * WN == 8 ? 1 : 2) void gemm_kernel
       fa[b ^ 1][i] = ra.read(i, b ^ 1);
       if constexpr (dma) {
 #pragma unroll
-        for (int d = i * DT / NI; d < (i + 1) * DT / NI; ++d) {
-          if (d < DA) a.issue(d, ldsA + dslot * SA, wave, lane);
-          else w.issue(d - DA, ldsW + dslot * SW, wave, lane);
-        }
+        for (int d = i * DT / NI; d < (i + 1) * DT / NI; ++d) issue(d, slot);
       }
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fa[b][i], fw[b][j], acc[i][j], 0, 0, 0);
+      for (int j = 0; j < NJ; ++j)
+        acc[i][j] = PERM ? __builtin_amdgcn_mfma_i32_16x16x64_i8(fa[b][i], fw[b][j], acc[i][j], 0, 0, 0)
+                         : __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[b][j], fa[b][i], acc[i][j], 0, 0, 0);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
 
-  stage_all(0);
-  stage_all(1);
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+  for (int q = 0; q < S; ++q) {
+    open();
+#pragma unroll
+    for (int d = 0; d < DT; ++d) issue(d, lds0 + q * SLOT);
+    is_next();
+  }
+  asm volatile("s_waitcnt vmcnt(%0)" :: "n"((S - 1) * DT) : "memory");
   wg_barrier();
-  int slot = 0;
-  bool ahead = false;
+  uint32_t slot = 0;  // byte offset of the slot that is multiplied
+  int ahead = 0;      // steps whose data is known to have arrived
   for (; u < u_end; u += u_step) {
     v4i acc[NI][NJ];
 #pragma unroll
@@ -749,22 +781,23 @@ __global__ __launch_bounds__(WM *WN * 64, WM * WN == 8 ? 1 : 2) void gemm_kernel
     for (int i = 0; i < NI; ++i) fa[0][i] = ra.read(i, 0);
     const int q0 = (u % p.splits) * p.ksteps;
     for (int left = min(kt, q0 + p.ksteps) - q0; left > 0; --left) {
-      half(acc, fa, fw, std::integral_constant<int, 0>(), std::false_type(), 0);
-      // the next step's data has arrived, and every wave holds this step's second half
-      if (ahead) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-      ahead = false;
+      half(acc, fa, fw, std::integral_constant<int, 0>(), 0);
+      // the next step's data has arrived (the DMA of S - 2 later steps may be under way), and every wave
+      // holds this step's second half
+      if (ahead > 0) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"((S - 2) * DT) : "memory");
+      --ahead;
       wg_barrier();
-      ra.shift(slot ? -SA : SA);
-      rw.shift(slot ? -SW : SW);
-      a.open(is_u < u_end);
-      w.open(is_u < u_end);
-      half(acc, fa, fw, std::integral_constant<int, 1>(), std::true_type(), slot);
+      const uint32_t by = slot == (S - 1) * SLOT ? 0u - (S - 1) * SLOT : SLOT;
+      ra.shift(by);
+      rw.shift(by);
+      open();
+      half(acc, fa, fw, std::integral_constant<int, 1>(), lds0 + slot);
       is_next();
-      slot ^= 1;
+      slot += by;
     }
     store(acc, u);
-    ahead = true;
+    ahead = S - 1;
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no DMA into LDS outlives the workgroup
 }
@@ -810,56 +843,66 @@ static void launch_combine(const Prob &p, hipStream_t st) {
 // int32 sums of |a w| <= 127^2 hold 133144 terms
 constexpr int kMaxSteps = 1024;
 
-// Tile, parts of the reduction, and steps of a part: the least time by a model of a launch (us): rounds of
-// units over the CUs, a step of 128 and a unit's start and end per tile form, and the combine's traffic.
-// The step times are those measured on 8192 x 8192 x 8192 (256 x 256 500 us, 256 x 192 557, 128 x 128 with
-// two workgroups per CU 719).
+// Tile, parts of the reduction, and steps of a part: the least time by a model of a launch (us), 5 + rounds of
+// units over the CUs * (steps * step + unit), and for parts their traffic at 4.5 TB/s and the combine's launch.
+// `step` and `unit` are fitted to measured products (us, best form and its neighbours): 8192^3 256 x 256 480,
+// 256 x 192 547, 128 x 128 614; 8192 x 1536 x 1536 256 x 192 24.7, 256 x 256 26, 128 x 128 30.3; 2047 x 1792
+// x 6869 128 x 128 alone on a CU 38.5, 64 x 128 40.5, two per CU with 2 parts 45.8; 2047 x 1792 x 1792 64 x
+// 128 15.9, 128 x 128 alone 18.1, 64 x 64 19.6; 1021 x 1792 x 597 64 x 64 8.5, 64 x 128 8.7, 128 x 128 11.1;
+// 300 x 333 x 500 64 x 64 5.4, 128 x 128 8.8.
 struct Form {
   int bm, bn, per_cu;
   float step, unit;
 };
-constexpr Form kForms[3] = {{256, 256, 1, 1.9f, 7.0f}, {256, 192, 1, 1.55f, 6.0f}, {128, 128, 2, 1.4f, 5.0f}};
+constexpr Form kForms[] = {{256, 256, 1, 1.82f, 3.5f}, {256, 192, 1, 1.4f, 2.6f}, {128, 128, 2, 1.1f, 2.2f},
+                           {128, 128, 1, 0.58f, 2.0f}, {64, 128, 2, 0.66f, 1.5f}, {64, 64, 2, 0.45f, 1.0f}};
+constexpr int kNumForms = sizeof(kForms) / sizeof(kForms[0]);
 
 struct Plan {
   int form, splits, ksteps;
 };
 static Plan plan(int64_t M, int64_t N, int64_t K) {
-  const int64_t kt = cdiv(K, BK);
+  const int64_t kt = cdiv(K, BK), s_min = cdiv(kt, kMaxSteps);
   Plan best{0, 1, (int)kt};
-  float best_t = 1e30f;
-  for (int f = 0; f < 3; ++f) {
+  double best_t = 1e30;
+  for (int f = 0; f < kNumForms; ++f) {
     const Form &c = kForms[f];
     const int64_t tiles = cdiv(M, c.bm) * cdiv(N, c.bn), slots = 256 * c.per_cu;
-    const int64_t s_min = cdiv(kt, kMaxSteps);
-    const int64_t s_max = std::max(s_min, std::min<int64_t>(cdiv(kt, 4), std::max<int64_t>(1, 2 * slots / tiles)));
-    for (int64_t s = s_min; s <= std::min<int64_t>(s_max, s_min + 64); ++s) {
-      const int64_t ks = cdiv(kt, s), sp = cdiv(kt, ks), units = tiles * sp, rounds = cdiv(units, slots);
-      // a CU that holds one workgroup of two runs it faster
-      const float step = c.per_cu == 2 && units <= 256 ? 0.7f * c.step : c.step;
-      float t = (float)rounds * ((float)ks * step + c.unit);
-      if (sp > 1) t += 4.0f + (float)(M * N) * 8.0f * (float)sp * 1.5e-7f;
+    const int64_t s_max = std::max(s_min, std::min<int64_t>({cdiv(kt, 4), std::max<int64_t>(1, 2 * slots / tiles), 64}));
+    for (int64_t s = s_min; s <= s_max; ++s) {
+      const int64_t ks = cdiv(kt, s), sp = cdiv(kt, ks), units = tiles * sp;
+      // one workgroup of two on a CU runs its steps faster
+      const double step = c.per_cu == 2 && units <= 256 ? 0.65 * c.step : c.step;
+      double t = 5.0 + (double)cdiv(units, slots) * ((double)ks * step + c.unit);
+      if (sp > 1) t += 3.0 + (double)(M * N) * (5.2 * (double)sp + 4.0) / 4.5e6;
       if (t < best_t) best_t = t, best = Plan{f, (int)sp, (int)ks};
     }
   }
   return best;
 }
 
-template <int BM, int BN, int WM, int WN, bool TA, bool TW, int OUT>
-static void launch_tile(const Prob &p, hipStream_t st) {
-  constexpr int lds = 2 * (BM + BN) * BK;
-  static const hipError_t set = hipFuncSetAttribute((const void *)gemm_kernel<BM, BN, WM, WN, TA, TW, OUT>,
+template <int BM, int BN, int WM, int WN, int S, bool TA, bool TW, int OUT>
+static void launch_tile(const Prob &p, int per_cu, hipStream_t st) {
+  constexpr int lds = S * (BM + BN) * BK;
+  static const hipError_t set = hipFuncSetAttribute((const void *)gemm_kernel<BM, BN, WM, WN, S, TA, TW, OUT>,
                                                     hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   (void)set;
   const int64_t units = cdiv(p.M, BM) * cdiv(p.N, BN) * p.splits;
-  const int64_t cus = cu_count() * (lds <= 80 * 1024 ? 2 : 1);
-  gemm_kernel<BM, BN, WM, WN, TA, TW, OUT><<<(unsigned)std::min(units, cus), WM * WN * 64, lds, st>>>(p);
+  gemm_kernel<BM, BN, WM, WN, S, TA, TW, OUT>
+      <<<(unsigned)std::min<int64_t>(units, (int64_t)cu_count() * per_cu), WM * WN * 64, lds, st>>>(p);
 }
 
 template <bool TA, bool TW, int OUT>
 static void launch_form(int form, const Prob &p, hipStream_t st) {
-  if (form == 0) launch_tile<256, 256, 2, 4, TA, TW, OUT>(p, st);
-  else if (form == 1) launch_tile<256, 192, 4, 2, TA, TW, OUT>(p, st);
-  else launch_tile<128, 128, 2, 2, TA, TW, OUT>(p, st);
+  const int n = kForms[form].per_cu;
+  switch (form) {
+    case 0: launch_tile<256, 256, 2, 4, 2, TA, TW, OUT>(p, n, st); break;
+    case 1: launch_tile<256, 192, 4, 2, 2, TA, TW, OUT>(p, n, st); break;
+    case 2: launch_tile<128, 128, 2, 2, 2, TA, TW, OUT>(p, n, st); break;
+    case 3: launch_tile<128, 128, 2, 2, 4, TA, TW, OUT>(p, n, st); break;
+    case 4: launch_tile<64, 128, 2, 2, 3, TA, TW, OUT>(p, n, st); break;
+    default: launch_tile<64, 64, 2, 2, 4, TA, TW, OUT>(p, n, st);
+  }
 }
 
 template <int OUT>
@@ -1090,9 +1133,12 @@ extern "C" int ksd_tc_gemm(const int8_t *a, int64_t lda, int a_t, const float *s
   if (M == 0 || N == 0) return KSD_OK;
   if (!a || !w || !y) return fail(KSD_EINVAL, "tc_gemm: null pointer");
   if (((uintptr_t)a) % 16 || ((uintptr_t)w) % 16) return fail(KSD_EINVAL, "tc_gemm: codes must be 16-byte aligned");
-  tc::Prob p{a, w, sa, sw, bias, residual, y, (int32_t *)workspace, lda, ldw, (int)M, (int)N, (int)K, 1, 0};
+  tc::Prob p{a, w, sa, sw, bias, residual, y, (int32_t *)workspace, lda, ldw, (int)M, (int)N, (int)K, 1, 0, 0};
   const tc::Plan pl = tc::plan(M, N, K);
   p.splits = pl.splits, p.ksteps = pl.ksteps;
+  // Where 16 lanes store whole 64-byte pieces (4 tokens' 150144 x 1536 product 1024 -> 933 us); pieces that
+  // other stores complete are put together in L2 (8192 x 1536 from a T operand: 28 us, non-temporal 40).
+  p.nt = !w_t && ((uintptr_t)y) % 64 == 0 && N * (out_dtype == KSD_F32 ? 4 : 2) % 64 == 0;
   const int64_t need = p.splits > 1 ? (int64_t)p.splits * M * N * 4 : 0;
   if (need > 0 && (!workspace || workspace_bytes < need))
     return fail(KSD_EINVAL, "tc_gemm: workspace of %lld bytes needed", (long long)need);
@@ -1126,21 +1172,25 @@ extern "C" int ksd_tc_quantize_grad(const void *g, int g_dtype, int64_t M, int64
   if (!g || !sx || !sw || !e || !f || !workspace || workspace_bytes < need)
     return fail(KSD_EINVAL, "tc_quantize_grad: null pointer or short workspace");
   const int rows = tc::stats_rows(M, N);
-  const int64_t ncb = cdiv(N, g_dtype == KSD_F32 ? 256 : 512), nrb = cdiv(M, rows);
-  if (nrb > 65535) return fail(KSD_EINVAL, "tc_quantize_grad: too many rows");
+  const bool large = tc::large_grad(M, N);
+  const int64_t ncb = cdiv(N, large && g_dtype != KSD_F32 ? 512 : 256), nrb = cdiv(M, rows);
+  if (nrb > 65535 || cdiv(M, 32) > 65535) return fail(KSD_EINVAL, "tc_quantize_grad: too many rows");
   uint32_t *row_part = (uint32_t *)workspace, *col_part = row_part + ncb * M;
   float *sum_part = (float *)(col_part + nrb * N), *einv = sum_part + nrb * N, *finv = einv + M;
+  float *sums = db ? sum_part : nullptr;
   hipStream_t st = (hipStream_t)stream;
-  const dim3 gs((unsigned)cdiv(ncb, 4), (unsigned)nrb), gq((unsigned)cdiv(ld, 512), (unsigned)cdiv(M, 64));
+  const dim3 gs((unsigned)cdiv(ncb, 4), (unsigned)nrb), gq((unsigned)cdiv(ld, 512), (unsigned)cdiv(M, large ? 64 : 32));
   const unsigned folds = (unsigned)(cdiv(M, 64) + cdiv(N, 64));
-#define KSD_TC(DT)                                                                                                    \
-  tc::grad_stats_kernel<DT><<<gs, 256, 0, st>>>(g, M, N, stride, rows, sx, sw, row_part, col_part, db ? sum_part : nullptr); \
+#define KSD_TC(DT, V)                                                                                                  \
+  if (large) tc::grad_stats_kernel<DT, V><<<gs, 256, 0, st>>>(g, M, N, stride, rows, sx, sw, row_part, col_part, sums); \
+  else tc::grad_stats_kernel<DT, 4><<<gs, 256, 0, st>>>(g, M, N, stride, rows, sx, sw, row_part, col_part, sums);       \
   tc::grad_fold_kernel<<<folds, 1024, 0, st>>>(row_part, col_part, sum_part, M, N, (int)ncb, (int)nrb, e, einv, f, finv, db); \
-  if (q || c) tc::grad_codes_kernel<DT><<<gq, 256, 0, st>>>(g, M, N, stride, sx, sw, einv, finv, q, c, ld);
+  if ((q || c) && large) tc::grad_codes_kernel<DT, 2><<<gq, 256, 0, st>>>(g, M, N, stride, sx, sw, einv, finv, q, c, ld); \
+  else if (q || c) tc::grad_codes_kernel<DT, 1><<<gq, 256, 0, st>>>(g, M, N, stride, sx, sw, einv, finv, q, c, ld);
   switch (g_dtype) {
-    case KSD_F32: KSD_TC(KSD_F32) break;
-    case KSD_BF16: KSD_TC(KSD_BF16) break;
-    default: KSD_TC(KSD_F16)
+    case KSD_F32: KSD_TC(KSD_F32, 4) break;
+    case KSD_BF16: KSD_TC(KSD_BF16, 8) break;
+    default: KSD_TC(KSD_F16, 8)
   }
 #undef KSD_TC
   return check_launch("tc_quantize_grad");

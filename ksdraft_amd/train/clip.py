@@ -45,14 +45,18 @@ class _Table:
             _lib.require_gpu(*grads, *(out or ()))
         if not all(map(_T.is_contiguous, grads)):  # False for sparse tensors too
             raise ValueError("a gradient is not dense and contiguous")
-        dtypes = list(map(_dtype_of, grads))
-        try:
-            codes = list(map(_CODE.__getitem__, dtypes))
-        except KeyError as e:
-            raise TypeError(f"unsupported gradient dtype {e.args[0]}") from None
+        dtypes = set(map(_dtype_of, grads))
+        for d in dtypes:
+            if d not in _CODE:
+                raise TypeError(f"unsupported gradient dtype {d}")
         sizes = list(map(_T.numel, grads))
-        if out is not None and (list(map(_dtype_of, out)) != dtypes or list(map(_T.numel, out)) != sizes
-                                or not all(map(_T.is_contiguous, out))):
+        if len(dtypes) == 1:
+            codes = [_CODE[d] for d in dtypes] * len(grads)
+        else:
+            codes = [_CODE[g.dtype] for g in grads]
+        if out is not None and (set(map(_dtype_of, out)) != dtypes or list(map(_T.numel, out)) != sizes
+                                or not all(map(_T.is_contiguous, out))
+                                or (len(dtypes) > 1 and [_CODE[o.dtype] for o in out] != codes)):
             raise ValueError("outputs must be contiguous and of their gradients' sizes and dtypes")
         self.n = len(grads)
         self.dev = grads[0].device
