@@ -89,7 +89,7 @@ __global__ __launch_bounds__(256) void lookup_kernel(const void *__restrict__ ta
 // rank = earlier tiles' + earlier waves' + earlier rounds of 64 + lower lanes with that digit, the last
 // from ballots over the digit's bits.
 constexpr int kDigits = 512;
-constexpr int kOne = 8192;   // keys that one workgroup sorts in LDS
+constexpr int kOne = 8192;  // keys that are placed by counting
 
 __device__ __forceinline__ uint32_t key_of(const void *ids, int wide, int64_t i, int64_t V, int64_t pad) {
   const int64_t id = load_id(ids, wide, i);
@@ -240,100 +240,39 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(const SortArgs a) {
   }
 }
 
-// Up to kOne keys: one workgroup sorts them, all passes in one launch (NT = 1024 threads: 8192 ids of
-// 150144 in MEASURED_SORT us). With NT = 256 the other workgroups clear `out` meanwhile; that form keeps little
-// in registers and LDS, so that a CU still holds 8 workgroups of the clearing.
-template <int NT>
-__global__ __launch_bounds__(NT) void sort_one_kernel(const SortArgs a, int passes, uint32_t *keys2, int32_t *pos2, const Fill f) {
-  constexpr int NW = NT / 64, R = kOne / NT, U = R < 4 ? R : 4;
-  __shared__ uint32_t h[NW * kDigits];
-  __shared__ uint32_t scratch[NW];
-  if (blockIdx.x > 0) {
-    if constexpr (NT == 256) fill(f, blockIdx.x - 1);
+// Up to kOne keys below 2^19: each key's place is the number of smaller (key, position) pairs, one word each,
+// counted by all CUs at 256 keys and 1024 others a workgroup: 8192 ids take MEASURED_RANK us where a radix sort's
+// four launches take 30. Workgroups past the counting ones clear `out` meanwhile.
+constexpr int kOthers = 1024;
+__device__ __forceinline__ uint32_t pair_of(const SortArgs &a, int i) {
+  return i < a.n ? key_of(a.ids, a.wide, i, a.V, a.pad) * (uint32_t)kOne + (uint32_t)i : 0xffffffffu;
+}
+__global__ __launch_bounds__(256) void rank_count_kernel(const SortArgs a, unsigned counting, const Fill f) {
+  __shared__ __attribute__((aligned(16))) uint32_t others[kOthers];
+  if (blockIdx.x >= counting) {
+    fill(f, blockIdx.x - counting);
     return;
   }
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int per = (a.n + NT - 1) / NT;  // rounds of a wave that hold keys
-  const uint32_t mask = (1u << a.bits) - 1;
-  const uint64_t below = (1ull << lane) - 1;
-  for (int pass = 0; pass < passes; ++pass) {
-    const int shift = pass * a.bits;
-    // the last pass ends in out_keys, out_pos
-    const bool even = (passes - 1 - pass) % 2 == 0;
-    uint32_t *const to_keys = even ? a.out_keys : keys2;
-    int32_t *const to_pos = even ? a.out_pos : pos2;
-    const uint32_t *const from_keys = even ? keys2 : a.out_keys;
-    const int32_t *const from_pos = even ? pos2 : a.out_pos;
-    auto load = [&](int r, uint32_t &key, int32_t &p, bool &in) __attribute__((always_inline)) {
-      const int i = (wave * per + r) * 64 + lane;
-      in = r < per && i < a.n;
-      const int j = in ? i : 0;
-      key = pass == 0 ? key_of(a.ids, a.wide, j, a.V, a.pad) : from_keys[j];
-      p = pass == 0 ? j : from_pos[j];
-    };
-    for (int i = tid; i < NW * kDigits; i += NT) h[i] = 0;
-    __syncthreads();
-    for (int r0 = 0; r0 < per; r0 += U) {
-      uint32_t key[U];
-      int32_t p[U];
-      bool in[U];
+  const int mine = (a.n + 255) / 256, slice = blockIdx.x / mine, i = (blockIdx.x % mine) * 256 + threadIdx.x;
 #pragma unroll
-      for (int r = 0; r < U; ++r) load(r0 + r, key[r], p[r], in[r]);
-#pragma unroll
-      for (int r = 0; r < U; ++r) {
-        const uint32_t d = (key[r] >> shift) & mask;
-        const uint64_t same = same_digit(d, a.bits, in[r]);
-        if (in[r] && (same & below) == 0) h[wave * kDigits + d] += (uint32_t)__popcll(same);
-        __builtin_amdgcn_wave_barrier();
-      }
-    }
-    __syncthreads();
-    // digit starts: NT = 256 threads hold two digits each
-    constexpr int E = NT < kDigits ? kDigits / NT : 1;
-    uint32_t all[E], sum = 0;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      all[e] = 0;
-      if (tid * E + e < kDigits)
-        for (int w = 0; w < NW; ++w) all[e] += h[w * kDigits + tid * E + e];
-      sum += all[e];
-    }
-    uint32_t at = exclusive_sum<NT>(sum, scratch);
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (tid * E + e < kDigits)
-        for (int w = 0; w < NW; ++w) {
-          const uint32_t c = h[w * kDigits + tid * E + e];
-          h[w * kDigits + tid * E + e] = at;
-          at += c;
-        }
-    __syncthreads();
-    for (int r0 = 0; r0 < per; r0 += U) {
-      uint32_t key[U];
-      int32_t p[U];
-      bool in[U];
-#pragma unroll
-      for (int r = 0; r < U; ++r) load(r0 + r, key[r], p[r], in[r]);
-#pragma unroll
-      for (int r = 0; r < U; ++r) {
-        const uint32_t d = (key[r] >> shift) & mask;
-        const uint64_t same = same_digit(d, a.bits, in[r]);
-        uint32_t first = 0;
-        if (in[r]) {
-          first = h[wave * kDigits + d];
-          const uint32_t to = first + (uint32_t)__popcll(same & below);
-          to_keys[to] = key[r];
-          to_pos[to] = p[r];
-        }
-        __builtin_amdgcn_wave_barrier();
-        if (in[r] && (same & below) == 0) h[wave * kDigits + d] = first + (uint32_t)__popcll(same);
-        __builtin_amdgcn_wave_barrier();
-      }
-    }
-    // this pass's keys are read by other waves of the workgroup in the next
-    __threadfence_block();
-    __syncthreads();
+  for (int k = 0; k < kOthers / 256; ++k) others[k * 256 + threadIdx.x] = pair_of(a, slice * kOthers + k * 256 + threadIdx.x);
+  const uint32_t c = pair_of(a, i);
+  __syncthreads();
+  uint32_t less = 0;
+#pragma unroll 8
+  for (int j = 0; j < kOthers; j += 4) {
+    const uint4 q = *(const uint4 *)(others + j);
+    less += (q.x < c) + (q.y < c) + (q.z < c) + (q.w < c);
   }
+  if (i < a.n) a.counts[(int64_t)slice * a.n + i] = less;
+}
+__global__ __launch_bounds__(256) void rank_scatter_kernel(const SortArgs a) {
+  const int i = blockIdx.x * 256 + threadIdx.x, slices = (a.n + kOthers - 1) / kOthers;
+  if (i >= a.n) return;
+  uint32_t to = 0;
+  for (int s = 0; s < slices; ++s) to += a.counts[(int64_t)s * a.n + i];
+  a.out_keys[to] = key_of(a.ids, a.wide, i, a.V, a.pad);
+  a.out_pos[to] = i;
 }
 
 // ------------------------------------------------------------------------------------ sums
@@ -569,10 +508,117 @@ __global__ __launch_bounds__(256) void join_kernel(const SumArgs a) {
   }
 }
 
+// Up to kFew tokens in one launch without a sort: workgroup b owns the rows b, b + grid, b + 2 grid, .. (so that
+// neighbouring frequent tokens meet different workgroups), lists the tokens of its rows in order, and sums or
+// clears its rows.
+constexpr int kFew = 1024;
+constexpr int kFewRows = 16;  // rows of a workgroup where all rows are written
+template <int DT, int OUT>
+__global__ __launch_bounds__(256) void few_tokens_kernel(const SumArgs a, const void *__restrict__ ids, int wide, int64_t pad) {
+  using T = typename Elem<DT>::T;
+  using TO = typename Elem<OUT>::T;
+  constexpr int NV = DT == KSD_F32 ? 4 : 8;
+  __shared__ uint32_t keys[kFew];
+  __shared__ uint16_t pos[kFew];
+  __shared__ uint8_t first[kFew];
+  __shared__ uint32_t counts[5];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const uint32_t grid = gridDim.x, me = blockIdx.x;
+  // the tokens of this workgroup's rows in order: thread t looks at the positions 4 t .. 4 t + 3
+  uint32_t k[4];
+  bool hit[4];
+  int mine = 0;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int i = tid * 4 + r;
+    k[r] = i < a.n ? key_of(ids, wide, i, a.V, pad) : (uint32_t)a.V;
+    hit[r] = k[r] < a.V && k[r] % grid == me;
+    mine += hit[r];
+  }
+  int incl = mine;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int u = __shfl_up(incl, o);
+    if (lane >= o) incl += u;
+  }
+  if (lane == 63) counts[wave] = incl;
+  __syncthreads();
+  int at = incl - mine, m = 0;
+  for (int w = 0; w < 4; ++w) {
+    if (w < wave) at += counts[w];
+    m += counts[w];
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    if (hit[r]) {
+      keys[at] = k[r];
+      pos[at++] = (uint16_t)(tid * 4 + r);
+    }
+  __syncthreads();
+  for (int e = tid; e < m; e += 256) {
+    bool f = true;
+    for (int j = 0; j < e && f; ++j) f = keys[j] != keys[e];
+    first[e] = f;
+  }
+  __syncthreads();
+  const int64_t step = 256 * NV;
+  for (int e = 0; e < m; ++e) {
+    if (!first[e]) continue;
+    const uint32_t key = keys[e];
+    for (int64_t cc = 0; cc < a.d; cc += step) {
+      const int64_t c = cc + tid * NV, c0 = max((int64_t)0, min(c, a.d - NV));
+      float acc[NV];
+#pragma unroll
+      for (int j = 0; j < NV; ++j) acc[j] = 0.0f;
+      for (int b = e; b < m; b += 64) {
+        uint64_t same = __ballot(b + lane < m && keys[min(b + lane, m - 1)] == key);
+        while (same) {  // 8 rows in flight
+          RawCols<DT, NV> v[8];
+          int n = 0;
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            const int j = same ? __builtin_ctzll(same) : 0;
+            if (same) {
+              v[r].load((const T *)a.g + (int64_t)__builtin_amdgcn_readfirstlane(pos[b + j]) * a.stride, c0, a.d);
+              same &= same - 1;
+              ++n;
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < 8; ++r)
+            if (r < n) {
+#pragma unroll
+              for (int j = 0; j < NV; ++j) acc[j] += v[r].at(j);
+            }
+        }
+      }
+      if (c < a.d) put_row<OUT, NV>(a, key, c, c0, acc);
+    }
+  }
+  if (a.add) return;
+  typedef uint32_t vec __attribute__((ext_vector_type(4), aligned(2)));
+  constexpr int NZ = 16 / sizeof(TO);
+  for (int64_t v = me + (int64_t)wave * grid; v < a.V; v += (int64_t)4 * grid) {  // a row per wave
+    bool there = false;
+    for (int b = 0; b < m && !there; b += 64) there = __ballot(b + lane < m && keys[min(b + lane, m - 1)] == (uint32_t)v) != 0;
+    if (there) continue;
+    TO *o = (TO *)a.out + v * a.d;
+#pragma unroll 4
+    for (int64_t c = lane * NZ; c < a.d; c += 64 * NZ) {
+      if (c + NZ <= a.d) {
+        __builtin_nontemporal_store((vec){0, 0, 0, 0}, (vec *)(o + c));
+      } else {
+        for (int64_t j = c; j < a.d; ++j) o[j] = (TO)0;
+      }
+    }
+  }
+}
+
 __global__ __launch_bounds__(256) void fill_kernel(const Fill f) { fill(f, blockIdx.x); }
 
-// Bytes whose clearing takes longer than the one-workgroup sort of NT = 256.
-constexpr int64_t kLongFill = 256 << 20;
+// Bytes that are cleared beside the counting, at a fill's own rate, rather than beside the sums (922 MB: 141 and
+// MEASURED_GAP us).
+constexpr int64_t kLongFill = 64 << 20;
 // Rounds of a tile: short tiles spread few keys over the CUs, long ones keep the tiles few whose counts every
 // workgroup adds up.
 static int rounds_of(int64_t n) { return n <= 131072 ? 4 : 16; }
@@ -598,7 +644,7 @@ static Layout layout(int64_t n, int64_t d) {
     return r;
   };
   for (int i = 0; i < 2; ++i) l.keys[i] = take(n * 4), l.pos[i] = take(n * 4);
-  l.counts = take(cdiv(n, 256 * rounds_of(n)) * kDigits * 4);
+  l.counts = take(std::max(cdiv(n, 256 * rounds_of(n)) * kDigits, n <= kOne ? cdiv(n, kOthers) * n : 0) * 4);
   l.parts = take(2 * cdiv(n, run_of(n)) * d * 4);
   l.bytes = at;
   return l;
@@ -610,6 +656,17 @@ static void launch_lookup(int out, unsigned g, const void *t, const void *ids, i
   if (out == KSD_F32) lookup_kernel<DT, KSD_F32><<<g, 256, 0, st>>>(t, ids, wide, n, V, d, stride, scale, y);
   else if (out == KSD_BF16) lookup_kernel<DT, KSD_BF16><<<g, 256, 0, st>>>(t, ids, wide, n, V, d, stride, scale, y);
   else lookup_kernel<DT, KSD_F16><<<g, 256, 0, st>>>(t, ids, wide, n, V, d, stride, scale, y);
+}
+template <int DT, int OUT>
+static void launch_few(const SumArgs &a, const SortArgs &s, hipStream_t st) {
+  const int64_t all = cdiv(a.V, kFewRows);
+  few_tokens_kernel<DT, OUT><<<(unsigned)(a.add ? std::min<int64_t>(all, 1024) : all), 256, 0, st>>>(a, s.ids, s.wide, s.pad);
+}
+template <int DT>
+static void launch_few(int out, const SumArgs &a, const SortArgs &s, hipStream_t st) {
+  if (out == KSD_F32) launch_few<DT, KSD_F32>(a, s, st);
+  else if (out == KSD_BF16) launch_few<DT, KSD_BF16>(a, s, st);
+  else launch_few<DT, KSD_F16>(a, s, st);
 }
 template <int DT, int OUT>
 static void launch_sums(SumArgs a, hipStream_t st) {
@@ -669,32 +726,36 @@ extern "C" int ksd_embedding_gradient(const void *g, int g_dtype, int64_t n, int
   if (!grid_fits(cdiv(chunks * slices, 4) + cdiv(V, emb::kGap), 256)) return fail(KSD_EINVAL, "embedding_gradient: too many ids");
   hipStream_t st = (hipStream_t)stream;
   const emb::Fill f{(char *)out, V * d * es};
-  const bool fits = grid_fits(emb::fill_blocks(f) + 1, 256);
   if (n == 0) {
     if (accumulate) return KSD_OK;
-    if (!fits) return fail(KSD_EINVAL, "embedding_gradient: table too large");
+    if (!grid_fits(emb::fill_blocks(f), 256)) return fail(KSD_EINVAL, "embedding_gradient: table too large");
     emb::fill_kernel<<<(unsigned)emb::fill_blocks(f), 256, 0, st>>>(f);
     return check_launch("embedding_gradient");
   }
   char *w = (char *)workspace;
   emb::SortArgs s{};
-  int passes, at = 0;
-  emb::digits(V, passes, s.bits);
   s.ids = ids, s.V = V, s.pad = padding, s.n = (int)n, s.wide = ids_wide;
-  int64_t rows = accumulate ? 0 : V;  // rows that the sums' launch clears where no token occurs
-  if (n <= emb::kOne) {
+  s.counts = (uint32_t *)(w + l.counts);
+  emb::SumArgs a{nullptr, nullptr, g, out, (float *)(w + l.parts), d, stride, V, accumulate ? 0 : V,
+                 (int)n, (int)chunks, run, (int)slices, accumulate, 0, scale};
+  if (n <= emb::kFew) {
+    if (g_dtype == KSD_F32) emb::launch_few<KSD_F32>(out_dtype, a, s, st);
+    else if (g_dtype == KSD_BF16) emb::launch_few<KSD_BF16>(out_dtype, a, s, st);
+    else emb::launch_few<KSD_F16>(out_dtype, a, s, st);
+    return check_launch("embedding_gradient");
+  }
+  int at = 0;
+  if (n <= emb::kOne && V < (1 << 19)) {
     s.out_keys = (uint32_t *)(w + l.keys[0]), s.out_pos = (int32_t *)(w + l.pos[0]);
-    uint32_t *keys2 = (uint32_t *)(w + l.keys[1]);
-    int32_t *pos2 = (int32_t *)(w + l.pos[1]);
-    if (!accumulate && f.n >= emb::kLongFill && fits) {
-      rows = 0;
-      emb::sort_one_kernel<256><<<(unsigned)(1 + emb::fill_blocks(f)), 256, 0, st>>>(s, passes, keys2, pos2, f);
-    } else {
-      emb::sort_one_kernel<1024><<<1, 1024, 0, st>>>(s, passes, keys2, pos2, f);
-    }
+    const bool blind = !accumulate && f.n >= emb::kLongFill && grid_fits(emb::fill_blocks(f) + 256, 256);
+    if (blind) a.rows = 0;
+    const unsigned counting = (unsigned)(cdiv(n, 256) * cdiv(n, emb::kOthers));
+    emb::rank_count_kernel<<<counting + (blind ? (unsigned)emb::fill_blocks(f) : 0), 256, 0, st>>>(s, counting, f);
+    emb::rank_scatter_kernel<<<(unsigned)cdiv(n, 256), 256, 0, st>>>(s);
   } else {
     const int rounds = emb::rounds_of(n);
-    s.counts = (uint32_t *)(w + l.counts);
+    int passes;
+    emb::digits(V, passes, s.bits);
     s.tiles = (int)cdiv(n, 256 * rounds);
     for (int p = 0; p < passes; ++p, at ^= 1) {
       if (p > 0) s.ids = nullptr;
@@ -711,8 +772,7 @@ extern "C" int ksd_embedding_gradient(const void *g, int g_dtype, int64_t n, int
     }
     at ^= 1;  // the last pass's output
   }
-  emb::SumArgs a{(uint32_t *)(w + l.keys[at]), (int32_t *)(w + l.pos[at]), g, out, (float *)(w + l.parts), d, stride, V, rows,
-                 (int)n, (int)chunks, run, (int)slices, accumulate, 0, scale};
+  a.keys = (uint32_t *)(w + l.keys[at]), a.pos = (int32_t *)(w + l.pos[at]);
 #define KSD_SUMS(DT)                                                        \
   if (out_dtype == KSD_F32) emb::launch_sums<DT, KSD_F32>(a, st);           \
   else if (out_dtype == KSD_BF16) emb::launch_sums<DT, KSD_BF16>(a, st);    \

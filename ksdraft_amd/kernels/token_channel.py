@@ -78,10 +78,12 @@ def _codes_operand(q: torch.Tensor, name: str, zeros: bool = False):
     if K == 0:
         raise ValueError(f"{name} has no columns")
     ld = q.stride(0) if M > 1 else _pitch(K)
-    end = (q.storage_offset() + max(M - 1, 0) * ld + _pitch(K))
-    if (not (zeros and K % 16) and q.stride(1) == 1 and ld % 16 == 0 and ld >= _pitch(K) and q.data_ptr() % 16 == 0
-            and end <= q.untyped_storage().nbytes()):
-        return q, ld
+    if q.stride(1) == 1 and ld % 16 == 0 and ld >= _pitch(K) and q.data_ptr() % 16 == 0:
+        if K % 16 == 0:
+            return q, ld
+        end = q.storage_offset() + max(M - 1, 0) * ld + _pitch(K)
+        if not zeros and end <= q.untyped_storage().nbytes():
+            return q, ld
     out = torch.zeros((M, _pitch(K)), dtype=torch.int8, device=q.device)
     out[:, :K] = q
     return out, _pitch(K)
