@@ -511,8 +511,7 @@ __global__ __launch_bounds__(256) void join_kernel(const SumArgs a) {
 // Up to kFew tokens in one launch without a sort: workgroup b owns the rows b, b + grid, b + 2 grid, .. (so that
 // neighbouring frequent tokens meet different workgroups), lists the tokens of its rows in order, and sums or
 // clears its rows.
-constexpr int kFew = 1024;
-constexpr int kFewRows = 16;  // rows of a workgroup where all rows are written
+constexpr int kFew = 2048;
 template <int DT, int OUT>
 __global__ __launch_bounds__(256) void few_tokens_kernel(const SumArgs a, const void *__restrict__ ids, int wide, int64_t pad) {
   using T = typename Elem<DT>::T;
@@ -521,16 +520,19 @@ __global__ __launch_bounds__(256) void few_tokens_kernel(const SumArgs a, const 
   __shared__ uint32_t keys[kFew];
   __shared__ uint16_t pos[kFew];
   __shared__ uint8_t first[kFew];
-  __shared__ uint32_t counts[5];
+  __shared__ uint16_t list[4][kFew];
+  __shared__ float part[4][64][NV];
+  __shared__ uint32_t counts[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const uint32_t grid = gridDim.x, me = blockIdx.x;
-  // the tokens of this workgroup's rows in order: thread t looks at the positions 4 t .. 4 t + 3
-  uint32_t k[4];
-  bool hit[4];
+  // the tokens of this workgroup's rows in order: thread t looks at positions 8 t .. 8 t + 7
+  constexpr int P = kFew / 256;
+  uint32_t k[P];
+  bool hit[P];
   int mine = 0;
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int i = tid * 4 + r;
+  for (int r = 0; r < P; ++r) {
+    const int i = tid * P + r;
     k[r] = i < a.n ? key_of(ids, wide, i, a.V, pad) : (uint32_t)a.V;
     hit[r] = k[r] < a.V && k[r] % grid == me;
     mine += hit[r];
@@ -549,10 +551,10 @@ __global__ __launch_bounds__(256) void few_tokens_kernel(const SumArgs a, const 
     m += counts[w];
   }
 #pragma unroll
-  for (int r = 0; r < 4; ++r)
+  for (int r = 0; r < P; ++r)
     if (hit[r]) {
       keys[at] = k[r];
-      pos[at++] = (uint16_t)(tid * 4 + r);
+      pos[at++] = (uint16_t)(tid * P + r);
     }
   __syncthreads();
   for (int e = tid; e < m; e += 256) {
@@ -561,38 +563,48 @@ __global__ __launch_bounds__(256) void few_tokens_kernel(const SumArgs a, const 
     first[e] = f;
   }
   __syncthreads();
-  const int64_t step = 256 * NV;
+  // the waves stand side by side over the columns, or share out a token's positions where few columns are left
+  const int across = a.d > 2 * 64 * NV ? 4 : a.d > 64 * NV ? 2 : 1, shares = 4 / across;
+  const int wc = wave % across, ws = wave / across;
   for (int e = 0; e < m; ++e) {
     if (!first[e]) continue;
     const uint32_t key = keys[e];
-    for (int64_t cc = 0; cc < a.d; cc += step) {
-      const int64_t c = cc + tid * NV, c0 = max((int64_t)0, min(c, a.d - NV));
+    int n = 0;  // its positions in order, each wave for itself
+    for (int b = e; b < m; b += 64) {
+      const bool same = b + lane < m && keys[min(b + lane, m - 1)] == key;
+      const uint64_t all = __ballot(same);
+      if (same) list[wave][n + __popcll(all & ((1ull << lane) - 1))] = pos[b + lane];
+      n += __popcll(all);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const int lo = n * ws / shares, hi = n * (ws + 1) / shares;
+    for (int64_t cc = 0; cc < a.d; cc += (int64_t)across * 64 * NV) {
+      const int64_t c = cc + (wc * 64 + lane) * NV, c0 = max((int64_t)0, min(c, a.d - NV));
       float acc[NV];
 #pragma unroll
       for (int j = 0; j < NV; ++j) acc[j] = 0.0f;
-      for (int b = e; b < m; b += 64) {
-        uint64_t same = __ballot(b + lane < m && keys[min(b + lane, m - 1)] == key);
-        while (same) {  // 8 rows in flight
-          RawCols<DT, NV> v[8];
-          int n = 0;
+      for (int b = lo; b < hi; b += 8) {  // 8 rows in flight
+        RawCols<DT, NV> v[8];
 #pragma unroll
-          for (int r = 0; r < 8; ++r) {
-            const int j = same ? __builtin_ctzll(same) : 0;
-            if (same) {
-              v[r].load((const T *)a.g + (int64_t)__builtin_amdgcn_readfirstlane(pos[b + j]) * a.stride, c0, a.d);
-              same &= same - 1;
-              ++n;
-            }
+        for (int r = 0; r < 8; ++r)
+          v[r].load((const T *)a.g + (int64_t)__builtin_amdgcn_readfirstlane(list[wave][min(b + r, hi - 1)]) * a.stride, c0, a.d);
+#pragma unroll
+        for (int r = 0; r < 8; ++r)
+          if (b + r < hi) {
+#pragma unroll
+            for (int j = 0; j < NV; ++j) acc[j] += v[r].at(j);
           }
-#pragma unroll
-          for (int r = 0; r < 8; ++r)
-            if (r < n) {
-#pragma unroll
-              for (int j = 0; j < NV; ++j) acc[j] += v[r].at(j);
-            }
-        }
       }
-      if (c < a.d) put_row<OUT, NV>(a, key, c, c0, acc);
+      if (shares > 1) {  // added in the order of the shares
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < NV; ++j) part[wave][lane][j] = acc[j];
+        __syncthreads();
+        for (int w = 1; w < shares; ++w)
+#pragma unroll
+          for (int j = 0; j < NV; ++j) acc[j] += part[w * across + wc][lane][j];
+      }
+      if (ws == 0 && c < a.d) put_row<OUT, NV>(a, key, c, c0, acc);
     }
   }
   if (a.add) return;
@@ -616,9 +628,6 @@ __global__ __launch_bounds__(256) void few_tokens_kernel(const SumArgs a, const 
 
 __global__ __launch_bounds__(256) void fill_kernel(const Fill f) { fill(f, blockIdx.x); }
 
-// Bytes that are cleared beside the counting, at a fill's own rate, rather than beside the sums (922 MB: 141 and
-// MEASURED_GAP us).
-constexpr int64_t kLongFill = 64 << 20;
 // Rounds of a tile: short tiles spread few keys over the CUs, long ones keep the tiles few whose counts every
 // workgroup adds up.
 static int rounds_of(int64_t n) { return n <= 131072 ? 4 : 16; }
@@ -659,8 +668,9 @@ static void launch_lookup(int out, unsigned g, const void *t, const void *ids, i
 }
 template <int DT, int OUT>
 static void launch_few(const SumArgs &a, const SortArgs &s, hipStream_t st) {
-  const int64_t all = cdiv(a.V, kFewRows);
-  few_tokens_kernel<DT, OUT><<<(unsigned)(a.add ? std::min<int64_t>(all, 1024) : all), 256, 0, st>>>(a, s.ids, s.wide, s.pad);
+  // at most 16 rows of a workgroup where all are written, at least one
+  const int64_t some = std::min<int64_t>(a.V, 1024), all = std::max<int64_t>(some, cdiv(a.V, 16));
+  few_tokens_kernel<DT, OUT><<<(unsigned)(a.add ? some : all), 256, 0, st>>>(a, s.ids, s.wide, s.pad);
 }
 template <int DT>
 static void launch_few(int out, const SumArgs &a, const SortArgs &s, hipStream_t st) {
@@ -747,7 +757,7 @@ extern "C" int ksd_embedding_gradient(const void *g, int g_dtype, int64_t n, int
   int at = 0;
   if (n <= emb::kOne && V < (1 << 19)) {
     s.out_keys = (uint32_t *)(w + l.keys[0]), s.out_pos = (int32_t *)(w + l.pos[0]);
-    const bool blind = !accumulate && f.n >= emb::kLongFill && grid_fits(emb::fill_blocks(f) + 256, 256);
+    const bool blind = !accumulate && grid_fits(emb::fill_blocks(f) + 256, 256);
     if (blind) a.rows = 0;
     const unsigned counting = (unsigned)(cdiv(n, 256) * cdiv(n, emb::kOthers));
     emb::rank_count_kernel<<<counting + (blind ? (unsigned)emb::fill_blocks(f) : 0), 256, 0, st>>>(s, counting, f);

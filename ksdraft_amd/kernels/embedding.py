@@ -146,7 +146,7 @@ class Int8Embedding(nn.Module):
 def _check_ids(ids: torch.Tensor, V: int, check: bool) -> torch.Tensor:
     if ids.dtype not in (torch.int64, torch.int32):
         raise TypeError("ids must be integer token indices")
-    flat = ids.reshape(-1).contiguous()
+    flat = ids if ids.dim() == 1 and ids.is_contiguous() else ids.reshape(-1).contiguous()
     if check and flat.numel():  # nn.Embedding raises for such ids (a host sync)
         bad = (flat < 0) | (flat >= V)
         if bool(bad.any()):
@@ -206,7 +206,7 @@ def embedding_gradient(grad: torch.Tensor, ids: torch.Tensor, num_embeddings: in
         raise ValueError(f"padding_idx {padding_idx} is out of range for {V} rows")
     pad = -1 if padding_idx is None else padding_idx % V
     flat = _check_ids(ids, V, check_ids)
-    g = _dense_rows(grad.reshape(-1, d)) if d else grad.reshape(-1, 0)
+    g = _dense_rows(grad if grad.dim() == 2 else grad.reshape(flat.numel(), d))
     n = flat.numel()
     if out is None:
         out = torch.empty((V, d), dtype=out_dtype, device=dev)

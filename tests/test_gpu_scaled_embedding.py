@@ -83,7 +83,7 @@ def check_gradient(got, g, ids, V, scale, pad, dtype, was=None):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
 @pytest.mark.parametrize("n,V,d,how,pad", [(1, 1, 1, "one", None), (1, 5, 8, "one", 4), (7, 3, 5, "zipf", 0), (32, 300, 64, "uniform", None),
-                                           (33, 2, 129, "one", None), (1024, 40, 130, "zipf", None), (1025, 3000, 20, "zipf", 1), (900, 1 << 20, 4, "uniform", None), (5000, 1 << 20, 4, "zipf", None), (5000, 600000, 3, "uniform", 7), (8192, 20000, 1030, "zipf", None), (500, 255, 1001, "zipf", None), (2048, 256, 24, "zipf", 255),
+                                           (33, 2, 129, "one", None), (1024, 40, 130, "zipf", None), (2048, 5, 33, "zipf", None), (2049, 3000, 20, "zipf", 1), (900, 1 << 20, 4, "uniform", None), (5000, 1 << 20, 4, "zipf", None), (5000, 600000, 3, "uniform", 7), (8192, 20000, 1030, "zipf", None), (500, 255, 1001, "zipf", None), (2048, 256, 24, "zipf", 255),
                                            (2049, 257, 40, "one", 0), (3000, 70000, 36, "zipf", None),
                                            (8192, 150144, 8, "uniform", -1), (8193, 65536, 33, "zipf", 0), (20000, 11, 2056, "zipf", None),
                                            (100003, 40000, 16, "zipf", 0)])
