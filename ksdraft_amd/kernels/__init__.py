@@ -3,9 +3,11 @@
 
 from .quant import GROUP_SIZE, SCALE_DTYPE, quantize_last_dim, dequantize_last_dim
 from .linear import Int8Linear
+from .token_channel import TokenChannelLinear
+from .embedding import ScaledEmbedding
 
 __all__ = [
     "GROUP_SIZE", "SCALE_DTYPE",
     "quantize_last_dim", "dequantize_last_dim",
-    "Int8Linear",
+    "Int8Linear", "TokenChannelLinear", "ScaledEmbedding",
 ]

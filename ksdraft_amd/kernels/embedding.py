@@ -234,6 +234,12 @@ class _ScaledLookup(torch.autograd.Function):
         return dw, None, None, None, None, None
 
 
+def scaled_rows(weight: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, padding_idx: int | None = None,
+                out_dtype: torch.dtype | None = None, check_ids: bool = True) -> torch.Tensor:
+    """embedding_lookup with embedding_gradient as its backward (a dense gradient of weight)."""
+    return _ScaledLookup.apply(weight, ids, scale, padding_idx, out_dtype, check_ids)
+
+
 class ScaledEmbedding(nn.Module):
     """nn.Embedding(V, d) whose rows come out times ``scale`` (a model's sqrt(d), for instance), in
     ``out_dtype``, with the gradient of embedding_gradient."""
@@ -256,4 +262,4 @@ class ScaledEmbedding(nn.Module):
         return emb
 
     def forward(self, ids: torch.Tensor) -> torch.Tensor:
-        return _ScaledLookup.apply(self.weight, ids, self.scale, self.padding_idx, self.out_dtype, self.check_ids)
+        return scaled_rows(self.weight, ids, self.scale, self.padding_idx, self.out_dtype, self.check_ids)

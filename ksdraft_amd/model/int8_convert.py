@@ -11,15 +11,20 @@ also swaps the embedding lookup for the int8 gather over the head's codes, and
 ``int8_injection=True`` the DSpine injection's low-rank maps for Int8Linear (their rank-32/64
 reductions pad to one 128-wide group, quant.py:9-10): the staged surfaces the reference's
 doctrine keeps float until gated.
+
+``to_token_channel(model)`` is the training conversion with one scale per token and output channel
+instead of one per 128 columns: the same linears become ``TokenChannelLinear``, the embedding a
+``ScaledEmbedding`` tied to the head (``train.token_channel_step.TokenChannelTrainer`` steps it).
 """
 
 from __future__ import annotations
 
 import copy
 
-from ..kernels.embedding import Int8Embedding
+from ..kernels.embedding import Int8Embedding, ScaledEmbedding
 from ..kernels.ks3_int8 import KS3Int8Cell
 from ..kernels.linear import Int8Linear
+from ..kernels.token_channel import TokenChannelLinear
 from .draft import KSDraftModel
 
 
@@ -63,6 +68,33 @@ def to_int8(model: KSDraftModel, group: int = 128, nonlinear: str = "int8", *,
     conv._int8_tier = {"group": group, "nonlinear": nonlinear, "swapped_surfaces": swapped,
                        "trainable": trainable, "int8_embedding": int8_embedding,
                        "int8_injection": int8_injection}
+    return conv
+
+
+def to_token_channel(model: KSDraftModel, group: int = 128, nonlinear: str = "int8", *,
+                     embedding_scale: float = 1.0, check_ids: bool = True) -> KSDraftModel:
+    """A copy of the model for training with int8 products scaled per token and channel: Rosa
+    q/k/v/out, ``teacher_proj`` and the tied head become TokenChannelLinear, the embedding a
+    ScaledEmbedding on the head's weight (rows times embedding_scale), the FFNs trainable
+    KS3Int8Cells as in ``to_int8``; norms, vectors and the injection stay float."""
+    conv = copy.deepcopy(model)
+    swapped = 0
+    for block in conv.blocks:
+        for name in ("q_proj", "k_proj", "v_proj", "out_proj"):
+            setattr(block.rosa, name, TokenChannelLinear.from_float(getattr(block.rosa, name)))
+            swapped += 1
+        block.ffn = KS3Int8Cell(cell=block.ffn, group=group, nonlinear=nonlinear, trainable=True)
+        swapped += 1
+    if conv.teacher_proj is not None:
+        conv.teacher_proj = TokenChannelLinear.from_float(conv.teacher_proj)
+        swapped += 1
+    head = TokenChannelLinear(conv.head.in_features, conv.head.out_features, bias=False)
+    head.weight = conv.embedding.weight  # tied, as KSDraftModel ties its head
+    conv.head = head
+    conv.embedding = ScaledEmbedding.from_float(conv.embedding, embedding_scale, check_ids=check_ids)
+    swapped += 2
+    conv._int8_tier = {"group": group, "nonlinear": nonlinear, "swapped_surfaces": swapped,
+                       "trainable": True, "scales": "token_channel"}
     return conv
 
 

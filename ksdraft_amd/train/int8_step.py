@@ -57,14 +57,17 @@ def _check_loss_scale(s: float) -> float:
 
 
 def transfer_space_loss(features, embedding_weight: torch.Tensor, tgt: torch.Tensor,
-                        sparse_row_grad: bool = False):
+                        sparse_row_grad: bool = False, rows: torch.Tensor | None = None):
     """distillation_losses' transfer term (train/__init__.py:79-85). On the GPU the
     per-layer cosines and their gradients are two HIP row kernels per layer
     (kernels.draft.TransferSpaceLoss); the normalized target embeddings stay torch ops.
     sparse_row_grad: the gather embedding_weight[tgt] returns its row gradients as a sparse
     gradient, which autograd adds into the tied head's dense one (the same values as the
-    dense embedding backward), instead of a dense (V, d) gradient."""
-    if sparse_row_grad and embedding_weight.requires_grad:
+    dense embedding backward), instead of a dense (V, d) gradient. rows: embedding_weight[tgt]
+    when the caller has looked it up."""
+    if rows is not None:
+        pass
+    elif sparse_row_grad and embedding_weight.requires_grad:
         from ..kernels.embedding import gather_rows_sparse_grad
         rows = gather_rows_sparse_grad(embedding_weight, tgt)
     else:
