@@ -288,9 +288,14 @@ class TokenChannelLinear(nn.Module):
         return super()._load_from_state_dict(*args, **kwargs)
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
+        """linear(x), or with ``residual`` (shaped like it) their sum, added in the product's store
+        where it has x's dtype."""
+        if residual is not None and residual.dtype != x.dtype:
+            return residual + self.forward(x)
+        bias = self.bias if self.bias is None or self.bias.dtype == torch.float32 else self.bias.float()
         if torch.is_grad_enabled() and (self.weight.requires_grad or x.requires_grad
                                         or (residual is not None and residual.requires_grad)):
             self._packed = None
-            return _LinearFunction.apply(x, self.weight, self.bias, residual)
+            return _LinearFunction.apply(x, self.weight, bias, residual)
         codes, scales = self._packed or quantize_rows(self.weight.detach())
-        return token_channel_linear(x, codes, scales, None if self.bias is None else self.bias.detach(), residual)
+        return token_channel_linear(x, codes, scales, None if bias is None else bias.detach(), residual)

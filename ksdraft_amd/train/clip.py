@@ -107,10 +107,18 @@ def clip_gradients(grads, max_norm: float, norm_type: float = 2.0, out=None, los
 
 
 def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, loss_scale: float = 1.0) -> torch.Tensor:
-    """torch.nn.utils.clip_grad_norm_ on the parameters' gradients, in place."""
+    """torch.nn.utils.clip_grad_norm_ on the parameters' gradients, in place (one that is not
+    contiguous through a copy)."""
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
     grads = [p.grad for p in parameters if p.grad is not None]
     if not grads:
         return torch.tensor(0.0)
-    return clip_gradients(grads, max_norm, norm_type, loss_scale=loss_scale)
+    copies = [(g, g.contiguous()) for g in grads if not g.is_sparse and not g.is_contiguous()]
+    if copies:
+        by_id = {id(g): c for g, c in copies}
+        grads = [by_id.get(id(g), g) for g in grads]
+    norm = clip_gradients(grads, max_norm, norm_type, loss_scale=loss_scale)
+    for g, c in copies:
+        g.copy_(c)
+    return norm

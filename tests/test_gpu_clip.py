@@ -125,6 +125,24 @@ def test_parameters_and_optimizer():
 
 
 @pytest.mark.gpu
+def test_gradients_of_other_layouts():
+    """A transposed gradient, an empty one, and one tensor as the parameters."""
+    p = torch.nn.Parameter(torch.zeros(50, 70, device=DEV))
+    g = tensors([(70, 50)], [torch.float32])[0].t()
+    p.grad = torch.empty(70, 50, device=DEV).t()
+    p.grad.copy_(g)
+    assert not p.grad.is_contiguous()
+    e = torch.nn.Parameter(torch.zeros(0, 3, device=DEV))
+    e.grad = torch.zeros(0, 3, device=DEV)
+    total, factor = reference([g], 1.0)
+    norm = clip_grad_norm_([p, e], 1.0)
+    assert abs(norm.item() - total) <= 3 * 2.0 ** -24 * total
+    assert (p.grad.double() - g.double() * factor).abs().max().item() <= 12 * 2.0 ** -24 * 5 * factor
+    assert abs(clip_grad_norm_(p, 2.0).item() - 1.0) <= 1e-5
+    assert clip_grad_norm_(e, 1.0).item() == 0.0
+
+
+@pytest.mark.gpu
 def test_refusals():
     t = torch.ones(4, 4, device=DEV)
     with pytest.raises(ValueError):

@@ -255,6 +255,55 @@ def test_module_and_strides():
 
 
 @pytest.mark.gpu
+def test_module_dtypes():
+    """Half precision masters, and a residual of another dtype."""
+    mod = tc.TokenChannelLinear.from_float(torch.nn.Linear(96, 50).to(DEV)).to(torch.bfloat16)
+    x = data(20, 96, "bf16", 1).requires_grad_(True)
+    r = data(20, 50, "fp32", 2)
+    with torch.no_grad():
+        plain = mod(x)
+        assert torch.equal(mod(x, residual=r), r + plain)
+    mod(x).backward(torch.ones(20, 50, device=DEV, dtype=torch.bfloat16))
+    assert mod.weight.grad.dtype == mod.bias.grad.dtype == torch.bfloat16 and x.grad.dtype == torch.bfloat16
+    assert torch.equal(mod.bias.grad, torch.full((50,), 20.0, device=DEV, dtype=torch.bfloat16))
+
+
+@pytest.mark.gpu
+def test_graph():
+    """A captured step (products, both gradients, embedding gradient, clipping), replayed between eager
+    work: every replay gives the eager bits."""
+    from ksdraft_amd.kernels.embedding import embedding_gradient, embedding_lookup
+    from ksdraft_amd.train.clip import clip_gradients
+    table, w = data(900, 256, "fp32", 1), data(384, 256, "fp32", 2)
+    ids = torch.randint(0, 900, (3000,), generator=torch.Generator().manual_seed(3)).to(DEV)
+    up = data(3000, 384, "fp32", 4)
+
+    def step():
+        x = embedding_lookup(table, ids, 16.0, check_ids=False)
+        y, s = tc.token_channel_linear_train(x, w)
+        few = tc.token_channel_linear(x[:4], s.wq[:, :256], s.ws)
+        dx, dw, db = tc.token_channel_linear_backward(up, s, need_db=True)
+        dt = embedding_gradient(dx, ids, 900, 16.0, check_ids=False)
+        out = [torch.empty_like(dw), torch.empty_like(dt)]
+        return [y, few, dx, dw, db, dt, clip_gradients([dw, dt], 1.0, out=out), *out]
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        eager = [t.clone() for t in step()]
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for _ in range(4):
+        for t in held:
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, eager))
+        step()
+        torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
 def test_operands_with_unknown_padding():
     """Bytes between a caller's rows take no part."""
     buf = torch.full((20, 48), 77, dtype=torch.int8, device=DEV)
