@@ -735,8 +735,11 @@ int ksd_tc_quantize_rows(const void *x, int x_dtype, int64_t M, int64_t K, int64
  *         16-byte aligned
  *   sa (M,), sw (N,), bias (N,) fp32 or NULL; residual (M, N) of the output type or NULL
  *   workspace: ksd_tc_gemm_workspace bytes
+ * ksd_tc_gemm_form: the tile, workgroups per CU and parts of the reduction that a shape gets.
  */
 int ksd_tc_gemm_workspace(int64_t M, int64_t N, int64_t K, int64_t *bytes);
+int ksd_tc_gemm_form(int64_t M, int64_t N, int64_t K, int *tile_m, int *tile_n, int *per_cu,
+                     int *splits);
 int ksd_tc_gemm(const int8_t *a, int64_t lda, int a_t, const float *sa, const int8_t *w,
                 int64_t ldw, int w_t, const float *sw, int64_t M, int64_t N, int64_t K,
                 const float *bias, const void *residual, void *y, int out_dtype, void *workspace,

@@ -89,6 +89,7 @@ SIGNATURES = {
                               _P, _P, _P, _P, _P],
     "ksd_tc_quantize_rows": [_P, _INT, _I64, _I64, _I64, _P, _I64, _P, _P],
     "ksd_tc_gemm_workspace": [_I64, _I64, _I64, _P],
+    "ksd_tc_gemm_form": [_I64, _I64, _I64, _P, _P, _P, _P],
     "ksd_tc_gemm": [_P, _I64, _INT, _P, _P, _I64, _INT, _P, _I64, _I64, _I64, _P, _P, _P, _INT, _P, _I64, _P],
     "ksd_tc_grad_workspace": [_I64, _I64, _P],
     "ksd_tc_quantize_grad": [_P, _INT, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P, _I64, _P, _P, _I64, _P],

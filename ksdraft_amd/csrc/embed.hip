@@ -241,9 +241,9 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(const SortArgs a) {
 }
 
 // Up to kOne keys below 2^19: each key's place is the number of smaller (key, position) pairs, one word each,
-// counted by all CUs at 256 keys and 1024 others a workgroup: 8192 ids take MEASURED_RANK us where a radix sort's
-// four launches take 30. Workgroups past the counting ones clear `out` meanwhile.
-constexpr int kOthers = 1024;
+// counted by all CUs at 256 keys and 1024 others a workgroup: 8192 ids take 16 us with the scatter, where a
+// radix sort's four launches take 30. Workgroups past the counting ones clear `out` meanwhile.
+constexpr int kOthers = 512;
 __device__ __forceinline__ uint32_t pair_of(const SortArgs &a, int i) {
   return i < a.n ? key_of(a.ids, a.wide, i, a.V, a.pad) * (uint32_t)kOne + (uint32_t)i : 0xffffffffu;
 }
@@ -563,8 +563,11 @@ __global__ __launch_bounds__(256) void few_tokens_kernel(const SumArgs a, const 
     first[e] = f;
   }
   __syncthreads();
-  // the waves stand side by side over the columns, or share out a token's positions where few columns are left
-  const int across = a.d > 2 * 64 * NV ? 4 : a.d > 64 * NV ? 2 : 1, shares = 4 / across;
+  // this workgroup's columns; its waves stand side by side over them, or share out a token's positions where
+  // few columns are left
+  const int64_t width = (int64_t)((a.slices + gridDim.y - 1) / gridDim.y) * 64 * NV;
+  const int64_t c_lo = blockIdx.y * width, c_hi = min(a.d, c_lo + width);
+  const int across = width > 2 * 64 * NV ? 4 : width > 64 * NV ? 2 : 1, shares = 4 / across;
   const int wc = wave % across, ws = wave / across;
   for (int e = 0; e < m; ++e) {
     if (!first[e]) continue;
@@ -578,7 +581,7 @@ __global__ __launch_bounds__(256) void few_tokens_kernel(const SumArgs a, const 
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     const int lo = n * ws / shares, hi = n * (ws + 1) / shares;
-    for (int64_t cc = 0; cc < a.d; cc += (int64_t)across * 64 * NV) {
+    for (int64_t cc = c_lo; cc < c_hi; cc += (int64_t)across * 64 * NV) {
       const int64_t c = cc + (wc * 64 + lane) * NV, c0 = max((int64_t)0, min(c, a.d - NV));
       float acc[NV];
 #pragma unroll
@@ -604,7 +607,7 @@ __global__ __launch_bounds__(256) void few_tokens_kernel(const SumArgs a, const 
 #pragma unroll
           for (int j = 0; j < NV; ++j) acc[j] += part[w * across + wc][lane][j];
       }
-      if (ws == 0 && c < a.d) put_row<OUT, NV>(a, key, c, c0, acc);
+      if (ws == 0 && c < c_hi) put_row<OUT, NV>(a, key, c, c0, acc);
     }
   }
   if (a.add) return;
@@ -616,11 +619,11 @@ __global__ __launch_bounds__(256) void few_tokens_kernel(const SumArgs a, const 
     if (there) continue;
     TO *o = (TO *)a.out + v * a.d;
 #pragma unroll 4
-    for (int64_t c = lane * NZ; c < a.d; c += 64 * NZ) {
-      if (c + NZ <= a.d) {
+    for (int64_t c = c_lo + lane * NZ; c < c_hi; c += 64 * NZ) {
+      if (c + NZ <= c_hi) {
         __builtin_nontemporal_store((vec){0, 0, 0, 0}, (vec *)(o + c));
       } else {
-        for (int64_t j = c; j < a.d; ++j) o[j] = (TO)0;
+        for (int64_t j = c; j < c_hi; ++j) o[j] = (TO)0;
       }
     }
   }
@@ -670,7 +673,10 @@ template <int DT, int OUT>
 static void launch_few(const SumArgs &a, const SortArgs &s, hipStream_t st) {
   // at most 16 rows of a workgroup where all are written, at least one
   const int64_t some = std::min<int64_t>(a.V, 1024), all = std::max<int64_t>(some, cdiv(a.V, 16));
-  few_tokens_kernel<DT, OUT><<<(unsigned)(a.add ? some : all), 256, 0, st>>>(a, s.ids, s.wide, s.pad);
+  const int64_t x = a.add ? some : all;
+  // columns apart where that gives more workgroups: a frequent token's rows are one workgroup's
+  const dim3 g((unsigned)x, (unsigned)std::max<int64_t>(1, std::min<int64_t>(a.slices, 2048 / x)));
+  few_tokens_kernel<DT, OUT><<<g, 256, 0, st>>>(a, s.ids, s.wide, s.pad);
 }
 template <int DT>
 static void launch_few(int out, const SumArgs &a, const SortArgs &s, hipStream_t st) {

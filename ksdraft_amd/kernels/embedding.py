@@ -171,7 +171,8 @@ def embedding_lookup(weight: torch.Tensor, ids: torch.Tensor, scale: float = 1.0
         raise TypeError(f"unsupported dtypes {weight.dtype} -> {out_dtype}")
     V, d = weight.shape
     flat = _check_ids(ids, V, check_ids)
-    weight = _dense_rows(weight)
+    if not weight.is_contiguous():
+        weight = _dense_rows(weight)
     out = torch.empty((*ids.shape, d), dtype=out_dtype, device=dev)
     _lib.call("ksd_embedding_lookup", weight.data_ptr(), _OUT[weight.dtype], V, d, weight.stride(0) if V > 1 else d,
               flat.data_ptr(), int(flat.dtype == torch.int64), flat.numel(), scale, out.data_ptr(), _OUT[out_dtype],

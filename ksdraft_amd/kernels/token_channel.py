@@ -147,12 +147,15 @@ def token_channel_linear(x: torch.Tensor, w_codes: torch.Tensor, w_scales: torch
     N, K = w_codes.shape
     if x.dim() == 0 or x.shape[-1] != K:
         raise ValueError(f"x has shape {tuple(x.shape)}, w_codes {tuple(w_codes.shape)}")
-    x2 = _matrix(x.reshape(-1, K), "x")
+    flat = x.dim() == 2  # a decode call's cost is this function's: no views that change nothing
+    x2 = _matrix(x if flat else x.reshape(-1, K), "x")
     M = x2.shape[0]
     out_dtype = out_dtype or x.dtype
-    bias, residual = _epilogue(M, N, bias, None if residual is None else residual.reshape(-1, N), out_dtype)
+    if residual is not None and not flat:
+        residual = residual.reshape(-1, N)
+    bias, residual = _epilogue(M, N, bias, residual, out_dtype)
     w_scales = _vector(w_scales, N, "w_scales")
-    y = torch.empty((*x.shape[:-1], N), dtype=out_dtype, device=dev)
+    y = torch.empty((M, N) if flat else (*x.shape[:-1], N), dtype=out_dtype, device=dev)
     need = ctypes.c_int64()
     _lib.call("ksd_tc_linear_workspace", M, N, K, ctypes.byref(need))
     work = torch.empty(need.value, dtype=torch.int8, device=dev) if need.value else None

@@ -86,7 +86,7 @@ def check_gradient(got, g, ids, V, scale, pad, dtype, was=None):
                                            (33, 2, 129, "one", None), (1024, 40, 130, "zipf", None), (2048, 5, 33, "zipf", None), (2049, 3000, 20, "zipf", 1), (900, 1 << 20, 4, "uniform", None), (5000, 1 << 20, 4, "zipf", None), (5000, 600000, 3, "uniform", 7), (8192, 20000, 1030, "zipf", None), (500, 255, 1001, "zipf", None), (2048, 256, 24, "zipf", 255),
                                            (2049, 257, 40, "one", 0), (3000, 70000, 36, "zipf", None),
                                            (8192, 150144, 8, "uniform", -1), (8193, 65536, 33, "zipf", 0), (20000, 11, 2056, "zipf", None),
-                                           (100003, 40000, 16, "zipf", 0)])
+                                           (100003, 40000, 16, "zipf", 0), (140001, 700, 12, "zipf", None)])
 def test_gradient(n, V, d, how, pad, dtype):
     g, ids = randn(n, d, dtype=dtype, seed=2), ids_of(n, V, 3, how)
     got = embedding_gradient(g, ids, V, 1.5, padding_idx=pad)

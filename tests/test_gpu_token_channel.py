@@ -6,11 +6,13 @@ two scales, bias, residual), each at most 2^-24 of the largest magnitude that it
 rounding to the output type (2^-24, 2^-11 or 2^-8 relative for fp32, fp16 and bf16; 2^-25 absolute
 for fp16's subnormals)."""
 
+import ctypes
 import math
 
 import pytest
 import torch
 
+from ksdraft_amd import _lib
 from ksdraft_amd.kernels import token_channel as tc
 
 DEV = "cuda"
@@ -158,6 +160,48 @@ def test_training(M, N, K, dtype):
     close(dw, main, main.abs(), torch.float32)
     close(db, gf.double().sum(0), gf.double().abs().sum(0), torch.float32, n_ops=M)
     assert dx.dtype == dt and dw.dtype == db.dtype == torch.float32
+
+
+# (M, N, K) and the tile (rows, columns, workgroups per CU) that one of its products gets: 0 the forward
+# (M, N, K), 1 dX (M, K, N), 2 dW (N, K, M)
+TILED = [(2617, 4477, 134, 0, (256, 256, 1)), (2574, 128, 4458, 1, (256, 256, 1)), (133, 4909, 2587, 2, (256, 256, 1)),
+         (4625, 1686, 131, 0, (256, 192, 1)), (2342, 128, 3512, 1, (256, 192, 1)), (128, 1808, 4725, 2, (256, 192, 1)),
+         (4685, 801, 129, 0, (128, 128, 2)), (961, 130, 4143, 1, (128, 128, 2)), (132, 3694, 1048, 2, (128, 128, 2)),
+         (4133, 479, 4157, 0, (128, 128, 1)), (523, 4305, 3639, 1, (128, 128, 1)), (4330, 4726, 394, 2, (128, 128, 1)),
+         (389, 4785, 137, 0, (64, 128, 2)), (840, 131, 2315, 1, (64, 128, 2)), (131, 4862, 387, 2, (64, 128, 2)),
+         (135, 5902, 5951, 0, (64, 128, 2)), (135, 128, 2952, 0, (64, 64, 2)), (141, 2855, 134, 1, (64, 64, 2)),
+         (2878, 131, 156, 2, (64, 64, 2)), (4600, 4700, 140, 0, (256, 192, 1)), (5003, 5009, 140, 0, (256, 256, 1))]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K,which,tile", TILED)
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_products_of_every_tile(M, N, K, which, tile, dtype):
+    """All three products at shapes that take each tile form, ragged at every edge, four of them with the
+    reduction in parts, the last two with several tiles to a workgroup: on the codes as they are, exact up to
+    the output's rounding."""
+    v = [ctypes.c_int() for _ in range(4)]
+    _lib.call("ksd_tc_gemm_form", *((M, N, K), (M, K, N), (N, K, M))[which], *[ctypes.byref(x) for x in v])
+    assert tuple(x.value for x in v[:3]) == tile
+    g = torch.Generator().manual_seed(M)
+    a = torch.randint(-127, 128, (M, K), generator=g, dtype=torch.int8).to(DEV)
+    w = torch.randint(-127, 128, (N, K), generator=g, dtype=torch.int8).to(DEV)
+    sa, sw = torch.rand(M, generator=g).to(DEV) + 0.5, torch.rand(N, generator=g).to(DEV) + 0.5
+    bias, res = data(1, N, "fp32", 3)[0], data(M, N, dtype, 4)
+    y = tc.token_channel_gemm(a, sa, w, sw, bias, res, TYPES[dtype])
+    main = (a.double() @ w.double().t()) * sa.double()[:, None] * sw.double()
+    size = main.abs() + bias.double().abs() + res.double().abs()
+    close(y, main + bias.double() + res.double(), size, TYPES[dtype])
+    x, wt, up = data(M, K, dtype, 5), data(N, K, "fp32", 6), data(M, N, dtype, 7)
+    _, s = tc.token_channel_linear_train(x, wt)
+    dx, dw, _ = tc.token_channel_linear_backward(up, s)
+    xq, wq, xs, ws = s.xq[:, :K].double(), s.wq[:, :K].double(), s.xs, s.ws
+    q, e = rows_cpu(up.float().cpu() * ws.cpu())
+    main = (q.to(DEV).double() @ wq) * e.to(DEV).double()[:, None]
+    close(dx, main, main.abs(), TYPES[dtype])
+    c, f = rows_cpu((up.float().cpu() * xs.cpu()[:, None]).t())
+    main = (c.to(DEV).double() @ xq) * f.to(DEV).double()[:, None]
+    close(dw, main, main.abs(), torch.float32)
 
 
 @pytest.mark.gpu
