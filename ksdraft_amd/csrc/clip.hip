@@ -69,6 +69,7 @@ __device__ __forceinline__ void chunk_norm(const Tensor &t, int64_t e0, double &
   }
 }
 
+// Bound by one read of the gradients. (509 fp32 tensors, 2.97 GB: 532 us, 5.6 TB/s.)
 template <bool MAX>
 __global__ __launch_bounds__(256) void norm_kernel(const Batch b, double *__restrict__ parts) {
   double sum = 0.0;
@@ -159,6 +160,7 @@ __device__ __forceinline__ void chunk_scale(const Tensor &t, int64_t e0, float f
   }
 }
 
+// Bound by a read and a write of the gradients. (The same tensors: 1190 us, 5.0 TB/s; a large copy 4.9.)
 __global__ __launch_bounds__(256) void scale_kernel(const Batch b, const float *__restrict__ factor) {
   const float f = factor[0];
   for (int c = blockIdx.x; c < b.chunks; c += gridDim.x) {

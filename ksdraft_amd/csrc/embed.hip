@@ -61,7 +61,7 @@ __device__ __forceinline__ void store_any(typename Elem<DT>::T *p, int n, const 
   }
 }
 
-// One wave per row.
+// One wave per row. (65521 tokens of a table 32003 x 1792, bf16 to bf16: 72 us, 6.5 TB/s; a few tokens: the launch.)
 template <int DT, int OUT>
 __global__ __launch_bounds__(256) void lookup_kernel(const void *__restrict__ table, const void *__restrict__ ids, int wide,
                                                      int64_t n, int64_t V, int64_t d, int64_t stride, float scale,
@@ -156,10 +156,15 @@ __device__ __forceinline__ uint32_t exclusive_sum(uint32_t v, uint32_t *scratch)
   return before + s - v;
 }
 
-// Tiles of 256 R keys, four waves of R rounds. Digit counts of the tiles.
+// Tiles of 256 R keys, four waves of R rounds. Digit counts of the tiles; workgroups past them clear `out`.
+// (65521 ids, per pass: 4.7 us, the scatter 8.9, both short launches at latency.)
 template <int R>
-__global__ __launch_bounds__(256) void sort_count_kernel(const SortArgs a) {
+__global__ __launch_bounds__(256) void sort_count_kernel(const SortArgs a, const Fill f) {
   __shared__ uint32_t h[kDigits];
+  if ((int)blockIdx.x >= a.tiles) {
+    fill(f, (int64_t)blockIdx.x - a.tiles);
+    return;
+  }
   const int tid = threadIdx.x, t0 = blockIdx.x * (256 * R);
   h[tid] = h[tid + 256] = 0;
   __syncthreads();
@@ -241,8 +246,8 @@ __global__ __launch_bounds__(256) void sort_scatter_kernel(const SortArgs a) {
 }
 
 // Up to kOne keys below 2^19: each key's place is the number of smaller (key, position) pairs, one word each,
-// counted by all CUs at 256 keys and 1024 others a workgroup: 8192 ids take 16 us with the scatter, where a
-// radix sort's four launches take 30. Workgroups past the counting ones clear `out` meanwhile.
+// counted by all CUs at 256 keys and kOthers others a workgroup. (8192 tokens of 942 by 93: the gradient takes
+// 22 us, with a radix sort's four launches 27.) Workgroups past the counting ones clear `out` meanwhile.
 constexpr int kOthers = 512;
 __device__ __forceinline__ uint32_t pair_of(const SortArgs &a, int i) {
   return i < a.n ? key_of(a.ids, a.wide, i, a.V, a.pad) * (uint32_t)kOne + (uint32_t)i : 0xffffffffu;
@@ -402,7 +407,8 @@ __device__ __forceinline__ void fill_gaps(const SumArgs &a, int64_t v0) {
 
 // One wave per chunk and slice of 64 NV columns: sums the chunk's runs in order, 8 rows in flight. A run
 // that lies in the chunk is finished; the pieces of runs that reach past it go to parts. Workgroups past
-// `sums` clear the rows without a token meanwhile, so every row of `out` is written once.
+// `sums` clear the rows without a token meanwhile, so every row of `out` is written once. (8192 x 1536 fp32 sums
+// alone 15 us; 65521 x 1792 bf16 into 32003 fp32 rows 105, 4.4 TB/s: rows gathered in 3.5 KB pieces.)
 template <int DT, int OUT>
 __global__ __launch_bounds__(256) void sum_kernel(const SumArgs a) {
   using T = typename Elem<DT>::T;
@@ -456,62 +462,80 @@ __global__ __launch_bounds__(256) void sum_kernel(const SumArgs a) {
   else put_row<OUT, NV>(a, key, c, c0, acc);
 }
 
-// Joins the pieces of runs that reach past the chunk they begin in: workgroup x looks at chunks 4 x .. 4 x + 3,
-// 256 columns each. The lanes find a run's last chunk 64 at a time; each of the 4 waves adds an equal share of
-// the pieces in order, the waves' sums are added in order.
-template <int OUT>
-__global__ __launch_bounds__(256) void join_kernel(const SumArgs a) {
-  __shared__ float part[4][64][4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  uint32_t key[4];
-  bool begins[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int b = (int)blockIdx.x * 4 + i, s0 = min(b, a.chunks - 1) * a.run, s1 = min(s0 + a.run, a.n - 1);
-    key[i] = a.keys[s1 - 1 > s0 ? s1 - 1 : s0];
-    begins[i] = b < a.chunks && b * a.run + a.run < a.n && key[i] < a.V && a.keys[s1] == key[i] &&
-                !(a.keys[s0] == key[i] && b > 0 && a.keys[s0 - 1] == key[i]);
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (!begins[i]) continue;
-    const int b = (int)blockIdx.x * 4 + i;
-    int last = b + 1;  // chunks b + 1 .. last - 1 begin with the key
-    while (true) {
-      const int q = last + lane;
-      const uint64_t hit = __ballot(q < a.chunks && a.keys[(int64_t)min(q, a.chunks - 1) * a.run] == key[i]);
-      const int more = hit == ~0ull ? 64 : __builtin_ctzll(~hit);
-      last += more;
-      if (more < 64) break;
-    }
-    const int m = last - b;  // pieces: the one that b ends in, then the beginnings of b + 1 .. last - 1
-    const int64_t c = ((int64_t)blockIdx.y * 64 + lane) * 4, c0 = max((int64_t)0, min(c, a.d - 4));
-    float acc[4] = {0, 0, 0, 0};
-    const int lo = (int)((int64_t)m * wave / 4), hi = (int)((int64_t)m * (wave + 1) / 4);
+// Joins the pieces of runs that reach past the chunk they begin in, 256 columns each: a wave looks at one chunk,
+// its lanes find the run's last chunk, 64 points of the range at a time. It adds a short run's pieces itself, in
+// order; a longer run's are shared out over the workgroup's waves, whose sums are added in order. (The
+// gradient for 131072 tokens, us: 942 x 93, all equal, shared by 4 waves 316, by 16 121; 32003 x 1792, a natural
+// text's frequencies, all runs shared by 4 waves 238, this way 218.)
+constexpr int kJoin = 16;   // waves of a workgroup
+constexpr int kAlone = 16;  // pieces of a short run
+__device__ __forceinline__ void add_pieces(const SumArgs &a, int b, int lo, int hi, int64_t c0, float *acc) {
 #pragma unroll 8
-    for (int q = lo; q < hi; ++q) {
-      float v[4];
-      load_cols<KSD_F32, 4>(a.parts + (q == 0 ? (int64_t)a.chunks + b : (int64_t)b + q) * a.d, c0, a.d, v);
+  for (int q = lo; q < hi; ++q) {
+    float v[4];
+    load_cols<KSD_F32, 4>(a.parts + (q == 0 ? (int64_t)a.chunks + b : (int64_t)b + q) * a.d, c0, a.d, v);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[j] += v[j];
+    for (int j = 0; j < 4; ++j) acc[j] += v[j];
+  }
+}
+template <int OUT>
+__global__ __launch_bounds__(64 * kJoin) void join_kernel(const SumArgs a) {
+  __shared__ float part[kJoin][64][4];
+  __shared__ int pieces[kJoin];
+  __shared__ uint32_t keys[kJoin];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t c = ((int64_t)blockIdx.y * 64 + lane) * 4, c0 = max((int64_t)0, min(c, a.d - 4));
+  const int first = (int)blockIdx.x * kJoin;
+  const int mine = first + wave, s0 = min(mine, a.chunks - 1) * a.run, s1 = min(s0 + a.run, a.n - 1);
+  const uint32_t key = a.keys[s1 - 1 > s0 ? s1 - 1 : s0];
+  const bool begins = mine < a.chunks && s0 + a.run < a.n && key < a.V && a.keys[s1] == key &&
+                      !(a.keys[s0] == key && mine > 0 && a.keys[s0 - 1] == key);
+  int m = 0;  // pieces: the one that the chunk ends in, then the beginnings of the next m - 1
+  if (begins) {
+    int last = mine + 2, end = a.chunks;  // chunks mine + 1 .. last - 1 begin with the key, chunk `end` does not
+    for (int step = 1; last < end; step = (end - last + 63) / 64) {
+      const int64_t q = last + (int64_t)lane * step;
+      const uint64_t hit = __ballot(q < end && a.keys[min(q, (int64_t)a.chunks - 1) * a.run] == key);
+      const int more = hit == ~0ull ? 64 : __builtin_ctzll(~hit);  // points with the key: all before the others
+      if (more < 64) end = (int)min((int64_t)end, last + (int64_t)more * step);
+      if (more > 0) last += (more - 1) * step + 1;
     }
-    __syncthreads();
+    m = last - mine;
+    if (m <= kAlone) {
+      float acc[4] = {0, 0, 0, 0};
+      add_pieces(a, mine, 0, m, c0, acc);
+      put_row<OUT, 4>(a, key, c, c0, acc);
+      m = 0;
+    }
+  }
+  if (lane == 0) pieces[wave] = m, keys[wave] = key;
+  __syncthreads();
+  for (int i = 0; i < kJoin; ++i) {
+    const int64_t n = pieces[i];
+    if (n == 0) continue;
+    float acc[4] = {0, 0, 0, 0};
+    add_pieces(a, first + i, (int)(n * wave / kJoin), (int)(n * (wave + 1) / kJoin), c0, acc);
+    __syncthreads();  // the last run's sums are read
 #pragma unroll
     for (int j = 0; j < 4; ++j) part[wave][lane][j] = acc[j];
     __syncthreads();
     if (wave == 0) {
-      for (int w = 1; w < 4; ++w)
+      for (int w = 1; w < kJoin; ++w)
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[j] += part[w][lane][j];
-      put_row<OUT, 4>(a, key[i], c, c0, acc);
+      put_row<OUT, 4>(a, keys[i], c, c0, acc);
     }
   }
 }
 
 // Up to kFew tokens in one launch without a sort: workgroup b owns the rows b, b + grid, b + 2 grid, .. (so that
 // neighbouring frequent tokens meet different workgroups), lists the tokens of its rows in order, and sums or
-// clears its rows.
-constexpr int kFew = 2048;
+// clears its rows. (The sorted form's time hardly depends on the tokens, this one's grows with the most frequent
+// one's: 942 x 93, us: 512 tokens 7.6, a third of them equal 21, sorted 21; 2048 tokens 8.7 and 63 against 22.)
+// Tables past kLarge are cleared by a launch of their own before (us: one token of 150144 x 1536, 922 MB, 143 and
+// here 167; 512 tokens of 32003 x 1792, 229 MB, 47 and 46).
+constexpr int64_t kLarge = (int64_t)256 << 20;
+constexpr int kFew = 512;
 template <int DT, int OUT>
 __global__ __launch_bounds__(256) void few_tokens_kernel(const SumArgs a, const void *__restrict__ ids, int wide, int64_t pad) {
   using T = typename Elem<DT>::T;
@@ -525,7 +549,7 @@ __global__ __launch_bounds__(256) void few_tokens_kernel(const SumArgs a, const 
   __shared__ uint32_t counts[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const uint32_t grid = gridDim.x, me = blockIdx.x;
-  // the tokens of this workgroup's rows in order: thread t looks at positions 8 t .. 8 t + 7
+  // the tokens of this workgroup's rows in order: thread t looks at positions P t .. P t + P - 1
   constexpr int P = kFew / 256;
   uint32_t k[P];
   bool hit[P];
@@ -610,10 +634,9 @@ __global__ __launch_bounds__(256) void few_tokens_kernel(const SumArgs a, const 
       if (ws == 0 && c < c_hi) put_row<OUT, NV>(a, key, c, c0, acc);
     }
   }
-  if (a.add) return;
   typedef uint32_t vec __attribute__((ext_vector_type(4), aligned(2)));
   constexpr int NZ = 16 / sizeof(TO);
-  for (int64_t v = me + (int64_t)wave * grid; v < a.V; v += (int64_t)4 * grid) {  // a row per wave
+  for (int64_t v = me + (int64_t)wave * grid; v < a.rows; v += (int64_t)4 * grid) {  // a row per wave
     bool there = false;
     for (int b = 0; b < m && !there; b += 64) there = __ballot(b + lane < m && keys[min(b + lane, m - 1)] == (uint32_t)v) != 0;
     if (there) continue;
@@ -632,8 +655,9 @@ __global__ __launch_bounds__(256) void few_tokens_kernel(const SumArgs a, const 
 __global__ __launch_bounds__(256) void fill_kernel(const Fill f) { fill(f, blockIdx.x); }
 
 // Rounds of a tile: short tiles spread few keys over the CUs, long ones keep the tiles few whose counts every
-// workgroup adds up.
-static int rounds_of(int64_t n) { return n <= 131072 ? 4 : 16; }
+// workgroup adds up. (942 x 93, us, 4 and 16 rounds: 131072 tokens 51 and 62, 262144 80 and 80, 524288 136 and
+// 114, 2^20 407 and 209.)
+static int rounds_of(int64_t n) { return n <= 262144 ? 4 : 16; }
 
 static void digits(int64_t V, int &passes, int &bits) {  // keys are 0 .. V
   int all = 1;
@@ -641,8 +665,9 @@ static void digits(int64_t V, int &passes, int &bits) {  // keys are 0 .. V
   passes = (all + 8) / 9;
   bits = (all + passes - 1) / passes;
 }
-// Short chunks where few rows would leave CUs idle.
-static int run_of(int64_t n) { return n <= 16384 ? 16 : 32; }
+// Short chunks where few rows would leave CUs idle. (942 x 93, us, 16 and 32: 3000 tokens 22 and 25, 8192 23
+// and 25.5; 32003 x 1792, 16384 tokens, a fifth of them equal: 87 and 74.)
+static int run_of(int64_t n) { return n <= 8192 ? 16 : 32; }
 
 struct Layout {
   int64_t keys[2], pos[2], counts, parts, bytes;
@@ -673,7 +698,7 @@ template <int DT, int OUT>
 static void launch_few(const SumArgs &a, const SortArgs &s, hipStream_t st) {
   // at most 16 rows of a workgroup where all are written, at least one
   const int64_t some = std::min<int64_t>(a.V, 1024), all = std::max<int64_t>(some, cdiv(a.V, 16));
-  const int64_t x = a.add ? some : all;
+  const int64_t x = a.rows == 0 ? some : all;
   // columns apart where that gives more workgroups: a frequent token's rows are one workgroup's
   const dim3 g((unsigned)x, (unsigned)std::max<int64_t>(1, std::min<int64_t>(a.slices, 2048 / x)));
   few_tokens_kernel<DT, OUT><<<g, 256, 0, st>>>(a, s.ids, s.wide, s.pad);
@@ -688,7 +713,8 @@ template <int DT, int OUT>
 static void launch_sums(SumArgs a, hipStream_t st) {
   a.sums = (unsigned)cdiv((int64_t)a.chunks * a.slices, 4);
   sum_kernel<DT, OUT><<<a.sums + (unsigned)cdiv(a.rows, kGap), 256, 0, st>>>(a);
-  if (a.chunks > 1) join_kernel<OUT><<<dim3((unsigned)cdiv(a.chunks, 4), (unsigned)cdiv(a.d, 256)), 256, 0, st>>>(a);
+  if (a.chunks > 1)
+    join_kernel<OUT><<<dim3((unsigned)cdiv(a.chunks, kJoin), (unsigned)cdiv(a.d, 256)), 64 * kJoin, 0, st>>>(a);
 }
 
 static bool float_type(int t) { return t == KSD_F32 || t == KSD_BF16 || t == KSD_F16; }
@@ -755,6 +781,10 @@ extern "C" int ksd_embedding_gradient(const void *g, int g_dtype, int64_t n, int
   emb::SumArgs a{nullptr, nullptr, g, out, (float *)(w + l.parts), d, stride, V, accumulate ? 0 : V,
                  (int)n, (int)chunks, run, (int)slices, accumulate, 0, scale};
   if (n <= emb::kFew) {
+    if (!accumulate && V * d * es > emb::kLarge && grid_fits(emb::fill_blocks(f), 256)) {
+      emb::fill_kernel<<<(unsigned)emb::fill_blocks(f), 256, 0, st>>>(f);
+      a.rows = 0;
+    }
     if (g_dtype == KSD_F32) emb::launch_few<KSD_F32>(out_dtype, a, s, st);
     else if (g_dtype == KSD_BF16) emb::launch_few<KSD_BF16>(out_dtype, a, s, st);
     else emb::launch_few<KSD_F16>(out_dtype, a, s, st);
@@ -773,16 +803,21 @@ extern "C" int ksd_embedding_gradient(const void *g, int g_dtype, int64_t n, int
     int passes;
     emb::digits(V, passes, s.bits);
     s.tiles = (int)cdiv(n, 256 * rounds);
+    // Where few rows have a token, clearing beside the sort costs less than in the sums' launch (us, uniform
+    // tokens: 150144 x 1536, 12000 tokens 185 and 198; 32003 x 1792, 12000 tokens 80 and 66).
+    const bool blind = !accumulate && n <= V / 4 && grid_fits(emb::fill_blocks(f) + s.tiles, 256);
+    if (blind) a.rows = 0;
     for (int p = 0; p < passes; ++p, at ^= 1) {
       if (p > 0) s.ids = nullptr;
       s.keys = (uint32_t *)(w + l.keys[at ^ 1]), s.pos = (int32_t *)(w + l.pos[at ^ 1]);
       s.out_keys = (uint32_t *)(w + l.keys[at]), s.out_pos = (int32_t *)(w + l.pos[at]);
       s.shift = p * s.bits;
+      const int64_t clear = blind && p == 0 ? emb::fill_blocks(f) : 0;
       if (rounds == 4) {
-        emb::sort_count_kernel<4><<<s.tiles, 256, 0, st>>>(s);
+        emb::sort_count_kernel<4><<<(unsigned)(s.tiles + clear), 256, 0, st>>>(s, f);
         emb::sort_scatter_kernel<4><<<s.tiles, 256, 0, st>>>(s);
       } else {
-        emb::sort_count_kernel<16><<<s.tiles, 256, 0, st>>>(s);
+        emb::sort_count_kernel<16><<<(unsigned)(s.tiles + clear), 256, 0, st>>>(s, f);
         emb::sort_scatter_kernel<16><<<s.tiles, 256, 0, st>>>(s);
       }
     }

@@ -807,7 +807,7 @@ __global__ __launch_bounds__(WM *WN * 64, WM *WN == 8 ? 1 : 2) void gemm_kernel(
 }
 
 // Joins the parts of a split reduction, V columns per thread. Their sum may pass 32 bits (K > 133144):
-// 64-bit integers.
+// 64-bit integers. (The 4096 x 1536 bf16 outputs of 150144 terms: 14 us of the product's 920.)
 template <int OUT, int V>
 __global__ __launch_bounds__(256) void combine_kernel(const Prob p) {
   const int per = p.N / V;
@@ -926,8 +926,8 @@ static void launch(int form, const Prob &p, bool ta, bool tw, hipStream_t st) {
 // y for few tokens in one launch: what bounds it is one read of the codes of W (or the launch itself).
 // Every workgroup quantizes the M tokens into LDS (their first W chunks are already on the way) and walks
 // tiles of 16 columns; its 4 waves take every fourth 64 steps of the reduction, W straight into MFMA registers
-// (each byte is used once), and meet in LDS. (bf16, us: 1 x 1536 -> 512 4.4, quantizing and a 128 x 128 product 13; 4 x 1536 -> 150144
-// 38, 6.1 TB/s, against 52.)
+// (each byte is used once), and meet in LDS. (bf16, us: 1 x 1536 -> 512 4.5, quantizing and a 128 x 128 product
+// 13; 4 x 1536 -> 150144 38, 6.1 TB/s, against 52.)
 struct Few {
   const void *x;
   const int8_t *W;
@@ -1149,7 +1149,7 @@ extern "C" int ksd_tc_gemm(const int8_t *a, int64_t lda, int a_t, const float *s
   tc::Prob p{a, w, sa, sw, bias, residual, y, (int32_t *)workspace, lda, ldw, (int)M, (int)N, (int)K, 1, 0, 0};
   const tc::Plan pl = tc::plan(M, N, K);
   p.splits = pl.splits, p.ksteps = pl.ksteps;
-  // Where 16 lanes store whole 64-byte pieces (4 tokens' 150144 x 1536 product 1024 -> 933 us); pieces that
+  // Where 16 lanes store whole 64-byte pieces (4096 x 150144 x 1536: 1024 -> 933 us); pieces that
   // other stores complete are put together in L2 (8192 x 1536 from a T operand: 28 us, non-temporal 40).
   p.nt = !w_t && ((uintptr_t)y) % 64 == 0 && N * (out_dtype == KSD_F32 ? 4 : 2) % 64 == 0;
   const int64_t need = p.splits > 1 ? (int64_t)p.splits * M * N * 4 : 0;

@@ -95,6 +95,31 @@ def test_gradient(n, V, d, how, pad, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n,V,d,how", [(1, 600, 70, "one"), (512, 300, 33, "zipf"), (513, 300, 33, "zipf"), (512, 9000, 132, "one"),
+                                       (40, 131101, 513, "zipf"), (511, 70001, 1025, "uniform"), (12000, 48000, 20, "zipf"),
+                                       (12000, 47999, 20, "zipf"), (9000, 600000, 9, "uniform"), (16385, 70000, 5, "one"),
+                                       (262144, 900, 6, "zipf"), (262145, 3, 70, "zipf"), (270001, 1, 258, "one")])
+def test_gradient_written_once(n, V, d, how):
+    """Tables of 256 MB and more, few and many tokens, one run through all: nothing of what `out` held stays."""
+    g, ids = randn(n, d, seed=7), ids_of(n, V, 8, how)
+    got = torch.full((V, d), math.nan, device=DEV)
+    embedding_gradient(g, ids, V, 0.5, padding_idx=0 if V > 1 else None, out=got)
+    if V * d < 1 << 24:
+        check_gradient(got, g, ids, V, 0.5, 0 if V > 1 else None, torch.float32)
+    else:
+        rows = ids.unique()
+        rows = rows[rows != 0]
+        check_gradient(got[rows], g, torch.searchsorted(rows, ids) + (ids == 0) * len(rows), len(rows), 0.5, None, torch.float32)
+        got[rows] = 0
+        assert not bool(got.any())
+    if V * d < 1 << 24:
+        was = randn(V, d, seed=9)
+        more = was.clone()
+        embedding_gradient(g, ids, V, 0.5, padding_idx=0 if V > 1 else None, out=more, accumulate=True)
+        check_gradient(more, g, ids, V, 0.5, 0 if V > 1 else None, torch.float32, was)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("out", ["fp32", "bf16", "fp16"])
 def test_gradient_accumulates(out):
     n, V, d = 700, 900, 52
