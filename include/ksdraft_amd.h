@@ -762,7 +762,8 @@ int ksd_tc_quantize_grad(const void *g, int g_dtype, int64_t M, int64_t N, int64
  * A layer's calls on those. The float operands have row strides in elements; out_dtype and residual
  * as for ksd_tc_gemm.
  * ksd_tc_linear: quantizes x (M, K) and multiplies with stored codes w (N, K) in rows of ldw bytes
- * with scales sw; up to 32 tokens in one launch (ksd_tc_linear_workspace is then 0).
+ * with scales sw; up to 16 tokens of short rows (a quarter of M, rounded up, times K up to
+ * 8192) in one launch (ksd_tc_linear_workspace is then 0).
  * ksd_tc_linear_train: quantizes x and the float master w into x_codes, w_codes (rows of K rounded up
  * to 16 bytes) and their scales, then y; workspace as for ksd_tc_gemm of (M, N, K).
  * ksd_tc_linear_backward: dx (M, K) of dx_dtype, dw (N, K) fp32 and db (N,) fp32 (each may be NULL)

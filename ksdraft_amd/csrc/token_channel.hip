@@ -938,13 +938,13 @@ struct Few {
   int M, N, K, pitch;  // pitch: bytes of an LDS row of codes, = 16 mod 256 (16 rows on 16 bank groups)
 };
 
-template <int DT, int OUT, int MT>
+template <int DT, int OUT>
 __global__ __launch_bounds__(256) void few_rows_kernel(const Few p) {
   using T = typename Elem<DT>::T;
   constexpr int U = 6;  // W chunks in flight per wave
-  extern __shared__ __attribute__((aligned(16))) int8_t smem[];  // codes, then 2 x 4 x MT x 256 int32 and M scales
+  extern __shared__ __attribute__((aligned(16))) int8_t smem[];  // codes, then 2 x 4 x 256 int32 and M scales
   int32_t *const part = (int32_t *)(smem + (int64_t)p.M * p.pitch);
-  float *const sx = (float *)(part + 2 * 4 * MT * 256);
+  float *const sx = (float *)(part + 2 * 4 * 256);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c16 = lane & 15, g = lane >> 4;
   const int nk = (p.K + 63) / 64, kb = (p.K + 15) & ~15, tiles = (p.N + 15) / 16;
@@ -1009,74 +1009,50 @@ __global__ __launch_bounds__(256) void few_rows_kernel(const Few p) {
     }
   }
   __syncthreads();
-  const int8_t *arow[MT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i) arow[i] = smem + (int64_t)min(i * 16 + c16, p.M - 1) * p.pitch + g * 16;
+  const int8_t *const arow = smem + (int64_t)min(c16, p.M - 1) * p.pitch + g * 16;
   int par = 0;
   for (; t < tiles; t += gridDim.x, par ^= 1) {
-    v4i acc[MT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i) acc[i] = (v4i){0, 0, 0, 0};
+    v4i acc = (v4i){0, 0, 0, 0};
     for (int k0 = wave; k0 < nk; k0 += 4 * U) {
 #pragma unroll
       for (int i = 0; i < U; ++i) {
         const int k = k0 + i * 4;
-        if (k < nk) {
-#pragma unroll
-          for (int r = 0; r < MT; ++r)
-            acc[r] = __builtin_amdgcn_mfma_i32_16x16x64_i8(*(const v4i *)(arow[r] + k * 64), w[i], acc[r], 0, 0, 0);
-        }
+        if (k < nk) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(*(const v4i *)(arow + k * 64), w[i], acc, 0, 0, 0);
       }
       if (k0 + 4 * U < nk) load(t, k0 + 4 * U);
       else if (t + (int)gridDim.x < tiles) load(t + gridDim.x, wave);
     }
     if (wave >= nk && t + (int)gridDim.x < tiles) load(t + gridDim.x, wave);
-    int32_t *const q = part + (par * 4 + wave) * MT * 256;
+    int32_t *const q = part + (par * 4 + wave) * 256;
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) q[i * 256 + (g * 4 + r) * 16 + c16] = acc[i][r];
+    for (int r = 0; r < 4; ++r) q[(g * 4 + r) * 16 + c16] = acc[r];
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      const int m = i * 16 + (tid >> 4), n = t * 16 + (tid & 15);
-      if (m < p.M && n < p.N) {
-        const int32_t *z = part + par * 4 * MT * 256 + i * 256 + tid;
-        const int32_t sum = z[0] + z[MT * 256] + z[2 * MT * 256] + z[3 * MT * 256];
-        float y = ((float)sum * sx[m]) * p.sw[n];
-        const int64_t at = (int64_t)m * p.N + n;
-        if (p.bias) y += p.bias[n];
-        if (p.R) y += load_out<OUT>(p.R, at);
-        store_out<OUT>(p.Y, at, y);
-      }
+    const int m = tid >> 4, n = t * 16 + (tid & 15);
+    if (m < p.M && n < p.N) {
+      const int32_t *z = part + par * 4 * 256 + tid;
+      const int32_t sum = z[0] + z[256] + z[2 * 256] + z[3 * 256];
+      float y = ((float)sum * sx[m]) * p.sw[n];
+      const int64_t at = (int64_t)m * p.N + n;
+      if (p.bias) y += p.bias[n];
+      if (p.R) y += load_out<OUT>(p.R, at);
+      store_out<OUT>(p.Y, at, y);
     }
   }
 }
 
-static int few_lds(int64_t M, int64_t K) {
-  const int64_t pitch = cdiv(K, 256) * 256 + 16, mt = cdiv(M, 16);
-  const int64_t b = M * pitch + 2 * 4 * mt * 1024 + 4 * M;
-  return b <= 160 * 1024 ? (int)b : 0;
-}
-// Up to 32 tokens whose codes leave room for two workgroups on a CU. K: int32 sums.
-static bool few_rows(int64_t M, int64_t K) {
-  return M <= 32 && K <= 65536 && few_lds(M, K) > 0 && few_lds(M, K) <= 80 * 1024;
-}
+// Every workgroup quantizes all tokens, a wave a quarter of them one after the other: up to 8192 values of a
+// wave. (us, against quantizing and the product: 16 x 1536 -> 512 8.0 and 10.7, 24 tokens 10.6 and 11.4, 16 x 512 ->
+// 32003 11.8 and 9.5; 4 x 6869 -> 1792 12.6 and 13.3, 8 tokens 19.9 and 13.4; 1 x 16384 -> 1024 22 and 16.)
+static bool few_rows(int64_t M, int64_t K) { return M <= 16 && cdiv(M, 4) * K <= 8192; }
 
 template <int DT, int OUT>
 static void launch_few(const Few &p, hipStream_t st) {
-  const int lds = few_lds(p.M, p.K), mt = (p.M + 15) / 16;
-  const int per_cu = std::min(8, 160 * 1024 / lds);
+  const int lds = p.M * p.pitch + 2 * 4 * 1024 + 4 * p.M;  // at most 42 KB
+  // 4 workgroups on a CU: more quantize more often (16 x 512 -> 32003, us: 4 11.8, 8 15.7), fewer read W more
+  // slowly (4 x 1536 -> 150144: 4 38, 1 50).
+  const int per_cu = std::min(4, 160 * 1024 / lds);
   const unsigned grid = (unsigned)std::min<int64_t>(cdiv(p.N, 16), (int64_t)cu_count() * per_cu);
-  if (mt == 1) {
-    static const hipError_t set = hipFuncSetAttribute((const void *)few_rows_kernel<DT, OUT, 1>, hipFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024);
-    (void)set;
-    few_rows_kernel<DT, OUT, 1><<<grid, 256, lds, st>>>(p);
-  } else {
-    static const hipError_t set = hipFuncSetAttribute((const void *)few_rows_kernel<DT, OUT, 2>, hipFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024);
-    (void)set;
-    few_rows_kernel<DT, OUT, 2><<<grid, 256, lds, st>>>(p);
-  }
+  few_rows_kernel<DT, OUT><<<grid, 256, lds, st>>>(p);
 }
 template <int DT>
 static void launch_few(int out, const Few &p, hipStream_t st) {

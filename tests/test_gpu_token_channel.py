@@ -362,6 +362,22 @@ def test_operands_with_unknown_padding():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K", [(16, 33, 2048), (17, 33, 2048), (13, 20000, 129), (12, 40, 2730), (8, 50, 4096), (8, 50, 4097),
+                                   (5, 17, 3001), (4, 21, 8192), (4, 21, 8193), (1, 16500, 70)])
+def test_few_tokens(M, N, K):
+    """Either side of the one-launch form: the same bits as the quantizer and the product apart."""
+    x = data(M, K, "bf16", 1)
+    wq, ws = tc.quantize_rows(data(N, K, "fp32", 2, K ** -0.5))
+    bias, res = data(1, N, "fp32", 3)[0], data(M, N, "bf16", 4)
+    q, s = tc.quantize_rows(x)
+    y = tc.token_channel_linear(x, wq, ws, bias, res)
+    assert torch.equal(y, tc.token_channel_gemm(q, s, wq, ws, bias, res, out_dtype=torch.bfloat16))
+    sums = (q.cpu().double() @ wq.cpu().double().t()).float()
+    exact = ((sums * s.cpu()[:, None] * ws.cpu()) + bias.cpu() + res.float().cpu()).bfloat16()
+    assert torch.equal(y.cpu(), exact)
+
+
+@pytest.mark.gpu
 def test_empty_and_repeat():
     wq, ws = tc.quantize_rows(data(40, 64, "fp32", 1))
     x = torch.empty(0, 64, device=DEV)
