@@ -279,6 +279,34 @@ __global__ __launch_bounds__(256) void rank_scatter_kernel(const SortArgs a) {
   a.out_keys[to] = key_of(a.ids, a.wide, i, a.V, a.pad);
   a.out_pos[to] = i;
 }
+// Up to kPlace keys: 64 a workgroup, counted against a quarter of all by each wave and placed at once. (1024 tokens
+// of 942 by 93: the gradient takes 20 us, by the two launches above 24.)
+constexpr int kPlace = 2048;
+__global__ __launch_bounds__(256) void rank_place_kernel(const SortArgs a, unsigned counting, const Fill f) {
+  __shared__ __attribute__((aligned(16))) uint32_t others[kPlace];
+  __shared__ uint32_t part[4][64];
+  if (blockIdx.x >= counting) {
+    fill(f, blockIdx.x - counting);
+    return;
+  }
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = blockIdx.x * 64 + lane;
+#pragma unroll
+  for (int k = 0; k < kPlace / 256; ++k) others[k * 256 + threadIdx.x] = pair_of(a, k * 256 + threadIdx.x);
+  const uint32_t c = pair_of(a, i);
+  __syncthreads();
+  uint32_t less = 0;
+#pragma unroll 8
+  for (int j = wave * (kPlace / 4); j < (wave + 1) * (kPlace / 4); j += 4) {
+    const uint4 q = *(const uint4 *)(others + j);
+    less += (q.x < c) + (q.y < c) + (q.z < c) + (q.w < c);
+  }
+  part[wave][lane] = less;
+  __syncthreads();
+  if (wave > 0 || i >= a.n) return;
+  const uint32_t to = part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane];
+  a.out_keys[to] = c / kOne;
+  a.out_pos[to] = i;
+}
 
 // ------------------------------------------------------------------------------------ sums
 struct SumArgs {
@@ -531,7 +559,7 @@ __global__ __launch_bounds__(64 * kJoin) void join_kernel(const SumArgs a) {
 // Up to kFew tokens in one launch without a sort: workgroup b owns the rows b, b + grid, b + 2 grid, .. (so that
 // neighbouring frequent tokens meet different workgroups), lists the tokens of its rows in order, and sums or
 // clears its rows. (The sorted form's time hardly depends on the tokens, this one's grows with the most frequent
-// one's: 942 x 93, us: 512 tokens 7.6, a third of them equal 21, sorted 21; 2048 tokens 8.7 and 63 against 22.)
+// one's: 942 x 93, us: 512 tokens 7, all equal 52, sorted 16 to 20; 2048 tokens 22, 186, 19 to 21.)
 // Tables past kLarge are cleared by a launch of their own before (us: one token of 150144 x 1536, 922 MB, 143 and
 // here 167; 512 tokens of 32003 x 1792, 229 MB, 47 and 46).
 constexpr int64_t kLarge = (int64_t)256 << 20;
@@ -795,9 +823,15 @@ extern "C" int ksd_embedding_gradient(const void *g, int g_dtype, int64_t n, int
     s.out_keys = (uint32_t *)(w + l.keys[0]), s.out_pos = (int32_t *)(w + l.pos[0]);
     const bool blind = !accumulate && grid_fits(emb::fill_blocks(f) + 256, 256);
     if (blind) a.rows = 0;
-    const unsigned counting = (unsigned)(cdiv(n, 256) * cdiv(n, emb::kOthers));
-    emb::rank_count_kernel<<<counting + (blind ? (unsigned)emb::fill_blocks(f) : 0), 256, 0, st>>>(s, counting, f);
-    emb::rank_scatter_kernel<<<(unsigned)cdiv(n, 256), 256, 0, st>>>(s);
+    const unsigned clear = blind ? (unsigned)emb::fill_blocks(f) : 0;
+    if (n <= emb::kPlace) {
+      const unsigned counting = (unsigned)cdiv(n, 64);
+      emb::rank_place_kernel<<<counting + clear, 256, 0, st>>>(s, counting, f);
+    } else {
+      const unsigned counting = (unsigned)(cdiv(n, 256) * cdiv(n, emb::kOthers));
+      emb::rank_count_kernel<<<counting + clear, 256, 0, st>>>(s, counting, f);
+      emb::rank_scatter_kernel<<<(unsigned)cdiv(n, 256), 256, 0, st>>>(s);
+    }
   } else {
     const int rounds = emb::rounds_of(n);
     int passes;

@@ -96,7 +96,8 @@ def test_gradient(n, V, d, how, pad, dtype):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("n,V,d,how", [(1, 600, 70, "one"), (512, 300, 33, "zipf"), (513, 300, 33, "zipf"), (512, 9000, 132, "one"),
-                                       (40, 131101, 513, "zipf"), (511, 70001, 1025, "uniform"), (12000, 48000, 20, "zipf"),
+                                       (40, 131101, 513, "zipf"), (511, 70001, 1025, "uniform"), (514, 524287, 3, "one"), (1025, 524287, 2, "uniform"),
+                                       (2047, 800, 60, "zipf"), (2048, 40000, 19, "uniform"), (1999, 3, 258, "zipf"), (12000, 48000, 20, "zipf"),
                                        (12000, 47999, 20, "zipf"), (9000, 600000, 9, "uniform"), (16385, 70000, 5, "one"),
                                        (262144, 900, 6, "zipf"), (262145, 3, 70, "zipf"), (270001, 1, 258, "one")])
 def test_gradient_written_once(n, V, d, how):
