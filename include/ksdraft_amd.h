@@ -812,8 +812,9 @@ int ksd_embedding_gradient(const void *g, int g_dtype, int64_t n, int64_t d, int
  *   norm   = (max_kind ? max |g| : sqrt(sum g^2)) / loss_scale, summed in fp64 in a fixed order
  *   factor = min(1, max_norm / (norm + 1e-6)) / loss_scale (NULL: not formed)
  * ksd_grad_scale writes outs[i] = grads[i] * factor[0] (an outs[i] may be grads[i]; a factor of exactly
- * 1 then leaves its memory untouched). grads, outs, sizes (elements) and types (KSD_F32, KSD_BF16,
- * KSD_F16) are host arrays of n entries; the tensors are dense, at any alignment of the element type.
+ * 1 then leaves its memory untouched). No outs[i] may share memory with another tensor of either list
+ * (KSD_EINVAL). grads, outs, sizes (elements) and types (KSD_F32, KSD_BF16, KSD_F16) are host arrays of n
+ * entries; the tensors are dense, at any alignment of the element type.
  */
 int ksd_grad_norm_workspace(const int64_t *sizes, int n, int64_t *bytes);
 int ksd_grad_norm(const void *const *grads, const int64_t *sizes, const int32_t *types, int n,

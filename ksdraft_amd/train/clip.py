@@ -93,7 +93,8 @@ def gradient_norm(grads, max_norm: float = math.inf, norm_type: float = 2.0, los
 
 def clip_gradients(grads, max_norm: float, norm_type: float = 2.0, out=None, loss_scale: float = 1.0) -> torch.Tensor:
     """Multiplies every gradient by the factor above, in place or into ``out`` (contiguous tensors of the
-    same sizes and dtypes), and returns the norm (0-d, on the device)."""
+    same sizes and dtypes), and returns the norm (0-d, on the device). A tensor that is written may share no
+    memory with another of either list (ValueError): the tensors are scaled side by side."""
     grads = list(grads)
     out = None if out is None else list(out)
     _check(grads, out, norm_type, loss_scale)
@@ -108,10 +109,11 @@ def clip_gradients(grads, max_norm: float, norm_type: float = 2.0, out=None, los
 
 def clip_grad_norm_(parameters, max_norm: float, norm_type: float = 2.0, loss_scale: float = 1.0) -> torch.Tensor:
     """torch.nn.utils.clip_grad_norm_ on the parameters' gradients, in place (one that is not
-    contiguous through a copy)."""
+    contiguous through a copy). A parameter that is listed more than once (a tied weight gathered
+    module by module) counts and is scaled once."""
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
-    grads = [p.grad for p in parameters if p.grad is not None]
+    grads = [p.grad for p in {id(p): p for p in parameters}.values() if p.grad is not None]
     if not grads:
         return torch.tensor(0.0)
     copies = [(g, g.contiguous()) for g in grads if not g.is_sparse and not g.is_contiguous()]
