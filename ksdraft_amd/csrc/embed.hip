@@ -821,14 +821,13 @@ extern "C" int ksd_embedding_gradient(const void *g, int g_dtype, int64_t n, int
   int at = 0;
   if (n <= emb::kOne && V < (1 << 19)) {
     s.out_keys = (uint32_t *)(w + l.keys[0]), s.out_pos = (int32_t *)(w + l.pos[0]);
-    const bool blind = !accumulate && grid_fits(emb::fill_blocks(f) + 256, 256);
+    const unsigned counting = (unsigned)(n <= emb::kPlace ? cdiv(n, 64) : cdiv(n, 256) * cdiv(n, emb::kOthers));
+    const bool blind = !accumulate && grid_fits(emb::fill_blocks(f) + counting, 256);
     if (blind) a.rows = 0;
     const unsigned clear = blind ? (unsigned)emb::fill_blocks(f) : 0;
     if (n <= emb::kPlace) {
-      const unsigned counting = (unsigned)cdiv(n, 64);
       emb::rank_place_kernel<<<counting + clear, 256, 0, st>>>(s, counting, f);
     } else {
-      const unsigned counting = (unsigned)(cdiv(n, 256) * cdiv(n, emb::kOthers));
       emb::rank_count_kernel<<<counting + clear, 256, 0, st>>>(s, counting, f);
       emb::rank_scatter_kernel<<<(unsigned)cdiv(n, 256), 256, 0, st>>>(s);
     }
