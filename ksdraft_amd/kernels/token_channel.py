@@ -297,6 +297,7 @@ class TokenChannelLinear(nn.Module):
             return residual + self.forward(x)
         bias = self.bias if self.bias is None or self.bias.dtype == torch.float32 else self.bias.float()
         if torch.is_grad_enabled() and (self.weight.requires_grad or x.requires_grad
+                                        or (bias is not None and bias.requires_grad)
                                         or (residual is not None and residual.requires_grad)):
             self._packed = None
             return _LinearFunction.apply(x, self.weight, bias, residual)
