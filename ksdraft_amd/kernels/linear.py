@@ -284,6 +284,7 @@ class Int8Linear(nn.Module):
         # call unless an optimizer handed over the codes of the master as it is now
         # (_codes_current); dithered codes are redrawn every call
         train = torch.is_grad_enabled() and (self.weight.requires_grad or x.requires_grad
+                                             or (self.bias is not None and self.bias.requires_grad)
                                              or (residual is not None and residual.requires_grad))
         xpre = None
         fuse_res = (residual is not None and x.dtype in _OUT_DTYPES

@@ -6,11 +6,11 @@ A sum of M terms in fp32 is within M roundings of the magnitudes' sum of the exa
 import pytest
 import torch
 
-from ksdraft_amd.kernels import TokenChannelLinear
+from ksdraft_amd.kernels import Int8Linear, TokenChannelLinear
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
-LAYERS = [TokenChannelLinear]
+LAYERS = [TokenChannelLinear, Int8Linear]
 
 
 @pytest.mark.parametrize("layer", LAYERS)
