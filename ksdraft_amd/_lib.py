@@ -202,6 +202,19 @@ def put(module: torch.nn.Module, **values) -> None:
 _buffer_hooks = getattr(torch.nn.modules.module, "_global_buffer_registration_hooks", {})
 
 
+def wrote(tensors) -> None:
+    """Counts a kernel's writes into a caller's tensors in their versions, as torch's in-place
+    operations do: autograd refuses a backward that needs the old values, and codes or caches
+    kept under a version go stale (20 us for 400 tensors). Inference tensors have no version."""
+    try:
+        _increment_version(tensors)
+    except RuntimeError:
+        _increment_version([t for t in tensors if not t.is_inference()])
+
+
+_increment_version = torch.autograd.graph.increment_version
+
+
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 

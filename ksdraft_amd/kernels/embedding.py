@@ -209,6 +209,7 @@ def embedding_gradient(grad: torch.Tensor, ids: torch.Tensor, num_embeddings: in
     flat = _check_ids(ids, V, check_ids)
     g = _dense_rows(grad if grad.dim() == 2 else grad.reshape(flat.numel(), d))
     n = flat.numel()
+    given = out is not None
     if out is None:
         out = torch.empty((V, d), dtype=out_dtype, device=dev)
     need = ctypes.c_int64()
@@ -217,6 +218,8 @@ def embedding_gradient(grad: torch.Tensor, ids: torch.Tensor, num_embeddings: in
     _lib.call("ksd_embedding_gradient", g.data_ptr(), _OUT[g.dtype], n, d, g.stride(0) if n > 1 else d, flat.data_ptr(),
               int(flat.dtype == torch.int64), V, pad, scale, int(accumulate), out.data_ptr(), _OUT[out_dtype],
               work.data_ptr(), need.value, _lib.stream_ptr(dev))
+    if given:
+        _lib.wrote((out,))
     return out
 
 

@@ -104,6 +104,7 @@ def clip_gradients(grads, max_norm: float, norm_type: float = 2.0, out=None, los
     res = _norm(t, norm_type, max_norm, loss_scale)
     _lib.call("ksd_grad_scale", _at(t.grads), _at(t.outs), _at(t.sizes), _at(t.types), t.n, res.data_ptr() + 4,
               _lib.stream_ptr(t.dev))
+    _lib.wrote(grads if out is None else out)
     return res[0]
 
 
