@@ -187,6 +187,7 @@ def adamw_requant_(param: torch.Tensor, grad: torch.Tensor, exp_avg: torch.Tenso
               1 - lr * weight_decay, 1 - beta1, beta2, 1 - beta2, eps, lr / bc1, bc2 ** 0.5,
               group, 0 if codes is None else codes.data_ptr(),
               0 if scales is None else scales.data_ptr(), _lib.stream_ptr(dev))
+    _lib.wrote((param, exp_avg, exp_avg_sq))
     return None if codes is None else (codes, scales)
 
 
@@ -241,6 +242,7 @@ def adamw_requant_multi_(items, lr: float, betas=(0.9, 0.999), eps: float = 1e-8
     cc = None if clip_coef is None else clip_coef.to(dtype=torch.float32).reshape(1).contiguous()
     _lib.call("ksd_adamw_requant_multi", arr.ctypes.data, len(items), 0 if cc is None else cc.data_ptr(),
               1 - lr * weight_decay, 1 - beta1, beta2, 1 - beta2, eps, group, _lib.stream_ptr(dev))
+    _lib.wrote([t for it in items for t in (it[0], it[2], it[3])])
     return out
 
 

@@ -4,6 +4,8 @@ import pytest
 import torch
 
 from ksdraft_amd.kernels.embedding import embedding_gradient
+from ksdraft_amd.kernels import Int8Linear
+from ksdraft_amd.train import AdamWRequant, adamw_requant_, adamw_requant_multi_
 from ksdraft_amd.train.clip import clip_grad_norm_, clip_gradients, gradient_norm
 
 pytestmark = pytest.mark.gpu
@@ -46,6 +48,38 @@ def test_embedding_gradient():
         was = out._version
         embedding_gradient(g, ids, 5, out=out, accumulate=accumulate)
         assert out._version > was
+
+
+@pytest.mark.parametrize("multi", [False, True])
+@pytest.mark.parametrize("quantize", [False, True])
+def test_optimizer_kernels(multi, quantize):
+    p, g, m, v = (torch.ones(8, 128, device=DEV) for _ in range(4))
+    was = versions([p, g, m, v])
+    if multi:
+        adamw_requant_multi_([(p, g, m, v, 1, quantize)], 1e-3)
+    else:
+        adamw_requant_(p, g, m, v, 1, 1e-3, quantize=quantize)
+    now = versions([p, g, m, v])
+    assert [a > b for a, b in zip(now, was)] == [True, False, True, True]
+
+
+def test_optimizer_step():
+    """Fused masters and torch's small ones alike; the registered layer's codes stay current, those of
+    another layer on the same master do not."""
+    lin, tied = Int8Linear(256, 512).to(DEV), Int8Linear(256, 512, bias=False).to(DEV)
+    tied.weight = lin.weight
+    plain = torch.nn.Parameter(torch.ones(1 << 17, device=DEV))
+    opt = AdamWRequant([*lin.parameters(), plain], lr=1e-2)
+    opt.register_int8(tied)
+    opt.register_int8(lin)
+    params = [lin.weight, lin.bias, plain]
+    for _ in range(2):
+        for p in params:
+            p.grad = torch.ones_like(p)
+        was = versions(params)
+        opt.step()
+        assert all(a > b for a, b in zip(versions(params), was))
+        assert lin._codes_current() and not tied._codes_current()
 
 
 def test_inference_tensors():
