@@ -252,8 +252,10 @@ class TokenChannelLinear(nn.Module):
     """nn.Linear with int8 products in both directions, scales per token and per output channel.
 
     The float master ``weight`` stays authoritative: its codes are rebuilt in every call, unless
-    ``pack()`` has stored them (serving: the master no longer changes); ``unpack()``, training
-    calls, moves and state-dict loads drop stored codes."""
+    ``pack()`` has stored them (serving). Stored codes belong to the master's tensor, storage and
+    version at that time: a call that finds another rebuilds and stores them again (a write that
+    torch does not version, through ``weight.data`` or a raw pointer, needs another ``pack()``).
+    ``unpack()``, training calls, moves and state-dict loads drop them."""
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True):
         super().__init__()
@@ -261,7 +263,7 @@ class TokenChannelLinear(nn.Module):
         self.out_features = out_features
         self.weight = nn.Parameter(torch.zeros(out_features, in_features))
         self.bias = nn.Parameter(torch.zeros(out_features)) if bias else None
-        self._packed = None
+        self._packed = self._packed_of = None  # codes and scales, and the master that they are of
 
     @classmethod
     def from_float(cls, module: nn.Linear) -> "TokenChannelLinear":
@@ -276,18 +278,30 @@ class TokenChannelLinear(nn.Module):
     def pack(self) -> "TokenChannelLinear":
         """Stores the codes of the master as it is now for calls without gradients."""
         self._packed = quantize_rows(self.weight.detach())
+        self._packed_of = self._master()
         return self
 
+    def _master(self):
+        w = self.weight
+        return w, w.data_ptr(), 0 if w.is_inference() else w._version
+
+    def _stored(self):
+        if self._packed is not None:
+            (was, at, version), (w, now_at, now) = self._packed_of, self._master()
+            if was is not w or at != now_at or version != now:
+                self.pack()
+        return self._packed
+
     def unpack(self) -> "TokenChannelLinear":
-        self._packed = None
+        self._packed = self._packed_of = None
         return self
 
     def _apply(self, fn, *args, **kwargs):
-        self._packed = None
+        self.unpack()
         return super()._apply(fn, *args, **kwargs)
 
     def _load_from_state_dict(self, *args, **kwargs):
-        self._packed = None
+        self.unpack()
         return super()._load_from_state_dict(*args, **kwargs)
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
@@ -299,7 +313,7 @@ class TokenChannelLinear(nn.Module):
         if torch.is_grad_enabled() and (self.weight.requires_grad or x.requires_grad
                                         or (bias is not None and bias.requires_grad)
                                         or (residual is not None and residual.requires_grad)):
-            self._packed = None
+            self.unpack()
             return _LinearFunction.apply(x, self.weight, bias, residual)
-        codes, scales = self._packed or quantize_rows(self.weight.detach())
+        codes, scales = self._stored() or quantize_rows(self.weight.detach())
         return token_channel_linear(x, codes, scales, None if bias is None else bias.detach(), residual)
