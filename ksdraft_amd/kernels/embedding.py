@@ -19,6 +19,7 @@ import ctypes
 
 import torch
 from torch import nn
+from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from .quant import GROUP_SIZE, SCALE_DTYPE, quantize_last_dim
@@ -231,6 +232,7 @@ class _ScaledLookup(torch.autograd.Function):
         return embedding_lookup(weight, ids, scale, out_dtype, check_ids)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad):
         (ids,) = ctx.saved_tensors
         V, scale, pad, dtype = ctx.args

@@ -21,6 +21,7 @@ import ctypes
 
 import torch
 from torch import nn
+from torch.autograd.function import once_differentiable
 
 from .. import _lib
 
@@ -237,6 +238,7 @@ class _LinearFunction(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad):
         s = Saved()
         s.xq, s.xs, s.wq, s.ws = ctx.saved_tensors
