@@ -263,6 +263,9 @@ class ScaledEmbedding(nn.Module):
 
     @classmethod
     def from_float(cls, module: nn.Embedding, scale: float = 1.0, **kwargs) -> "ScaledEmbedding":
+        for name in ("max_norm", "scale_grad_by_freq", "sparse"):
+            if getattr(module, name) not in (None, False):
+                raise ValueError(f"ScaledEmbedding has no {name}, and the embedding's is {getattr(module, name)}")
         emb = cls(module.num_embeddings, module.embedding_dim, scale, module.padding_idx, **kwargs)
         emb.weight = module.weight  # the same master (a tied head keeps its tie)
         return emb
