@@ -253,6 +253,8 @@ class ScaledEmbedding(nn.Module):
     def __init__(self, num_embeddings: int, embedding_dim: int, scale: float = 1.0, padding_idx: int | None = None,
                  out_dtype: torch.dtype | None = None, check_ids: bool = True):
         super().__init__()
+        if padding_idx is not None and not -num_embeddings <= padding_idx < num_embeddings:
+            raise ValueError(f"padding_idx {padding_idx} is out of range for {num_embeddings} rows")
         self.num_embeddings = num_embeddings
         self.embedding_dim = embedding_dim
         self.scale = float(scale)

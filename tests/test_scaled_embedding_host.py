@@ -16,3 +16,11 @@ def test_from_float_keeps_the_master():
     emb = torch.nn.Embedding(10, 4, padding_idx=-2)
     mod = ScaledEmbedding.from_float(emb, 2.0, out_dtype=torch.bfloat16, check_ids=False)
     assert mod.weight is emb.weight and (mod.padding_idx, mod.scale, mod.out_dtype, mod.check_ids) == (8, 2.0, torch.bfloat16, False)
+
+
+@pytest.mark.parametrize("idx", [10, -11, 1 << 40])
+def test_padding_out_of_range(idx):
+    """Refused at once, not in the first backward."""
+    with pytest.raises(ValueError, match="padding_idx"):
+        ScaledEmbedding(10, 4, padding_idx=idx)
+    assert ScaledEmbedding(10, 4, padding_idx=-10).padding_idx == -10
