@@ -178,6 +178,12 @@ static void launch_rows(const Rows &a, int t, hipStream_t st) {
 // and 5.4 TB/s.)
 // A wave takes `rows` (a multiple of 16) x 64 V columns: lane l holds columns V l .. V l + V - 1, 16 rows'
 // loads in flight. A row's maximum crosses the lanes through LDS, 16 rows at once.
+// Row blocks run along y, and along z past the 65535 that y holds.
+__device__ __forceinline__ int64_t row_block() { return (int64_t)blockIdx.z * gridDim.y + blockIdx.y; }
+static dim3 row_grid(int64_t x, int64_t rows) {
+  const int64_t z = cdiv(rows, 65535);
+  return dim3((unsigned)x, (unsigned)cdiv(rows, z), (unsigned)z);
+}
 template <int DT, int V>
 __device__ __forceinline__ void load_vec(const typename Elem<DT>::T *p, float *v) {
   if constexpr (V == 8) {
@@ -207,9 +213,9 @@ __global__ __launch_bounds__(256) void grad_stats_kernel(const void *__restrict_
   __shared__ uint32_t rmax_all[4][16][65];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   uint32_t(*const rmax)[65] = rmax_all[wave];
-  const int64_t cb = (int64_t)blockIdx.x * 4 + wave, rb = blockIdx.y, c = (cb * 64 + lane) * V;
+  const int64_t cb = (int64_t)blockIdx.x * 4 + wave, rb = row_block(), c = (cb * 64 + lane) * V;
   const int64_t m0 = rb * rows, m1 = min(M, m0 + rows);
-  if (cb * 64 * V >= N) return;
+  if (cb * 64 * V >= N || m0 >= M) return;
   const bool cols = (cb + 1) * 64 * V <= N;
   float w[V], sum[V];
   uint32_t cm[V];
@@ -312,7 +318,7 @@ __global__ __launch_bounds__(256) void grad_codes_kernel(const void *__restrict_
                                                          int8_t *__restrict__ q, int8_t *__restrict__ cq, int64_t ld) {
   using T = typename Elem<DT>::T;
   const int64_t c = ((int64_t)blockIdx.x * 64 + (threadIdx.x & 63)) * 8;
-  const int64_t m0 = (int64_t)blockIdx.y * (32 * H) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * (8 * H);
+  const int64_t m0 = row_block() * (32 * H) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * (8 * H);
   if (c >= ld) return;
   const bool cols = (int64_t)(blockIdx.x + 1) * 512 <= N;
   float w[8], fi[8];
@@ -1163,12 +1169,12 @@ extern "C" int ksd_tc_quantize_grad(const void *g, int g_dtype, int64_t M, int64
   const int rows = tc::stats_rows(M, N);
   const bool large = tc::large_grad(M, N);
   const int64_t ncb = cdiv(N, large && g_dtype != KSD_F32 ? 512 : 256), nrb = cdiv(M, rows);
-  if (nrb > 65535 || cdiv(M, 32) > 65535) return fail(KSD_EINVAL, "tc_quantize_grad: too many rows");
+  if (!grid_fits(cdiv(M, 64) + cdiv(N, 64), 1024)) return fail(KSD_EINVAL, "tc_quantize_grad: too many rows or columns");
   uint32_t *row_part = (uint32_t *)workspace, *col_part = row_part + ncb * M;
   float *sum_part = (float *)(col_part + nrb * N), *einv = sum_part + nrb * N, *finv = einv + M;
   float *sums = db ? sum_part : nullptr;
   hipStream_t st = (hipStream_t)stream;
-  const dim3 gs((unsigned)cdiv(ncb, 4), (unsigned)nrb), gq((unsigned)cdiv(ld, 512), (unsigned)cdiv(M, large ? 64 : 32));
+  const dim3 gs = tc::row_grid(cdiv(ncb, 4), nrb), gq = tc::row_grid(cdiv(ld, 512), cdiv(M, large ? 64 : 32));
   const unsigned folds = (unsigned)(cdiv(M, 64) + cdiv(N, 64));
 #define KSD_TC(DT, V)                                                                                                  \
   if (large) tc::grad_stats_kernel<DT, V><<<gs, 256, 0, st>>>(g, M, N, stride, rows, sx, sw, row_part, col_part, sums); \
