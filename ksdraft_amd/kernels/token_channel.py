@@ -109,13 +109,14 @@ def _gemm(a, lda, a_t, sa, w, ldw, w_t, sw, M, N, K, bias, residual, out_dtype, 
     return y
 
 
-def _epilogue(M: int, N: int, bias, residual, out_dtype):
+def _epilogue(lead, N: int, bias, residual, out_dtype):
+    """Checks what is added to an output (*lead, N)."""
     if out_dtype not in _OUT:
         raise TypeError(f"unsupported output dtype {out_dtype}")
     bias = _vector(bias, N, "bias")
     if residual is not None:
-        if residual.shape != (M, N) or residual.dtype != out_dtype:
-            raise ValueError(f"residual must be ({M}, {N}) {out_dtype}, got {tuple(residual.shape)} {residual.dtype}")
+        if residual.shape != (*lead, N) or residual.dtype != out_dtype:
+            raise ValueError(f"residual must be {(*lead, N)} {out_dtype}, got {tuple(residual.shape)} {residual.dtype}")
         residual = residual.contiguous()
     return bias, residual
 
@@ -132,7 +133,7 @@ def token_channel_gemm(a_codes: torch.Tensor, a_scales: torch.Tensor, w_codes: t
     (M, K), (N, Kw) = a_codes.shape, w_codes.shape
     if K != Kw:
         raise ValueError(f"a_codes has {K} columns, w_codes {Kw}")
-    bias, residual = _epilogue(M, N, bias, residual, out_dtype)
+    bias, residual = _epilogue((M,), N, bias, residual, out_dtype)
     return _gemm(a, lda, 0, _vector(a_scales, M, "a_scales"), w, ldw, 0, _vector(w_scales, N, "w_scales"), M, N, K,
                  bias, residual, out_dtype, dev)
 
@@ -152,9 +153,7 @@ def token_channel_linear(x: torch.Tensor, w_codes: torch.Tensor, w_scales: torch
     x2 = _matrix(x if flat else x.reshape(-1, K), "x")
     M = x2.shape[0]
     out_dtype = out_dtype or x.dtype
-    if residual is not None and not flat:
-        residual = residual.reshape(-1, N)
-    bias, residual = _epilogue(M, N, bias, residual, out_dtype)
+    bias, residual = _epilogue(x.shape[:-1], N, bias, residual, out_dtype)
     w_scales = _vector(w_scales, N, "w_scales")
     y = torch.empty((M, N) if flat else (*x.shape[:-1], N), dtype=out_dtype, device=dev)
     need = ctypes.c_int64()
@@ -185,7 +184,7 @@ def token_channel_linear_train(x: torch.Tensor, weight: torch.Tensor, bias: torc
     x2 = _matrix(x.reshape(-1, K), "x")
     s = Saved()
     s.M, s.N, s.K, s.dtype, s.lead, s.has_bias = x2.shape[0], N, K, x.dtype, x.shape[:-1], bias is not None
-    bias, residual = _epilogue(s.M, N, bias, None if residual is None else residual.reshape(-1, N), x.dtype)
+    bias, residual = _epilogue(s.lead, N, bias, residual, x.dtype)
     M, ld = s.M, _pitch(K)
     codes = torch.empty((M + N, ld), dtype=torch.int8, device=dev)
     scales = torch.empty(M + N, dtype=torch.float32, device=dev)
