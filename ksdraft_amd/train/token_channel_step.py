@@ -6,8 +6,8 @@
     clip       train.clip.gradient_norm over every gradient; the factor goes to the optimizer
     optimizer  AdamWRequant (the factor applied as the gradients are loaded)
 
-``to_token_channel(model)`` converts a float model; apart from the losses' target check nothing is
-read back to the host.
+``to_token_channel(model)`` converts a float model. The host reads back two checks a step, that the
+inputs and that the targets are tokens; a model converted with ``check_ids=False`` reads back nothing.
 """
 
 from __future__ import annotations
@@ -23,10 +23,24 @@ from .clip import gradient_norm
 from .int8_step import Int8DraftTrainer, _check_loss_scale, transfer_space_loss
 
 
+def check_targets(tgt: torch.Tensor, V: int, check: bool) -> torch.Tensor:
+    """The targets as the losses take them. All must be tokens (a masked target has no row for the
+    transfer term): IndexError, before anything runs on them (a host read). Unchecked, those out of
+    range become IGNORE_INDEX, on which torch's cross entropy does not abort."""
+    bad = (tgt < 0) | (tgt >= V)
+    if not check:
+        return tgt.masked_fill(bad, IGNORE_INDEX)
+    if bool(bad.any()):
+        raise IndexError(f"target {int(tgt[bad][0])} is out of range for {V} rows")
+    return tgt
+
+
 class TokenChannelTrainer(Int8DraftTrainer):
     """Int8DraftTrainer's interface (``loss``, ``backward``, ``optimizer_step``, ``step``) on a
     ``to_token_channel`` model. ``grad_norm`` holds the last step's gradient norm (0-d, on the
-    device)."""
+    device). Every target must be a token. Where the model does not check its ids, an input out of
+    range is a row of zeros, a target out of range is left out of the cross entropy and counts as a
+    cosine of 0 in the transfer term."""
 
     def __init__(self, model, lr: float = 3e-4, betas=(0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 0.01, grad_clip: float = 1.0, transfer_weight: float = 0.5,
@@ -46,12 +60,11 @@ class TokenChannelTrainer(Int8DraftTrainer):
 
     def loss(self, tokens: torch.Tensor, teacher_states: torch.Tensor | None = None):
         """(loss, ce, transfer) as device tensors, with the graph for backward."""
-        model = self.model
-        inp, tgt = tokens[:, :-1], tokens[:, 1:]
+        model, emb = self.model, self.model.embedding
+        inp, tgt = tokens[:, :-1], check_targets(tokens[:, 1:], emb.num_embeddings, emb.check_ids)
         h, features = model.backbone(inp, teacher_states)
-        # the targets' rows: the batch's ids were checked by the lookup, its last column's here
-        rows = scaled_rows(model.embedding.weight, tgt, check_ids=model.embedding.check_ids)
-        ts = transfer_space_loss(features, model.embedding.weight, tgt, rows=rows)
+        rows = scaled_rows(emb.weight, tgt, check_ids=False)
+        ts = transfer_space_loss(features, emb.weight, tgt, rows=rows)
         logits = model.head(h.reshape(-1, h.shape[-1]))
         ce = F.cross_entropy(logits.float(), tgt.reshape(-1), ignore_index=IGNORE_INDEX)
         return ce + self.transfer_weight * ts, ce, ts
