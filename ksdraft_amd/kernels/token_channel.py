@@ -12,18 +12,27 @@ dY is quantized,
     dX = e[m] sum_n q[m, n] wq[n, k],   (q, e) = quantize_rows(dY * sw)
     dW = f[n] sum_m c[m, n] xq[m, k],   (c, f) = the same per column of dY * sx
 
+What of a row of dY * sw (dX) or a column of dY * sx (dW) lies below 1/254 of the largest value there
+is lost. That is a small part of a projection's gradient and nearly all of a vocabulary head's: a cross
+entropy's dY is about -1 at the target and a probability elsewhere, and at 20000 classes the target's
+code is the only one left of a row. Such a layer takes its gradients from dY in groups of 128
+(``group_gradient``).
+
 ``TokenChannelLinear`` is an nn.Linear drop-in on them. There is no CPU path.
 """
 
 from __future__ import annotations
 
 import ctypes
+import math
 
 import torch
 from torch import nn
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
+from .linear import w8a8_linear_backward
+from .quant import quantize_dual
 
 _OUT = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 
@@ -249,8 +258,59 @@ class _LinearFunction(torch.autograd.Function):
         return dx, None if dw is None else dw.to(ctx.weight_dtype), db, grad if need[3] else None
 
 
+def _lift(g: torch.Tensor):
+    """(g * s, 1 / s) for the power of two s that brings max |g| to [2^20, 2^21), without a host read.
+    The groups' fp16 scales keep all their bits from 2^-14 on, so 28 binades below the largest value do
+    (a mean loss over 8192 tokens has probabilities near 1e-9 in its gradient). For a g with NaN or inf
+    the second is NaN: a group's code of inf is finite."""
+    from ..train.clip import gradient_norm
+    if g.dtype == torch.float16:
+        g = g.float()  # 2^20 is past its range
+    top = gradient_norm([g], norm_type=math.inf)[0].view(torch.int32) >> 23  # biased exponent
+    shift = torch.where(top == 255, 0, 127 + 20 - top).clamp(max=126)
+    s = ((127 + shift) << 23).view(torch.float32)
+    back = torch.where(top == 255, 0x7fc00000, (127 - shift) << 23).view(torch.float32)
+    return g * s.to(g.dtype), back
+
+
+class _GroupGradientFunction(torch.autograd.Function):
+    """_LinearFunction's forward with Int8Linear's backward: dY, X and W in groups of 128 along what
+    each product contracts."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual):
+        y, saved = token_channel_linear_train(x, weight, bias, residual)
+        ctx.shape = (saved.M, saved.N, saved.K, x.dtype, saved.lead)
+        xt = (None, None)
+        if ctx.needs_input_grad[1] and saved.M:  # dW's operand instead of x itself
+            xt = quantize_dual(x.reshape(-1, saved.K), t_from_codes=True)[2:]
+        ctx.save_for_backward(weight, *xt)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        weight, *xt = ctx.saved_tensors
+        M, N, K, dtype, lead = ctx.shape
+        need_dx, need_dw, need_db, need_res = ctx.needs_input_grad
+        g = grad if grad.dtype in _OUT else grad.float()
+        dres = g if need_res else None
+        if M == 0 or not (need_dx or need_dw):
+            return (torch.empty((*lead, K), dtype=dtype, device=g.device) if need_dx else None,
+                    torch.zeros_like(weight) if need_dw else None, g.reshape(-1, N).float().sum(0) if need_db else None, dres)
+        g, back = _lift(g.reshape(-1, N).contiguous())
+        wt = quantize_dual(weight.float(), t_from_codes=True)[2:] if need_dx else None
+        dx, dw, *db = w8a8_linear_backward(g, None, None, None, None, need_dx=need_dx, need_dw=need_dw,
+                                           xt=xt if need_dw else None, wt=wt, want_db=need_db)
+        return ((dx * back).to(dtype).reshape(*lead, K) if need_dx else None,
+                dw.mul_(back).to(weight.dtype) if need_dw else None, db[0] * back if need_db else None, dres)
+
+
 class TokenChannelLinear(nn.Module):
     """nn.Linear with int8 products in both directions, scales per token and per output channel.
+    With ``group_gradient`` the backward's operands have a scale per 128 values of what is contracted,
+    as Int8Linear's: for a layer whose upstream gradient holds values of very different size in one
+    row, as a vocabulary head's.
 
     The float master ``weight`` stays authoritative: its codes are rebuilt in every call, unless
     ``pack()`` has stored them (serving). Stored codes belong to the master's tensor, storage and
@@ -258,17 +318,18 @@ class TokenChannelLinear(nn.Module):
     torch does not version, through ``weight.data`` or a raw pointer, needs another ``pack()``).
     ``unpack()``, training calls, moves and state-dict loads drop them."""
 
-    def __init__(self, in_features: int, out_features: int, bias: bool = True):
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, group_gradient: bool = False):
         super().__init__()
         self.in_features = in_features
         self.out_features = out_features
+        self.group_gradient = group_gradient
         self.weight = nn.Parameter(torch.zeros(out_features, in_features))
         self.bias = nn.Parameter(torch.zeros(out_features)) if bias else None
         self._packed = self._packed_of = None  # codes and scales, and the master that they are of
 
     @classmethod
-    def from_float(cls, module: nn.Linear) -> "TokenChannelLinear":
-        lin = cls(module.in_features, module.out_features, bias=module.bias is not None)
+    def from_float(cls, module: nn.Linear, group_gradient: bool = False) -> "TokenChannelLinear":
+        lin = cls(module.in_features, module.out_features, module.bias is not None, group_gradient)
         lin = lin.to(module.weight.device)
         with torch.no_grad():
             lin.weight.copy_(module.weight)
@@ -315,6 +376,7 @@ class TokenChannelLinear(nn.Module):
                                         or (bias is not None and bias.requires_grad)
                                         or (residual is not None and residual.requires_grad)):
             self.unpack()
-            return _LinearFunction.apply(x, self.weight, bias, residual)
+            function = _GroupGradientFunction if self.group_gradient else _LinearFunction
+            return function.apply(x, self.weight, bias, residual)
         codes, scales = self._stored() or quantize_rows(self.weight.detach())
         return token_channel_linear(x, codes, scales, None if bias is None else bias.detach(), residual)

@@ -74,9 +74,10 @@ def to_int8(model: KSDraftModel, group: int = 128, nonlinear: str = "int8", *,
 def to_token_channel(model: KSDraftModel, group: int = 128, nonlinear: str = "int8", *,
                      embedding_scale: float = 1.0, check_ids: bool = True) -> KSDraftModel:
     """A copy of the model for training with int8 products scaled per token and channel: Rosa
-    q/k/v/out, ``teacher_proj`` and the tied head become TokenChannelLinear, the embedding a
-    ScaledEmbedding on the head's weight (rows times embedding_scale), the FFNs trainable
-    KS3Int8Cells as in ``to_int8``; norms, vectors and the injection stay float."""
+    q/k/v/out, ``teacher_proj`` and the tied head become TokenChannelLinear (the head's gradients in
+    groups of 128), the embedding a ScaledEmbedding on the head's weight (rows times
+    embedding_scale), the FFNs trainable KS3Int8Cells as in ``to_int8``; norms, vectors and the
+    injection stay float."""
     conv = copy.deepcopy(model)
     swapped = 0
     for block in conv.blocks:
@@ -88,7 +89,8 @@ def to_token_channel(model: KSDraftModel, group: int = 128, nonlinear: str = "in
     if conv.teacher_proj is not None:
         conv.teacher_proj = TokenChannelLinear.from_float(conv.teacher_proj)
         swapped += 1
-    head = TokenChannelLinear(conv.head.in_features, conv.head.out_features, bias=False)
+    # a cross entropy's gradient over a vocabulary needs more than a scale per token
+    head = TokenChannelLinear(conv.head.in_features, conv.head.out_features, bias=False, group_gradient=True)
     head.weight = conv.embedding.weight  # tied, as KSDraftModel ties its head
     conv.head = head
     conv.embedding = ScaledEmbedding.from_float(conv.embedding, embedding_scale, check_ids=check_ids)

@@ -1,7 +1,8 @@
 """A training step of the draft model with int8 products scaled per token and output channel:
 
     lookup     ScaledEmbedding (its gradient by sorted tokens, without atomics)
-    linears    TokenChannelLinear: y, dX and dW as int8 products on the same codes
+    linears    TokenChannelLinear: y, dX and dW as int8 products on the same codes (the head's dX
+               and dW in groups of 128)
     loss       cross entropy of the head's logits + transfer_weight * the transfer term
     clip       train.clip.gradient_norm over every gradient; the factor goes to the optimizer
     optimizer  AdamWRequant (the factor applied as the gradients are loaded)
