@@ -180,3 +180,30 @@ def test_int8_head_agrees():
         grads.append((xg.grad.double().cpu(), head.weight.grad.double().cpu()))
     _, _, bx, bw = bounds(dy.double().cpu(), x.double().cpu(), head.weight.detach().double().cpu())
     assert bool(((grads[0][0] - grads[1][0]).abs() <= 2 * bx).all()) and bool(((grads[0][1] - grads[1][1]).abs() <= 2 * bw).all())
+
+
+def test_captured_step():
+    """Captured, the layer's calls give the eager bits on every replay."""
+    lin = TokenChannelLinear.from_float(torch.nn.Linear(256, 1000).to(DEV), group_gradient=True)
+    g = torch.Generator().manual_seed(0)
+    x = torch.randn(300, 256, generator=g).to(DEV).requires_grad_(True)
+    dy = torch.randn(300, 1000, generator=g).to(DEV)
+
+    def step():
+        y = lin(x)
+        return [y.detach(), *torch.autograd.grad(y, [x, lin.weight, lin.bias], dy)]
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for k in range(4):
+        dy.mul_(0.5)  # another lift each time
+        for t in held:
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, step()))
+        torch.cuda.synchronize()
