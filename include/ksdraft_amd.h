@@ -795,8 +795,8 @@ int ksd_embedding_lookup(const void *table, int table_dtype, int64_t V, int64_t 
                          const void *ids, int ids_wide, int64_t n, float scale, void *out,
                          int out_dtype, void *stream);
 /*
- * Its gradient: out[v] (+)= scale * sum of g[i] over ids[i] = v, positions in order, fp32 sums,
- * without the id `padding` (-1 for none) and ids out of range. g (n, d) of row stride `stride`; out
+ * Its gradient: out[v] (+)= scale * sum of g[i] over ids[i] = v, fp32 sums in an order that the ids and
+ * sizes fix, without the id `padding` (-1 for none) and ids out of range. g (n, d) of row stride `stride`; out
  * (V, d) dense, 16-byte aligned; accumulate = 0 writes all of it, else only the rows of ids that
  * occur are read and written. The same inputs give the same bits on every call.
  */

@@ -214,8 +214,8 @@ static int check(const List &l, const char *who, bool out) {
 }
 
 // Two workgroups must not write one element, nor one read what another writes: an output's memory may meet
-// its own gradient's only where both are the same, and no other tensor's. (392 tensors in any order: 10 us of host
-// while the norm runs.)
+// its own gradient's only where both are the same, and no other tensor's. (392 tensors in any order: 6 us of host in
+// place, 14 into other tensors, while the norm runs.)
 struct Span {
   uintptr_t lo, hi;
   int i;

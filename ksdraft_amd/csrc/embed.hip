@@ -1,12 +1,14 @@
 // Embedding lookup with a scale, and the table's gradient by sorted tokens.
 //
 //   y[i]  = round(scale * W[id_i])
-//   dW[v] = scale * sum of g[i] over the positions i with id_i = v, in the order of i, in fp32
+//   dW[v] = scale * sum of g[i] over the positions i with id_i = v, in fp32
 //
 // The positions are sorted by token (stable radix sort), so every token's rows are one run of the
-// sorted list and no float atomics are needed: the sums have a fixed order and repeated calls give
-// the same bits. Runs are cut at multiples of 32 sorted positions, so a token that fills the batch
-// is spread over the device like any other; the pieces of a cut run are joined in order.
+// sorted list and no float atomics are needed. Runs are cut at multiples of 16 or 32 sorted positions, so a
+// token that fills the batch is spread over the device like any other. Rows are added in the order of
+// their positions within a piece, the pieces of a cut run in order, a long run's in 16 shares whose sums are
+// added in order (few tokens: a token's positions in up to 4 such shares). That is not the sum of the rows one
+// after the other, but it depends on the ids and sizes alone: repeated calls give the same bits.
 #include "ksd_common.h"
 
 #include <algorithm>

@@ -5,9 +5,10 @@
 // The scales stand outside the sum, so the whole reduction stays in the int8 matrix unit with exact
 // int32 sums; the group-128 product of gemm.hip rescales every 128 steps on the VALU instead.
 //
-// What bounds it (us, bf16 output): long products the power that the matrix unit draws, 8192^3 480 (2290
-// TOPS) on random codes and 334 on zeros; at K = 1536 a launch's start and a tile's end as well, 8192 x 1536 x
-// 1536 24.5 (1580 TOPS), 4096 x 150144 x 1536 935 (2020 TOPS).
+// What bounds it (us, bf16 output, one product over and over): long products the power that the matrix unit
+// draws, 8192^3 410 to 480 by card (2290 TOPS and more) on random codes and 334 on zeros; at K = 1536 a launch's
+// start and a tile's end as well, 8192 x 1536 x 1536 22 to 25 (1580 TOPS and more), with a residual 27 to 29, 4096 x
+// 150144 x 1536 920 to 955 (2.0 POPS; 1016 to 1062 between the other passes of a training call).
 //
 // Row quantization (ksd_tc_quantize_rows): a = max |x[r,:]|; where a < 2^-100 the row's scale and
 // codes are 0, else scale = a / 127, code = rint(x * (127 / a)), each operation rounded to fp32.
@@ -1047,8 +1048,11 @@ __global__ __launch_bounds__(256) void few_rows_kernel(const Few p) {
 }
 
 // Every workgroup quantizes all tokens, a wave a quarter of them one after the other: up to 8192 values of a
-// wave. (us, against quantizing and the product: 16 x 1536 -> 512 8.0 and 10.7, 24 tokens 10.6 and 11.4, 16 x 512 ->
-// 32003 11.8 and 9.5; 4 x 6869 -> 1792 12.6 and 13.3, 8 tokens 19.9 and 13.4; 1 x 16384 -> 1024 22 and 16.)
+// wave. (us, against quantizing and the product, in a graph: 1536 -> 512 2 tokens 3.6 and 9.2, 16 tokens 7.2 and
+// 9.8; 1536 -> 150144 2 tokens 37 and 39, 8 tokens 37 and 41, 16 tokens 41.7 and 40.7; outside one 24 x 1536 -> 512
+// 10.6 and 11.4, 4 x 6869 -> 1792 12.6 and 13.3, 8 tokens 19.9 and 13.4, 1 x 16384 -> 1024 22 and 16. The rule does not
+// look at N: short rows onto many columns are quantized in more workgroups than pays, 512 -> 32003 8 tokens 8.6 and
+// 8.3, 16 tokens 10.6 and 8.4.)
 static bool few_rows(int64_t M, int64_t K) { return M <= 16 && cdiv(M, 4) * K <= 8192; }
 
 template <int DT, int OUT>
@@ -1131,7 +1135,7 @@ extern "C" int ksd_tc_gemm(const int8_t *a, int64_t lda, int a_t, const float *s
   tc::Prob p{a, w, sa, sw, bias, residual, y, (int32_t *)workspace, lda, ldw, (int)M, (int)N, (int)K, 1, 0, 0};
   const tc::Plan pl = tc::plan(M, N, K);
   p.splits = pl.splits, p.ksteps = pl.ksteps;
-  // Where 16 lanes store whole 64-byte pieces (4096 x 150144 x 1536: 1024 -> 933 us); pieces that
+  // Where 16 lanes store whole 64-byte pieces (4096 x 150144 x 1536 over and over: 1090 -> 925 us); pieces that
   // other stores complete are put together in L2 (8192 x 1536 from a T operand: 28 us, non-temporal 40).
   p.nt = !w_t && ((uintptr_t)y) % 64 == 0 && N * (out_dtype == KSD_F32 ? 4 : 2) % 64 == 0;
   const int64_t need = p.splits > 1 ? (int64_t)p.splits * M * N * 4 : 0;

@@ -43,7 +43,7 @@ def embedding_gather_int8(codes: torch.Tensor, scales: torch.Tensor, ids: torch.
     if code is None:
         raise TypeError(f"unsupported output dtype {out_dtype}")
     flat = ids.reshape(-1).to(torch.int64).contiguous()
-    if check_ids and flat.numel():  # nn.Embedding raises for such ids (a host sync)
+    if check_ids and flat.numel():  # as nn.Embedding does on the CPU (a host read)
         bad = (flat < 0) | (flat >= V)
         if bool(bad.any()):
             raise IndexError(f"index {int(flat[bad][0])} is out of range for {V} rows")
@@ -148,7 +148,7 @@ def _check_ids(ids: torch.Tensor, V: int, check: bool) -> torch.Tensor:
     if ids.dtype not in (torch.int64, torch.int32):
         raise TypeError("ids must be integer token indices")
     flat = ids if ids.dim() == 1 and ids.is_contiguous() else ids.reshape(-1).contiguous()
-    if check and flat.numel():  # nn.Embedding raises for such ids (a host sync)
+    if check and flat.numel():  # as nn.Embedding does on the CPU (a host read)
         bad = (flat < 0) | (flat >= V)
         if bool(bad.any()):
             raise IndexError(f"index {int(flat[bad][0])} is out of range for {V} rows")
@@ -186,12 +186,12 @@ def embedding_gradient(grad: torch.Tensor, ids: torch.Tensor, num_embeddings: in
                        out: torch.Tensor | None = None, accumulate: bool = False,
                        check_ids: bool = True) -> torch.Tensor:
     """The gradient of embedding_lookup's table: dW[v] = scale * sum of grad[i] over ids[i] == v, in
-    fp32 in the order of the positions, rounded once to out_dtype; the row of padding_idx is 0.
+    fp32, rounded once to out_dtype; the row of padding_idx is 0.
 
     grad (..., d) float, ids of its leading shape -> (num_embeddings, d). ``out`` (dense) takes the
     result; with accumulate=True the sums are added to what it holds and only the rows of ids that
-    occur are touched (a tied head's dense gradient). Without atomics: repeated calls give the same
-    bits. With check_ids=False (no host sync) ids out of range are left out."""
+    occur are touched (a tied head's dense gradient). Without atomics, in an order that the ids and
+    sizes fix: repeated calls give the same bits. With check_ids=False (no host sync) ids out of range are left out."""
     dev = _lib.require_gpu(grad, ids, out)
     if grad.shape[:-1] != ids.shape:
         raise ValueError(f"grad {tuple(grad.shape)} does not match ids {tuple(ids.shape)}")
