@@ -823,6 +823,46 @@ int ksd_grad_norm(const void *const *grads, const int64_t *sizes, const int32_t 
 int ksd_grad_scale(const void *const *grads, void *const *outs, const int64_t *sizes,
                    const int32_t *types, int n, const float *factor, void *stream);
 
+/*
+ * Dropout with a mask that is made from a counter and stored nowhere (no reference counterpart):
+ *   out[m, c] = round(x[m, c] * (u[m, c] >= drop ? 65536 / (65536 - drop) : 0) (+ residual[m, c]))
+ * in fp32, a dropped value counting as 0 whatever it held; drop = 0..65536 is 65536 times the probability.
+ * u: 16 bits, half c % 8 (low halves first) of Philox4x32 with 10 rounds at the counter (c / 8, m, m >> 32,
+ * stream_id) under the key `seed` (low word first). The same call on the gradient is the backward pass.
+ *   x (rows, d) and residual (or NULL) of row strides in elements, out (rows, d) dense, all of dtype (KSD_F32,
+ *   KSD_BF16, KSD_F16); out may be x or residual themselves where they are dense
+ *   seed_from: NULL, or a device address of the 64-bit seed (a replayed graph then gets new masks)
+ */
+int ksd_dropout(const void *x, int dtype, int64_t rows, int64_t d, int64_t stride, int64_t drop,
+                uint64_t seed, const void *seed_from, int64_t stream_id, const void *residual,
+                int64_t residual_stride, void *out, void *stream);
+
+/*
+ * Verification of drafted tokens from given random numbers (no reference counterpart; with L = 0, drawing a
+ * token). Per stream b, with p = softmax(target[b, t] / T), q = softmax(draft[b, t] / T) and u = uniforms[b]:
+ *   position t < len is accepted while u[t] q(token) < p(token); q(token) = 1 without draft logits
+ *   out[b] = the accepted tokens, one drawn token, then -1; accepted[b] = how many were
+ *   drawn: the first token whose running sum of weights passes u[L] times their sum; weights
+ *   max(p - q, 0) where a token was refused (without draft logits p without it; p where they are all 0), p
+ *   behind the last one
+ *   T not above 0: greedy; a token is accepted where it is the row's largest logit (the lowest index of equal
+ *   ones), which is drawn too
+ * Uniforms lie in [0, 1). A draft token outside [0, V) is refused. A row without a finite logit, or with NaN or
+ * +inf (greedy: NaN), has no distribution: a target's is refused and draws -1, a draft's with NaN or +inf refuses its
+ * token and draws from p. Sums of the row that is drawn from are 64-bit, those of the tests 32-bit.
+ *   target (B, L + 1, V), draft (B, L, V) or NULL: dtype, last stride 1, the others in elements
+ *   tokens (B, L) int64; uniforms (B, L + 1) fp32, or fp64 where uniforms_wide (NULL if all are greedy)
+ *   temperatures (B,) fp32, or NULL: `temperature` for all
+ *   lengths (B,) int64, clamped to [0, L], or NULL (L)
+ *   out (B, L + 1), accepted (B,) int64; workspace: ksd_verify_draft_workspace bytes
+ */
+int ksd_verify_draft_workspace(int64_t B, int64_t L, int64_t V, int draft, int64_t *bytes);
+int ksd_verify_draft(const void *target, const void *draft, int dtype, int64_t B, int64_t L, int64_t V,
+                     int64_t target_b, int64_t target_t, int64_t draft_b, int64_t draft_t,
+                     const int64_t *tokens, const void *uniforms, int uniforms_wide,
+                     const float *temperatures, float temperature, const int64_t *lengths, int64_t *out,
+                     int64_t *accepted, void *workspace, int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

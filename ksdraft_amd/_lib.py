@@ -23,6 +23,7 @@ _DTYPE_CODE = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
 
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
+_U64 = ctypes.c_uint64
 _INT = ctypes.c_int
 _F = ctypes.c_float
 
@@ -105,6 +106,9 @@ SIGNATURES = {
     "ksd_grad_norm_workspace": [_P, _INT, _P],
     "ksd_grad_norm": [_P, _P, _P, _INT, _INT, _F, _F, _P, _P, _P, _I64, _P],
     "ksd_grad_scale": [_P, _P, _P, _P, _INT, _P, _P],
+    "ksd_verify_draft_workspace": [_I64, _I64, _I64, _INT, _P],
+    "ksd_verify_draft": [_P, _P, _INT, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _INT, _P, _F, _P, _P, _P, _P, _I64, _P],
+    "ksd_dropout": [_P, _INT, _I64, _I64, _I64, _I64, _U64, _P, _I64, _P, _I64, _P, _P],
 }
 
 _lib = None
@@ -147,6 +151,20 @@ def call(name: str, *args) -> None:
     status = getattr(_lib or load(), name)(*args)
     if status:
         check(status)
+
+
+def call_on(dev: torch.device, name: str, *args) -> None:
+    """``call`` with dev as the current device and its current stream as the last argument: a launch
+    goes to the current device, whatever device its tensors are on."""
+    if dev.index == _current_device():
+        call(name, *args, stream_ptr(dev))
+    else:
+        with torch.cuda.device(dev):
+            call(name, *args, stream_ptr(dev))
+
+
+def _current_device() -> int:
+    return torch._C._cuda_getDevice()
 
 
 def require_gpu(*tensors: torch.Tensor) -> torch.device:

@@ -20,49 +20,6 @@ __device__ __forceinline__ int64_t load_id(const void *ids, int wide, int64_t i)
   return wide ? ((const int64_t *)ids)[i] : (int64_t)((const int32_t *)ids)[i];
 }
 
-template <int DT>
-__device__ __forceinline__ void load_any(const typename Elem<DT>::T *p, int n, float *v) {
-  if (n >= 8) {
-    struct __attribute__((packed, aligned(DT == KSD_F32 ? 4 : 2))) Any { uint4 q; };
-    Raw8<DT> r;
-    r.a = ((const Any *)p)->q;
-    if constexpr (DT == KSD_F32) r.b = ((const Any *)(p + 4))->q;
-    cvt_raw8<DT>(r, true, v);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j < n ? Elem<DT>::load(p + j) : 0.0f;
-  }
-}
-template <int DT>
-__device__ __forceinline__ void store_any(typename Elem<DT>::T *p, int n, const float *v) {
-  struct __attribute__((packed, aligned(DT == KSD_F32 ? 4 : 2))) Any { uint4 q; };
-  if (n >= 8) {
-    if constexpr (DT == KSD_F32) {
-      uint4 a, b;
-      a.x = __builtin_bit_cast(uint32_t, v[0]), a.y = __builtin_bit_cast(uint32_t, v[1]);
-      a.z = __builtin_bit_cast(uint32_t, v[2]), a.w = __builtin_bit_cast(uint32_t, v[3]);
-      b.x = __builtin_bit_cast(uint32_t, v[4]), b.y = __builtin_bit_cast(uint32_t, v[5]);
-      b.z = __builtin_bit_cast(uint32_t, v[6]), b.w = __builtin_bit_cast(uint32_t, v[7]);
-      ((Any *)p)->q = a;
-      ((Any *)(p + 4))->q = b;
-    } else {
-      uint32_t w[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        uint16_t lo, hi;
-        store_out<DT>(&lo, 0, v[2 * k]);
-        store_out<DT>(&hi, 0, v[2 * k + 1]);
-        w[k] = lo | (uint32_t)hi << 16;
-      }
-      ((Any *)p)->q = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < n) store_out<DT>(p, j, v[j]);
-  }
-}
-
 // One wave per row. (65521 tokens of a table 32003 x 1792, bf16 to bf16: 72 us, 6.5 TB/s; a few tokens: the launch.)
 template <int DT, int OUT>
 __global__ __launch_bounds__(256) void lookup_kernel(const void *__restrict__ table, const void *__restrict__ ids, int wide,

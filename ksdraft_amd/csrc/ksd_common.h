@@ -357,4 +357,49 @@ template <> __device__ __forceinline__ void store_out<KSD_F16_SAT>(void *y, int6
   ((uint16_t *)y)[idx] = __builtin_bit_cast(uint16_t, h);
 }
 
+// Up to 8 consecutive elements at any alignment of the element type, as floats (zeros from n on),
+// and their store; whole chunks move as 16-byte vectors.
+template <int DT>
+__device__ __forceinline__ void load_any(const typename Elem<DT>::T *p, int n, float *v) {
+  if (n >= 8) {
+    struct __attribute__((packed, aligned(DT == KSD_F32 ? 4 : 2))) Any { uint4 q; };
+    Raw8<DT> r;
+    r.a = ((const Any *)p)->q;
+    if constexpr (DT == KSD_F32) r.b = ((const Any *)(p + 4))->q;
+    cvt_raw8<DT>(r, true, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j < n ? Elem<DT>::load(p + j) : 0.0f;
+  }
+}
+template <int DT>
+__device__ __forceinline__ void store_any(typename Elem<DT>::T *p, int n, const float *v) {
+  struct __attribute__((packed, aligned(DT == KSD_F32 ? 4 : 2))) Any { uint4 q; };
+  if (n >= 8) {
+    if constexpr (DT == KSD_F32) {
+      uint4 a, b;
+      a.x = __builtin_bit_cast(uint32_t, v[0]), a.y = __builtin_bit_cast(uint32_t, v[1]);
+      a.z = __builtin_bit_cast(uint32_t, v[2]), a.w = __builtin_bit_cast(uint32_t, v[3]);
+      b.x = __builtin_bit_cast(uint32_t, v[4]), b.y = __builtin_bit_cast(uint32_t, v[5]);
+      b.z = __builtin_bit_cast(uint32_t, v[6]), b.w = __builtin_bit_cast(uint32_t, v[7]);
+      ((Any *)p)->q = a;
+      ((Any *)(p + 4))->q = b;
+    } else {
+      uint32_t w[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        uint16_t lo, hi;
+        store_out<DT>(&lo, 0, v[2 * k]);
+        store_out<DT>(&hi, 0, v[2 * k + 1]);
+        w[k] = lo | (uint32_t)hi << 16;
+      }
+      ((Any *)p)->q = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < n) store_out<DT>(p, j, v[j]);
+  }
+}
+
 }  // namespace ksd
