@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import weakref
 
 import torch
 
@@ -106,6 +107,11 @@ SIGNATURES = {
     "ksd_grad_norm_workspace": [_P, _INT, _P],
     "ksd_grad_norm": [_P, _P, _P, _INT, _INT, _F, _F, _P, _P, _P, _I64, _P],
     "ksd_grad_scale": [_P, _P, _P, _P, _INT, _P, _P],
+    "ksd_adapter_linear": [_P, _INT, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _P, _INT, _I64, _P, _P, _I64, _I64, _U64, _P,
+                           _I64, _P, _P, _P],
+    "ksd_adapter_linear_backward_workspace": [_I64, _I64, _I64, _I64, _I64, _INT, _P],
+    "ksd_adapter_linear_backward": [_P, _INT, _I64, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _I64, _I64, _P, _INT, _I64, _P, _P,
+                                    _I64, _I64, _U64, _P, _I64, _P, _P, _P, _P, _I64, _P],
     "ksd_verify_draft_workspace": [_I64, _I64, _I64, _INT, _P],
     "ksd_verify_draft": [_P, _P, _INT, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _INT, _P, _F, _P, _P, _P, _P, _I64, _P],
     "ksd_dropout": [_P, _INT, _I64, _I64, _I64, _I64, _U64, _P, _I64, _P, _I64, _P, _P],
@@ -195,6 +201,34 @@ def stream_ptr(dev: torch.device) -> int:
     if _raw_stream is None or dev.index is None:
         return torch.cuda.current_stream(dev).cuda_stream
     return _raw_stream(dev.index)
+
+
+class _EagerGraph:
+    __slots__ = ("leaves", "stream", "__weakref__")
+
+
+_eager_graphs = weakref.WeakSet()  # of the living autograd graphs that ``capture_guard`` was called for
+
+
+def capture_guard(dev: torch.device, *tensors):
+    """Called in the forward of an autograd function; what it returns is kept in ctx. torch ends the process
+    (in the capture's end) where a backward pass is captured while an eager graph of the same leaf made on another
+    stream lives: the leaf's accumulation node belongs to that stream. Captured calls on such leaves raise
+    instead, as far as the eager graph is of a function that calls this too."""
+    leaves = {id(t) for t in tensors if t is not None and t.requires_grad and t.is_leaf}
+    if not leaves:
+        return None
+    stream = stream_ptr(dev)
+    if torch.cuda.is_current_stream_capturing():
+        for g in list(_eager_graphs):
+            if g.stream != stream and not leaves.isdisjoint(g.leaves):
+                raise RuntimeError("an eager graph of the same leaf tensors is alive: drop it (its outputs and losses) "
+                                   "before their backward pass is captured")
+        return None
+    g = _EagerGraph()
+    g.leaves, g.stream = leaves, stream
+    _eager_graphs.add(g)
+    return g
 
 
 def put(module: torch.nn.Module, **values) -> None:

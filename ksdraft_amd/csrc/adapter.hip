@@ -49,6 +49,14 @@ __device__ __forceinline__ typename Oct<DT>::V load_oct(const typename Elem<DT>:
   }
   return v;
 }
+__device__ __forceinline__ f32x4 load_four(const float *row, int c, int n) {
+  struct __attribute__((packed, aligned(4))) Any { f32x4 v; };
+  if (c + 4 <= n) return ((const Any *)(row + c))->v;
+  f32x4 v;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = c + j < n ? row[c + j] : 0.0f;
+  return v;
+}
 template <int DT>
 __device__ __forceinline__ void to_floats(const typename Oct<DT>::V &v, float *f) {
 #pragma unroll
@@ -278,6 +286,7 @@ __global__ __launch_bounds__(64 * kWaves) void pair_kernel(const PairArgs p) {
       }
     }
   }
+  if (!p.y) return;
   const int64_t n0 = (int64_t)blockIdx.y * p.cols, n1 = min(p.N, n0 + p.cols);
   for (int64_t c = n0 + wave * 64; c < n1; c += 64 * kWaves) {
     const int64_t at = c + grp * 16;
@@ -302,7 +311,7 @@ __global__ __launch_bounds__(64 * kWaves) void pair_kernel(const PairArgs p) {
 #pragma unroll
         for (int q = 0; q < R16; ++q) {
           if constexpr (DT == KSD_F32) {
-            const V w = load_oct<DT>(b, q * 16 + grp * 4, min(p.r, q * 16 + grp * 4 + 4));
+            const f32x4 w = load_four(b, q * 16 + grp * 4, p.r);
 #pragma unroll
             for (int u = 0; u < RT; ++u)
 #pragma unroll
@@ -346,7 +355,13 @@ __global__ __launch_bounds__(64 * kWaves) void pair_kernel(const PairArgs p) {
 template <int DT, int R16, int RT>
 static void launch_pair(const PairArgs &p, bool mask, hipStream_t st) {
   const dim3 g((unsigned)cdiv(p.M, p.rows), (unsigned)cdiv(p.N, p.cols));
-  const size_t lds = (size_t)kWaves * 16 * RT * (16 * R16 + 4) * 4;
+  constexpr int lds = kWaves * 16 * RT * (16 * R16 + 4) * 4;
+  if constexpr (lds > 65536) {  // past HIP's default
+    static const hipError_t set[2] = {
+        hipFuncSetAttribute((const void *)pair_kernel<DT, R16, RT, false>, hipFuncAttributeMaxDynamicSharedMemorySize, lds),
+        hipFuncSetAttribute((const void *)pair_kernel<DT, R16, RT, true>, hipFuncAttributeMaxDynamicSharedMemorySize, lds)};
+    (void)set;
+  }
   if (mask) pair_kernel<DT, R16, RT, true><<<g, 64 * kWaves, lds, st>>>(p);
   else pair_kernel<DT, R16, RT, false><<<g, 64 * kWaves, lds, st>>>(p);
 }
@@ -403,7 +418,9 @@ __global__ __launch_bounds__(256) void group_kernel(const GroupArgs a) {
   __syncthreads();
   const int start = sums[0][0] + sums[0][1] + sums[0][2] + sums[0][3], len = sums[1][0] + sums[1][1] + sums[1][2] + sums[1][3];
   const int slot = start / kPiece + i, next = (start + len) / kPiece + i + 1, pieces = (len + kPiece - 1) / kPiece;
-  for (int s = slot + tid; s < next; s += 256) {
+  // the last adapter's workgroup empties the slots behind it too: tokens without an adapter take none
+  const int upto = i == a.n - 1 ? (int)(a.M / kPiece) + a.n : next;
+  for (int s = slot + tid; s < upto; s += 256) {
     const int at = start + (s - slot) * kPiece;
     a.slots[s] = s - slot < pieces ? Slot{i, at, min(at + kPiece, start + len), 0} : Slot{-1, 0, 0, 0};
   }

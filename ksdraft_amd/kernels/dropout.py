@@ -63,6 +63,7 @@ def _dropout(x, p, seed, stream, residual):
 class _DropoutFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, p, seed, stream, residual):
+        ctx.guard = _lib.capture_guard(_lib.require_gpu(x), x, residual)
         if isinstance(seed, torch.Tensor):  # the caller may count it on before the backward pass
             seed = seed.clone()
             ctx.save_for_backward(seed)
