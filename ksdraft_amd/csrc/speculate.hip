@@ -10,7 +10,7 @@
 // need p and q of one token a row, and an error of 2^-24 there moves one test in ten million. The drawn token is
 // another matter: with 150144 tokens a running sum has as many borders, and sums in 32 bits would move about one draw in
 // a hundred across one. The one row of a stream that is drawn from is therefore read again with powers and sums in 64
-// bits (total_kernel, draw_kernel). Logits of -inf have probability 0; a row without a finite logit, or with NaN or
+// bits (total_kernel, weight_kernel, draw_kernel). Logits of -inf have probability 0; a row without a finite logit, or with NaN or
 // +inf, has no distribution: a target's is refused and draws -1, a draft's refuses the token and draws from p.
 #include "ksd_common.h"
 
@@ -38,9 +38,14 @@ struct Args {
   int64_t *out, *accepted;
   Part *parts;                 // (B, 2 L + 1, splits): target rows, then draft rows
   double *totals, *weights;    // (B, pieces, 2) each
-  int *arrived;                // (B,)
+  struct Draw *draws;          // (B,)
+  int *refused;                // (kRanges, B): the first refused position, as far as the ranges before one tell
   int B, L, V, splits, chunk, pieces, piece;
+  int range, t0, t1, before;   // positions of this launch of stats_kernel, and where its predecessor's began
 };
+constexpr int kRanges = 6, kNone = 0x7fffffff;
+// Logits from which positions go in several launches, and of the first of them
+constexpr int64_t kSeveral = 64 << 20, kFirst = 40 << 20;
 
 __device__ __forceinline__ float temperature(const Args &a, int b) { return a.temps ? a.temps[b] : a.temp; }
 __device__ __forceinline__ float clamped(float t) { return fminf(fmaxf(t, 1e-37f), 1e37f); }
@@ -73,7 +78,38 @@ __device__ __forceinline__ void load_logits(const typename Elem<DT>::T *row, int
   }
 }
 
-// ------------------------------------------------------------------------------- row statistics
+// ------------------------------------------------------------------------------- powers
+// 2^y in 64 bits for y <= 0: 2^k times the Taylor polynomial of e^(r ln 2), |r| <= 1/2, to the 11th power, whose rest
+// is below 9e-15 of it, roundings included. NaN stays NaN; below 2^-1100 it is 0. (About 20 instructions for each of the two rows' logits,
+// twice; with the library's exp the two launches took 24 and 30 us for 64 streams of 150144 tokens.)
+__device__ __forceinline__ double power2(double y) {
+  y = y < -1100.0 ? -1100.0 : y;
+  const double k = __builtin_rint(y), r = y - k;
+  constexpr double l = 0.693147180559945309417232121458;
+  constexpr double c1 = l, c2 = c1 * l / 2, c3 = c2 * l / 3, c4 = c3 * l / 4, c5 = c4 * l / 5, c6 = c5 * l / 6, c7 = c6 * l / 7,
+                   c8 = c7 * l / 8, c9 = c8 * l / 9, c10 = c9 * l / 10, c11 = c10 * l / 11;
+  double p = fma(c11, r, c10);
+  p = fma(p, r, c9);
+  p = fma(p, r, c8);
+  p = fma(p, r, c7);
+  p = fma(p, r, c6);
+  p = fma(p, r, c5);
+  p = fma(p, r, c4);
+  p = fma(p, r, c3);
+  p = fma(p, r, c2);
+  p = fma(p, r, c1);
+  p = fma(p, r, 1.0);
+  return __builtin_amdgcn_ldexp(p, (int)k);
+}
+constexpr double kLog2e = 1.44269504088896340735992468100189214;
+// e^((z - m) / T) = power2((z - m) c), c = log2(e) / T; the difference first, which is 0 at the largest logit at any T
+struct Exponent {
+  double c, m;
+};
+__device__ __forceinline__ Exponent exponent(float T, float m) { return Exponent{kLog2e / (double)clamped(T), (double)m}; }
+__device__ __forceinline__ double power(double z, Exponent e) { return power2((z - e.m) * e.c); }
+
+// ------------------------------------------------------------------------------- reductions
 struct Best {
   float m;
   int at;
@@ -81,68 +117,180 @@ struct Best {
 __device__ __forceinline__ Best better(Best x, Best y) {
   return y.m > x.m || (y.m == x.m && y.at < x.at) ? y : x;
 }
+__device__ __forceinline__ double block_sum(double v, double *scratch) {  // 256 threads
+#pragma unroll
+  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return scratch[0] + scratch[1] + scratch[2] + scratch[3];
+}
+__device__ __forceinline__ float block_max(float v, float *scratch) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return fmaxf(fmaxf(scratch[0], scratch[1]), fmaxf(scratch[2], scratch[3]));
+}
+
+// The largest logit of a piece of a row (greedy streams).
+template <int DT>
+__device__ __forceinline__ void best_part(const typename Elem<DT>::T *row, int from, int to, Part *out) {
+  __shared__ Best found[4];
+  __shared__ int bads[4];
+  Best best{-INFINITY, kNone};
+  bool bad = false;
+  for (int k = from + threadIdx.x * 8; k < to; k += 2048) {
+    float v[8];
+    load_logits<DT>(row, k, to, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      bad |= v[j] != v[j];
+      if (v[j] > best.m) best = Best{v[j], k + j};
+    }
+  }
+#pragma unroll
+  for (int o = 32; o; o >>= 1) best = better(best, Best{__shfl_xor(best.m, o), __shfl_xor(best.at, o)});
+  const int any = __ballot(bad) != 0;
+  if ((threadIdx.x & 63) == 0) found[threadIdx.x >> 6] = best, bads[threadIdx.x >> 6] = any;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 4; ++w) best = better(best, found[w]);
+    *out = Part{best.m, 0.0f, best.at, bads[0] | bads[1] | bads[2] | bads[3]};
+  }
+}
+
+// ------------------------------------------------------------------------------- acceptance
+// What 16 lanes make of a row's pieces (at most 32): every lane gets the result.
+struct Stat {
+  float m;
+  double s;
+};
+__device__ __forceinline__ Stat row_stat(const Args &a, const Part *p, float c) {
+  const int i = threadIdx.x & 15;
+  Part x{-FLT_MAX, 0, 0, 0}, y = x;
+  if (i < a.splits) x = p[i];
+  if (i + 16 < a.splits) y = p[i + 16];
+  float m = fmaxf(x.m, y.m);
+#pragma unroll
+  for (int o = 8; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  double s = (double)(x.s * __builtin_amdgcn_exp2f((x.m - m) * c)) + (double)(y.s * __builtin_amdgcn_exp2f((y.m - m) * c));
+#pragma unroll
+  for (int o = 8; o; o >>= 1) s += __shfl_xor(s, o);
+  return Stat{m, s};
+}
+// The place of a greedy row's largest logit; -1 where it has none.
+__device__ __forceinline__ int row_best(const Args &a, const Part *p, int splits) {
+  Best best{-INFINITY, kNone};
+  int bad = 0;
+  for (int i = threadIdx.x & 15; i < splits; i += 16) {
+    const Part x = p[i];
+    best = better(best, Best{x.m, x.at}), bad |= x.bad;
+  }
+#pragma unroll
+  for (int o = 8; o; o >>= 1) {
+    best = better(best, Best{__shfl_xor(best.m, o), __shfl_xor(best.at, o)});
+    bad |= __shfl_xor(bad, o);
+  }
+  return bad || best.m == -INFINITY ? -1 : best.at;
+}
 
 template <int DT>
-__global__ __launch_bounds__(256) void stats_kernel(const Args a, int t0, int nt) {
+__device__ __forceinline__ bool accepts(const Args &a, int b, int t, float T) {  // 16 lanes
+  const int64_t token = a.tokens[(int64_t)b * a.L + t];
+  if (!(T > 0)) return row_best(a, parts_of(a, b, t), a.splits) == token && token >= 0;
+  const bool in = token >= 0 && token < a.V;
+  const float c = 1.4426950408889634f / clamped(T);
+  const float zp = in ? Elem<DT>::load(target_row<DT>(a, b, t) + token) : 0.0f;
+  const float zq = in && a.draft ? Elem<DT>::load(draft_row<DT>(a, b, t) + token) : 0.0f;
+  const double u = uniform(a, b, t);
+  const Stat p = row_stat(a, parts_of(a, b, t), c);
+  const double pt = power((double)zp, exponent(T, p.m)) / p.s;
+  double qt = 1.0;
+  if (a.draft) {
+    const Stat q = row_stat(a, parts_of(a, b, a.L + 1 + t), c);
+    qt = q.s == 0 ? 0.0 : power((double)zq, exponent(T, q.m)) / q.s;
+  }
+  return in && u * qt < pt;
+}
+
+// The first refused position in [from, to), else kNone: a workgroup of 256 threads, 16 positions at a time.
+template <int DT>
+__device__ __forceinline__ int refused_in(const Args &a, int b, int from, int to, float T) {
+  __shared__ int first;
+  if (threadIdx.x == 0) first = kNone;
+  __syncthreads();
+  for (int base = from; base < to; base += 16) {
+    const int t = base + (threadIdx.x >> 4);
+    if (t < to && !accepts<DT>(a, b, t, T) && (threadIdx.x & 15) == 0) atomicMin(&first, t);
+    __syncthreads();
+    const int r = first;
+    __syncthreads();  // before the next positions' refusals
+    if (r != kNone) return r;
+  }
+  return kNone;
+}
+
+// ------------------------------------------------------------------------------- row statistics
+// The rows of the positions [t0, t1). A long batch goes through its positions in several launches: a stream's rows
+// behind a refused token need not be read, and a launch knows what its predecessors' rows refuse.
+template <int DT>
+__global__ __launch_bounds__(256) void stats_kernel(const Args a) {
   // blocks: split fastest, then target and draft, then requests, then positions
   const int split = blockIdx.x % a.splits;
   int i = blockIdx.x / a.splits;
   const int sides = a.draft ? 2 : 1;
   const bool drafted = i % sides;
   i /= sides;
-  const int b = i % a.B, t = t0 + i / a.B;
+  const int b = i % a.B, t = a.t0 + i / a.B;
   const int len = length(a, b);
   const float T = temperature(a, b);
   const bool greedy = !(T > 0);
-  if (t > len || (drafted && (t == len || greedy))) return;
+  const bool note = a.range > 0 && t == a.t0 && split == 0 && !drafted;  // whose workgroup writes down what was refused
+  const bool idle = t > len || (drafted && (t == len || greedy));
+  if (idle && !note) return;
+  if (a.range > 0) {
+    int r = a.range > 1 ? a.refused[(int64_t)(a.range - 1) * a.B + b] : kNone;
+    if (r == kNone) r = refused_in<DT>(a, b, a.before, min(a.t0, len), T);
+    if (note && threadIdx.x == 0) a.refused[(int64_t)a.range * a.B + b] = r;
+    if (r != kNone || idle) return;
+  }
   const typename Elem<DT>::T *const row = drafted ? draft_row<DT>(a, b, t) : target_row<DT>(a, b, t);
   const int from = split * a.chunk, to = min(a.V, from + a.chunk);
-  const float c = 1.4426950408889634f / clamped(T);
-  __shared__ float sm[4], ss[4];
-  __shared__ int si[4];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  constexpr int U = 4;
   Part *const out = const_cast<Part *>(parts_of(a, b, drafted ? a.L + 1 + t : t)) + split;
   if (greedy) {
-    Best best{-INFINITY, 0x7fffffff};
-    bool bad = false;
-    for (int k = from + threadIdx.x * 8; k < to; k += 2048) {
-      float v[8];
-      load_logits<DT>(row, k, to, v);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        bad |= v[j] != v[j];
-        if (v[j] > best.m) best = Best{v[j], k + j};
-      }
-    }
-#pragma unroll
-    for (int o = 32; o; o >>= 1) best = better(best, Best{__shfl_xor(best.m, o), __shfl_xor(best.at, o)});
-    const int any = __ballot(bad) != 0;
-    if (lane == 0) sm[wave] = best.m, si[wave] = best.at, ss[wave] = any ? 1.0f : 0.0f;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      for (int w = 1; w < 4; ++w) best = better(best, Best{sm[w], si[w]});
-      *out = Part{best.m, 0.0f, best.at, ss[0] + ss[1] + ss[2] + ss[3] > 0};
-    }
+    best_part<DT>(row, from, to, out);
     return;
   }
+  const float c = 1.4426950408889634f / clamped(T);
+  __shared__ float sm[4], ss[4];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int U = 4;
   float m = -FLT_MAX, s = 0.0f;  // not -inf: a piece of nothing but -inf then has differences of -inf and sum 0
   for (int k = from + threadIdx.x * 8; k < to; k += 2048 * U) {
     float v[U][8];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (k + u * 2048 < to) load_logits<DT>(row, k + u * 2048, to, v[u]);
-#pragma unroll
     for (int u = 0; u < U; ++u) {
-      if (k + u * 2048 >= to) break;
-      float top = m;
+      if (k + u * 2048 < to) {
+        load_logits<DT>(row, k + u * 2048, to, v[u]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[u][j] = -INFINITY;
+      }
+    }
+    float top = m;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int j = 0; j < 8; ++j) top = fmaxf(top, v[u][j]);
-      s *= __builtin_amdgcn_exp2f((m - top) * c);
-      m = top;
+    float sum[U] = {};
 #pragma unroll
-      for (int j = 0; j < 8; ++j) s += __builtin_amdgcn_exp2f((v[u][j] - m) * c);
-    }
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum[u] += __builtin_amdgcn_exp2f((v[u][j] - top) * c);
+    s = s * __builtin_amdgcn_exp2f((m - top) * c) + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+    m = top;
   }
   const auto join = [&](float m2, float s2) {
     const float top = fmaxf(m, m2);
@@ -159,99 +307,45 @@ __global__ __launch_bounds__(256) void stats_kernel(const Args a, int t0, int nt
   }
 }
 
-// ------------------------------------------------------------------------------- acceptance
-struct Stat {
-  float m;
-  double s;
-};
-__device__ __forceinline__ Stat row_stat(const Args &a, const Part *p, float c) {
-  Stat r{-FLT_MAX, 0.0};
-  for (int i = 0; i < a.splits; ++i) r.m = fmaxf(r.m, p[i].m);
-  for (int i = 0; i < a.splits; ++i) r.s += (double)(p[i].s * __builtin_amdgcn_exp2f((p[i].m - r.m) * c));
-  return r;
-}
-// The place of a greedy row's largest logit; -1 where it has none.
-__device__ __forceinline__ int row_best(const Args &a, const Part *p) {
-  Best best{-INFINITY, 0x7fffffff};
-  int bad = 0;
-  for (int i = 0; i < a.splits; ++i) best = better(best, Best{p[i].m, p[i].at}), bad |= p[i].bad;
-  return bad || best.m == -INFINITY ? -1 : best.at;
-}
-__device__ __forceinline__ double power(float z, float m, double inv) {  // e^((z - m) / T)
-  return exp(((double)z - (double)m) * inv);
-}
-
-template <int DT>
-__device__ __forceinline__ bool accepts(const Args &a, int b, int t, float T) {
-  const int64_t token = a.tokens[(int64_t)b * a.L + t];
-  if (!(T > 0)) return row_best(a, parts_of(a, b, t)) == token && token >= 0;
-  if (token < 0 || token >= a.V) return false;
-  const float c = 1.4426950408889634f / clamped(T);
-  const double inv = 1.0 / (double)clamped(T);
-  const Stat p = row_stat(a, parts_of(a, b, t), c);
-  const double pt = power(Elem<DT>::load(target_row<DT>(a, b, t) + token), p.m, inv) / p.s;
-  double qt = 1.0;
-  if (a.draft) {
-    const Stat q = row_stat(a, parts_of(a, b, a.L + 1 + t), c);
-    qt = q.s == 0 ? 0.0 : power(Elem<DT>::load(draft_row<DT>(a, b, t) + token), q.m, inv) / q.s;
-  }
-  return uniform(a, b, t) * qt < pt;
-}
-
-// Accepted positions among the first `most` (a whole wave; every lane gets the result).
-template <int DT>
-__device__ __forceinline__ int accepted_of(const Args &a, int b, int most, float T) {
-  const int lane = threadIdx.x & 63;
-  for (int base = 0; base < most; base += 64) {
-    const int t = base + lane;
-    const bool refused = t < most && !accepts<DT>(a, b, t, T);
-    const uint64_t m = __ballot(refused);
-    if (m) return base + __builtin_ctzll(m);
-  }
-  return most;
-}
-
 // ------------------------------------------------------------------------------- the drawn token
-template <int NT>
-__device__ __forceinline__ double block_sum(double v, double *scratch) {
-#pragma unroll
-  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
-  __syncthreads();
-  double r = 0;
-#pragma unroll
-  for (int w = 0; w < NT / 64; ++w) r += scratch[w];
-  return r;
-}
-
 // What the draw of a stream works on.
 struct Draw {
-  int at, refused;     // position, and whether its token was refused
-  float mp, mq;        // largest logits
-  double inv;
-  int64_t token;       // the refused token
+  int at, rest;        // position; whether a refused token's draft row is subtracted
+  Exponent p, q;
+  int64_t without;     // the token that is left out (refused, and no draft logits), or -1
 };
 
+// Without a draft there is nothing to test: a piece's largest logit and sum of powers in 64 bits at once.
 template <int DT>
-__device__ __forceinline__ void draw_of(const Args &a, int b, Draw &d) {  // wave 0 writes d (in LDS)
+__global__ __launch_bounds__(256) void sample_kernel(const Args a) {
+  const int b = blockIdx.x / a.pieces, piece = blockIdx.x % a.pieces;
   const float T = temperature(a, b);
-  const int len = length(a, b);
-  const int at = accepted_of<DT>(a, b, len, T);
-  if ((threadIdx.x & 63) == 0) {
-    d.at = at, d.refused = at < len;
-    d.inv = 1.0 / (double)clamped(T);
-    d.token = at < len ? a.tokens[(int64_t)b * a.L + at] : -1;
-    float m = -FLT_MAX;
-    const Part *p = parts_of(a, b, at);
-    for (int i = 0; i < a.splits; ++i) m = fmaxf(m, p[i].m);
-    d.mp = m;
-    m = -FLT_MAX;
-    if (d.refused && a.draft) {
-      p = parts_of(a, b, a.L + 1 + at);
-      for (int i = 0; i < a.splits; ++i) m = fmaxf(m, p[i].m);
-    }
-    d.mq = m;
+  const typename Elem<DT>::T *const row = target_row<DT>(a, b, 0);
+  const int from = piece * a.piece, to = min(a.V, from + a.piece);
+  if (!(T > 0)) {
+    best_part<DT>(row, from, to, a.parts + (int64_t)b * a.pieces + piece);
+    return;
+  }
+  __shared__ float tops[4];
+  __shared__ double scratch[4];
+  float m = -FLT_MAX, v[8];
+  for (int k = from + threadIdx.x * 8; k < to; k += 2048) {
+    load_logits<DT>(row, k, to, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = fmaxf(m, v[j]);
+  }
+  m = block_max(m, tops);
+  const Exponent e = exponent(T, m);
+  double s = 0;
+  for (int k = from + threadIdx.x * 8; k < to; k += 2048) {
+    if (a.piece > 2048) load_logits<DT>(row, k, to, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s += power((double)v[j], e);
+  }
+  s = block_sum(s, scratch);
+  if (threadIdx.x == 0) {
+    double *const o = a.totals + ((int64_t)b * a.pieces + piece) * 2;
+    o[0] = s, o[1] = (double)m;
   }
 }
 
@@ -259,185 +353,228 @@ __device__ __forceinline__ void draw_of(const Args &a, int b, Draw &d) {  // wav
 template <int DT>
 __global__ __launch_bounds__(256) void total_kernel(const Args a) {
   const int b = blockIdx.x / a.pieces, piece = blockIdx.x % a.pieces;
-  if (!(temperature(a, b) > 0)) {
-    if (piece == 0 && threadIdx.x == 0) a.arrived[b] = 0;
-    return;
-  }
+  const float T = temperature(a, b);
+  const int len = length(a, b);
+  if (!(T > 0) && piece) return;
   __shared__ Draw d;
   __shared__ double scratch[4];
-  if (threadIdx.x < 64) draw_of<DT>(a, b, d);
+  int r = a.range > 0 ? a.refused[(int64_t)a.range * a.B + b] : kNone;
+  if (r == kNone) r = refused_in<DT>(a, b, a.range > 0 ? a.t0 : 0, len, T);
+  const int at = min(r, len);
+  if (T > 0 && threadIdx.x < 16) {
+    const bool refused = at < len;
+    const float c = 1.4426950408889634f / clamped(T);
+    const float mp = row_stat(a, parts_of(a, b, at), c).m;
+    const float mq = refused && a.draft ? row_stat(a, parts_of(a, b, a.L + 1 + at), c).m : 0.0f;
+    if (threadIdx.x == 0)
+      d = Draw{at, refused && a.draft, exponent(T, mp), exponent(T, mq),
+               refused && !a.draft ? a.tokens[(int64_t)b * a.L + at] : -1};
+  }
+  if (!(T > 0) && threadIdx.x == 0) d.at = at;
   __syncthreads();
+  if (piece == 0 && threadIdx.x == 0) a.draws[b] = d;
+  if (!(T > 0)) return;
   const int from = piece * a.piece, to = min(a.V, from + a.piece);
-  const bool both = d.refused && a.draft;
-  double sp = 0, sq = 0;
+  double s0 = 0, s1 = 0;
   for (int k = from + threadIdx.x * 8; k < to; k += 2048) {
-    float v[8];
+    float v[8], w[8];
     load_logits<DT>(target_row<DT>(a, b, d.at), k, to, v);
+    if (d.rest) load_logits<DT>(draft_row<DT>(a, b, d.at), k, to, w);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) sp += power(v[j], d.mp, d.inv);
-    if (both) {
-      load_logits<DT>(draft_row<DT>(a, b, d.at), k, to, v);
+    for (int j = 0; j < 8; ++j) {
+      const double e = power((double)v[j], d.p);
+      if (k + j == d.without) s1 += e;
+      else s0 += e;
+    }
+    if (d.rest) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sq += power(v[j], d.mq, d.inv);
+      for (int j = 0; j < 8; ++j) s1 += power((double)w[j], d.q);
     }
   }
-  sp = block_sum<256>(sp, scratch);
-  sq = block_sum<256>(sq, scratch);
+  s0 = block_sum(s0, scratch);
+  s1 = block_sum(s1, scratch);
   if (threadIdx.x == 0) {
     double *const o = a.totals + ((int64_t)b * a.pieces + piece) * 2;
-    o[0] = sp, o[1] = sq;
-    if (piece == 0) a.arrived[b] = 0;
+    o[0] = s0, o[1] = s1;
   }
 }
 
-// The weights of 8 tokens from column k on: rest[j] = what is drawn from, chance[j] = p.
+// The pieces' values of one of two sides, i and i + 64 of them in lane i (at most 128 pieces).
+__device__ __forceinline__ double piece_value(const double *v, int i, int n, int side) {
+  return i < n ? v[2 * i + side] : 0.0;
+}
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+
+// Reciprocals of the sums of the drawn row's powers and of its draft's (1 and 0 where p need not be normalised).
+struct Norms {
+  double rp, rq;
+};
+__device__ __forceinline__ Norms norms_of(const Args &a, int b, int lane) {
+  const double *const t = a.totals + (int64_t)b * a.pieces * 2;
+  const double sp = wave_sum(piece_value(t, lane, a.pieces, 0) + piece_value(t, lane + 64, a.pieces, 0));
+  const double sq = wave_sum(piece_value(t, lane, a.pieces, 1) + piece_value(t, lane + 64, a.pieces, 1));
+  return Norms{1.0 / sp, sq > 0 ? 1.0 / sq : sq};  // an empty draft row: q = 0; NaN stays
+}
+
+// The weights of 8 tokens from column k on: rest[j] = what is drawn from, chance[j] = p (or a multiple of it).
 template <int DT>
-__device__ __forceinline__ void weights_of(const Args &a, int b, const Draw &d, double rp, double rq, int k, int to,
-                                           double *rest, double *chance) {
-  float v[8];
+__device__ __forceinline__ void weights_of(const Args &a, int b, const Draw &d, Norms n, int k, int to, double *rest,
+                                           double *chance) {
+  float v[8], w[8];
   load_logits<DT>(target_row<DT>(a, b, d.at), k, to, v);
+  if (d.rest) load_logits<DT>(draft_row<DT>(a, b, d.at), k, to, w);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) rest[j] = chance[j] = power(v[j], d.mp, d.inv) * rp;
-  if (!d.refused) return;
-  if (a.draft) {
-    load_logits<DT>(draft_row<DT>(a, b, d.at), k, to, v);
+  for (int j = 0; j < 8; ++j) {
+    chance[j] = power((double)v[j], d.p) * n.rp;
+    rest[j] = k + j == d.without ? 0.0 : chance[j];
+  }
+  if (d.rest) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) rest[j] = fmax(rest[j] - power(v[j], d.mq, d.inv) * rq, 0.0);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (k + j == d.token) rest[j] = 0.0;
+    for (int j = 0; j < 8; ++j) rest[j] = fmax(rest[j] - power((double)w[j], d.q) * n.rq, 0.0);
   }
 }
 
-// Sums of the weights of a piece; the stream's last workgroup finds the drawn token. Only the order in which
-// workgroups end decides which one that is: sums are added by piece.
+// Sums of the weights of a piece, where a draft row is subtracted (elsewhere total_kernel's sums are the weights).
 template <int DT>
-__global__ __launch_bounds__(256) void draw_kernel(const Args a) {
-  const int b = blockIdx.x / a.pieces, piece = blockIdx.x % a.pieces, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  __shared__ Draw d;
+__global__ __launch_bounds__(256) void weight_kernel(const Args a) {
+  const int b = blockIdx.x / a.pieces, piece = blockIdx.x % a.pieces, lane = threadIdx.x & 63;
+  if (!(temperature(a, b) > 0)) return;
+  const Draw d = a.draws[b];
+  if (!d.rest) return;
   __shared__ double scratch[4];
-  __shared__ int last, found;
-  const float T = temperature(a, b);
-  const bool greedy = !(T > 0);
-  if (greedy && piece) return;
-  if (tid < 64) {
-    if (greedy) {
-      const int at = accepted_of<DT>(a, b, length(a, b), T);
-      if (lane == 0) d.at = at, found = row_best(a, parts_of(a, b, at));
-    } else {
-      draw_of<DT>(a, b, d);
-    }
-  }
-  __syncthreads();
-  if (!greedy) {
-    double sp = 0, sq = 0;
-    for (int i = 0; i < a.pieces; ++i) {
-      const double *const o = a.totals + ((int64_t)b * a.pieces + i) * 2;
-      sp += o[0], sq += o[1];
-    }
-    const double rp = 1.0 / sp, rq = sq > 0 ? 1.0 / sq : sq;  // an empty draft row: q = 0; NaN stays
-    double rest[8], chance[8], sr = 0, sc = 0;
-    {
-      const int from = piece * a.piece, to = min(a.V, from + a.piece);
-      for (int k = from + tid * 8; k < to; k += 2048) {
-        weights_of<DT>(a, b, d, rp, rq, k, to, rest, chance);
+  const Norms n = norms_of(a, b, lane);
+  double rest[8], chance[8], sr = 0, sc = 0;
+  const int from = piece * a.piece, to = min(a.V, from + a.piece);
+  for (int k = from + threadIdx.x * 8; k < to; k += 2048) {
+    weights_of<DT>(a, b, d, n, k, to, rest, chance);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sr += rest[j], sc += chance[j];
+    for (int j = 0; j < 8; ++j) sr += rest[j], sc += chance[j];
+  }
+  sr = block_sum(sr, scratch);
+  sc = block_sum(sc, scratch);
+  if (threadIdx.x == 0) {
+    double *const o = a.weights + ((int64_t)b * a.pieces + piece) * 2;
+    o[0] = sr, o[1] = sc;
+  }
+}
+
+// A workgroup finds a stream's drawn token and writes its row of the result. The running sum goes by piece (each wave
+// for itself), then by 8192 tokens of the piece, by thread and by token. In a launch of its own: a stream's last
+// workgroup of weight_kernel could do it, but the fence that every workgroup then needs writes its XCD's L2 back
+// (64 streams of 150144 tokens: 97 us, as two launches 27).
+template <int DT>
+__global__ __launch_bounds__(1024) void draw_kernel(const Args a) {
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ double scratch[16];
+  __shared__ int2 hits[16];
+  const float T = temperature(a, b);
+  const double *const totals = a.totals + (int64_t)b * a.pieces * 2;
+  Draw d;
+  int found = -1;
+  if (!(T > 0)) {
+    d.at = a.L ? a.draws[b].at : 0;
+    found = row_best(a, a.L ? parts_of(a, b, d.at) : a.parts + (int64_t)b * a.pieces, a.L ? a.splits : a.pieces);
+  } else {
+    // weights of the pieces lane and lane + 64; of the second choice, p itself
+    double lo = piece_value(totals, lane, a.pieces, 0), hi = piece_value(totals, lane + 64, a.pieces, 0);
+    double lo1 = piece_value(totals, lane, a.pieces, 1), hi1 = piece_value(totals, lane + 64, a.pieces, 1);
+    Norms n{1.0, 0.0};
+    if (!a.L) {  // pieces with largest logits of their own
+      float m = fmaxf(lane < a.pieces ? (float)lo1 : -FLT_MAX, lane + 64 < a.pieces ? (float)hi1 : -FLT_MAX);
+#pragma unroll
+      for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+      d = Draw{0, 0, exponent(T, m), Exponent{0, 0}, -1};
+      lo *= power(lo1, d.p), hi *= power(hi1, d.p);
+      lo1 = lo, hi1 = hi;
+    } else {
+      d = a.draws[b];
+      if (d.rest) {
+        n = norms_of(a, b, lane);
+        const double *const w = a.weights + (int64_t)b * a.pieces * 2;
+        lo = piece_value(w, lane, a.pieces, 0), hi = piece_value(w, lane + 64, a.pieces, 0);
+        lo1 = piece_value(w, lane, a.pieces, 1), hi1 = piece_value(w, lane + 64, a.pieces, 1);
+      } else {
+        lo1 += lo, hi1 += hi;
       }
-      sr = block_sum<256>(sr, scratch);
-      sc = block_sum<256>(sc, scratch);
     }
-    if (tid == 0) {
-      double *const o = a.weights + ((int64_t)b * a.pieces + piece) * 2;
-      o[0] = sr, o[1] = sc;
-      __threadfence();
-      last = atomicAdd(&a.arrived[b], 1) == a.pieces - 1;
-      __threadfence();
-    }
-    __syncthreads();
-    if (!last) return;
-    // the running sum by piece, then by 2048 tokens of the piece, then by thread and token
-    const double *const w = a.weights + (int64_t)b * a.pieces * 2;
-    double whole = 0, all = 0;
-    for (int i = 0; i < a.pieces; ++i) whole += __builtin_nontemporal_load(w + 2 * i), all += __builtin_nontemporal_load(w + 2 * i + 1);
-    const int side = whole > 0 ? 0 : 1;
-    if (side) whole = all;
-    if (tid == 0) found = -1;
+    const bool side = !(wave_sum(lo + hi) > 0);
+    if (side) lo = lo1, hi = hi1;
+    const auto scan = [&](double v) {
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const double u = __shfl_up(v, o);
+        if (lane >= o) v += u;
+      }
+      return v;
+    };
+    const double run_lo = scan(lo), half = __shfl(run_lo, 63), run_hi = half + scan(hi), whole = __shfl(run_hi, 63);
     if (whole > 0 && whole <= DBL_MAX) {
       const double goal = uniform(a, b, a.L) * whole;
-      double run = 0;
-      int at = -1, some = -1;
-      for (int i = 0; i < a.pieces; ++i) {
-        const double s = __builtin_nontemporal_load(w + 2 * i + side);
-        if (s > 0) some = i;
-        if (s > 0 && run + s > goal) {
-          at = i;
-          break;
-        }
-        run += s;
+      const uint64_t in_lo = __ballot(lo > 0 && run_lo > goal), in_hi = __ballot(hi > 0 && run_hi > goal);
+      int at;
+      if (in_lo) at = __builtin_ctzll(in_lo);
+      else if (in_hi) at = 64 + __builtin_ctzll(in_hi);
+      else {  // a number of 1 or more, or none: the last token with a weight
+        const uint64_t some_lo = __ballot(lo > 0), some_hi = __ballot(hi > 0);
+        at = some_hi ? 127 - __builtin_clzll(some_hi) : 63 - __builtin_clzll(some_lo);
       }
-      if (at < 0) {  // a number of 1 or more, or none: the last token with a weight
-        at = some;
-        for (run = 0, some = 0; some < at; ++some) run += __builtin_nontemporal_load(w + 2 * some + side);
-      }
+      // what runs before the piece: the sums of the pieces before it, so that no difference is taken
+      double run = at & 63 ? __shfl(at < 64 ? run_lo : run_hi, (at & 63) - 1) : (at < 64 ? 0.0 : half);
       const int from = at * a.piece, to = min(a.V, from + a.piece);
-      __shared__ int first, final;
-      if (tid == 0) first = 0x7fffffff, final = -1;
-      __syncthreads();
-      for (int base = from; base < to; base += 2048) {
+      int some = -1;
+      for (int base = from; base < to && found < 0; base += 8192) {
         const int k = base + tid * 8;
-        double mine = 0;
+        double rest[8], chance[8], mine = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) rest[j] = 0;
         if (k < to) {
-          weights_of<DT>(a, b, d, rp, rq, k, to, rest, chance);
-          if (side) {
+          weights_of<DT>(a, b, d, n, k, to, rest, chance);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) rest[j] = chance[j];
+          for (int j = 0; j < 8; ++j) {
+            rest[j] = side ? chance[j] : rest[j];
+            mine += rest[j];
           }
-#pragma unroll
-          for (int j = 0; j < 8; ++j) mine += rest[j];
         }
-        double s = mine;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-          const double u = __shfl_up(s, o);
-          if (lane >= o) s += u;
-        }
+        const double s = scan(mine);
+        __syncthreads();  // the last 8192 tokens' sums and hits have been read
         if (lane == 63) scratch[wave] = s;
         __syncthreads();
         double before = run;
         for (int v = 0; v < wave; ++v) before += scratch[v];
-        double end = run;
-        for (int v = 0; v < 4; ++v) end += scratch[v];
+        for (int v = 0; v < 16; ++v) run += scratch[v];
         before += s - mine;
-        if (k < to) {
-          for (int j = 0; j < 8; ++j) {
-            if (rest[j] > 0) {
-              before += rest[j];
-              atomicMax(&final, k + j);
-              if (before > goal) {
-                atomicMin(&first, k + j);
-                break;
-              }
-            }
+        int first = kNone, final = -1;  // the first token past the goal, and the last one with a weight
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          before += rest[j];
+          if (rest[j] > 0) {
+            final = k + j;
+            if (before > goal && first == kNone) first = k + j;
           }
         }
+#pragma unroll
+        for (int o = 32; o; o >>= 1) first = min(first, __shfl_xor(first, o)), final = max(final, __shfl_xor(final, o));
+        if (lane == 0) hits[wave] = make_int2(first, final);
         __syncthreads();
-        run = end;
-        if (first != 0x7fffffff) break;
+        for (int v = 0; v < 16; ++v) first = min(first, hits[v].x), final = max(final, hits[v].y);
+        some = max(some, final);
+        if (first != kNone) found = first;
       }
-      if (tid == 0) found = first != 0x7fffffff ? first : final;
+      if (found < 0) found = some;
     }
-    __syncthreads();
   }
-  for (int t = tid; t <= a.L; t += 256)
+  for (int t = tid; t <= a.L; t += 1024)
     a.out[(int64_t)b * (a.L + 1) + t] = t < d.at ? a.tokens[(int64_t)b * a.L + t] : t == d.at ? found : -1;
   if (tid == 0) a.accepted[b] = d.at;
 }
 
 struct Layout {
-  int splits, chunk, pieces, piece;
-  int64_t parts, totals, weights, arrived, bytes;
+  int splits, chunk, pieces, piece, ranges;
+  int64_t parts, totals, weights, draws, refused, bytes;
 };
 // Pieces of whole 2048 tokens (256 threads, 16 or 32 bytes each), enough of them to occupy the device a few times over.
 static void cut(int64_t V, int64_t rows, int64_t most, int &n, int &size) {
@@ -445,9 +582,28 @@ static void cut(int64_t V, int64_t rows, int64_t most, int &n, int &size) {
   size = (int)(cdiv(cdiv(V, want), 2048) * 2048);
   n = (int)cdiv(V, size);
 }
+// Positions of the launches of stats_kernel: the last of them ends with L + 1.
+static int ranges_of(int64_t B, int64_t L, int64_t V, int draft, int *ends) {
+  int n = 0;
+  const int64_t logits = B * V * (draft ? 2 : 1);  // of a position
+  if (logits * (L + 1) < kSeveral) {
+    ends[n++] = (int)L + 1;
+    return n;
+  }
+  int64_t at = 0, step = std::max<int64_t>(1, cdiv(kFirst, logits));
+  while (n < kRanges - 1 && at + 2 * step < L + 1) {
+    at += step;
+    ends[n++] = (int)at;
+    step += (step + 1) / 2;
+  }
+  ends[n++] = (int)L + 1;
+  return n;
+}
 static Layout layout(int64_t B, int64_t L, int64_t V, int draft) {
   Layout l;
-  cut(V, B * (L + 1 + (draft ? L : 0)), 32, l.splits, l.chunk);
+  int ends[kRanges];
+  l.ranges = ranges_of(B, L, V, draft, ends);
+  cut(V, B * ends[0] * (L && draft ? 2 : 1), 32, l.splits, l.chunk);
   cut(V, B, 128, l.pieces, l.piece);
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
@@ -455,20 +611,33 @@ static Layout layout(int64_t B, int64_t L, int64_t V, int draft) {
     at += (bytes + 255) / 256 * 256;
     return r;
   };
-  l.parts = take(B * (2 * L + 1) * l.splits * (int64_t)sizeof(Part));
+  l.parts = take(L ? B * (2 * L + 1) * l.splits * (int64_t)sizeof(Part) : B * l.pieces * (int64_t)sizeof(Part));
   l.totals = take(B * l.pieces * 16);
   l.weights = take(B * l.pieces * 16);
-  l.arrived = take(B * 4);
+  l.draws = take(B * (int64_t)sizeof(Draw));
+  l.refused = take(kRanges * B * 4);
   l.bytes = at;
   return l;
 }
 
 template <int DT>
-static void launch(const Args &a, hipStream_t st) {
-  const int sides = a.draft ? 2 : 1;
-  stats_kernel<DT><<<(unsigned)((int64_t)a.splits * sides * a.B * (a.L + 1)), 256, 0, st>>>(a, 0, a.L + 1);
-  total_kernel<DT><<<(unsigned)((int64_t)a.B * a.pieces), 256, 0, st>>>(a);
-  draw_kernel<DT><<<(unsigned)((int64_t)a.B * a.pieces), 256, 0, st>>>(a);
+static void launch(Args a, hipStream_t st) {
+  const unsigned all = (unsigned)((int64_t)a.B * a.pieces);
+  if (a.L) {
+    int ends[kRanges];
+    const int n = ranges_of(a.B, a.L, a.V, a.draft != nullptr, ends);
+    for (a.range = 0; a.range < n; ++a.range) {
+      a.before = a.range > 1 ? ends[a.range - 2] : 0;
+      a.t0 = a.range ? ends[a.range - 1] : 0, a.t1 = ends[a.range];
+      stats_kernel<DT><<<(unsigned)((int64_t)a.splits * (a.draft ? 2 : 1) * a.B * (a.t1 - a.t0)), 256, 0, st>>>(a);
+    }
+    --a.range;
+    total_kernel<DT><<<all, 256, 0, st>>>(a);
+  } else {
+    sample_kernel<DT><<<all, 256, 0, st>>>(a);
+  }
+  if (a.draft) weight_kernel<DT><<<all, 256, 0, st>>>(a);
+  draw_kernel<DT><<<(unsigned)a.B, 1024, 0, st>>>(a);
 }
 
 static bool fits(int64_t B, int64_t L, int64_t V) {
@@ -502,7 +671,8 @@ extern "C" int ksd_verify_draft(const void *target, const void *draft, int dtype
   char *w = (char *)workspace;
   spec::Args a{target, L ? draft : nullptr, target_b, target_t, draft_b, draft_t, tokens, uniforms, uniforms_wide, temperatures,
                temperature, lengths, out, accepted, (spec::Part *)(w + l.parts), (double *)(w + l.totals), (double *)(w + l.weights),
-               (int *)(w + l.arrived), (int)B, (int)L, (int)V, l.splits, l.chunk, l.pieces, l.piece};
+               (spec::Draw *)(w + l.draws), (int *)(w + l.refused), (int)B, (int)L, (int)V, l.splits,
+               l.chunk, l.pieces, l.piece, 0, 0, 0, 0};
   hipStream_t st = (hipStream_t)stream;
   if (!grid_fits((int64_t)l.splits * 2 * B * (L + 1), 256) || !grid_fits(B * l.pieces, 256))
     return fail(KSD_EINVAL, "verify_draft: too many rows");

@@ -137,6 +137,31 @@ def test_long_rows(dtype, V):
         assert torch.equal(got[k].cpu(), verify_cpu(target[:, :1], None, u[:, k:k + 1], None, temps)[0][:, 0])
 
 
+def test_positions_in_several_launches():
+    """A long batch: streams refused early, late and never, greedy ones, every length; rows shared between the
+    streams (strides of 0), their tokens and numbers their own."""
+    B, L, V = 64, 20, 30000
+    target, draft, _, _, _ = make(1, L, V, "bf16", 51, peaks=4)
+    g = torch.Generator().manual_seed(3)
+    temps = torch.full((B,), 0.9)
+    temps[::7] = 0
+    tokens = torch.multinomial(torch.softmax(draft[0].float() / 0.9, 1), B, replacement=True, generator=g).t().contiguous()
+    tokens[::7] = target[0, :L].float().argmax(1)
+    tokens[7, 4], tokens[14, 0], tokens[21, 19], tokens[28, 12] = 1, 2, 3, 4
+    u = torch.rand(B, L + 1, generator=g) * (torch.arange(B)[:, None] % 3 / 2).clamp(min=1e-3)  # 0.001, 0.5 and 1 times
+    lengths = torch.randint(0, L + 1, (B,), generator=g)
+    lengths[::2] = L
+    for d in (draft, None):
+        want = verify_cpu(target.expand(B, L + 1, V), tokens, u, None if d is None else d.expand(B, L, V), temps, lengths)
+        for n in (lengths, None):
+            if n is None:
+                want = verify_cpu(target.expand(B, L + 1, V), tokens, u, None if d is None else d.expand(B, L, V), temps)
+            got = verify_draft(gpu(target).expand(B, L + 1, V), gpu(tokens), gpu(u), None if d is None else gpu(d).expand(B, L, V),
+                               gpu(temps), gpu(n))
+            assert torch.equal(got[0].cpu(), want[0]) and torch.equal(got[1].cpu(), want[1])
+        assert len(set(want[1].tolist())) > 5
+
+
 def test_masks():
     """-inf and the type's lowest values, rows with one finite logit, with none, with NaN and +inf."""
     inf, nan = math.inf, math.nan
@@ -197,8 +222,8 @@ def test_temperatures():
     target, draft, tokens, u, _ = make(8, 3, 700, "bf16", 23)
     cold = torch.tensor([1e-30, 1e-3, 1e-2, 0.1, 10.0, 1e4, -1.0, math.nan])
     got = verify_draft(gpu(target), gpu(tokens), gpu(u), gpu(draft), gpu(cold))
-    want = verify_cpu(target[2:], tokens[2:], u[2:], draft[2:], cold[2:])
-    assert torch.equal(got[0][2:].cpu(), want[0]) and torch.equal(got[1][2:].cpu(), want[1])
+    want = verify_cpu(target, tokens, u, draft, cold)
+    assert torch.equal(got[0].cpu(), want[0]) and torch.equal(got[1].cpu(), want[1])
     assert torch.equal(verify_draft(gpu(target), gpu(tokens), gpu(u), gpu(draft), 0.7)[0],
                        verify_draft(gpu(target), gpu(tokens), gpu(u), gpu(draft), torch.full((8,), 0.7, device=DEV))[0])
     assert torch.equal(verify_draft(gpu(target), gpu(tokens), None, temperatures=0.0)[0].cpu(),
