@@ -49,14 +49,6 @@ __device__ __forceinline__ typename Oct<DT>::V load_oct(const typename Elem<DT>:
   }
   return v;
 }
-__device__ __forceinline__ f32x4 load_four(const float *row, int c, int n) {
-  struct __attribute__((packed, aligned(4))) Any { f32x4 v; };
-  if (c + 4 <= n) return ((const Any *)(row + c))->v;
-  f32x4 v;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) v[j] = c + j < n ? row[c + j] : 0.0f;
-  return v;
-}
 template <int DT>
 __device__ __forceinline__ void to_floats(const typename Oct<DT>::V &v, float *f) {
 #pragma unroll
@@ -116,6 +108,15 @@ __device__ __forceinline__ f32x4 product(const typename Oct<DT>::V &a, const typ
   }
 }
 
+// Tokens are listed by adapter (stable; those without one last, as adapter n), each list in pieces. Piece j of adapter
+// i is slot start_i / piece + i + j: slots of different adapters never meet, and a slot knows its adapter without a sum
+// over the earlier ones' pieces.
+constexpr int kTile = 32, kPiece = 256;  // of the products by rows; of the gradients' sums
+
+struct Slot {
+  int adapter, from, to, pad;  // -1: empty
+};
+
 struct PairArgs {
   const void *x;           // (M, K), row stride
   int64_t x_stride, M, K, N;
@@ -132,93 +133,191 @@ struct PairArgs {
   int n, r, rows, cols;    // rows and columns (a multiple of 64) of a workgroup
   Mask mask;
   int mask_x, mask_y;
+  const int32_t *order;    // tokens listed by adapter, and the pieces of the lists (NULL: rows as they lie)
+  const Slot *slots;
+  int tiles;               // workgroups of a piece
 };
 
 __device__ __forceinline__ int adapter_of(const void *index, int wide, int64_t per, int64_t m, int n) {
-  const int64_t at = per == 1 ? m : m / per;
+  const int64_t at = per == 1 ? m : (uint32_t)m / (uint32_t)per;
   const int64_t i = wide ? ((const int64_t *)index)[at] : (int64_t)((const int32_t *)index)[at];
   return i >= 0 && i < n ? (int)i : -1;
 }
 
+// 8 elements from c on that lie inside a row.
+template <int DT>
+__device__ __forceinline__ typename Oct<DT>::V whole_oct(const typename Elem<DT>::T *row, int64_t c) {
+  struct __attribute__((packed, aligned(sizeof(typename Elem<DT>::T)))) Any { typename Oct<DT>::V v; };
+  return ((const Any *)(row + c))->v;
+}
+
+// The dropped ones of 8 values become 0; the kept ones stay as they are (fp32: are scaled). 16-bit values would be
+// rounded by the scale, which their sums take instead.
+template <int DT>
+__device__ __forceinline__ void drop_oct(const Mask &m, uint4 bits, typename Oct<DT>::V &v) {
+  const uint32_t w[4] = {bits.x, bits.y, bits.z, bits.w};
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t u = j & 1 ? w[j / 2] >> 16 : w[j / 2] & 0xffffu;
+    if constexpr (DT == KSD_F32) v[j] = u >= m.drop ? v[j] * m.scale : 0.0f;
+    else v[j] = u >= m.drop ? v[j] : (short)0;
+  }
+}
+
+// U steps of 32 columns of the narrow product. Rows of other adapters and ranks from r on are read from a
+// row that exists: their results are not used. `whole`: no step passes the row's end.
+template <int DT, int R16, int RT, int U, bool MASK>
+__device__ __forceinline__ void narrow(const PairArgs &p, const typename Elem<DT>::T *const (&xr)[RT],
+                                       const typename Elem<DT>::T *const (&ar)[R16], int64_t s, bool whole, MaskKey key,
+                                       const int64_t (&row)[RT], int grp, f32x4 (&acc)[RT][R16]) {
+  using V = typename Oct<DT>::V;
+  V xv[U][RT], av[U][R16];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t k = (s + u) * 32 + grp * 8;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) xv[u][t] = whole ? whole_oct<DT>(xr[t], k) : load_oct<DT>(xr[t], k, p.K);
+#pragma unroll
+    for (int q = 0; q < R16; ++q) av[u][q] = whole ? whole_oct<DT>(ar[q], k) : load_oct<DT>(ar[q], k, p.K);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if constexpr (MASK) {
+      if (p.mask_x) {
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+          drop_oct<DT>(p.mask, mask_bits(p.mask, key, row[t], (uint32_t)((s + u) * 4 + grp)), xv[u][t]);
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int q = 0; q < R16; ++q) acc[t][q] = product<DT>(av[u][q], xv[u][t], acc[t][q]);
+  }
+}
+
+// What a lane takes of a bank row of r ranks in a block of 16: fp32 ranks 4 grp .. + 3, 16-bit types ranks 8 (grp % 2) ..
+// + 7; zeros from r on. ALIGNED: r is a multiple of that, else value by value (r = 23: 8 loads for one).
+template <int DT, bool ALIGNED>
+__device__ __forceinline__ typename Oct<DT>::V bank_oct(const typename Elem<DT>::T *row, int q, int grp, int r) {
+  using V = typename Oct<DT>::V;
+  constexpr int W = DT == KSD_F32 ? 4 : 8;
+  const int c = q * 16 + (DT == KSD_F32 ? grp : grp & 1) * W;
+  V w{};
+  if constexpr (!ALIGNED) {
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      const auto e = row[min(c + j, r - 1)];
+      w[j] = c + j < r ? e : 0;
+    }
+  } else if constexpr (DT == KSD_F32) {
+    struct __attribute__((packed, aligned(4))) Any { f32x4 v; };
+    const f32x4 v = ((const Any *)(row + (c < r ? c : 0)))->v;
+#pragma unroll
+    for (int j = 0; j < W; ++j) w[j] = c < r ? v[j] : 0.0f;
+  } else {
+    w = whole_oct<DT>(row, c < r ? c : 0);
+    w = c < r ? w : V{};
+  }
+  return w;
+}
+
 // R16: blocks of 16 ranks; RT: blocks of 16 rows.
-template <int DT, int R16, int RT, bool MASK>
+template <int DT, int R16, int RT, bool MASK, bool ALIGNED>
 __global__ __launch_bounds__(64 * kWaves) void pair_kernel(const PairArgs p) {
   using T = typename Elem<DT>::T;
   using V = typename Oct<DT>::V;
-  constexpr int R = 16 * R16, U = DT == KSD_F32 ? (R16 <= 2 ? 2 : 1) : (R16 <= 2 ? 4 : 2);
+  constexpr int R = 16 * R16, U = DT == KSD_F32 ? (R16 <= 1 ? 4 : R16 <= 2 ? 2 : 1) : (R16 <= 1 ? 6 : R16 <= 2 ? 4 : 2);
+  constexpr int TB = R16 <= 2 ? 4 : R16 == 4 ? 2 : 1;  // products whose bank rows are loaded together
+  constexpr bool kAhead = R16 == 1;  // the next bank rows are loaded during a block's products: more ranks, no registers for it
   constexpr int pitch = R + 4;  // floats: a row's four lanes of 16 bytes start 4 banks further than the last row's
   extern __shared__ float lds[];  // (kWaves, 16 RT, pitch): sums of a wave's columns; the first holds h
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, grp = lane >> 4;
-  const int64_t row0 = (int64_t)blockIdx.x * p.rows;
-  const int rows = (int)min((int64_t)p.rows, p.M - row0);
-  // lane l < 16 RT: the adapter of row l
-  const int mine = lane < rows ? adapter_of(p.index, p.wide, p.per, row0 + lane, p.n) : -1;
+  // lane l < rows: its token and the token's adapter
+  int rows, mine = -1, token = 0;
+  if (p.slots) {
+    const Slot s = p.slots[blockIdx.x / p.tiles];
+    const int from = s.from + (int)(blockIdx.x % p.tiles) * p.rows;
+    rows = s.adapter < 0 ? 0 : min(p.rows, s.to - from);
+    if (rows <= 0) return;
+    if (lane < rows) token = p.order[from + lane], mine = s.adapter < p.n ? s.adapter : -1;
+  } else {
+    const int64_t row0 = (int64_t)blockIdx.x * p.rows;
+    rows = (int)min((int64_t)p.rows, p.M - row0);
+    if (lane < rows) token = (int)row0 + lane, mine = adapter_of(p.index, p.wide, p.per, token, p.n);
+  }
   int of[RT];  // of the rows that this lane's columns of the products are
+  int64_t at_row[RT];
 #pragma unroll
-  for (int t = 0; t < RT; ++t) of[t] = __shfl(mine, t * 16 + col);
+  for (int t = 0; t < RT; ++t) {
+    of[t] = __shfl(mine, t * 16 + col);
+    at_row[t] = __shfl(token, t * 16 + col < rows ? t * 16 + col : 0);
+  }
   const uint64_t with = __ballot(mine >= 0);
   MaskKey key{};
   if constexpr (MASK) key = mask_key(p.mask);
 
+  const int64_t n0 = (int64_t)blockIdx.y * p.cols, n1 = min(p.N, n0 + p.cols);
+  // base of a block of 64 columns: 16 of them per lane
+  const auto load_base = [&](int64_t c, V (&v)[RT][2]) {
+    const int64_t at = c + grp * 16;
+    const bool whole = c + 64 <= p.N;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      const T *const row = (const T *)p.base + at_row[t] * p.base_stride;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) v[t][e] = whole ? whole_oct<DT>(row, at + e * 8) : load_oct<DT>(row, at + e * 8, p.N);
+    }
+  };
+  V bv[RT][2] = {};
+  int64_t c = n0 + wave * 64;
+  const bool based = p.base && p.y;
+  if (based && c < n1) load_base(c, bv);
+  // An adapter's bank rows for tiles t0 .. of a block: row i of product t is column (i / 4) 16 + 4 t + i % 4 of the block,
+  // so a lane ends with 16 consecutive columns of its token.
+  const auto load_bank = [&](int64_t c, int i, int t0, V (&w)[TB][R16]) {
+    const T *const b = (const T *)p.b + (int64_t)i * p.N * p.r;
+    const bool whole = c + 64 <= p.N;
+#pragma unroll
+    for (int t = 0; t < TB; ++t) {
+      const int64_t n = c + (col >> 2) * 16 + (t0 + t) * 4 + (col & 3);
+#pragma unroll
+      for (int q = 0; q < R16; ++q) w[t][q] = bank_oct<DT, ALIGNED>(b + (whole ? n : min(n, p.N - 1)) * p.r, q, grp, p.r);
+    }
+  };
+  const auto lowest = [&](uint64_t rows) { return __shfl(mine, __builtin_ctzll(rows)); };
+  V w[TB][R16] = {};
+  if (kAhead && with && p.y && c < n1) load_bank(c, lowest(with), 0, w);
+
   if (with) {
     // ---- h: D[rank][token] = A x^T over this wave's columns
-    const int64_t steps = (p.K + 31) / 32, share = ((steps + kWaves - 1) / kWaves + 1) & ~1ll;
-    const int64_t from = wave * share, to = min(steps, from + share);
+    const T *xr[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) xr[t] = (const T *)p.x + at_row[t] * p.x_stride;
+    const int64_t steps = (p.K + 31) / 32, full = p.K / 32, share = ((steps + kWaves - 1) / kWaves + 1) & ~1ll;
+    const int64_t from = wave * share, to = min(steps, from + share), upto = min(to, full);
     for (uint64_t left = with; left;) {
       const int i = __shfl(mine, __builtin_ctzll(left));
       left &= ~__ballot(mine == i);
       const T *const a = (const T *)p.a + (int64_t)i * p.r * p.K;
+      const T *ar[R16];
+#pragma unroll
+      for (int q = 0; q < R16; ++q) ar[q] = a + (int64_t)min(q * 16 + col, p.r - 1) * p.K;
       f32x4 acc[RT][R16] = {};
-      for (int64_t s = from; s < to; s += U) {
-        V xv[U][RT], av[U][R16];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int64_t k = (s + u) * 32 + grp * 8;
-          const bool in = s + u < to;
-#pragma unroll
-          for (int t = 0; t < RT; ++t) {
-            xv[u][t] = V{};
-            if (in && of[t] == i) xv[u][t] = load_oct<DT>((const T *)p.x + (row0 + t * 16 + col) * p.x_stride, k, p.K);
-          }
-#pragma unroll
-          for (int q = 0; q < R16; ++q) {
-            av[u][q] = V{};
-            if (in && q * 16 + col < p.r) av[u][q] = load_oct<DT>(a + (int64_t)(q * 16 + col) * p.K, k, p.K);
-          }
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          if constexpr (MASK) {
-            if (p.mask_x) {
-#pragma unroll
-              for (int t = 0; t < RT; ++t) {
-                float f[8];
-                to_floats<DT>(xv[u][t], f);
-                apply_mask(p.mask, mask_bits(p.mask, key, row0 + t * 16 + col, (uint32_t)((s + u) * 4 + grp)), f);
-                // 16-bit: the scaled value would be rounded; the scale goes to h instead
-                if constexpr (DT != KSD_F32) {
-#pragma unroll
-                  for (int j = 0; j < 8; ++j) xv[u][t][j] = f[j] == 0.0f ? (short)0 : xv[u][t][j];
-                } else {
-                  xv[u][t] = from_floats<DT>(f);
-                }
-              }
-            }
-          }
-#pragma unroll
-          for (int t = 0; t < RT; ++t)
-#pragma unroll
-            for (int q = 0; q < R16; ++q) acc[t][q] = product<DT>(av[u][q], xv[u][t], acc[t][q]);
-        }
+      int64_t s = from;
+      for (; s + U <= upto; s += U) narrow<DT, R16, RT, U, MASK>(p, xr, ar, s, true, key, at_row, grp, acc);
+      if constexpr (U > 2) {
+        for (; s + 2 <= upto; s += 2) narrow<DT, R16, RT, 2, MASK>(p, xr, ar, s, true, key, at_row, grp, acc);
       }
-      float s = p.scales ? p.scales[i] : 1.0f;
-      if constexpr (MASK && DT != KSD_F32) s *= p.mask_x ? p.mask.scale : 1.0f;
+      for (; s < to; ++s) narrow<DT, R16, RT, 1, MASK>(p, xr, ar, s, s < full, key, at_row, grp, acc);
+      float scale = p.scales ? p.scales[i] : 1.0f;
+      if constexpr (MASK && DT != KSD_F32) scale *= p.mask_x ? p.mask.scale : 1.0f;
 #pragma unroll
       for (int t = 0; t < RT; ++t)
         if (of[t] == i) {
           float *const o = lds + ((int64_t)wave * 16 * RT + t * 16 + col) * pitch + grp * 4;
 #pragma unroll
-          for (int q = 0; q < R16; ++q) *(f32x4 *)(o + q * 16) = acc[t][q] * s;
+          for (int q = 0; q < R16; ++q) *(f32x4 *)(o + q * 16) = acc[t][q] * scale;
         }
     }
     __syncthreads();
@@ -228,21 +327,21 @@ __global__ __launch_bounds__(64 * kWaves) void pair_kernel(const PairArgs p) {
         float v = lds[t * pitch + q];
 #pragma unroll
         for (int w = 1; w < kWaves; ++w) v += lds[(w * 16 * RT + t) * pitch + q];
-        lds[t * pitch + q] = v;
-        if (p.hidden && blockIdx.y == 0 && q < p.r) p.hidden[(row0 + t) * p.r + q] = v;
+        lds[t * pitch + q] = q < p.r ? v : 0.0f;
       }
     }
     __syncthreads();
   }
-  if (p.hidden && blockIdx.y == 0) {  // rows without an adapter
-    for (int e = threadIdx.x; e < rows * p.r; e += 64 * kWaves)
-      if (!(with >> (e / p.r) & 1)) p.hidden[row0 * p.r + e] = 0.0f;
+  if (p.hidden && blockIdx.y == 0) {
+    for (int t = wave; t < rows; t += kWaves) {
+      const int64_t m = __shfl(token, t);
+      for (int q = lane; q < p.r; q += 64) p.hidden[m * p.r + q] = with >> t & 1 ? lds[t * pitch + q] : 0.0f;
+    }
   }
+  if (!p.y) return;
 
-  // ---- y: D[column][token] = B h^T. Row i of product t is column (i / 4) 16 + 4 t + i % 4 of a block of 64, so a
-  // lane ends with 16 consecutive columns of its token.
-  using H = typename Oct<DT>::V;
-  H hv[RT][R16];
+  // ---- y: D[column][token] = B h^T
+  V hv[RT][R16];
   float back[RT];
   if (with) {
 #pragma unroll
@@ -253,7 +352,7 @@ __global__ __launch_bounds__(64 * kWaves) void pair_kernel(const PairArgs p) {
 #pragma unroll
         for (int q = 0; q < R16; ++q) {
           const f32x4 v = *(const f32x4 *)(h + q * 16 + grp * 4);
-          hv[t][q] = H{v.x, v.y, v.z, v.w, 0, 0, 0, 0};
+          hv[t][q] = V{v.x, v.y, v.z, v.w, 0, 0, 0, 0};
         }
       } else {  // ranks 8 (grp % 2) .. + 7: rounded in the lower two groups, the rest in the upper two
         float up = 1.0f;
@@ -286,41 +385,44 @@ __global__ __launch_bounds__(64 * kWaves) void pair_kernel(const PairArgs p) {
       }
     }
   }
-  if (!p.y) return;
-  const int64_t n0 = (int64_t)blockIdx.y * p.cols, n1 = min(p.N, n0 + p.cols);
-  for (int64_t c = n0 + wave * 64; c < n1; c += 64 * kWaves) {
+  for (; c < n1; c += 64 * kWaves) {
     const int64_t at = c + grp * 16;
-    V bv[RT][2];
-#pragma unroll
-    for (int t = 0; t < RT; ++t)
-#pragma unroll
-      for (int v = 0; v < 2; ++v) {
-        bv[t][v] = V{};
-        if (p.base && t * 16 + col < rows && at + v * 8 < p.N)
-          bv[t][v] = load_oct<DT>((const T *)p.base + (row0 + t * 16 + col) * p.base_stride, at + v * 8, p.N);
-      }
+    const bool whole = c + 64 <= p.N;
+    V next[RT][2] = {};
+    if (based && c + 64 * kWaves < n1) load_base(c + 64 * kWaves, next);
     f32x4 acc[RT][4] = {};
     for (uint64_t left = with; left;) {
-      const int i = __shfl(mine, __builtin_ctzll(left));
+      const int i = lowest(left);
       left &= ~__ballot(mine == i);
       f32x4 d[RT][4] = {};
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const int64_t n = min(c + (col >> 2) * 16 + t * 4 + (col & 3), p.N - 1);
-        const T *const b = (const T *)p.b + ((int64_t)i * p.N + n) * p.r;
+      for (int t0 = 0; t0 < 4; t0 += TB) {
+        V ahead[TB][R16] = {};
+        if constexpr (kAhead) {  // the next adapter's or the next block's rows are on the way during these products
+          const int64_t then = left ? c : c + 64 * kWaves;
+          if (then < n1) load_bank(then, lowest(left ? left : with), 0, ahead);
+        } else {
+          load_bank(c, i, t0, w);
+        }
 #pragma unroll
-        for (int q = 0; q < R16; ++q) {
-          if constexpr (DT == KSD_F32) {
-            const f32x4 w = load_four(b, q * 16 + grp * 4, p.r);
+        for (int t = 0; t < TB; ++t)
 #pragma unroll
-            for (int u = 0; u < RT; ++u)
+          for (int q = 0; q < R16; ++q)
 #pragma unroll
-              for (int j = 0; j < 4; ++j) d[u][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[j], hv[u][q][j], d[u][t], 0, 0, 0);
-          } else {
-            const V w = load_oct<DT>(b, q * 16 + (grp & 1) * 8, p.r);
+            for (int u = 0; u < RT; ++u) {
+              f32x4 &o = d[u][t0 + t];
+              if constexpr (DT == KSD_F32) {
 #pragma unroll
-            for (int u = 0; u < RT; ++u) d[u][t] = product<DT>(w, hv[u][q], d[u][t]);
-          }
+                for (int j = 0; j < 4; ++j) o = __builtin_amdgcn_mfma_f32_16x16x4f32(w[t][q][j], hv[u][q][j], o, 0, 0, 0);
+              } else {
+                o = product<DT>(w[t][q], hv[u][q], o);
+              }
+            }
+        if constexpr (kAhead) {
+#pragma unroll
+          for (int t = 0; t < TB; ++t)
+#pragma unroll
+            for (int q = 0; q < R16; ++q) w[t][q] = ahead[t][q];
         }
       }
 #pragma unroll
@@ -330,123 +432,169 @@ __global__ __launch_bounds__(64 * kWaves) void pair_kernel(const PairArgs p) {
     }
 #pragma unroll
     for (int u = 0; u < RT; ++u) {
-      if (u * 16 + col >= rows) continue;
-      const int64_t m = row0 + u * 16 + col;
+      const int64_t m = at_row[u];
+      T *const out = (T *)p.y + m * p.N;
 #pragma unroll
       for (int v = 0; v < 2; ++v) {
-        if (at + v * 8 >= p.N) continue;
         float f[8], g[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[j] = acc[u][v * 2 + j / 4][j & 3];
         if constexpr (MASK) {
           if (p.mask_y) apply_mask(p.mask, mask_bits(p.mask, key, m, (uint32_t)((at >> 3) + v)), f);
         }
-        to_floats<DT>(bv[u][v], g);
-        if (p.base) {
+        if (based) {
+          to_floats<DT>(bv[u][v], g);
 #pragma unroll
           for (int j = 0; j < 8; ++j) f[j] = of[u] >= 0 ? f[j] + g[j] : g[j];
         }
-        store_oct<DT>((T *)p.y + m * p.N, at + v * 8, p.N, f);
+        if (u * 16 + col < rows) {
+          if (whole) {
+            struct __attribute__((packed, aligned(sizeof(T)))) Any { V v; };
+            ((Any *)(out + at + v * 8))->v = from_floats<DT>(f);
+          } else {
+            store_oct<DT>(out, at + v * 8, p.N, f);
+          }
+        }
       }
     }
+#pragma unroll
+    for (int t = 0; t < RT; ++t) bv[t][0] = next[t][0], bv[t][1] = next[t][1];
   }
 }
 
-template <int DT, int R16, int RT>
-static void launch_pair(const PairArgs &p, bool mask, hipStream_t st) {
-  const dim3 g((unsigned)cdiv(p.M, p.rows), (unsigned)cdiv(p.N, p.cols));
+template <int DT, int R16, int RT, bool MASK, bool ALIGNED>
+static void launch_pair(const PairArgs &p, unsigned tiles, hipStream_t st) {
+  const dim3 g(tiles, (unsigned)cdiv(p.N, p.cols));
   constexpr int lds = kWaves * 16 * RT * (16 * R16 + 4) * 4;
   if constexpr (lds > 65536) {  // past HIP's default
-    static const hipError_t set[2] = {
-        hipFuncSetAttribute((const void *)pair_kernel<DT, R16, RT, false>, hipFuncAttributeMaxDynamicSharedMemorySize, lds),
-        hipFuncSetAttribute((const void *)pair_kernel<DT, R16, RT, true>, hipFuncAttributeMaxDynamicSharedMemorySize, lds)};
+    static const hipError_t set = hipFuncSetAttribute((const void *)pair_kernel<DT, R16, RT, MASK, ALIGNED>,
+                                                      hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     (void)set;
   }
-  if (mask) pair_kernel<DT, R16, RT, true><<<g, 64 * kWaves, lds, st>>>(p);
-  else pair_kernel<DT, R16, RT, false><<<g, 64 * kWaves, lds, st>>>(p);
+  pair_kernel<DT, R16, RT, MASK, ALIGNED><<<g, 64 * kWaves, lds, st>>>(p);
+}
+template <int DT, int R16, int RT>
+static void launch_pair(const PairArgs &p, bool mask, unsigned tiles, hipStream_t st) {
+  if constexpr (RT == 1) {
+    if (p.r % (DT == KSD_F32 ? 4 : 8)) {
+      if (mask) launch_pair<DT, R16, RT, true, false>(p, tiles, st);
+      else launch_pair<DT, R16, RT, false, false>(p, tiles, st);
+      return;
+    }
+  }
+  if (mask) launch_pair<DT, R16, RT, true, true>(p, tiles, st);
+  else launch_pair<DT, R16, RT, false, true>(p, tiles, st);
 }
 template <int DT>
-static void launch_pair(const PairArgs &p, bool mask, hipStream_t st) {
+static void launch_pair(const PairArgs &p, bool mask, unsigned tiles, hipStream_t st) {
   const bool one = p.rows <= 16;
-  if (p.r <= 16) one ? launch_pair<DT, 1, 1>(p, mask, st) : launch_pair<DT, 1, 2>(p, mask, st);
-  else if (p.r <= 32) one ? launch_pair<DT, 2, 1>(p, mask, st) : launch_pair<DT, 2, 2>(p, mask, st);
-  else if (p.r <= 64) one ? launch_pair<DT, 4, 1>(p, mask, st) : launch_pair<DT, 4, 2>(p, mask, st);
-  else launch_pair<DT, 8, 1>(p, mask, st);
+  if (p.r <= 16) one ? launch_pair<DT, 1, 1>(p, mask, tiles, st) : launch_pair<DT, 1, 2>(p, mask, tiles, st);
+  else if (p.r <= 32) one ? launch_pair<DT, 2, 1>(p, mask, tiles, st) : launch_pair<DT, 2, 2>(p, mask, tiles, st);
+  else if (p.r <= 64) one ? launch_pair<DT, 4, 1>(p, mask, tiles, st) : launch_pair<DT, 4, 2>(p, mask, tiles, st);
+  else launch_pair<DT, 8, 1>(p, mask, tiles, st);
 }
 
-// Rows and columns of a workgroup.
-static void shape(PairArgs &p) {
-  const int most = p.r <= 64 ? 32 : 16;
-  p.rows = (int)std::max<int64_t>(1, std::min<int64_t>(most, cdiv(p.M, 256)));
-  if (p.rows > 16 && p.rows < 32) p.rows = 16;
+// Rows and columns of a workgroup. Rows that may have several adapters and do not go by lists: one at a time (64 tokens of
+// as many adapters, 1536 x 1536, rank 16: 8.8 us, two 10.4). Else up to 16, whose products fill the instructions
+// (1021 tokens, 1536 x 1536: 9.9 us with 16 rows and 11.0 with 4; 256 tokens: 9.4 and 8.7), and 32 where 256
+// workgroups are left (8192 tokens: 18.6 us, with 16 rows 19.2; rank 64: 33 and 45). Columns are shared out where
+// fewer workgroups than CUs would run, each part forming h again: not where that is the longer product (2047 tokens,
+// 6869 to 1792: 43 us, in two parts 69; 1792 to 6869: 54 us, in 4 parts 47).
+static void shape(PairArgs &p, bool aligned) {
+  if (!p.slots && p.n > 1 && p.per < 16) p.rows = (int)std::min<int64_t>(16, cdiv(p.M, 1024));
+  else p.rows = p.M <= 64 ? 1 : p.M <= 256 ? 4 : p.M <= 512 ? 8 : p.M >= 8192 && p.r <= 64 && aligned ? 32 : 16;
+  if (p.slots)
+    while (kTile % p.rows) --p.rows;
   const int64_t tiles = cdiv(p.M, p.rows), blocks = cdiv(p.N, 64);
-  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(cdiv(blocks, kWaves), cdiv(512, tiles)));
-  p.cols = (int)(cdiv(blocks, parts) * 64);
+  const int64_t parts = std::min({blocks / 6, cdiv(blocks < 64 ? 256 : 512, tiles), 4 * p.N / p.K});
+  p.cols = (int)(cdiv(blocks, std::max<int64_t>(1, parts)) * 64);
 }
 
-// ------------------------------------------------------------------------------- the adapters' gradients
-// Tokens are listed by adapter (stable), each adapter's list in pieces of kPiece. Piece j of adapter i is slot
-// start_i / kPiece + i + j: slots of different adapters never meet, and a slot knows its adapter without a sum over the
-// earlier ones' pieces.
-constexpr int kPiece = 256;
-
-struct Slot {
-  int adapter, from, to, pad;  // -1: empty
-};
-
+// ------------------------------------------------------------------------------- lists by adapter
 struct GroupArgs {
   const void *index;
   int wide, n;
   int64_t per, M;
-  int32_t *order;   // (M,)
-  Slot *slots;      // (M / kPiece + n,)
-  int2 *spans;      // (n,): first slot, slots
+  int32_t *order;        // (M,)
+  Slot *tiles, *pieces;  // (M / kTile + n + 1,), (M / kPiece + n + 1,)
+  int2 *spans;           // (n + 1,): an adapter's first of `pieces`, and how many
 };
 
-// Workgroup i lists adapter i's tokens.
-__global__ __launch_bounds__(256) void group_kernel(const GroupArgs a) {
+// Workgroup i lists adapter i's tokens, workgroup n those without one: 8192 tokens at a time, whose indices are
+// loaded together.
+__global__ __launch_bounds__(1024) void group_kernel(const GroupArgs a) {
+  constexpr int U = 8;
   const int i = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  __shared__ int sums[2][4], counts[4];
+  __shared__ int sums[2][16], counts[2][U][16];
+  int v[U];
+  const auto load = [&](int64_t base) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t m = base + u * 1024 + tid;
+      v[u] = a.n + 1;  // in no list
+      if (m < a.M) {
+        v[u] = adapter_of(a.index, a.wide, a.per, m, a.n);
+        v[u] = v[u] < 0 ? a.n : v[u];
+      }
+    }
+  };
   int less = 0, mine = 0;
-  for (int64_t m = tid; m < a.M; m += 256) {
-    const int v = adapter_of(a.index, a.wide, a.per, m, a.n);
-    less += v >= 0 && v < i, mine += v == i;
+  for (int64_t base = 0; base < a.M; base += U * 1024) {
+    load(base);
+#pragma unroll
+    for (int u = 0; u < U; ++u) less += v[u] < i, mine += v[u] == i;
   }
 #pragma unroll
   for (int o = 32; o; o >>= 1) less += __shfl_xor(less, o), mine += __shfl_xor(mine, o);
   if (lane == 0) sums[0][wave] = less, sums[1][wave] = mine;
   __syncthreads();
-  const int start = sums[0][0] + sums[0][1] + sums[0][2] + sums[0][3], len = sums[1][0] + sums[1][1] + sums[1][2] + sums[1][3];
-  const int slot = start / kPiece + i, next = (start + len) / kPiece + i + 1, pieces = (len + kPiece - 1) / kPiece;
-  // the last adapter's workgroup empties the slots behind it too: tokens without an adapter take none
-  const int upto = i == a.n - 1 ? (int)(a.M / kPiece) + a.n : next;
-  for (int s = slot + tid; s < upto; s += 256) {
-    const int at = start + (s - slot) * kPiece;
-    a.slots[s] = s - slot < pieces ? Slot{i, at, min(at + kPiece, start + len), 0} : Slot{-1, 0, 0, 0};
-  }
-  if (tid == 0) a.spans[i] = make_int2(slot, pieces);
-  if (len == 0) return;
-  int done = start;
-  for (int64_t base = 0; base < a.M; base += 256) {
-    const int64_t m = base + tid;
-    const bool in = m < a.M && adapter_of(a.index, a.wide, a.per, m, a.n) == i;
-    const uint64_t b = __ballot(in);
-    __syncthreads();
-    if (lane == 0) counts[wave] = __popcll(b);
-    __syncthreads();
-    int at = done;
-    for (int w = 0; w < wave; ++w) at += counts[w];
-    if (in) a.order[at + __popcll(b & ((1ull << lane) - 1))] = (int32_t)m;
-    done += counts[0] + counts[1] + counts[2] + counts[3];
+  int start = 0, len = 0;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) start += sums[0][w], len += sums[1][w];
+  const auto cut = [&](Slot *slots, int piece) {
+    // every slot is written: all tokens are in one of the n + 1 lists, so the last one ends at M / piece + n + 1
+    const int slot = start / piece + i, next = (start + len) / piece + i + 1, pieces = (len + piece - 1) / piece;
+    for (int s = slot + tid; s < next; s += 1024) {
+      const int at = start + (s - slot) * piece;
+      slots[s] = s - slot < pieces ? Slot{i, at, min(at + piece, start + len), 0} : Slot{-1, 0, 0, 0};
+    }
+    return make_int2(slot, pieces);
+  };
+  cut(a.tiles, kTile);
+  const int2 span = cut(a.pieces, kPiece);
+  if (tid == 0) a.spans[i] = span;
+  int done = start, turn = 0;
+  for (int64_t base = 0; base < a.M && done < start + len; base += U * 1024, turn ^= 1) {
+    if (a.M > U * 1024) load(base);
+    uint64_t b[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      b[u] = __ballot(v[u] == i);
+      if (lane == 0) counts[turn][u][wave] = __popcll(b[u]);
+    }
+    __syncthreads();  // the other half of counts is read until the next round's
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      int at = done;
+#pragma unroll
+      for (int w = 0; w < 16; ++w) {
+        const int n = counts[turn][u][w];
+        at += w < wave ? n : 0;
+        done += n;
+      }
+      if (v[u] == i) a.order[at + __popcll(b[u] & ((1ull << lane) - 1))] = (int32_t)(base + u * 1024 + tid);
+    }
   }
 }
 
-// out[i][c][r] = in[i][r][c] of 16- or 32-bit values, tiles of 32 x 32.
+// ------------------------------------------------------------------------------- the adapters' gradients
+// out[i][c][r] = in[i][r][c] of 16- or 32-bit values, tiles of 32 x 32; two banks in one launch.
 template <typename T>
-__global__ __launch_bounds__(256) void turn_kernel(const T *__restrict__ in, T *__restrict__ out, int64_t rows, int64_t cols) {
+__device__ __forceinline__ void turn(const T *__restrict__ in, T *__restrict__ out, int64_t rows, int64_t cols, unsigned block) {
   __shared__ T tile[32][33];
-  const int64_t tr = (rows + 31) / 32, tc = (cols + 31) / 32;
-  const int64_t t = blockIdx.x % (tr * tc), i = blockIdx.x / (tr * tc), r0 = t / tc * 32, c0 = t % tc * 32;
+  const unsigned tr = (unsigned)((rows + 31) / 32), tc = (unsigned)((cols + 31) / 32);
+  const unsigned t = block % (tr * tc);
+  const int64_t i = block / (tr * tc), r0 = t / tc * 32, c0 = t % tc * 32;
   in += i * rows * cols, out += i * rows * cols;
   for (int e = threadIdx.x; e < 1024; e += 256) {
     const int64_t r = r0 + e / 32, c = c0 + e % 32;
@@ -458,6 +606,12 @@ __global__ __launch_bounds__(256) void turn_kernel(const T *__restrict__ in, T *
     if (r < rows && c < cols) out[c * rows + r] = tile[e % 32][e / 32];
   }
 }
+template <typename T>
+__global__ __launch_bounds__(256) void turn_kernel(const T *__restrict__ a, T *__restrict__ at, const T *__restrict__ b,
+                                                   T *__restrict__ bt, int64_t r, int64_t K, int64_t N, unsigned a_blocks) {
+  if (blockIdx.x < a_blocks) turn<T>(a, at, r, K, blockIdx.x);
+  else turn<T>(b, bt, N, r, blockIdx.x - a_blocks);
+}
 
 struct GradArgs {
   const void *x, *g;        // (M, K), (M, N)
@@ -466,48 +620,71 @@ struct GradArgs {
   const int32_t *order;
   const Slot *slots;
   float *parts;             // (slots, r K + N r)
-  int r, a_blocks, masked;
+  int r, n, a_blocks, masked;
   Mask mask;
 };
 
-// A slot's sums over its tokens for 128 columns of dA or dB and 64 ranks: D[rank][column] = p^T z in fp32 matrix
-// instructions of 4 tokens, which read both operands as they lie in memory.
-template <int DT>
+// A slot's sums over its tokens for 128 columns of dA or dB and 16 RB ranks: D[rank][column] = p^T z in fp32 matrix
+// instructions of 4 tokens, which read both operands as they lie in memory. A wave takes 16 tokens at a time and has
+// the next 16 on the way.
+template <int DT, int RB>
 __global__ __launch_bounds__(256) void grad_kernel(const GradArgs p) {
   using T = typename Elem<DT>::T;
+  using V = typename Oct<DT>::V;
   const Slot s = p.slots[blockIdx.y];
-  if (s.adapter < 0) return;
+  if (s.adapter < 0 || s.adapter >= p.n) return;
   const bool of_a = (int)blockIdx.x < p.a_blocks;
   const int64_t width = of_a ? p.K : p.N, stride = of_a ? p.x_stride : p.g_stride;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, grp = lane >> 4;
   const int64_t c = (int64_t)(of_a ? blockIdx.x : blockIdx.x - p.a_blocks) * 128 + col * 8;
+  const bool whole = c + 8 <= width;
   const T *const z = (const T *)(of_a ? p.x : p.g);
   const float *const q = of_a ? p.gh : p.h;
   const int r0 = blockIdx.z * 64;
+  const bool masked = of_a && p.masked;
   const MaskKey key = p.masked ? mask_key(p.mask) : MaskKey{};
-  f32x4 acc[4][8] = {};
-  for (int m0 = s.from + wave * 4; m0 < s.to; m0 += 16) {
-    const bool in = m0 + grp < s.to;
-    const int64_t m = in ? p.order[m0 + grp] : 0;
-    float f[8] = {};
-    if (in && c < width) {
-      to_floats<DT>(load_oct<DT>(z + m * stride, c, width), f);
-      if (of_a && p.masked) apply_mask(p.mask, mask_bits(p.mask, key, m, (uint32_t)(c >> 3)), f);
-    }
+  struct Step {
+    V z[4];
+    float p[4][RB];
+    int m[4];
+  };
+  const auto load = [&](int m0, Step &o) {
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      if (r0 + b * 16 >= p.r) break;
-      const int rank = r0 + b * 16 + col;
-      const float v = in && rank < p.r ? q[m * p.r + rank] : 0.0f;
+    for (int u = 0; u < 4; ++u) {
+      const bool in = m0 + u * 4 + grp < s.to;
+      const int64_t m = p.order[in ? m0 + u * 4 + grp : s.from];
+      o.m[u] = (int)m;
+      o.z[u] = V{};
+      if (in) o.z[u] = whole ? whole_oct<DT>(z + m * stride, c) : load_oct<DT>(z + m * stride, c, width);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) acc[b][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, f[j], acc[b][j], 0, 0, 0);
+      for (int b = 0; b < RB; ++b) {
+        const int rank = r0 + b * 16 + col;
+        o.p[u][b] = in && rank < p.r ? q[m * p.r + rank] : 0.0f;
+      }
     }
+  };
+  f32x4 acc[RB][8] = {};
+  Step now, next;
+  int m0 = s.from + wave * 16;
+  if (m0 < s.to) load(m0, now);
+  for (; m0 < s.to; m0 += 64) {
+    if (m0 + 64 < s.to) load(m0 + 64, next);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      float f[8];
+      to_floats<DT>(now.z[u], f);
+      if (masked) apply_mask(p.mask, mask_bits(p.mask, key, now.m[u], (uint32_t)(c >> 3)), f);
+#pragma unroll
+      for (int b = 0; b < RB; ++b)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[b][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(now.p[u][b], f[j], acc[b][j], 0, 0, 0);
+    }
+    now = next;
   }
   __shared__ f32x4 sum[4][8][64];
   float *const out = p.parts + (int64_t)blockIdx.y * p.r * (p.K + p.N);
 #pragma unroll
-  for (int b = 0; b < 4; ++b) {
-    if (r0 + b * 16 >= p.r) break;
+  for (int b = 0; b < RB; ++b) {
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < 8; ++j) sum[wave][j][lane] = acc[b][j];
@@ -530,44 +707,61 @@ __global__ __launch_bounds__(256) void grad_kernel(const GradArgs p) {
   }
 }
 
-// da, db: an adapter's slots added in order.
+// da, db: an adapter's slots added by four waves, every fourth slot each, and the four sums in order.
 __global__ __launch_bounds__(256) void join_kernel(const float *__restrict__ parts, const int2 *__restrict__ spans, int64_t na,
                                                    int64_t nb, float *__restrict__ da, float *__restrict__ db) {
-  const int i = blockIdx.y;
+  __shared__ float sums[4][64];
+  const int i = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int2 s = spans[i];
-  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (e >= na + nb) return;
+  const int64_t e = (int64_t)blockIdx.x * 64 + lane;
   float v = 0.0f;
-  for (int j = 0; j < s.y; ++j) v += parts[(s.x + j) * (na + nb) + e];
-  if (e < na) {
-    if (da) da[i * na + e] = v;
-  } else if (db) {
-    db[i * nb + e - na] = v;
+  if (e < na + nb) {
+#pragma unroll 4
+    for (int j = wave; j < s.y; j += 4) v += parts[(s.x + j) * (na + nb) + e];
   }
+  sums[wave][lane] = v;
+  __syncthreads();
+  if (wave || e >= na + nb) return;
+  v = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
+  if (e < na) da[i * na + e] = v;
+  else db[i * nb + e - na] = v;
 }
 
 static bool float_type(int t) { return t == KSD_F32 || t == KSD_BF16 || t == KSD_F16; }
 static int64_t size_of(int t) { return t == KSD_F32 ? 4 : 2; }
 
+struct Take {
+  int64_t at = 0;
+  int64_t operator()(int64_t bytes) {
+    const int64_t v = at;
+    at += (bytes + 255) / 256 * 256;
+    return v;
+  }
+};
+struct Groups {
+  int64_t order, tiles, pieces, spans, bytes;
+};
+static Groups groups(int64_t M, int64_t n) {
+  Take take;
+  Groups l;
+  l.order = take(M * 4);
+  l.tiles = take((M / kTile + n + 1) * (int64_t)sizeof(Slot));
+  l.pieces = take((M / kPiece + n + 1) * (int64_t)sizeof(Slot));
+  l.spans = take((n + 1) * 8);
+  l.bytes = take.at;
+  return l;
+}
 struct Layout {
-  int64_t order, slots, spans, at, bt, gh, parts, bytes;
+  int64_t at, bt, gh, parts, bytes;
 };
 static Layout layout(int64_t M, int64_t K, int64_t N, int64_t r, int64_t n, int dtype) {
+  Take take;
   Layout l;
-  int64_t at = 0;
-  auto take = [&](int64_t b) {
-    const int64_t v = at;
-    at += (b + 255) / 256 * 256;
-    return v;
-  };
-  l.order = take(M * 4);
-  l.slots = take((M / kPiece + n) * (int64_t)sizeof(Slot));
-  l.spans = take(n * 8);
   l.at = take(n * r * K * size_of(dtype));
   l.bt = take(n * r * N * size_of(dtype));
   l.gh = take(M * r * 4);
-  l.parts = take((M / kPiece + n) * r * (K + N) * 4);
-  l.bytes = at;
+  l.parts = take((M / kPiece + n + 1) * r * (K + N) * 4);
+  l.bytes = take.at;
   return l;
 }
 
@@ -579,18 +773,43 @@ static bool fits(int64_t M, int64_t K, int64_t N, int64_t r, int64_t n) {
 
 static int run_pair(const PairArgs &args, int dtype, bool mask, hipStream_t st) {
   PairArgs p = args;
-  shape(p);
-  if (!grid_fits(cdiv(p.M, p.rows), 64 * kWaves) || cdiv(p.N, p.cols) > 65535)
+  shape(p, p.r % (dtype == KSD_F32 ? 4 : 8) == 0);
+  int64_t tiles = cdiv(p.M, p.rows);
+  if (p.slots) {
+    p.tiles = kTile / p.rows;
+    tiles = (p.M / kTile + p.n + 1) * p.tiles;
+  }
+  if (!grid_fits(tiles, 64 * kWaves) || cdiv(p.N, p.cols) > 65535)
     return fail(KSD_EINVAL, "adapter_linear: too many rows or columns");
-  if (dtype == KSD_F32) launch_pair<KSD_F32>(p, mask, st);
-  else if (dtype == KSD_BF16) launch_pair<KSD_BF16>(p, mask, st);
-  else launch_pair<KSD_F16>(p, mask, st);
+  if (dtype == KSD_F32) launch_pair<KSD_F32>(p, mask, (unsigned)tiles, st);
+  else if (dtype == KSD_BF16) launch_pair<KSD_BF16>(p, mask, (unsigned)tiles, st);
+  else launch_pair<KSD_F16>(p, mask, (unsigned)tiles, st);
   return check_launch("adapter_linear");
 }
 
+// Whether the products go by the lists: tokens in any order whose adapters, read for each token by itself, would be
+// more than 32 MB (the list's launch costs as much as that, about 5 us).
+static bool by_lists(int64_t M, int64_t K, int64_t N, int64_t r, int64_t n, int64_t per, int dtype) {
+  return n > 1 && per < 16 && M > 64 && M * r * (K + N) * size_of(dtype) > (32 << 20);
+}
+
+static void group(const void *index, int wide, int64_t per, int64_t M, int64_t n, char *w, hipStream_t st) {
+  const Groups l = groups(M, n);
+  group_kernel<<<(unsigned)(n + 1), 1024, 0, st>>>(GroupArgs{index, wide, (int)n, per, M, (int32_t *)(w + l.order),
+                                                            (Slot *)(w + l.tiles), (Slot *)(w + l.pieces), (int2 *)(w + l.spans)});
+}
+
+template <int DT>
+static void launch_grad(const GradArgs &q, dim3 grid, hipStream_t st) {
+  if (q.r <= 16) grad_kernel<DT, 1><<<grid, 256, 0, st>>>(q);
+  else if (q.r <= 32) grad_kernel<DT, 2><<<grid, 256, 0, st>>>(q);
+  else grad_kernel<DT, 4><<<grid, 256, 0, st>>>(q);
+}
 template <typename T>
-static void turn(const void *in, void *out, int64_t n, int64_t rows, int64_t cols, hipStream_t st) {
-  turn_kernel<T><<<(unsigned)(n * cdiv(rows, 32) * cdiv(cols, 32)), 256, 0, st>>>((const T *)in, (T *)out, rows, cols);
+static void turn_banks(const void *a, void *at, const void *b, void *bt, int64_t n, int64_t r, int64_t K, int64_t N, hipStream_t st) {
+  const unsigned blocks = (unsigned)(n * cdiv(r, 32) * cdiv(K, 32));
+  turn_kernel<T><<<blocks + (unsigned)(n * cdiv(r, 32) * cdiv(N, 32)), 256, 0, st>>>((const T *)a, (T *)at, (const T *)b, (T *)bt,
+                                                                                      r, K, N, blocks);
 }
 
 }  // namespace adp
@@ -598,20 +817,37 @@ static void turn(const void *in, void *out, int64_t n, int64_t rows, int64_t col
 
 using namespace ksd;
 
+extern "C" int ksd_adapter_linear_groups(int64_t M, int64_t K, int64_t N, int64_t r, int64_t n, int64_t rows_per_index, int dtype,
+                                         int train, int64_t *bytes) {
+  if (!bytes || !adp::fits(M, K, N, r, n) || !adp::float_type(dtype) || rows_per_index < 1) return fail(KSD_EINVAL, "adapter_linear_groups: bad arguments");
+  *bytes = train || adp::by_lists(M, K, N, r, n, rows_per_index, dtype) ? adp::groups(M, n).bytes : 0;
+  return KSD_OK;
+}
+
 extern "C" int ksd_adapter_linear(const void *x, int dtype, int64_t M, int64_t K, int64_t x_stride, const void *a, const void *b,
                                   int64_t n, int64_t r, int64_t N, const void *index, int index_wide, int64_t rows_per_index,
                                   const float *scales, const void *base, int64_t base_stride, int64_t drop, uint64_t seed,
-                                  const void *seed_from, int64_t stream_id, void *y, float *hidden, void *stream) {
-  if (!adp::fits(M, K, N, r, n) || rows_per_index < 1 || (M > 1 && (x_stride < K || (base && base_stride < N))))
+                                  const void *seed_from, int64_t stream_id, void *y, float *hidden, void *groups,
+                                  int64_t groups_bytes, void *stream) {
+  using namespace adp;
+  if (!fits(M, K, N, r, n) || rows_per_index < 1 || (M > 1 && (x_stride < K || (base && base_stride < N))))
     return fail(KSD_EINVAL, "adapter_linear: bad shape");
-  if (!adp::float_type(dtype)) return fail(KSD_ETYPE, "adapter_linear: unsupported element type");
+  if (!float_type(dtype)) return fail(KSD_ETYPE, "adapter_linear: unsupported element type");
   Mask m;
   if (!make_mask(m, drop, seed, seed_from, stream_id)) return fail(KSD_EINVAL, "adapter_linear: bad probability, seed or stream");
-  if (M == 0) return KSD_OK;
-  if (!x || !a || !b || !index || !y) return fail(KSD_EINVAL, "adapter_linear: null pointer");
-  adp::PairArgs p{x, x_stride, M, K, N, a, b, index, index_wide, rows_per_index, scales, base, base_stride, y, hidden,
-                  (int)n, (int)r, 0, 0, m, 1, 0};
-  return adp::run_pair(p, dtype, drop > 0, (hipStream_t)stream);
+  const bool lists = by_lists(M, K, N, r, n, rows_per_index, dtype);
+  const Groups l = adp::groups(M, n);
+  if ((groups || lists) && (!groups || groups_bytes < l.bytes || (uintptr_t)groups % 16))
+    return fail(KSD_EINVAL, "adapter_linear: short or misaligned groups");
+  if (M > 0 && (!x || !a || !b || !index || !y)) return fail(KSD_EINVAL, "adapter_linear: null pointer");
+  hipStream_t st = (hipStream_t)stream;
+  char *const w = (char *)groups;
+  if (w) group(index, index_wide, rows_per_index, M, n, w, st);
+  if (M == 0) return w ? check_launch("adapter_linear") : KSD_OK;
+  PairArgs p{x, x_stride, M, K, N, a, b, index, index_wide, rows_per_index, scales, base, base_stride, y, hidden,
+             (int)n, (int)r, 0, 0, m, 1, 0, nullptr, nullptr, 1};
+  if (lists) p.order = (const int32_t *)(w + l.order), p.slots = (const Slot *)(w + l.tiles);
+  return run_pair(p, dtype, drop > 0, st);
 }
 
 extern "C" int ksd_adapter_linear_backward_workspace(int64_t M, int64_t K, int64_t N, int64_t r, int64_t n, int dtype,
@@ -623,11 +859,12 @@ extern "C" int ksd_adapter_linear_backward_workspace(int64_t M, int64_t K, int64
 }
 
 extern "C" int ksd_adapter_linear_backward(const void *g, int dtype, int64_t M, int64_t N, int64_t g_stride, const void *x,
-                                           int64_t K, int64_t x_stride, const float *hidden, const void *a, const void *b,
-                                           int64_t n, int64_t r, const void *index, int index_wide, int64_t rows_per_index,
-                                           const float *scales, const void *base, int64_t base_stride, int64_t drop,
-                                           uint64_t seed, const void *seed_from, int64_t stream_id, void *dx, float *da,
-                                           float *db, void *workspace, int64_t workspace_bytes, void *stream) {
+                                           int64_t K, int64_t x_stride, const float *hidden, const void *groups,
+                                           int64_t groups_bytes, const void *a, const void *b, int64_t n, int64_t r,
+                                           const void *index, int index_wide, int64_t rows_per_index, const float *scales,
+                                           const void *base, int64_t base_stride, int64_t drop, uint64_t seed,
+                                           const void *seed_from, int64_t stream_id, void *dx, float *da, float *db,
+                                           void *workspace, int64_t workspace_bytes, void *stream) {
   using namespace adp;
   if (!fits(M, K, N, r, n) || rows_per_index < 1 ||
       (M > 1 && (x_stride < K || g_stride < N || (base && base_stride < K))))
@@ -636,42 +873,41 @@ extern "C" int ksd_adapter_linear_backward(const void *g, int dtype, int64_t M, 
   Mask m;
   if (!make_mask(m, drop, seed, seed_from, stream_id))
     return fail(KSD_EINVAL, "adapter_linear_backward: bad probability, seed or stream");
-  if (M > 0 && (!g || !x || !hidden || !a || !b || !index)) return fail(KSD_EINVAL, "adapter_linear_backward: null pointer");
+  if ((M > 0 && (!g || !x || !hidden || !a || !b || !index)) || !da != !db)
+    return fail(KSD_EINVAL, "adapter_linear_backward: null pointer");
   const Layout l = layout(M, K, N, r, n, dtype);
-  if (!workspace || workspace_bytes < l.bytes || (uintptr_t)workspace % 16)
-    return fail(KSD_EINVAL, "adapter_linear_backward: short or misaligned workspace");
-  const int64_t slots = M / kPiece + n, blocks_a = cdiv(K, 128), blocks_b = cdiv(N, 128), each = r * (K + N);
-  if (slots > 65535 || !grid_fits(blocks_a + blocks_b, 256) || !grid_fits(cdiv(each, 256), 256) ||
-      !grid_fits(n * cdiv(r, 32) * std::max(cdiv(K, 32), cdiv(N, 32)), 256))
+  const Groups gl = adp::groups(M, n);
+  if (!workspace || workspace_bytes < l.bytes || (uintptr_t)workspace % 16 || !groups || groups_bytes < gl.bytes ||
+      (uintptr_t)groups % 16)
+    return fail(KSD_EINVAL, "adapter_linear_backward: short or misaligned workspace or groups");
+  const int64_t slots = M / kPiece + n + 1, blocks_a = cdiv(K, 128), blocks_b = cdiv(N, 128), each = r * (K + N);
+  if (slots > 65535 || !grid_fits(blocks_a + blocks_b, 256) || !grid_fits(cdiv(each, 64), 256) ||
+      !grid_fits(n * cdiv(r, 32) * (cdiv(K, 32) + cdiv(N, 32)), 256))
     return fail(KSD_EINVAL, "adapter_linear_backward: too many tokens, columns or adapters");
   hipStream_t st = (hipStream_t)stream;
   char *const w = (char *)workspace;
-  // the narrow product contracts dY's columns, the wide one the ranks: both banks the other way round
-  if (dtype == KSD_F32) {
-    turn<uint32_t>(a, w + l.at, n, r, K, st);
-    turn<uint32_t>(b, w + l.bt, n, N, r, st);
-  } else {
-    turn<uint16_t>(a, w + l.at, n, r, K, st);
-    turn<uint16_t>(b, w + l.bt, n, N, r, st);
-  }
+  const char *const gw = (const char *)groups;
   float *const gh = (float *)(w + l.gh);
   if (M > 0) {
+    // the narrow product contracts dY's columns, the wide one the ranks: both banks the other way round
+    if (dtype == KSD_F32) turn_banks<uint32_t>(a, w + l.at, b, w + l.bt, n, r, K, N, st);
+    else turn_banks<uint16_t>(a, w + l.at, b, w + l.bt, n, r, K, N, st);
     PairArgs p{g, g_stride, M, N, K, w + l.bt, w + l.at, index, index_wide, rows_per_index, scales, base, base_stride, dx, gh,
-               (int)n, (int)r, 0, 0, m, 0, 1};
+               (int)n, (int)r, 0, 0, m, 0, 1, nullptr, nullptr, 1};
+    if (by_lists(M, K, N, r, n, rows_per_index, dtype)) p.order = (const int32_t *)(gw + gl.order), p.slots = (const Slot *)(gw + gl.tiles);
     const int rc = run_pair(p, dtype, drop > 0, st);
     if (rc) return rc;
   }
-  if (!da && !db) return KSD_OK;
-  GroupArgs ga{index, index_wide, (int)n, rows_per_index, M, (int32_t *)(w + l.order), (Slot *)(w + l.slots), (int2 *)(w + l.spans)};
-  group_kernel<<<(unsigned)n, 256, 0, st>>>(ga);
+  if (!da) return KSD_OK;
   float *const parts = (float *)(w + l.parts);
   if (M > 0) {
-    GradArgs q{x, g, x_stride, g_stride, K, N, gh, hidden, ga.order, ga.slots, parts, (int)r, (int)blocks_a, drop > 0, m};
+    GradArgs q{x, g, x_stride, g_stride, K, N, gh, hidden, (const int32_t *)(gw + gl.order), (const Slot *)(gw + gl.pieces), parts,
+               (int)r, (int)n, (int)blocks_a, drop > 0, m};
     const dim3 grid((unsigned)(blocks_a + blocks_b), (unsigned)slots, (unsigned)cdiv(r, 64));
-    if (dtype == KSD_F32) grad_kernel<KSD_F32><<<grid, 256, 0, st>>>(q);
-    else if (dtype == KSD_BF16) grad_kernel<KSD_BF16><<<grid, 256, 0, st>>>(q);
-    else grad_kernel<KSD_F16><<<grid, 256, 0, st>>>(q);
+    if (dtype == KSD_F32) launch_grad<KSD_F32>(q, grid, st);
+    else if (dtype == KSD_BF16) launch_grad<KSD_BF16>(q, grid, st);
+    else launch_grad<KSD_F16>(q, grid, st);
   }
-  join_kernel<<<dim3((unsigned)cdiv(each, 256), (unsigned)n), 256, 0, st>>>(parts, ga.spans, r * K, r * N, da, db);
+  join_kernel<<<dim3((unsigned)cdiv(each, 64), (unsigned)n), 256, 0, st>>>(parts, (const int2 *)(gw + gl.spans), r * K, r * N, da, db);
   return check_launch("adapter_linear_backward");
 }

@@ -14,6 +14,7 @@ CPU path.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -72,7 +73,7 @@ def _bank(x, a, b, index, scales, base):
             None if scales is None else scales.contiguous(), None if base is None else _rows(base, N))
 
 
-def _forward(x, a, b, index, scales, base, out, mask, hidden):
+def _forward(x, a, b, index, scales, base, out, mask, train):
     dev = _lib.require_gpu(x, a, b, index, scales, base, out)
     x2, a, b, index, per, scales, base2 = _bank(x, a, b, index, scales, base)
     (M, K), (n, N, r) = x2.shape, b.shape
@@ -87,14 +88,25 @@ def _forward(x, a, b, index, scales, base, out, mask, hidden):
                 raise ValueError(f"out shares memory with {name}")
         if base2 is not None and _shared(out, base2) and (base2.data_ptr() != out.data_ptr() or _pitch(base2) != N):
             raise ValueError("out shares memory with base and is not base itself")
-    h = torch.empty((M, r), dtype=torch.float32, device=dev) if hidden else None
-    if M:
+    h = torch.empty((M, r), dtype=torch.float32, device=dev) if train else None
+    groups, size = None, _groups_bytes(M, K, N, r, n, per, _lib.dtype_code(x.dtype), train)
+    if size:
+        groups = torch.empty(size, dtype=torch.int8, device=dev)
+    if M or train:
         _lib.call_on(dev, "ksd_adapter_linear", x2.data_ptr(), _lib.dtype_code(x.dtype), M, K, _pitch(x2), a.data_ptr(),
                      b.data_ptr(), n, r, N, index.data_ptr(), int(index.dtype == torch.int64), per, _lib.ptr(scales),
-                     _lib.ptr(base2), 0 if base2 is None else _pitch(base2), *mask, y.data_ptr(), _lib.ptr(h))
+                     _lib.ptr(base2), 0 if base2 is None else _pitch(base2), *mask, y.data_ptr(), _lib.ptr(h),
+                     _lib.ptr(groups), size)
     if out is not None:
         _lib.wrote((out,))
-    return y, (x2, a, b, index, per, scales, h)
+    return y, (x2, a, b, index, per, scales, h, groups)
+
+
+@functools.lru_cache(maxsize=4096)
+def _groups_bytes(M: int, K: int, N: int, r: int, n: int, per: int, dtype: int, train: bool) -> int:
+    need = ctypes.c_int64()
+    _lib.call("ksd_adapter_linear_groups", M, K, N, r, n, per, dtype, int(train), ctypes.byref(need))
+    return need.value
 
 
 _NO_MASK = (0, 0, None, 0)
@@ -112,9 +124,10 @@ def adapter_linear(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, index: tor
 
 
 class Saved:
-    """What adapter_linear_backward needs of a training forward: its inputs, and h (r floats a token)."""
+    """What adapter_linear_backward needs of a training forward: its inputs, h (r floats a token) and the tokens
+    listed by adapter."""
 
-    __slots__ = ("x", "a", "b", "index", "per", "scales", "hidden", "lead", "mask", "seed")
+    __slots__ = ("x", "a", "b", "index", "per", "scales", "hidden", "groups", "lead", "mask", "seed")
 
 
 def adapter_linear_train(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, index: torch.Tensor,
@@ -128,7 +141,7 @@ def adapter_linear_train(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, inde
     mask = mask_arguments(dropout, seed, stream, dev)
     s = Saved()
     s.mask, s.seed, s.lead = mask, seed, x.shape[:-1]
-    y, (s.x, s.a, s.b, s.index, s.per, s.scales, s.hidden) = _forward(x, a, b, index, scales, base, None, mask, True)
+    y, (s.x, s.a, s.b, s.index, s.per, s.scales, s.hidden, s.groups) = _forward(x, a, b, index, scales, base, None, mask, True)
     return y, s
 
 
@@ -156,7 +169,7 @@ def adapter_linear_backward(grad: torch.Tensor, saved: Saved, base: torch.Tensor
     _lib.call("ksd_adapter_linear_backward_workspace", M, K, N, r, n, dt, ctypes.byref(need))
     work = torch.empty(need.value, dtype=torch.int8, device=dev)
     _lib.call_on(dev, "ksd_adapter_linear_backward", g.data_ptr(), dt, M, N, _pitch(g), x.data_ptr(), K, _pitch(x),
-                 saved.hidden.data_ptr(), a.data_ptr(), b.data_ptr(), n, r, saved.index.data_ptr(),
+                 saved.hidden.data_ptr(), saved.groups.data_ptr(), saved.groups.numel(), a.data_ptr(), b.data_ptr(), n, r, saved.index.data_ptr(),
                  int(saved.index.dtype == torch.int64), saved.per, _lib.ptr(saved.scales), _lib.ptr(base),
                  0 if base is None else _pitch(base), *saved.mask, _lib.ptr(dx) if M else None, _lib.ptr(da), _lib.ptr(db),
                  work.data_ptr(), need.value)
@@ -170,18 +183,18 @@ class _AdapterFunction(torch.autograd.Function):
         y, s = adapter_linear_train(x, a, b, index, scales, base, p, seed, stream)
         # through save_for_backward, so that they are freed with the graph and writes into them are noticed
         device_seed = s.seed if isinstance(s.seed, torch.Tensor) else None
-        ctx.save_for_backward(x, a, b, s.index, s.scales, s.hidden, device_seed)
+        ctx.save_for_backward(x, a, b, s.index, s.scales, s.hidden, s.groups, device_seed)
         ctx.args = (s.per, s.lead, s.mask)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        x, a, b, index, scales, hidden, seed = ctx.saved_tensors
+        x, a, b, index, scales, hidden, groups, seed = ctx.saved_tensors
         s = Saved()
         s.per, s.lead, s.mask = ctx.args
         s.x, s.a, s.b = _rows(x, x.shape[-1]), a.contiguous(), b.contiguous()
-        s.index, s.scales, s.hidden, s.seed = index, scales, hidden, seed
+        s.index, s.scales, s.hidden, s.groups, s.seed = index, scales, hidden, groups, seed
         need = ctx.needs_input_grad
         dx = da = db = None
         if need[0] or need[1] or need[2]:

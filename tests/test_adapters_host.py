@@ -7,18 +7,21 @@ from ksdraft_amd import _lib
 P = ctypes.c_void_p(256)  # never dereferenced
 
 
-def forward(x=P, dtype=0, M=4, K=8, stride=8, a=P, n=2, r=4, N=16, index=P, per=1, base=P, base_stride=16, drop=0, stream_id=0, y=P):
+def forward(x=P, dtype=0, M=4, K=8, stride=8, a=P, n=2, r=4, N=16, index=P, per=1, base=P, base_stride=16, drop=0, stream_id=0, y=P, groups=None,
+            size=0):
     return _lib.load().ksd_adapter_linear(x, dtype, M, K, stride, a, P, n, r, N, index, 1, per, P, base, base_stride, drop, 1, None,
-                                          stream_id, y, None, None)
+                                          stream_id, y, None, groups, size, None)
 
 
-def backward(dtype=0, M=4, N=16, stride=16, K=8, hidden=P, n=2, r=4, per=1, drop=0, work=P, size=1 << 50):
-    return _lib.load().ksd_adapter_linear_backward(P, dtype, M, N, stride, P, K, 8, hidden, P, P, n, r, P, 1, per, P, None, 0, drop, 1,
-                                                   None, 0, P, P, P, work, size, None)
+def backward(dtype=0, M=4, N=16, stride=16, K=8, hidden=P, n=2, r=4, per=1, drop=0, work=P, size=1 << 50, da=P, groups=P,
+             groups_size=1 << 50):
+    return _lib.load().ksd_adapter_linear_backward(P, dtype, M, N, stride, P, K, 8, hidden, groups, groups_size, P, P, n, r, P, 1, per, P, None, 0, drop, 1,
+                                                   None, 0, P, da, P, work, size, None)
 
 
 def test_forward():
     assert forward(M=0) == 0
+    assert forward(M=600000) == 1 and forward(M=600000, groups=P, size=64) == 1 and forward(groups=ctypes.c_void_p(8), size=1 << 30) == 1
     for bad in (dict(M=-1), dict(K=0), dict(N=0), dict(r=0), dict(r=129), dict(n=0), dict(n=1 << 16), dict(per=0), dict(stride=7),
                 dict(base_stride=15), dict(drop=65537), dict(drop=-1), dict(stream_id=-1), dict(x=None), dict(a=None), dict(index=None),
                 dict(y=None), dict(M=1 << 31), dict(K=1 << 31), dict(N=1 << 31)):
@@ -28,7 +31,8 @@ def test_forward():
 
 def test_backward():
     for bad in (dict(M=-1), dict(K=0), dict(N=0), dict(r=129), dict(n=0), dict(per=0), dict(stride=15), dict(hidden=None),
-                dict(drop=70000), dict(work=None), dict(size=16), dict(work=ctypes.c_void_p(8)), dict(M=1 << 25)):
+                dict(drop=70000), dict(work=None), dict(size=16), dict(work=ctypes.c_void_p(8)), dict(M=1 << 25), dict(da=None),
+                dict(groups=None), dict(groups_size=64)):
         assert backward(**bad) == 1, bad
     assert backward(dtype=9) == 2
     need = ctypes.c_int64()
