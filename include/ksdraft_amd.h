@@ -854,7 +854,7 @@ int ksd_dropout(const void *x, int dtype, int64_t rows, int64_t d, int64_t strid
  *   tokens (B, L) int64; uniforms (B, L + 1) fp32, or fp64 where uniforms_wide (NULL if all are greedy)
  *   temperatures (B,) fp32, or NULL: `temperature` for all
  *   lengths (B,) int64, clamped to [0, L], or NULL (L)
- *   out (B, L + 1), accepted (B,) int64; workspace: ksd_verify_draft_workspace bytes
+ *   out (B, L + 1), accepted (B,) int64 (or NULL where L = 0); workspace: ksd_verify_draft_workspace bytes
  */
 int ksd_verify_draft_workspace(int64_t B, int64_t L, int64_t V, int draft, int64_t *bytes);
 int ksd_verify_draft(const void *target, const void *draft, int dtype, int64_t B, int64_t L, int64_t V,
@@ -871,26 +871,26 @@ int ksd_verify_draft(const void *target, const void *draft, int dtype, int64_t B
  *   x (M, K), base (M, N) or NULL: row strides in elements; y (M, N) dense, may be base itself where that is
  *   dense; a (n, r, K), b (n, N, r) dense; all of dtype; r <= 128, n <= 65535
  *   index int64 (index_wide) or int32; scales (n,) fp32 or NULL (1); hidden (M, r) fp32 or NULL: h
- *   groups: ksd_adapter_linear_groups bytes, 16-byte aligned, written by the call (the tokens listed by adapter);
- *   NULL where that is 0
- * The backward pass from g = dY and the forward's hidden and groups, g'[m] = scales[i] g[m] B_i:
+ *   workspace: ksd_adapter_linear_workspace bytes, 16-byte aligned (NULL where that is 0)
+ * The backward pass from g = dY and the forward's hidden and workspace, left as it was (tokens listed by adapter), g'[m] = scales[i] g[m] B_i:
  *   dx[m] = base[m] + mask(g'[m] A_i) (base (M, K): another branch's gradient, or NULL); NULL: not wanted
  *   da_i = sum of g'[m]^T x~[m] (n, r, K), db_i = sum of g[m]^T h[m] (n, N, r), fp32, sums in an order that
  *   index and sizes fix; both NULL: not wanted
  */
-int ksd_adapter_linear_groups(int64_t M, int64_t K, int64_t N, int64_t r, int64_t n, int64_t rows_per_index,
-                              int dtype, int train, int64_t *bytes);
+int ksd_adapter_linear_workspace(int64_t M, int64_t K, int64_t N, int64_t r, int64_t n, int64_t rows_per_index,
+                                 int dtype, int64_t *bytes);
 int ksd_adapter_linear(const void *x, int dtype, int64_t M, int64_t K, int64_t x_stride, const void *a,
                        const void *b, int64_t n, int64_t r, int64_t N, const void *index, int index_wide,
                        int64_t rows_per_index, const float *scales, const void *base, int64_t base_stride,
                        int64_t drop, uint64_t seed, const void *seed_from, int64_t stream_id, void *y,
-                       float *hidden, void *groups, int64_t groups_bytes, void *stream);
-int ksd_adapter_linear_backward_workspace(int64_t M, int64_t K, int64_t N, int64_t r, int64_t n, int dtype,
-                                          int64_t *bytes);
+                       float *hidden, void *workspace,
+                       int64_t workspace_bytes, void *stream);
+int ksd_adapter_linear_backward_workspace(int64_t M, int64_t K, int64_t N, int64_t r, int64_t n,
+                                          int64_t rows_per_index, int dtype, int64_t *bytes);
 int ksd_adapter_linear_backward(const void *g, int dtype, int64_t M, int64_t N, int64_t g_stride,
                                 const void *x, int64_t K, int64_t x_stride, const float *hidden,
-                                const void *groups, int64_t groups_bytes, const void *a, const void *b,
-                                int64_t n, int64_t r, const void *index,
+                                const void *forward_workspace, int64_t forward_bytes, const void *a,
+                                const void *b, int64_t n, int64_t r, const void *index,
                                 int index_wide, int64_t rows_per_index, const float *scales,
                                 const void *base, int64_t base_stride, int64_t drop, uint64_t seed,
                                 const void *seed_from, int64_t stream_id, void *dx, float *da, float *db,

@@ -107,10 +107,10 @@ SIGNATURES = {
     "ksd_grad_norm_workspace": [_P, _INT, _P],
     "ksd_grad_norm": [_P, _P, _P, _INT, _INT, _F, _F, _P, _P, _P, _I64, _P],
     "ksd_grad_scale": [_P, _P, _P, _P, _INT, _P, _P],
-    "ksd_adapter_linear_groups": [_I64, _I64, _I64, _I64, _I64, _I64, _INT, _INT, _P],
+    "ksd_adapter_linear_workspace": [_I64, _I64, _I64, _I64, _I64, _I64, _INT, _P],
     "ksd_adapter_linear": [_P, _INT, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _P, _INT, _I64, _P, _P, _I64, _I64, _U64, _P,
                            _I64, _P, _P, _P, _I64, _P],
-    "ksd_adapter_linear_backward_workspace": [_I64, _I64, _I64, _I64, _I64, _INT, _P],
+    "ksd_adapter_linear_backward_workspace": [_I64, _I64, _I64, _I64, _I64, _I64, _INT, _P],
     "ksd_adapter_linear_backward": [_P, _INT, _I64, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _P, _P, _I64, _I64, _P, _INT, _I64,
                                     _P, _P, _I64, _I64, _U64, _P, _I64, _P, _P, _P, _P, _I64, _P],
     "ksd_verify_draft_workspace": [_I64, _I64, _I64, _INT, _P],

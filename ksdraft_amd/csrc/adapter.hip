@@ -111,7 +111,7 @@ __device__ __forceinline__ f32x4 product(const typename Oct<DT>::V &a, const typ
 // Tokens are listed by adapter (stable; those without one last, as adapter n), each list in pieces. Piece j of adapter
 // i is slot start_i / piece + i + j: slots of different adapters never meet, and a slot knows its adapter without a sum
 // over the earlier ones' pieces.
-constexpr int kTile = 32, kPiece = 256;  // of the products by rows; of the gradients' sums
+constexpr int kTile = 32, kLeast = 64;  // of the products by rows; the smallest of the gradients' sums
 
 struct Slot {
   int adapter, from, to, pad;  // -1: empty
@@ -136,6 +136,9 @@ struct PairArgs {
   const int32_t *order;    // tokens listed by adapter, and the pieces of the lists (NULL: rows as they lie)
   const Slot *slots;
   int tiles;               // workgroups of a piece
+  int splits;              // > 0: the narrow product's columns in so many parts, in a launch of its own
+  int phase;               // 0: both products; 1: the narrow one's part blockIdx.y into sums; 2: the wide one from sums
+  float *sums;             // (splits, M, r)
 };
 
 __device__ __forceinline__ int adapter_of(const void *index, int wide, int64_t per, int64_t m, int n) {
@@ -260,42 +263,60 @@ __global__ __launch_bounds__(64 * kWaves) void pair_kernel(const PairArgs p) {
   const int64_t n0 = (int64_t)blockIdx.y * p.cols, n1 = min(p.N, n0 + p.cols);
   // base of a block of 64 columns: 16 of them per lane
   const auto load_base = [&](int64_t c, V (&v)[RT][2]) {
-    const int64_t at = c + grp * 16;
     const bool whole = c + 64 <= p.N;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       const T *const row = (const T *)p.base + at_row[t] * p.base_stride;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) v[t][e] = whole ? whole_oct<DT>(row, at + e * 8) : load_oct<DT>(row, at + e * 8, p.N);
+      for (int e = 0; e < 2; ++e) {
+        const int64_t at = c + e * 32 + grp * 8;
+        v[t][e] = whole ? whole_oct<DT>(row, at) : load_oct<DT>(row, at, p.N);
+      }
     }
   };
   V bv[RT][2] = {};
   int64_t c = n0 + wave * 64;
-  const bool based = p.base && p.y;
+  const bool wide = p.y && p.phase != 1, based = p.base && wide;
   if (based && c < n1) load_base(c, bv);
-  // An adapter's bank rows for tiles t0 .. of a block: row i of product t is column (i / 4) 16 + 4 t + i % 4 of the block,
-  // so a lane ends with 16 consecutive columns of its token.
+  // An adapter's bank rows for tiles t0 .. of a block. Which of its columns row i of product t is: such that a lane ends
+  // with two runs of 8 columns of its token, and four lanes' runs lie side by side.
   const auto load_bank = [&](int64_t c, int i, int t0, V (&w)[TB][R16]) {
     const T *const b = (const T *)p.b + (int64_t)i * p.N * p.r;
     const bool whole = c + 64 <= p.N;
 #pragma unroll
     for (int t = 0; t < TB; ++t) {
-      const int64_t n = c + (col >> 2) * 16 + (t0 + t) * 4 + (col & 3);
+      const int64_t n = c + (t0 + t) / 2 * 32 + (col >> 2) * 8 + (t0 + t) % 2 * 4 + (col & 3);
 #pragma unroll
       for (int q = 0; q < R16; ++q) w[t][q] = bank_oct<DT, ALIGNED>(b + (whole ? n : min(n, p.N - 1)) * p.r, q, grp, p.r);
     }
   };
   const auto lowest = [&](uint64_t rows) { return __shfl(mine, __builtin_ctzll(rows)); };
   V w[TB][R16] = {};
-  if (kAhead && with && p.y && c < n1) load_bank(c, lowest(with), 0, w);
+  if (kAhead && with && wide && c < n1) load_bank(c, lowest(with), 0, w);
 
-  if (with) {
+  if (with && p.phase == 2) {
+    __shared__ int tokens[16 * RT];
+    if (wave == 0 && lane < 16 * RT) tokens[lane] = token;
+    __syncthreads();
+    for (int e = threadIdx.x; e < 16 * RT * R; e += 64 * kWaves) {
+      const int t = e / R, q = e % R;
+      float v = 0.0f;
+      if (t < rows && (with >> t & 1) && q < p.r) {
+        const float *const from = p.sums + (int64_t)tokens[t] * p.r + q;
+        for (int k = 0; k < p.splits; ++k) v += from[k * p.M * p.r];
+      }
+      lds[t * pitch + q] = v;
+    }
+    __syncthreads();
+  } else if (with) {
     // ---- h: D[rank][token] = A x^T over this wave's columns
     const T *xr[RT];
 #pragma unroll
     for (int t = 0; t < RT; ++t) xr[t] = (const T *)p.x + at_row[t] * p.x_stride;
-    const int64_t steps = (p.K + 31) / 32, full = p.K / 32, share = ((steps + kWaves - 1) / kWaves + 1) & ~1ll;
-    const int64_t from = wave * share, to = min(steps, from + share), upto = min(to, full);
+    const int64_t steps = (p.K + 31) / 32, full = p.K / 32;
+    const int waves = p.phase ? kWaves * p.splits : kWaves, mark = p.phase ? blockIdx.y * kWaves + wave : wave;
+    const int64_t share = ((steps + waves - 1) / waves + 1) & ~1ll;
+    const int64_t from = mark * share, to = min(steps, from + share), upto = min(to, full);
     for (uint64_t left = with; left;) {
       const int i = __shfl(mine, __builtin_ctzll(left));
       left &= ~__ballot(mine == i);
@@ -332,13 +353,21 @@ __global__ __launch_bounds__(64 * kWaves) void pair_kernel(const PairArgs p) {
     }
     __syncthreads();
   }
+  if (p.phase == 1) {
+    for (int t = wave; t < rows; t += kWaves) {
+      float *const to = p.sums + ((int64_t)blockIdx.y * p.M + __shfl(token, t)) * p.r;
+      if (with >> t & 1)
+        for (int q = lane; q < p.r; q += 64) to[q] = lds[t * pitch + q];
+    }
+    return;
+  }
   if (p.hidden && blockIdx.y == 0) {
     for (int t = wave; t < rows; t += kWaves) {
       const int64_t m = __shfl(token, t);
       for (int q = lane; q < p.r; q += 64) p.hidden[m * p.r + q] = with >> t & 1 ? lds[t * pitch + q] : 0.0f;
     }
   }
-  if (!p.y) return;
+  if (!wide) return;
 
   // ---- y: D[column][token] = B h^T
   V hv[RT][R16];
@@ -386,7 +415,6 @@ __global__ __launch_bounds__(64 * kWaves) void pair_kernel(const PairArgs p) {
     }
   }
   for (; c < n1; c += 64 * kWaves) {
-    const int64_t at = c + grp * 16;
     const bool whole = c + 64 <= p.N;
     V next[RT][2] = {};
     if (based && c + 64 * kWaves < n1) load_base(c + 64 * kWaves, next);
@@ -436,11 +464,12 @@ __global__ __launch_bounds__(64 * kWaves) void pair_kernel(const PairArgs p) {
       T *const out = (T *)p.y + m * p.N;
 #pragma unroll
       for (int v = 0; v < 2; ++v) {
+        const int64_t at = c + v * 32 + grp * 8;
         float f[8], g[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[j] = acc[u][v * 2 + j / 4][j & 3];
         if constexpr (MASK) {
-          if (p.mask_y) apply_mask(p.mask, mask_bits(p.mask, key, m, (uint32_t)((at >> 3) + v)), f);
+          if (p.mask_y) apply_mask(p.mask, mask_bits(p.mask, key, m, (uint32_t)(at >> 3)), f);
         }
         if (based) {
           to_floats<DT>(bv[u][v], g);
@@ -450,9 +479,9 @@ __global__ __launch_bounds__(64 * kWaves) void pair_kernel(const PairArgs p) {
         if (u * 16 + col < rows) {
           if (whole) {
             struct __attribute__((packed, aligned(sizeof(T)))) Any { V v; };
-            ((Any *)(out + at + v * 8))->v = from_floats<DT>(f);
+            ((Any *)(out + at))->v = from_floats<DT>(f);
           } else {
-            store_oct<DT>(out, at + v * 8, p.N, f);
+            store_oct<DT>(out, at, p.N, f);
           }
         }
       }
@@ -464,7 +493,7 @@ __global__ __launch_bounds__(64 * kWaves) void pair_kernel(const PairArgs p) {
 
 template <int DT, int R16, int RT, bool MASK, bool ALIGNED>
 static void launch_pair(const PairArgs &p, unsigned tiles, hipStream_t st) {
-  const dim3 g(tiles, (unsigned)cdiv(p.N, p.cols));
+  const dim3 g(tiles, (unsigned)(p.phase == 1 ? p.splits : cdiv(p.N, p.cols)));
   constexpr int lds = kWaves * 16 * RT * (16 * R16 + 4) * 4;
   if constexpr (lds > 65536) {  // past HIP's default
     static const hipError_t set = hipFuncSetAttribute((const void *)pair_kernel<DT, R16, RT, MASK, ALIGNED>,
@@ -500,13 +529,16 @@ static void launch_pair(const PairArgs &p, bool mask, unsigned tiles, hipStream_
 // workgroups are left (8192 tokens: 18.6 us, with 16 rows 19.2; rank 64: 33 and 45). Columns are shared out where
 // fewer workgroups than CUs would run, each part forming h again: not where that is the longer product (2047 tokens,
 // 6869 to 1792: 43 us, in two parts 69; 1792 to 6869: 54 us, in 4 parts 47).
-static void shape(PairArgs &p, bool aligned) {
-  if (!p.slots && p.n > 1 && p.per < 16) p.rows = (int)std::min<int64_t>(16, cdiv(p.M, 1024));
+static void shape(PairArgs &p, bool lists, bool aligned) {
+  if (!lists && p.n > 1 && p.per < 16) p.rows = (int)std::max<int64_t>(1, std::min<int64_t>(16, cdiv(p.M, 1024)));
   else p.rows = p.M <= 64 ? 1 : p.M <= 256 ? 4 : p.M <= 512 ? 8 : p.M >= 8192 && p.r <= 64 && aligned ? 32 : 16;
-  if (p.slots)
+  if (lists)
     while (kTile % p.rows) --p.rows;
-  const int64_t tiles = cdiv(p.M, p.rows), blocks = cdiv(p.N, 64);
-  const int64_t parts = std::min({blocks / 6, cdiv(blocks < 64 ? 256 : 512, tiles), 4 * p.N / p.K});
+  const int64_t tiles = std::max<int64_t>(1, cdiv(p.M, p.rows)), blocks = cdiv(p.N, 64);
+  // a long narrow product of few rows goes to several workgroups first (2047 tokens, 6869 to 1792: 44 us, so 34; one
+  // token 24 and 13), whose sums the wide product's add
+  p.splits = p.K >= 4096 && tiles < 256 ? 4 : 0;
+  const int64_t parts = std::min({blocks / 6, cdiv(blocks < 64 ? 256 : 512, tiles), p.splits ? blocks : 4 * p.N / p.K});
   p.cols = (int)(cdiv(blocks, std::max<int64_t>(1, parts)) * 64);
 }
 
@@ -516,15 +548,16 @@ struct GroupArgs {
   int wide, n;
   int64_t per, M;
   int32_t *order;        // (M,)
-  Slot *tiles, *pieces;  // (M / kTile + n + 1,), (M / kPiece + n + 1,)
+  Slot *tiles, *pieces;  // (M / kTile + n + 1,), (M / piece + n + 1,)
   int2 *spans;           // (n + 1,): an adapter's first of `pieces`, and how many
+  int piece;             // tokens of one of `pieces`
 };
 
 // Workgroup i lists adapter i's tokens, workgroup n those without one: 8192 tokens at a time, whose indices are
 // loaded together.
-__global__ __launch_bounds__(1024) void group_kernel(const GroupArgs a) {
+__device__ __forceinline__ void list_tokens(const GroupArgs &a, int i) {
   constexpr int U = 8;
-  const int i = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   __shared__ int sums[2][16], counts[2][U][16];
   int v[U];
   const auto load = [&](int64_t base) {
@@ -561,7 +594,7 @@ __global__ __launch_bounds__(1024) void group_kernel(const GroupArgs a) {
     return make_int2(slot, pieces);
   };
   cut(a.tiles, kTile);
-  const int2 span = cut(a.pieces, kPiece);
+  const int2 span = cut(a.pieces, a.piece);
   if (tid == 0) a.spans[i] = span;
   int done = start, turn = 0;
   for (int64_t base = 0; base < a.M && done < start + len; base += U * 1024, turn ^= 1) {
@@ -587,30 +620,30 @@ __global__ __launch_bounds__(1024) void group_kernel(const GroupArgs a) {
   }
 }
 
+__global__ __launch_bounds__(1024) void group_kernel(const GroupArgs a) { list_tokens(a, blockIdx.x); }
+
 // ------------------------------------------------------------------------------- the adapters' gradients
-// out[i][c][r] = in[i][r][c] of 16- or 32-bit values, tiles of 32 x 32; two banks in one launch.
+// out[i][c][r] = in[i][r][c] of 16- or 32-bit values, tiles of 32 x 32.
 template <typename T>
 __device__ __forceinline__ void turn(const T *__restrict__ in, T *__restrict__ out, int64_t rows, int64_t cols, unsigned block) {
   __shared__ T tile[32][33];
   const unsigned tr = (unsigned)((rows + 31) / 32), tc = (unsigned)((cols + 31) / 32);
   const unsigned t = block % (tr * tc);
   const int64_t i = block / (tr * tc), r0 = t / tc * 32, c0 = t % tc * 32;
+  const int y = threadIdx.x >> 5, x = threadIdx.x & 31;
   in += i * rows * cols, out += i * rows * cols;
-  for (int e = threadIdx.x; e < 1024; e += 256) {
-    const int64_t r = r0 + e / 32, c = c0 + e % 32;
-    if (r < rows && c < cols) tile[e / 32][e % 32] = in[r * cols + c];
-  }
+  if (r0 + y < rows && c0 + x < cols) tile[y][x] = in[(r0 + y) * cols + c0 + x];
   __syncthreads();
-  for (int e = threadIdx.x; e < 1024; e += 256) {
-    const int64_t c = c0 + e / 32, r = r0 + e % 32;
-    if (r < rows && c < cols) out[c * rows + r] = tile[e % 32][e / 32];
-  }
+  if (r0 + x < rows && c0 + y < cols) out[(c0 + y) * rows + r0 + x] = tile[x][y];
 }
+// What the backward pass starts with: both banks the other way round, and the lists where the forward made none.
 template <typename T>
-__global__ __launch_bounds__(256) void turn_kernel(const T *__restrict__ a, T *__restrict__ at, const T *__restrict__ b,
-                                                   T *__restrict__ bt, int64_t r, int64_t K, int64_t N, unsigned a_blocks) {
-  if (blockIdx.x < a_blocks) turn<T>(a, at, r, K, blockIdx.x);
-  else turn<T>(b, bt, N, r, blockIdx.x - a_blocks);
+__global__ __launch_bounds__(1024) void prepare_kernel(const T *__restrict__ a, T *__restrict__ at, const T *__restrict__ b,
+                                                       T *__restrict__ bt, int64_t r, int64_t K, int64_t N, unsigned a_blocks,
+                                                       unsigned lists, const GroupArgs g) {
+  if (blockIdx.x < lists) list_tokens(g, blockIdx.x);
+  else if (blockIdx.x - lists < a_blocks) turn<T>(a, at, r, K, blockIdx.x - lists);
+  else turn<T>(b, bt, N, r, blockIdx.x - lists - a_blocks);
 }
 
 struct GradArgs {
@@ -738,6 +771,13 @@ struct Take {
     return v;
   }
 };
+// Tokens of a piece of the gradients' sums: such that the columns and pieces give the device enough workgroups (train
+// calls, 8192 tokens of 1536 to 1536: 256 tokens 123 us, 128 tokens 128, 512 tokens 134; 2047 of 1792 to 6869: 119, 113, 134).
+static int piece_of(int64_t M, int64_t K, int64_t N) {
+  int piece = 256;
+  while (piece > kLeast && cdiv(M, piece) * (cdiv(K, 128) + cdiv(N, 128)) < 768) piece /= 2;
+  return piece;
+}
 struct Groups {
   int64_t order, tiles, pieces, spans, bytes;
 };
@@ -746,21 +786,46 @@ static Groups groups(int64_t M, int64_t n) {
   Groups l;
   l.order = take(M * 4);
   l.tiles = take((M / kTile + n + 1) * (int64_t)sizeof(Slot));
-  l.pieces = take((M / kPiece + n + 1) * (int64_t)sizeof(Slot));
+  l.pieces = take((M / kLeast + n + 1) * (int64_t)sizeof(Slot));
   l.spans = take((n + 1) * 8);
   l.bytes = take.at;
   return l;
 }
-struct Layout {
-  int64_t at, bt, gh, parts, bytes;
+// Whether the products go by the lists: tokens in any order whose adapters, read for each token by itself, would be
+// more than 32 MB (the list's launch costs as much as that, about 5 us).
+static bool by_lists(int64_t M, int64_t K, int64_t N, int64_t r, int64_t n, int64_t per, int dtype) {
+  return n > 1 && per < 16 && M > 64 && M * r * (K + N) * size_of(dtype) > (32 << 20);
+}
+static bool aligned_rank(int64_t r, int dtype) { return r % (dtype == KSD_F32 ? 4 : 8) == 0; }
+
+// The workspace of a forward pass: lists, then the narrow product's parts.
+struct Forward {
+  bool lists;
+  int64_t sums, bytes;
 };
-static Layout layout(int64_t M, int64_t K, int64_t N, int64_t r, int64_t n, int dtype) {
+static Forward forward(int64_t M, int64_t K, int64_t N, int64_t r, int64_t n, int64_t per, int dtype) {
+  Forward l;
+  l.lists = by_lists(M, K, N, r, n, per, dtype);
+  PairArgs p{};
+  p.M = M, p.K = K, p.N = N, p.r = (int)r, p.n = (int)n, p.per = per;
+  shape(p, l.lists, aligned_rank(r, dtype));
+  l.sums = l.lists ? groups(M, n).bytes : 0;
+  l.bytes = l.sums + p.splits * M * r * 4;
+  return l;
+}
+struct Layout {
+  int64_t at, bt, gh, parts, groups, sums, bytes;
+};
+static Layout layout(int64_t M, int64_t K, int64_t N, int64_t r, int64_t n, int64_t per, int dtype) {
   Take take;
   Layout l;
   l.at = take(n * r * K * size_of(dtype));
   l.bt = take(n * r * N * size_of(dtype));
   l.gh = take(M * r * 4);
-  l.parts = take((M / kPiece + n + 1) * r * (K + N) * 4);
+  l.parts = take((M / piece_of(M, K, N) + n + 1) * r * (K + N) * 4);
+  const Forward f = forward(M, N, K, r, n, per, dtype);
+  l.groups = take(groups(M, n).bytes);
+  l.sums = take(f.bytes - f.sums);
   l.bytes = take.at;
   return l;
 }
@@ -773,7 +838,7 @@ static bool fits(int64_t M, int64_t K, int64_t N, int64_t r, int64_t n) {
 
 static int run_pair(const PairArgs &args, int dtype, bool mask, hipStream_t st) {
   PairArgs p = args;
-  shape(p, p.r % (dtype == KSD_F32 ? 4 : 8) == 0);
+  shape(p, p.slots != nullptr, aligned_rank(p.r, dtype));
   int64_t tiles = cdiv(p.M, p.rows);
   if (p.slots) {
     p.tiles = kTile / p.rows;
@@ -781,22 +846,18 @@ static int run_pair(const PairArgs &args, int dtype, bool mask, hipStream_t st) 
   }
   if (!grid_fits(tiles, 64 * kWaves) || cdiv(p.N, p.cols) > 65535)
     return fail(KSD_EINVAL, "adapter_linear: too many rows or columns");
-  if (dtype == KSD_F32) launch_pair<KSD_F32>(p, mask, (unsigned)tiles, st);
-  else if (dtype == KSD_BF16) launch_pair<KSD_BF16>(p, mask, (unsigned)tiles, st);
-  else launch_pair<KSD_F16>(p, mask, (unsigned)tiles, st);
+  for (p.phase = p.splits ? 1 : 0; p.phase < 3; p.phase += p.splits ? 1 : 3) {
+    if (dtype == KSD_F32) launch_pair<KSD_F32>(p, mask, (unsigned)tiles, st);
+    else if (dtype == KSD_BF16) launch_pair<KSD_BF16>(p, mask, (unsigned)tiles, st);
+    else launch_pair<KSD_F16>(p, mask, (unsigned)tiles, st);
+  }
   return check_launch("adapter_linear");
 }
 
-// Whether the products go by the lists: tokens in any order whose adapters, read for each token by itself, would be
-// more than 32 MB (the list's launch costs as much as that, about 5 us).
-static bool by_lists(int64_t M, int64_t K, int64_t N, int64_t r, int64_t n, int64_t per, int dtype) {
-  return n > 1 && per < 16 && M > 64 && M * r * (K + N) * size_of(dtype) > (32 << 20);
-}
-
-static void group(const void *index, int wide, int64_t per, int64_t M, int64_t n, char *w, hipStream_t st) {
+static GroupArgs group_args(const void *index, int wide, int64_t per, int64_t M, int64_t K, int64_t N, int64_t n, char *w) {
   const Groups l = groups(M, n);
-  group_kernel<<<(unsigned)(n + 1), 1024, 0, st>>>(GroupArgs{index, wide, (int)n, per, M, (int32_t *)(w + l.order),
-                                                            (Slot *)(w + l.tiles), (Slot *)(w + l.pieces), (int2 *)(w + l.spans)});
+  return GroupArgs{index, wide, (int)n, per, M, (int32_t *)(w + l.order), (Slot *)(w + l.tiles), (Slot *)(w + l.pieces),
+                   (int2 *)(w + l.spans), piece_of(M, K, N)};
 }
 
 template <int DT>
@@ -806,10 +867,11 @@ static void launch_grad(const GradArgs &q, dim3 grid, hipStream_t st) {
   else grad_kernel<DT, 4><<<grid, 256, 0, st>>>(q);
 }
 template <typename T>
-static void turn_banks(const void *a, void *at, const void *b, void *bt, int64_t n, int64_t r, int64_t K, int64_t N, hipStream_t st) {
-  const unsigned blocks = (unsigned)(n * cdiv(r, 32) * cdiv(K, 32));
-  turn_kernel<T><<<blocks + (unsigned)(n * cdiv(r, 32) * cdiv(N, 32)), 256, 0, st>>>((const T *)a, (T *)at, (const T *)b, (T *)bt,
-                                                                                      r, K, N, blocks);
+static void launch_prepare(const void *a, void *at, const void *b, void *bt, int64_t n, int64_t r, int64_t K, int64_t N, bool lists,
+                           const GroupArgs &g, hipStream_t st) {
+  const unsigned blocks = (unsigned)(n * cdiv(r, 32) * cdiv(K, 32)), lists_n = lists ? (unsigned)n + 1 : 0;
+  prepare_kernel<T><<<lists_n + blocks + (unsigned)(n * cdiv(r, 32) * cdiv(N, 32)), 1024, 0, st>>>(
+      (const T *)a, (T *)at, (const T *)b, (T *)bt, r, K, N, blocks, lists_n, g);
 }
 
 }  // namespace adp
@@ -817,50 +879,53 @@ static void turn_banks(const void *a, void *at, const void *b, void *bt, int64_t
 
 using namespace ksd;
 
-extern "C" int ksd_adapter_linear_groups(int64_t M, int64_t K, int64_t N, int64_t r, int64_t n, int64_t rows_per_index, int dtype,
-                                         int train, int64_t *bytes) {
-  if (!bytes || !adp::fits(M, K, N, r, n) || !adp::float_type(dtype) || rows_per_index < 1) return fail(KSD_EINVAL, "adapter_linear_groups: bad arguments");
-  *bytes = train || adp::by_lists(M, K, N, r, n, rows_per_index, dtype) ? adp::groups(M, n).bytes : 0;
+extern "C" int ksd_adapter_linear_workspace(int64_t M, int64_t K, int64_t N, int64_t r, int64_t n, int64_t rows_per_index, int dtype,
+                                            int64_t *bytes) {
+  if (!bytes || !adp::fits(M, K, N, r, n) || !adp::float_type(dtype) || rows_per_index < 1)
+    return fail(KSD_EINVAL, "adapter_linear_workspace: bad arguments");
+  *bytes = adp::forward(M, K, N, r, n, rows_per_index, dtype).bytes;
   return KSD_OK;
 }
 
 extern "C" int ksd_adapter_linear(const void *x, int dtype, int64_t M, int64_t K, int64_t x_stride, const void *a, const void *b,
                                   int64_t n, int64_t r, int64_t N, const void *index, int index_wide, int64_t rows_per_index,
                                   const float *scales, const void *base, int64_t base_stride, int64_t drop, uint64_t seed,
-                                  const void *seed_from, int64_t stream_id, void *y, float *hidden, void *groups,
-                                  int64_t groups_bytes, void *stream) {
+                                  const void *seed_from, int64_t stream_id, void *y, float *hidden, void *workspace,
+                                  int64_t workspace_bytes, void *stream) {
   using namespace adp;
   if (!fits(M, K, N, r, n) || rows_per_index < 1 || (M > 1 && (x_stride < K || (base && base_stride < N))))
     return fail(KSD_EINVAL, "adapter_linear: bad shape");
   if (!float_type(dtype)) return fail(KSD_ETYPE, "adapter_linear: unsupported element type");
   Mask m;
   if (!make_mask(m, drop, seed, seed_from, stream_id)) return fail(KSD_EINVAL, "adapter_linear: bad probability, seed or stream");
-  const bool lists = by_lists(M, K, N, r, n, rows_per_index, dtype);
-  const Groups l = adp::groups(M, n);
-  if ((groups || lists) && (!groups || groups_bytes < l.bytes || (uintptr_t)groups % 16))
-    return fail(KSD_EINVAL, "adapter_linear: short or misaligned groups");
-  if (M > 0 && (!x || !a || !b || !index || !y)) return fail(KSD_EINVAL, "adapter_linear: null pointer");
+  if (M == 0) return KSD_OK;
+  const Forward l = forward(M, K, N, r, n, rows_per_index, dtype);
+  if (l.bytes && (!workspace || workspace_bytes < l.bytes || (uintptr_t)workspace % 16))
+    return fail(KSD_EINVAL, "adapter_linear: short or misaligned workspace");
+  if (!x || !a || !b || !index || !y) return fail(KSD_EINVAL, "adapter_linear: null pointer");
   hipStream_t st = (hipStream_t)stream;
-  char *const w = (char *)groups;
-  if (w) group(index, index_wide, rows_per_index, M, n, w, st);
-  if (M == 0) return w ? check_launch("adapter_linear") : KSD_OK;
+  char *const w = (char *)workspace;
   PairArgs p{x, x_stride, M, K, N, a, b, index, index_wide, rows_per_index, scales, base, base_stride, y, hidden,
-             (int)n, (int)r, 0, 0, m, 1, 0, nullptr, nullptr, 1};
-  if (lists) p.order = (const int32_t *)(w + l.order), p.slots = (const Slot *)(w + l.tiles);
+             (int)n, (int)r, 0, 0, m, 1, 0, nullptr, nullptr, 1, 0, 0, (float *)(w + l.sums)};
+  if (l.lists) {
+    const GroupArgs g = group_args(index, index_wide, rows_per_index, M, K, N, n, w);
+    group_kernel<<<(unsigned)(n + 1), 1024, 0, st>>>(g);
+    p.order = g.order, p.slots = g.tiles;
+  }
   return run_pair(p, dtype, drop > 0, st);
 }
 
-extern "C" int ksd_adapter_linear_backward_workspace(int64_t M, int64_t K, int64_t N, int64_t r, int64_t n, int dtype,
-                                                     int64_t *bytes) {
-  if (!bytes || !adp::fits(M, K, N, r, n) || !adp::float_type(dtype))
+extern "C" int ksd_adapter_linear_backward_workspace(int64_t M, int64_t K, int64_t N, int64_t r, int64_t n, int64_t rows_per_index,
+                                                     int dtype, int64_t *bytes) {
+  if (!bytes || !adp::fits(M, K, N, r, n) || !adp::float_type(dtype) || rows_per_index < 1)
     return fail(KSD_EINVAL, "adapter_linear_backward_workspace: bad arguments");
-  *bytes = adp::layout(M, K, N, r, n, dtype).bytes;
+  *bytes = adp::layout(M, K, N, r, n, rows_per_index, dtype).bytes;
   return KSD_OK;
 }
 
 extern "C" int ksd_adapter_linear_backward(const void *g, int dtype, int64_t M, int64_t N, int64_t g_stride, const void *x,
-                                           int64_t K, int64_t x_stride, const float *hidden, const void *groups,
-                                           int64_t groups_bytes, const void *a, const void *b, int64_t n, int64_t r,
+                                           int64_t K, int64_t x_stride, const float *hidden, const void *forward_workspace,
+                                           int64_t forward_bytes, const void *a, const void *b, int64_t n, int64_t r,
                                            const void *index, int index_wide, int64_t rows_per_index, const float *scales,
                                            const void *base, int64_t base_stride, int64_t drop, uint64_t seed,
                                            const void *seed_from, int64_t stream_id, void *dx, float *da, float *db,
@@ -875,39 +940,41 @@ extern "C" int ksd_adapter_linear_backward(const void *g, int dtype, int64_t M, 
     return fail(KSD_EINVAL, "adapter_linear_backward: bad probability, seed or stream");
   if ((M > 0 && (!g || !x || !hidden || !a || !b || !index)) || !da != !db)
     return fail(KSD_EINVAL, "adapter_linear_backward: null pointer");
-  const Layout l = layout(M, K, N, r, n, dtype);
-  const Groups gl = adp::groups(M, n);
-  if (!workspace || workspace_bytes < l.bytes || (uintptr_t)workspace % 16 || !groups || groups_bytes < gl.bytes ||
-      (uintptr_t)groups % 16)
-    return fail(KSD_EINVAL, "adapter_linear_backward: short or misaligned workspace or groups");
-  const int64_t slots = M / kPiece + n + 1, blocks_a = cdiv(K, 128), blocks_b = cdiv(N, 128), each = r * (K + N);
+  const Layout l = layout(M, K, N, r, n, rows_per_index, dtype);
+  const Forward f = forward(M, K, N, r, n, rows_per_index, dtype);
+  if (!workspace || workspace_bytes < l.bytes || (uintptr_t)workspace % 16 ||
+      (M > 0 && f.lists && (!forward_workspace || forward_bytes < f.sums || (uintptr_t)forward_workspace % 16)))
+    return fail(KSD_EINVAL, "adapter_linear_backward: short or misaligned workspace");
+  const int64_t slots = M / piece_of(M, K, N) + n + 1, blocks_a = cdiv(K, 128), blocks_b = cdiv(N, 128), each = r * (K + N);
   if (slots > 65535 || !grid_fits(blocks_a + blocks_b, 256) || !grid_fits(cdiv(each, 64), 256) ||
-      !grid_fits(n * cdiv(r, 32) * (cdiv(K, 32) + cdiv(N, 32)), 256))
+      !grid_fits(n * cdiv(r, 32) * (cdiv(K, 32) + cdiv(N, 32)) + n + 1, 1024))
     return fail(KSD_EINVAL, "adapter_linear_backward: too many tokens, columns or adapters");
   hipStream_t st = (hipStream_t)stream;
   char *const w = (char *)workspace;
-  const char *const gw = (const char *)groups;
+  if (M == 0) {  // no slot has a token: zeros
+    if (!da) return KSD_OK;
+    group_kernel<<<(unsigned)(n + 1), 1024, 0, st>>>(group_args(index, index_wide, rows_per_index, M, K, N, n, w + l.groups));
+    join_kernel<<<dim3((unsigned)cdiv(each, 64), (unsigned)n), 256, 0, st>>>(
+        nullptr, (const int2 *)(w + l.groups + groups(M, n).spans), r * K, r * N, da, db);
+    return check_launch("adapter_linear_backward");
+  }
+  const bool lists = f.lists;
+  const GroupArgs ga = group_args(index, index_wide, rows_per_index, M, K, N, n, lists ? (char *)forward_workspace : w + l.groups);
   float *const gh = (float *)(w + l.gh);
-  if (M > 0) {
-    // the narrow product contracts dY's columns, the wide one the ranks: both banks the other way round
-    if (dtype == KSD_F32) turn_banks<uint32_t>(a, w + l.at, b, w + l.bt, n, r, K, N, st);
-    else turn_banks<uint16_t>(a, w + l.at, b, w + l.bt, n, r, K, N, st);
-    PairArgs p{g, g_stride, M, N, K, w + l.bt, w + l.at, index, index_wide, rows_per_index, scales, base, base_stride, dx, gh,
-               (int)n, (int)r, 0, 0, m, 0, 1, nullptr, nullptr, 1};
-    if (by_lists(M, K, N, r, n, rows_per_index, dtype)) p.order = (const int32_t *)(gw + gl.order), p.slots = (const Slot *)(gw + gl.tiles);
-    const int rc = run_pair(p, dtype, drop > 0, st);
-    if (rc) return rc;
-  }
-  if (!da) return KSD_OK;
+  // the narrow product contracts dY's columns, the wide one the ranks: both banks the other way round
+  if (dtype == KSD_F32) launch_prepare<uint32_t>(a, w + l.at, b, w + l.bt, n, r, K, N, !lists && da, ga, st);
+  else launch_prepare<uint16_t>(a, w + l.at, b, w + l.bt, n, r, K, N, !lists && da, ga, st);
+  PairArgs p{g, g_stride, M, N, K, w + l.bt, w + l.at, index, index_wide, rows_per_index, scales, base, base_stride, dx, gh,
+             (int)n, (int)r, 0, 0, m, 0, 1, nullptr, nullptr, 1, 0, 0, (float *)(w + l.sums)};
+  if (lists) p.order = ga.order, p.slots = ga.tiles;
+  const int rc = run_pair(p, dtype, drop > 0, st);
+  if (rc || !da) return rc;
   float *const parts = (float *)(w + l.parts);
-  if (M > 0) {
-    GradArgs q{x, g, x_stride, g_stride, K, N, gh, hidden, (const int32_t *)(gw + gl.order), (const Slot *)(gw + gl.pieces), parts,
-               (int)r, (int)n, (int)blocks_a, drop > 0, m};
-    const dim3 grid((unsigned)(blocks_a + blocks_b), (unsigned)slots, (unsigned)cdiv(r, 64));
-    if (dtype == KSD_F32) launch_grad<KSD_F32>(q, grid, st);
-    else if (dtype == KSD_BF16) launch_grad<KSD_BF16>(q, grid, st);
-    else launch_grad<KSD_F16>(q, grid, st);
-  }
-  join_kernel<<<dim3((unsigned)cdiv(each, 64), (unsigned)n), 256, 0, st>>>(parts, (const int2 *)(gw + gl.spans), r * K, r * N, da, db);
+  GradArgs q{x, g, x_stride, g_stride, K, N, gh, hidden, ga.order, ga.pieces, parts, (int)r, (int)n, (int)blocks_a, drop > 0, m};
+  const dim3 grid((unsigned)(blocks_a + blocks_b), (unsigned)slots, (unsigned)cdiv(r, 64));
+  if (dtype == KSD_F32) launch_grad<KSD_F32>(q, grid, st);
+  else if (dtype == KSD_BF16) launch_grad<KSD_BF16>(q, grid, st);
+  else launch_grad<KSD_F16>(q, grid, st);
+  join_kernel<<<dim3((unsigned)cdiv(each, 64), (unsigned)n), 256, 0, st>>>(parts, ga.spans, r * K, r * N, da, db);
   return check_launch("adapter_linear_backward");
 }

@@ -569,7 +569,7 @@ __global__ __launch_bounds__(1024) void draw_kernel(const Args a) {
   }
   for (int t = tid; t <= a.L; t += 1024)
     a.out[(int64_t)b * (a.L + 1) + t] = t < d.at ? a.tokens[(int64_t)b * a.L + t] : t == d.at ? found : -1;
-  if (tid == 0) a.accepted[b] = d.at;
+  if (tid == 0 && a.accepted) a.accepted[b] = d.at;
 }
 
 struct Layout {
@@ -663,7 +663,7 @@ extern "C" int ksd_verify_draft(const void *target, const void *draft, int dtype
   if (!spec::fits(B, L, V)) return fail(KSD_EINVAL, "verify_draft: bad shape");
   if (dtype != KSD_F32 && dtype != KSD_BF16 && dtype != KSD_F16) return fail(KSD_ETYPE, "verify_draft: unsupported element type");
   if (B == 0) return KSD_OK;
-  if (!target || (!uniforms && (temperatures || temperature > 0)) || !out || !accepted || !workspace || (L > 0 && !tokens))
+  if (!target || (!uniforms && (temperatures || temperature > 0)) || !out || (L > 0 && !accepted) || !workspace || (L > 0 && !tokens))
     return fail(KSD_EINVAL, "verify_draft: null pointer");
   if (target_b < 0 || target_t < 0 || draft_b < 0 || draft_t < 0) return fail(KSD_EINVAL, "verify_draft: negative stride");
   const spec::Layout l = spec::layout(B, L, V, draft != nullptr);

@@ -23,15 +23,21 @@ from .. import _lib
 from .dropout import mask_arguments
 
 _TYPES = (torch.float32, torch.bfloat16, torch.float16)
+_INDEX = (torch.int64, torch.int32)
 
 
-def _rows(t: torch.Tensor, width: int) -> torch.Tensor:
+def _rows(t: torch.Tensor, width: int):
+    """(t or a copy, its rows, their pitch) of a tensor (..., width) as the kernels read it."""
+    if t.is_contiguous():
+        return t, t.numel() // width, width
     t = t if t.dim() == 2 else t.reshape(-1, width)
-    return t if t.stride(1) == 1 and (t.shape[0] <= 1 or t.stride(0) >= width) else t.contiguous()
+    if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < width):
+        t = t.contiguous()
+    return t, t.shape[0], t.stride(0) if t.shape[0] > 1 else width
 
 
-def _pitch(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _dense(t: torch.Tensor) -> torch.Tensor:
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _shared(p: torch.Tensor, q: torch.Tensor) -> bool:
@@ -45,67 +51,75 @@ def _shared(p: torch.Tensor, q: torch.Tensor) -> bool:
     return a < d and c < b
 
 
-def _bank(x, a, b, index, scales, base):
-    """Checks a call: (x as rows, a, b, index, rows of one index, scales, base as rows)."""
-    if x.dim() < 2:
-        raise ValueError(f"x must be (..., K) with one dimension or more of rows, got {tuple(x.shape)}")
-    if x.dtype not in _TYPES:
-        raise TypeError(f"unsupported dtype {x.dtype}")
-    if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2] or a.shape[2] != x.shape[-1]:
-        raise ValueError(f"a must be (n, r, {x.shape[-1]}) and b (n, N, r), got {tuple(a.shape)} and {tuple(b.shape)}")
-    if a.dtype != x.dtype or b.dtype != x.dtype:
-        raise TypeError(f"adapters must be of x's {x.dtype}, got {a.dtype} and {b.dtype}")
-    n, r, K = a.shape
-    N = b.shape[1]
+def _check(x, a, b, index, scales, base):
+    """(M's leading dimensions, K, n, r, N), with the calls that are refused."""
+    xs, shape_a, shape_b, at, dtype = x.shape, a.shape, b.shape, index.shape, x.dtype
+    if len(xs) < 2:
+        raise ValueError(f"x must be (..., K) with one dimension or more of rows, got {tuple(xs)}")
+    if dtype not in _TYPES:
+        raise TypeError(f"unsupported dtype {dtype}")
+    if (len(shape_a) != 3 or len(shape_b) != 3 or shape_a[0] != shape_b[0] or shape_a[1] != shape_b[2]
+            or shape_a[2] != xs[-1]):
+        raise ValueError(f"a must be (n, r, {xs[-1]}) and b (n, N, r), got {tuple(shape_a)} and {tuple(shape_b)}")
+    if a.dtype != dtype or b.dtype != dtype:
+        raise TypeError(f"adapters must be of x's {dtype}, got {a.dtype} and {b.dtype}")
+    n, r, K = shape_a
+    N = shape_b[1]
     if not (n and r and K and N) or r > 128 or n > 65535:
-        raise ValueError(f"a bank holds 1 to 65535 adapters of rank 1 to 128, got {tuple(a.shape)} and {tuple(b.shape)}")
-    if index.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"a bank holds 1 to 65535 adapters of rank 1 to 128, got {tuple(shape_a)} and {tuple(shape_b)}")
+    if index.dtype not in _INDEX:
         raise TypeError(f"index must be integers, got {index.dtype}")
-    if index.dim() == 0 or index.dim() >= x.dim() or index.shape != x.shape[:index.dim()]:
-        raise ValueError(f"index must be of x's leading dimensions {tuple(x.shape[:-1])}, got {tuple(index.shape)}")
-    if scales is not None and (scales.dtype != torch.float32 or tuple(scales.shape) != (n,)):
+    lead = xs[:-1]
+    if at != lead and (not at or at != lead[:len(at)]):
+        raise ValueError(f"index must be of x's leading dimensions {tuple(lead)}, got {tuple(at)}")
+    if scales is not None and (scales.dtype != torch.float32 or scales.shape != (n,)):
         raise ValueError(f"scales must be {n} float32 values, got {tuple(scales.shape)} {scales.dtype}")
-    if base is not None and (base.shape != (*x.shape[:-1], N) or base.dtype != x.dtype):
-        raise ValueError(f"base must be {(*x.shape[:-1], N)} {x.dtype}, got {tuple(base.shape)} {base.dtype}")
-    x2 = _rows(x, K)
-    per = x2.shape[0] // max(1, index.numel())
-    return (x2, a.contiguous(), b.contiguous(), index.contiguous(), max(1, per),
-            None if scales is None else scales.contiguous(), None if base is None else _rows(base, N))
+    if base is not None and (base.dtype != dtype or base.shape != (*lead, N)):
+        raise ValueError(f"base must be {(*lead, N)} {dtype}, got {tuple(base.shape)} {base.dtype}")
+    return lead, K, n, r, N
 
 
 def _forward(x, a, b, index, scales, base, out, mask, train):
     dev = _lib.require_gpu(x, a, b, index, scales, base, out)
-    x2, a, b, index, per, scales, base2 = _bank(x, a, b, index, scales, base)
-    (M, K), (n, N, r) = x2.shape, b.shape
+    lead, K, n, r, N = _check(x, a, b, index, scales, base)
+    x, M, pitch = _rows(x, K)
+    a, b, index = _dense(a), _dense(b), _dense(index)
+    per = M // (index.numel() or 1) or 1
+    if scales is not None:
+        scales = _dense(scales)
+    base_at, base_pitch = None, 0
+    if base is not None:
+        base, _, base_pitch = _rows(base, N)
+        base_at = base.data_ptr()
     y = out
     if out is None:
-        y = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=dev)
+        y = torch.empty((*lead, N), dtype=x.dtype, device=dev)
     else:
-        if out.shape != (*x.shape[:-1], N) or out.dtype != x.dtype or not out.is_contiguous():
-            raise ValueError(f"out must be a contiguous {(*x.shape[:-1], N)} {x.dtype} tensor")
-        for name, t in (("x", x2), ("a", a), ("b", b), ("index", index)):
+        if out.shape != (*lead, N) or out.dtype != x.dtype or not out.is_contiguous():
+            raise ValueError(f"out must be a contiguous {(*lead, N)} {x.dtype} tensor")
+        for name, t in (("x", x), ("a", a), ("b", b), ("index", index)):
             if _shared(out, t):
                 raise ValueError(f"out shares memory with {name}")
-        if base2 is not None and _shared(out, base2) and (base2.data_ptr() != out.data_ptr() or _pitch(base2) != N):
+        if base is not None and _shared(out, base) and (base_at != out.data_ptr() or base_pitch != N):
             raise ValueError("out shares memory with base and is not base itself")
+    dt = _lib.dtype_code(x.dtype)
     h = torch.empty((M, r), dtype=torch.float32, device=dev) if train else None
-    groups, size = None, _groups_bytes(M, K, N, r, n, per, _lib.dtype_code(x.dtype), train)
-    if size:
-        groups = torch.empty(size, dtype=torch.int8, device=dev)
-    if M or train:
-        _lib.call_on(dev, "ksd_adapter_linear", x2.data_ptr(), _lib.dtype_code(x.dtype), M, K, _pitch(x2), a.data_ptr(),
-                     b.data_ptr(), n, r, N, index.data_ptr(), int(index.dtype == torch.int64), per, _lib.ptr(scales),
-                     _lib.ptr(base2), 0 if base2 is None else _pitch(base2), *mask, y.data_ptr(), _lib.ptr(h),
-                     _lib.ptr(groups), size)
+    size = _workspace("ksd_adapter_linear_workspace", M, K, N, r, n, per, dt)
+    work = torch.empty(size, dtype=torch.int8, device=dev) if size else None
+    if M:
+        _lib.call_on(dev, "ksd_adapter_linear", x.data_ptr(), dt, M, K, pitch, a.data_ptr(), b.data_ptr(), n, r, N,
+                     index.data_ptr(), index.dtype == torch.int64, per, None if scales is None else scales.data_ptr(), base_at,
+                     base_pitch, *mask, y.data_ptr(), None if h is None else h.data_ptr(),
+                     None if work is None else work.data_ptr(), size)
     if out is not None:
         _lib.wrote((out,))
-    return y, (x2, a, b, index, per, scales, h, groups)
+    return y, (x, pitch, a, b, index, per, scales, h, work)
 
 
 @functools.lru_cache(maxsize=4096)
-def _groups_bytes(M: int, K: int, N: int, r: int, n: int, per: int, dtype: int, train: bool) -> int:
+def _workspace(name: str, *sizes: int) -> int:
     need = ctypes.c_int64()
-    _lib.call("ksd_adapter_linear_groups", M, K, N, r, n, per, dtype, int(train), ctypes.byref(need))
+    _lib.call(name, *sizes, ctypes.byref(need))
     return need.value
 
 
@@ -124,10 +138,10 @@ def adapter_linear(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, index: tor
 
 
 class Saved:
-    """What adapter_linear_backward needs of a training forward: its inputs, h (r floats a token) and the tokens
-    listed by adapter."""
+    """What adapter_linear_backward needs of a training forward: its inputs, h (r floats a token) and its
+    workspace, where tokens of many adapters are listed by adapter."""
 
-    __slots__ = ("x", "a", "b", "index", "per", "scales", "hidden", "groups", "lead", "mask", "seed")
+    __slots__ = ("x", "pitch", "a", "b", "index", "per", "scales", "hidden", "work", "lead", "mask", "seed")
 
 
 def adapter_linear_train(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, index: torch.Tensor,
@@ -141,7 +155,7 @@ def adapter_linear_train(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, inde
     mask = mask_arguments(dropout, seed, stream, dev)
     s = Saved()
     s.mask, s.seed, s.lead = mask, seed, x.shape[:-1]
-    y, (s.x, s.a, s.b, s.index, s.per, s.scales, s.hidden, s.groups) = _forward(x, a, b, index, scales, base, None, mask, True)
+    y, (s.x, s.pitch, s.a, s.b, s.index, s.per, s.scales, s.hidden, s.work) = _forward(x, a, b, index, scales, base, None, mask, True)
     return y, s
 
 
@@ -152,27 +166,30 @@ def adapter_linear_backward(grad: torch.Tensor, saved: Saved, base: torch.Tensor
     None; an adapter that no token has gets zeros."""
     dev = _lib.require_gpu(grad, saved.x, base)
     x, a, b = saved.x, saved.a, saved.b
-    (M, K), (n, N, r) = x.shape, b.shape
+    (n, N, r), K = b.shape, a.shape[2]
+    M = saved.hidden.shape[0]
     if grad.shape != (*saved.lead, N) or grad.dtype != x.dtype:
         raise ValueError(f"grad must be {(*saved.lead, N)} {x.dtype}, got {tuple(grad.shape)} {grad.dtype}")
     if base is not None and (base.shape != (*saved.lead, K) or base.dtype != x.dtype):
         raise ValueError(f"base must be {(*saved.lead, K)} {x.dtype}, got {tuple(base.shape)} {base.dtype}")
     if not need_dx and not need_dab:
         return None, None, None
-    g = _rows(grad, N)
-    base = None if base is None or not need_dx else _rows(base, K)
+    g, _, pitch = _rows(grad, N)
+    base_at, base_pitch = None, 0
+    if base is not None and need_dx:
+        base, _, base_pitch = _rows(base, K)
+        base_at = base.data_ptr()
     dx = torch.empty((*saved.lead, K), dtype=x.dtype, device=dev) if need_dx else None
     da = torch.empty((n, r, K), dtype=torch.float32, device=dev) if need_dab else None
     db = torch.empty((n, N, r), dtype=torch.float32, device=dev) if need_dab else None
-    need = ctypes.c_int64()
     dt = _lib.dtype_code(x.dtype)
-    _lib.call("ksd_adapter_linear_backward_workspace", M, K, N, r, n, dt, ctypes.byref(need))
-    work = torch.empty(need.value, dtype=torch.int8, device=dev)
-    _lib.call_on(dev, "ksd_adapter_linear_backward", g.data_ptr(), dt, M, N, _pitch(g), x.data_ptr(), K, _pitch(x),
-                 saved.hidden.data_ptr(), saved.groups.data_ptr(), saved.groups.numel(), a.data_ptr(), b.data_ptr(), n, r, saved.index.data_ptr(),
-                 int(saved.index.dtype == torch.int64), saved.per, _lib.ptr(saved.scales), _lib.ptr(base),
-                 0 if base is None else _pitch(base), *saved.mask, _lib.ptr(dx) if M else None, _lib.ptr(da), _lib.ptr(db),
-                 work.data_ptr(), need.value)
+    size = _workspace("ksd_adapter_linear_backward_workspace", M, K, N, r, n, saved.per, dt)
+    work = torch.empty(size, dtype=torch.int8, device=dev)
+    _lib.call_on(dev, "ksd_adapter_linear_backward", g.data_ptr(), dt, M, N, pitch, x.data_ptr(), K, saved.pitch,
+                 saved.hidden.data_ptr(), _lib.ptr(saved.work), 0 if saved.work is None else saved.work.numel(), a.data_ptr(),
+                 b.data_ptr(), n, r, saved.index.data_ptr(), saved.index.dtype == torch.int64, saved.per,
+                 _lib.ptr(saved.scales), base_at, base_pitch, *saved.mask, _lib.ptr(dx) if M else None, _lib.ptr(da),
+                 _lib.ptr(db), work.data_ptr(), size)
     return dx, da, db
 
 
@@ -183,18 +200,18 @@ class _AdapterFunction(torch.autograd.Function):
         y, s = adapter_linear_train(x, a, b, index, scales, base, p, seed, stream)
         # through save_for_backward, so that they are freed with the graph and writes into them are noticed
         device_seed = s.seed if isinstance(s.seed, torch.Tensor) else None
-        ctx.save_for_backward(x, a, b, s.index, s.scales, s.hidden, s.groups, device_seed)
+        ctx.save_for_backward(x, a, b, s.index, s.scales, s.hidden, s.work, device_seed)
         ctx.args = (s.per, s.lead, s.mask)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        x, a, b, index, scales, hidden, groups, seed = ctx.saved_tensors
+        x, a, b, index, scales, hidden, work, seed = ctx.saved_tensors
         s = Saved()
         s.per, s.lead, s.mask = ctx.args
-        s.x, s.a, s.b = _rows(x, x.shape[-1]), a.contiguous(), b.contiguous()
-        s.index, s.scales, s.hidden, s.groups, s.seed = index, scales, hidden, groups, seed
+        (s.x, _, s.pitch), s.a, s.b = _rows(x, x.shape[-1]), _dense(a), _dense(b)
+        s.index, s.scales, s.hidden, s.work, s.seed = index, scales, hidden, work, seed
         need = ctx.needs_input_grad
         dx = da = db = None
         if need[0] or need[1] or need[2]:

@@ -34,9 +34,14 @@ def mask_arguments(p: float, seed, stream: int, dev: torch.device):
     return round(p * 65536), seed, None, stream
 
 
-def _rows(t: torch.Tensor, d: int) -> torch.Tensor:
+def _rows(t: torch.Tensor, d: int):
+    """(t or a copy, its rows, their pitch) of a tensor (..., d) as the kernel reads it."""
+    if t.is_contiguous():
+        return t, t.numel() // d, d
     t = t if t.dim() == 2 else t.reshape(-1, d)
-    return t if t.stride(1) == 1 and (t.shape[0] <= 1 or t.stride(0) >= d) else t.contiguous()
+    if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < d):
+        t = t.contiguous()
+    return t, t.shape[0], t.stride(0) if t.shape[0] > 1 else d
 
 
 def _dropout(x, p, seed, stream, residual):
@@ -49,14 +54,16 @@ def _dropout(x, p, seed, stream, residual):
         raise ValueError(f"residual must be {tuple(x.shape)} {x.dtype}, got {tuple(residual.shape)} {residual.dtype}")
     mask = mask_arguments(p, seed, stream, dev)
     out = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    d = x.shape[-1]
     if out.numel() == 0:
         return out
-    d = x.shape[-1]
-    x2 = _rows(x, d)
-    r2 = None if residual is None else _rows(residual, d)
-    rows = x2.shape[0]
-    _lib.call_on(dev, "ksd_dropout", x2.data_ptr(), _lib.dtype_code(x.dtype), rows, d, x2.stride(0) if rows > 1 else d,
-                 *mask, _lib.ptr(r2), 0 if r2 is None else r2.stride(0) if rows > 1 else d, out.data_ptr())
+    x, rows, pitch = _rows(x, d)
+    at, residual_pitch = None, 0
+    if residual is not None:
+        residual, _, residual_pitch = _rows(residual, d)
+        at = residual.data_ptr()
+    _lib.call_on(dev, "ksd_dropout", x.data_ptr(), _lib.dtype_code(x.dtype), rows, d, pitch, *mask, at, residual_pitch,
+                 out.data_ptr())
     return out
 
 

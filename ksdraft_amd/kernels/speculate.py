@@ -11,6 +11,7 @@ host.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -19,68 +20,43 @@ from .. import _lib
 _TYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
-def _logits(t: torch.Tensor, shape, name: str) -> torch.Tensor:
-    if t.dim() != 3 or (shape is not None and tuple(t.shape) != shape):
-        raise ValueError(f"{name} must be {shape or '(streams, positions, tokens)'}, got {tuple(t.shape)}")
-    if t.dtype not in _TYPES:
-        raise TypeError(f"{name}: unsupported dtype {t.dtype}")
-    return t if t.stride(2) == 1 else t.contiguous()
-
-
 def _integers(t: torch.Tensor, shape, name: str) -> torch.Tensor:
     if t.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"{name} must be integers, got {t.dtype}")
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
-    return t.to(torch.int64).contiguous()
+    return t if t.dtype == torch.int64 and t.is_contiguous() else t.to(torch.int64).contiguous()
 
 
-def _verify(target, tokens, uniforms, draft, temperatures, lengths):
-    dev = _lib.require_gpu(target, tokens, uniforms, draft, lengths,
-                           temperatures if isinstance(temperatures, torch.Tensor) else None)
-    target = _logits(target, None, "target_logits")
-    B, rows, V = target.shape
-    L = rows - 1
-    if L < 0 or V == 0:
-        raise ValueError(f"target_logits must hold a row more than drafted tokens, got {tuple(target.shape)}")
-    if L:
-        tokens = _integers(tokens, (B, L), "draft_tokens")
-    if draft is not None:
-        draft = _logits(draft, (B, L, V), "draft_logits")
-        if draft.dtype != target.dtype:
-            raise TypeError(f"draft_logits are {draft.dtype}, target_logits {target.dtype}")
+def _numbers(uniforms, temperatures, shape, lead):
+    """(uniforms, whether they are fp64, temperatures on the device or None, else one for all)."""
     temps, temp = None, 1.0
     if isinstance(temperatures, torch.Tensor):
-        if temperatures.dtype != torch.float32 or tuple(temperatures.shape) != (B,):
-            raise ValueError(f"temperatures must be {B} float32 values, got {tuple(temperatures.shape)} {temperatures.dtype}")
-        temps = temperatures.contiguous()
+        if temperatures.dtype != torch.float32 or temperatures.shape != lead:
+            raise ValueError(f"temperatures must be {tuple(lead)} float32 values, got {tuple(temperatures.shape)} {temperatures.dtype}")
+        temps = temperatures if temperatures.is_contiguous() else temperatures.contiguous()
     elif temperatures is not None:
         temp = float(temperatures)
         if not temp >= 0:
             raise ValueError(f"temperature must not be negative, got {temp}")
+    wide = False
     if uniforms is not None:
         if uniforms.dtype not in (torch.float32, torch.float64):
             raise TypeError(f"uniforms must be float32 or float64, got {uniforms.dtype}")
-        if tuple(uniforms.shape) != (B, L + 1):
-            raise ValueError(f"uniforms must be {(B, L + 1)}, got {tuple(uniforms.shape)}")
-        uniforms = uniforms.contiguous()
+        if uniforms.shape != shape:
+            raise ValueError(f"uniforms must be {tuple(shape)}, got {tuple(uniforms.shape)}")
+        wide = uniforms.dtype == torch.float64
+        uniforms = uniforms if uniforms.is_contiguous() else uniforms.contiguous()
     elif temps is not None or temp > 0:
         raise ValueError("only temperature 0 draws without uniforms")
-    if lengths is not None:
-        lengths = _integers(lengths, (B,), "lengths")
-    out = torch.empty((B, L + 1), dtype=torch.int64, device=dev)
-    accepted = torch.empty(B, dtype=torch.int64, device=dev)
-    if B == 0:
-        return out, accepted
+    return uniforms, wide, temps, temp
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace(B: int, L: int, V: int, draft: bool) -> int:
     need = ctypes.c_int64()
-    _lib.call("ksd_verify_draft_workspace", B, L, V, int(draft is not None), ctypes.byref(need))
-    work = torch.empty(need.value, dtype=torch.int8, device=dev)
-    db, dt = (0, 0) if draft is None else (draft.stride(0), draft.stride(1))
-    _lib.call_on(dev, "ksd_verify_draft", target.data_ptr(), _lib.ptr(draft), _lib.dtype_code(target.dtype), B, L, V,
-                 target.stride(0), target.stride(1), db, dt, tokens.data_ptr() if L else None, _lib.ptr(uniforms),
-                 int(uniforms is not None and uniforms.dtype == torch.float64), _lib.ptr(temps), temp, _lib.ptr(lengths),
-                 out.data_ptr(), accepted.data_ptr(), work.data_ptr(), need.value)
-    return out, accepted
+    _lib.call("ksd_verify_draft_workspace", B, L, V, draft, ctypes.byref(need))
+    return need.value
 
 
 def verify_draft(target_logits: torch.Tensor, draft_tokens: torch.Tensor, uniforms: torch.Tensor | None,
@@ -100,7 +76,38 @@ def verify_draft(target_logits: torch.Tensor, draft_tokens: torch.Tensor, unifor
     without a finite logit, or with NaN or +inf, refuses its token and draws -1."""
     if draft_tokens is None:
         raise ValueError("draft_tokens are needed; sample_tokens draws without a draft")
-    return _verify(target_logits, draft_tokens, uniforms, draft_logits, temperatures, lengths)
+    dev = _lib.require_gpu(target_logits, draft_tokens, uniforms, draft_logits, lengths,
+                           temperatures if isinstance(temperatures, torch.Tensor) else None)
+    target, draft, dtype = target_logits, draft_logits, target_logits.dtype
+    if target.dim() != 3 or target.shape[1] == 0 or target.shape[2] == 0:
+        raise ValueError(f"target_logits must be (streams, a row more than drafted tokens, tokens), got {tuple(target.shape)}")
+    if dtype not in _TYPES:
+        raise TypeError(f"target_logits: unsupported dtype {dtype}")
+    B, rows, V = target.shape
+    L = rows - 1
+    target = target if target.stride(2) == 1 else target.contiguous()
+    tokens = _integers(draft_tokens, (B, L), "draft_tokens")
+    db = dt = 0
+    if draft is not None:
+        if draft.shape != (B, L, V):
+            raise ValueError(f"draft_logits must be {(B, L, V)}, got {tuple(draft.shape)}")
+        if draft.dtype != dtype:
+            raise TypeError(f"draft_logits are {draft.dtype}, target_logits {dtype}")
+        draft = draft if draft.stride(2) == 1 else draft.contiguous()
+        db, dt, _ = draft.stride()
+    uniforms, wide, temps, temp = _numbers(uniforms, temperatures, (B, rows), (B,))
+    if lengths is not None:
+        lengths = _integers(lengths, (B,), "lengths")
+    out = torch.empty((B, rows), dtype=torch.int64, device=dev)
+    accepted = torch.empty(B, dtype=torch.int64, device=dev)
+    if B:
+        size = _workspace(B, L, V, draft is not None)
+        work = torch.empty(size, dtype=torch.int8, device=dev)
+        tb, tt, _ = target.stride()
+        _lib.call_on(dev, "ksd_verify_draft", target.data_ptr(), _lib.ptr(draft), _lib.dtype_code(dtype), B, L, V, tb, tt, db, dt,
+                     tokens.data_ptr(), _lib.ptr(uniforms), wide, _lib.ptr(temps), temp, _lib.ptr(lengths), out.data_ptr(),
+                     accepted.data_ptr(), work.data_ptr(), size)
+    return out, accepted
 
 
 def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor | None = None,
@@ -108,18 +115,20 @@ def sample_tokens(logits: torch.Tensor, uniforms: torch.Tensor | None = None,
     """A token for each row of logits (..., V): the first whose running sum of softmax(logits / T) passes its
     number of uniforms (...), or the largest logit at T = 0 (uniforms may then be None for a T given as a
     number); -1 for a row without a distribution. temperatures: (...) float32, a number or None (1). int64 (...)."""
-    if logits.dim() == 0:
-        raise ValueError("logits must have a last dimension of tokens")
-    lead = logits.shape[:-1]
-
-    def flat(t, name):
-        if t is not None and isinstance(t, torch.Tensor) and t.shape != lead:
-            raise ValueError(f"{name} must be {tuple(lead)}, got {tuple(t.shape)}")
-        return t
-    uniforms = flat(uniforms, "uniforms")
-    temperatures = flat(temperatures, "temperatures")
-    if isinstance(temperatures, torch.Tensor):
-        temperatures = temperatures.reshape(-1)
-    rows = logits.reshape(-1, 1, logits.shape[-1]) if logits.shape[-1] else logits.new_empty((0, 1, 0))
-    out, _ = _verify(rows, None, None if uniforms is None else uniforms.reshape(-1, 1), None, temperatures, None)
-    return out.reshape(lead)
+    dev = _lib.require_gpu(logits, uniforms, temperatures if isinstance(temperatures, torch.Tensor) else None)
+    if logits.dim() == 0 or logits.shape[-1] == 0:
+        raise ValueError(f"logits must have a last dimension of tokens, got {tuple(logits.shape)}")
+    if logits.dtype not in _TYPES:
+        raise TypeError(f"logits: unsupported dtype {logits.dtype}")
+    lead, V = logits.shape[:-1], logits.shape[-1]
+    uniforms, wide, temps, temp = _numbers(uniforms, temperatures, lead, lead)
+    rows = logits if logits.dim() == 2 else logits.reshape(-1, V)
+    rows = rows if rows.stride(1) == 1 else rows.contiguous()
+    B = rows.shape[0]
+    out = torch.empty(lead, dtype=torch.int64, device=dev)
+    if B:
+        size = _workspace(B, 0, V, False)
+        work = torch.empty(size, dtype=torch.int8, device=dev)
+        _lib.call_on(dev, "ksd_verify_draft", rows.data_ptr(), None, _lib.dtype_code(rows.dtype), B, 0, V, rows.stride(0), 0, 0, 0,
+                     None, _lib.ptr(uniforms), wide, _lib.ptr(temps), temp, None, out.data_ptr(), None, work.data_ptr(), size)
+    return out

@@ -21,7 +21,7 @@ def backward(dtype=0, M=4, N=16, stride=16, K=8, hidden=P, n=2, r=4, per=1, drop
 
 def test_forward():
     assert forward(M=0) == 0
-    assert forward(M=600000) == 1 and forward(M=600000, groups=P, size=64) == 1 and forward(groups=ctypes.c_void_p(8), size=1 << 30) == 1
+    assert forward(M=600000) == 1 and forward(M=600000, groups=P, size=64) == 1 and forward(M=600000, groups=ctypes.c_void_p(8), size=1 << 40) == 1
     for bad in (dict(M=-1), dict(K=0), dict(N=0), dict(r=0), dict(r=129), dict(n=0), dict(n=1 << 16), dict(per=0), dict(stride=7),
                 dict(base_stride=15), dict(drop=65537), dict(drop=-1), dict(stream_id=-1), dict(x=None), dict(a=None), dict(index=None),
                 dict(y=None), dict(M=1 << 31), dict(K=1 << 31), dict(N=1 << 31)):
@@ -32,14 +32,16 @@ def test_forward():
 def test_backward():
     for bad in (dict(M=-1), dict(K=0), dict(N=0), dict(r=129), dict(n=0), dict(per=0), dict(stride=15), dict(hidden=None),
                 dict(drop=70000), dict(work=None), dict(size=16), dict(work=ctypes.c_void_p(8)), dict(M=1 << 25), dict(da=None),
-                dict(groups=None), dict(groups_size=64)):
+                dict(M=600000, groups=None), dict(M=600000, groups_size=64), dict(M=600000, groups=ctypes.c_void_p(8))):
         assert backward(**bad) == 1, bad
     assert backward(dtype=9) == 2
     need = ctypes.c_int64()
     f = _lib.load().ksd_adapter_linear_backward_workspace
-    assert f(4, 8, 16, 4, 2, 0, ctypes.byref(need)) == 0 and need.value > 0
-    assert f(4, 8, 16, 4, 2, 7, ctypes.byref(need)) == 1 and f(4, 8, 16, 0, 2, 0, ctypes.byref(need)) == 1
-    assert f(4, 8, 16, 4, 2, 0, None) == 1
+    assert f(4, 8, 16, 4, 2, 1, 0, ctypes.byref(need)) == 0 and need.value > 0
+    assert f(0, 8, 16, 4, 2, 1, 0, ctypes.byref(need)) == 0
+    assert _lib.load().ksd_adapter_linear_workspace(0, 8, 16, 4, 2, 1, 0, ctypes.byref(need)) == 0 and need.value == 0
+    assert f(4, 8, 16, 4, 2, 1, 7, ctypes.byref(need)) == 1 and f(4, 8, 16, 0, 2, 1, 0, ctypes.byref(need)) == 1
+    assert f(4, 8, 16, 4, 2, 0, 0, ctypes.byref(need)) == 1 and f(4, 8, 16, 4, 2, 1, 0, None) == 1
 
 
 def test_capture_guard(monkeypatch):
