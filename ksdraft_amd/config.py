@@ -27,12 +27,15 @@ class KSDraftConfig:
     anchor_stride: int = 64
     dtype: str = "int8"
     tie_word_embeddings: bool = True
+    dropout: float = 0.0  # on each block's mixer and FFN before their residual adds, in training
 
     def __post_init__(self) -> None:
         if self.dtype not in VALID_DTYPES:
             raise ValueError(f"dtype must be one of {VALID_DTYPES}, got {self.dtype!r}")
         if not 1 <= self.rosa_bits <= 64:
             raise ValueError("rosa_bits must be in [1, 64] (Rosa packed symbol width)")
+        if not 0 <= self.dropout <= 1:
+            raise ValueError(f"dropout must lie in [0, 1], got {self.dropout}")
 
     @property
     def n_heads(self) -> int:

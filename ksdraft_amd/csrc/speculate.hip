@@ -21,9 +21,10 @@
 namespace ksd {
 namespace spec {
 
-struct Part {  // of a row's piece: largest logit, sum of 2^((z - m) c); greedy: largest logit, -, its place
-  float m, s;
-  int at, bad;
+struct Part {  // of a row's piece: largest logit, sum of 2^((z - m) c); greedy: largest logit (NaN where there is one), its place
+  float m;
+  int at;
+  double s;
 };
 
 struct Args {
@@ -42,10 +43,11 @@ struct Args {
   int *refused;                // (kRanges, B): the first refused position, as far as the ranges before one tell
   int B, L, V, splits, chunk, pieces, piece;
   int range, t0, t1, before;   // positions of this launch of stats_kernel, and where its predecessor's began
+  int exact;                   // stats_kernel's sums are 64-bit already
 };
-constexpr int kRanges = 6, kNone = 0x7fffffff;
+constexpr int kRanges = 6, kNone = 0x7fffffff, kHeld = 4;
 // Logits from which positions go in several launches, and of the first of them
-constexpr int64_t kSeveral = 64 << 20, kFirst = 40 << 20;
+constexpr int64_t kSeveral = 64 << 20, kFirst = 40 << 20, kFew = 12 << 20;
 
 __device__ __forceinline__ float temperature(const Args &a, int b) { return a.temps ? a.temps[b] : a.temp; }
 __device__ __forceinline__ float clamped(float t) { return fminf(fmaxf(t, 1e-37f), 1e37f); }
@@ -138,7 +140,6 @@ __device__ __forceinline__ float block_max(float v, float *scratch) {
 template <int DT>
 __device__ __forceinline__ void best_part(const typename Elem<DT>::T *row, int from, int to, Part *out) {
   __shared__ Best found[4];
-  __shared__ int bads[4];
   Best best{-INFINITY, kNone};
   bool bad = false;
   for (int k = from + threadIdx.x * 8; k < to; k += 2048) {
@@ -152,12 +153,12 @@ __device__ __forceinline__ void best_part(const typename Elem<DT>::T *row, int f
   }
 #pragma unroll
   for (int o = 32; o; o >>= 1) best = better(best, Best{__shfl_xor(best.m, o), __shfl_xor(best.at, o)});
-  const int any = __ballot(bad) != 0;
-  if ((threadIdx.x & 63) == 0) found[threadIdx.x >> 6] = best, bads[threadIdx.x >> 6] = any;
+  if (__ballot(bad)) best.m = NAN;
+  if ((threadIdx.x & 63) == 0) found[threadIdx.x >> 6] = best;
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int w = 1; w < 4; ++w) best = better(best, found[w]);
-    *out = Part{best.m, 0.0f, best.at, bads[0] | bads[1] | bads[2] | bads[3]};
+    for (int w = 1; w < 4; ++w) best = best.m != best.m || found[w].m != found[w].m ? Best{NAN, 0} : better(best, found[w]);
+    *out = Part{best.m, best.at, 0.0};
   }
 }
 
@@ -167,15 +168,22 @@ struct Stat {
   float m;
   double s;
 };
-__device__ __forceinline__ Stat row_stat(const Args &a, const Part *p, float c) {
+__device__ __forceinline__ Stat row_stat(const Args &a, const Part *p, float T) {
   const int i = threadIdx.x & 15;
-  Part x{-FLT_MAX, 0, 0, 0}, y = x;
+  Part x{-FLT_MAX, 0, 0.0}, y = x;
   if (i < a.splits) x = p[i];
   if (i + 16 < a.splits) y = p[i + 16];
   float m = fmaxf(x.m, y.m);
 #pragma unroll
   for (int o = 8; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-  double s = (double)(x.s * __builtin_amdgcn_exp2f((x.m - m) * c)) + (double)(y.s * __builtin_amdgcn_exp2f((y.m - m) * c));
+  double s;
+  if (a.exact) {
+    const Exponent e = exponent(T, m);
+    s = x.s * power((double)x.m, e) + y.s * power((double)y.m, e);
+  } else {
+    const float c = 1.4426950408889634f / clamped(T);
+    s = x.s * (double)__builtin_amdgcn_exp2f((x.m - m) * c) + y.s * (double)__builtin_amdgcn_exp2f((y.m - m) * c);
+  }
 #pragma unroll
   for (int o = 8; o; o >>= 1) s += __shfl_xor(s, o);
   return Stat{m, s};
@@ -186,7 +194,7 @@ __device__ __forceinline__ int row_best(const Args &a, const Part *p, int splits
   int bad = 0;
   for (int i = threadIdx.x & 15; i < splits; i += 16) {
     const Part x = p[i];
-    best = better(best, Best{x.m, x.at}), bad |= x.bad;
+    best = better(best, Best{x.m, x.at}), bad |= x.m != x.m;
   }
 #pragma unroll
   for (int o = 8; o; o >>= 1) {
@@ -201,27 +209,26 @@ __device__ __forceinline__ bool accepts(const Args &a, int b, int t, float T) { 
   const int64_t token = a.tokens[(int64_t)b * a.L + t];
   if (!(T > 0)) return row_best(a, parts_of(a, b, t), a.splits) == token && token >= 0;
   const bool in = token >= 0 && token < a.V;
-  const float c = 1.4426950408889634f / clamped(T);
   const float zp = in ? Elem<DT>::load(target_row<DT>(a, b, t) + token) : 0.0f;
   const float zq = in && a.draft ? Elem<DT>::load(draft_row<DT>(a, b, t) + token) : 0.0f;
   const double u = uniform(a, b, t);
-  const Stat p = row_stat(a, parts_of(a, b, t), c);
+  const Stat p = row_stat(a, parts_of(a, b, t), T);
   const double pt = power((double)zp, exponent(T, p.m)) / p.s;
   double qt = 1.0;
   if (a.draft) {
-    const Stat q = row_stat(a, parts_of(a, b, a.L + 1 + t), c);
+    const Stat q = row_stat(a, parts_of(a, b, a.L + 1 + t), T);
     qt = q.s == 0 ? 0.0 : power((double)zq, exponent(T, q.m)) / q.s;
   }
   return in && u * qt < pt;
 }
 
-// The first refused position in [from, to), else kNone: a workgroup of 256 threads, 16 positions at a time.
+// The first refused position in [from, to), else kNone: a workgroup, 16 threads a position.
 template <int DT>
 __device__ __forceinline__ int refused_in(const Args &a, int b, int from, int to, float T) {
   __shared__ int first;
   if (threadIdx.x == 0) first = kNone;
   __syncthreads();
-  for (int base = from; base < to; base += 16) {
+  for (int base = from; base < to; base += blockDim.x >> 4) {
     const int t = base + (threadIdx.x >> 4);
     if (t < to && !accepts<DT>(a, b, t, T) && (threadIdx.x & 15) == 0) atomicMin(&first, t);
     __syncthreads();
@@ -261,6 +268,32 @@ __global__ __launch_bounds__(256) void stats_kernel(const Args a) {
   Part *const out = const_cast<Part *>(parts_of(a, b, drafted ? a.L + 1 + t : t)) + split;
   if (greedy) {
     best_part<DT>(row, from, to, out);
+    return;
+  }
+  if (a.exact) {  // few rows: their pieces fit the registers
+    __shared__ float tops[4];
+    __shared__ double scratch[4];
+    float v[kHeld][8], m = -FLT_MAX;
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u) {
+      const int k = from + (u * 256 + threadIdx.x) * 8;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[u][j] = -INFINITY;
+      if (k < to) load_logits<DT>(row, k, to, v[u]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m = fmaxf(m, v[u][j]);
+    }
+    m = block_max(m, tops);
+    const Exponent e = exponent(T, m);
+    double s = 0;
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u)
+      if (u * 2048 < a.chunk) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s += power((double)v[u][j], e);
+      }
+    s = block_sum(s, scratch);
+    if (threadIdx.x == 0) *out = Part{m, 0, s};
     return;
   }
   const float c = 1.4426950408889634f / clamped(T);
@@ -303,7 +336,7 @@ __global__ __launch_bounds__(256) void stats_kernel(const Args a) {
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int w = 1; w < 4; ++w) join(sm[w], ss[w]);
-    *out = Part{m, s, 0, 0};
+    *out = Part{m, 0, (double)s};
   }
 }
 
@@ -312,8 +345,29 @@ __global__ __launch_bounds__(256) void stats_kernel(const Args a) {
 struct Draw {
   int at, rest;        // position; whether a refused token's draft row is subtracted
   Exponent p, q;
+  double rp, rq;       // reciprocals of the sums of powers, where stats_kernel's sums are 64-bit
   int64_t without;     // the token that is left out (refused, and no draft logits), or -1
 };
+__device__ __forceinline__ double reciprocal(double s) { return s > 0 ? 1.0 / s : s; }  // an empty draft row: q = 0; NaN stays
+// A workgroup tests its stream's tokens; d is in LDS.
+template <int DT>
+__device__ __forceinline__ void find_draw(const Args &a, int b, float T, Draw &d) {
+  const int len = length(a, b);
+  int r = a.range > 0 ? a.refused[(int64_t)a.range * a.B + b] : kNone;
+  if (r == kNone) r = refused_in<DT>(a, b, a.range > 0 ? a.t0 : 0, len, T);
+  const int at = min(r, len);
+  if (!(T > 0)) {
+    if (threadIdx.x == 0) d.at = at;
+  } else if (threadIdx.x < 16) {
+    const bool refused = at < len, rest = refused && a.draft;
+    const Stat p = row_stat(a, parts_of(a, b, at), T);
+    const Stat q = rest ? row_stat(a, parts_of(a, b, a.L + 1 + at), T) : Stat{0.0f, 0.0};
+    if (threadIdx.x == 0)
+      d = Draw{at, rest, exponent(T, p.m), exponent(T, q.m), 1.0 / p.s, reciprocal(q.s),
+               refused && !a.draft ? a.tokens[(int64_t)b * a.L + at] : -1};
+  }
+  __syncthreads();
+}
 
 // Without a draft there is nothing to test: a piece's largest logit and sum of powers in 64 bits at once.
 template <int DT>
@@ -354,24 +408,10 @@ template <int DT>
 __global__ __launch_bounds__(256) void total_kernel(const Args a) {
   const int b = blockIdx.x / a.pieces, piece = blockIdx.x % a.pieces;
   const float T = temperature(a, b);
-  const int len = length(a, b);
   if (!(T > 0) && piece) return;
   __shared__ Draw d;
   __shared__ double scratch[4];
-  int r = a.range > 0 ? a.refused[(int64_t)a.range * a.B + b] : kNone;
-  if (r == kNone) r = refused_in<DT>(a, b, a.range > 0 ? a.t0 : 0, len, T);
-  const int at = min(r, len);
-  if (T > 0 && threadIdx.x < 16) {
-    const bool refused = at < len;
-    const float c = 1.4426950408889634f / clamped(T);
-    const float mp = row_stat(a, parts_of(a, b, at), c).m;
-    const float mq = refused && a.draft ? row_stat(a, parts_of(a, b, a.L + 1 + at), c).m : 0.0f;
-    if (threadIdx.x == 0)
-      d = Draw{at, refused && a.draft, exponent(T, mp), exponent(T, mq),
-               refused && !a.draft ? a.tokens[(int64_t)b * a.L + at] : -1};
-  }
-  if (!(T > 0) && threadIdx.x == 0) d.at = at;
-  __syncthreads();
+  find_draw<DT>(a, b, T, d);
   if (piece == 0 && threadIdx.x == 0) a.draws[b] = d;
   if (!(T > 0)) return;
   const int from = piece * a.piece, to = min(a.V, from + a.piece);
@@ -417,7 +457,7 @@ __device__ __forceinline__ Norms norms_of(const Args &a, int b, int lane) {
   const double *const t = a.totals + (int64_t)b * a.pieces * 2;
   const double sp = wave_sum(piece_value(t, lane, a.pieces, 0) + piece_value(t, lane + 64, a.pieces, 0));
   const double sq = wave_sum(piece_value(t, lane, a.pieces, 1) + piece_value(t, lane + 64, a.pieces, 1));
-  return Norms{1.0 / sp, sq > 0 ? 1.0 / sq : sq};  // an empty draft row: q = 0; NaN stays
+  return Norms{1.0 / sp, reciprocal(sq)};
 }
 
 // The weights of 8 tokens from column k on: rest[j] = what is drawn from, chance[j] = p (or a multiple of it).
@@ -442,11 +482,20 @@ __device__ __forceinline__ void weights_of(const Args &a, int b, const Draw &d, 
 template <int DT>
 __global__ __launch_bounds__(256) void weight_kernel(const Args a) {
   const int b = blockIdx.x / a.pieces, piece = blockIdx.x % a.pieces, lane = threadIdx.x & 63;
-  if (!(temperature(a, b) > 0)) return;
-  const Draw d = a.draws[b];
-  if (!d.rest) return;
+  const float T = temperature(a, b);
+  __shared__ Draw d;
   __shared__ double scratch[4];
-  const Norms n = norms_of(a, b, lane);
+  if (!(T > 0) && (piece || !a.exact)) return;
+  if (a.exact) {
+    find_draw<DT>(a, b, T, d);
+    if (piece == 0 && threadIdx.x == 0) a.draws[b] = d;
+    if (!(T > 0)) return;
+  } else {
+    if (threadIdx.x == 0) d = a.draws[b];
+    __syncthreads();
+  }
+  if (!d.rest) return;
+  const Norms n = a.exact ? Norms{d.rp, d.rq} : norms_of(a, b, lane);
   double rest[8], chance[8], sr = 0, sc = 0;
   const int from = piece * a.piece, to = min(a.V, from + a.piece);
   for (int k = from + threadIdx.x * 8; k < to; k += 2048) {
@@ -471,34 +520,63 @@ __global__ __launch_bounds__(1024) void draw_kernel(const Args a) {
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   __shared__ double scratch[16];
   __shared__ int2 hits[16];
+  __shared__ Draw d;
   const float T = temperature(a, b);
   const double *const totals = a.totals + (int64_t)b * a.pieces * 2;
-  Draw d;
-  int found = -1;
+  int found = -1, pieces = a.pieces, piece = a.piece;
+  if (a.L && a.exact && !a.draft) {
+    find_draw<DT>(a, b, T, d);
+  } else if (a.L) {
+    if (tid == 0) d = a.draws[b];
+  } else if (T > 0) {
+    float m = fmaxf(lane < pieces ? (float)totals[2 * lane + 1] : -FLT_MAX,
+                    lane + 64 < pieces ? (float)totals[2 * (lane + 64) + 1] : -FLT_MAX);
+#pragma unroll
+    for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    if (tid == 0) d = Draw{0, 0, exponent(T, m), Exponent{0, 0}, 1.0, 0.0, -1};
+  } else if (tid == 0) {
+    d.at = 0;
+  }
+  __syncthreads();
   if (!(T > 0)) {
-    d.at = a.L ? a.draws[b].at : 0;
     found = row_best(a, a.L ? parts_of(a, b, d.at) : a.parts + (int64_t)b * a.pieces, a.L ? a.splits : a.pieces);
   } else {
     // weights of the pieces lane and lane + 64; of the second choice, p itself
-    double lo = piece_value(totals, lane, a.pieces, 0), hi = piece_value(totals, lane + 64, a.pieces, 0);
-    double lo1 = piece_value(totals, lane, a.pieces, 1), hi1 = piece_value(totals, lane + 64, a.pieces, 1);
+    double lo, hi = 0, lo1, hi1 = 0;
     Norms n{1.0, 0.0};
-    if (!a.L) {  // pieces with largest logits of their own
-      float m = fmaxf(lane < a.pieces ? (float)lo1 : -FLT_MAX, lane + 64 < a.pieces ? (float)hi1 : -FLT_MAX);
+    if (a.L && a.exact && !d.rest) {  // stats_kernel's pieces, with largest logits of their own
+      pieces = a.splits, piece = a.chunk;
+      const Part p = lane < pieces ? parts_of(a, b, d.at)[lane] : Part{-FLT_MAX, 0, 0.0};
+      lo = lo1 = p.s * power((double)p.m, d.p);
+      if (d.without >= 0 && d.without < a.V) {  // its piece again without it: a difference could leave what is not there
+        const int own = (int)(d.without / piece), to = min(a.V, (own + 1) * piece);
+        double s = 0;
+        for (int k = own * piece + tid * 8; k < to; k += 8192) {
+          float v[8];
+          load_logits<DT>(target_row<DT>(a, b, d.at), k, to, v);
 #pragma unroll
-      for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-      d = Draw{0, 0, exponent(T, m), Exponent{0, 0}, -1};
-      lo *= power(lo1, d.p), hi *= power(hi1, d.p);
-      lo1 = lo, hi1 = hi;
+          for (int j = 0; j < 8; ++j) s += k + j == d.without ? 0.0 : power((double)v[j], d.p);
+        }
+        s = wave_sum(s);
+        if (lane == 0) scratch[wave] = s;
+        __syncthreads();
+        s = 0;
+        for (int v = 0; v < 16; ++v) s += scratch[v];
+        if (lane == own) lo = s;
+      }
+    } else if (d.rest) {
+      n = a.exact ? Norms{d.rp, d.rq} : norms_of(a, b, lane);
+      const double *const w = a.weights + (int64_t)b * pieces * 2;
+      lo = piece_value(w, lane, pieces, 0), hi = piece_value(w, lane + 64, pieces, 0);
+      lo1 = piece_value(w, lane, pieces, 1), hi1 = piece_value(w, lane + 64, pieces, 1);
     } else {
-      d = a.draws[b];
-      if (d.rest) {
-        n = norms_of(a, b, lane);
-        const double *const w = a.weights + (int64_t)b * a.pieces * 2;
-        lo = piece_value(w, lane, a.pieces, 0), hi = piece_value(w, lane + 64, a.pieces, 0);
-        lo1 = piece_value(w, lane, a.pieces, 1), hi1 = piece_value(w, lane + 64, a.pieces, 1);
-      } else {
+      lo = piece_value(totals, lane, pieces, 0), hi = piece_value(totals, lane + 64, pieces, 0);
+      lo1 = piece_value(totals, lane, pieces, 1), hi1 = piece_value(totals, lane + 64, pieces, 1);
+      if (a.L) {
         lo1 += lo, hi1 += hi;
+      } else {  // pieces with largest logits of their own
+        lo *= power(lo1, d.p), hi *= power(hi1, d.p);
+        lo1 = lo, hi1 = hi;
       }
     }
     const bool side = !(wave_sum(lo + hi) > 0);
@@ -524,7 +602,7 @@ __global__ __launch_bounds__(1024) void draw_kernel(const Args a) {
       }
       // what runs before the piece: the sums of the pieces before it, so that no difference is taken
       double run = at & 63 ? __shfl(at < 64 ? run_lo : run_hi, (at & 63) - 1) : (at < 64 ? 0.0 : half);
-      const int from = at * a.piece, to = min(a.V, from + a.piece);
+      const int from = at * piece, to = min(a.V, from + piece);
       int some = -1;
       for (int base = from; base < to && found < 0; base += 8192) {
         const int k = base + tid * 8;
@@ -573,7 +651,7 @@ __global__ __launch_bounds__(1024) void draw_kernel(const Args a) {
 }
 
 struct Layout {
-  int splits, chunk, pieces, piece, ranges;
+  int splits, chunk, pieces, piece, ranges, exact;
   int64_t parts, totals, weights, draws, refused, bytes;
 };
 // Pieces of whole 2048 tokens (256 threads, 16 or 32 bytes each), enough of them to occupy the device a few times over.
@@ -605,6 +683,9 @@ static Layout layout(int64_t B, int64_t L, int64_t V, int draft) {
   l.ranges = ranges_of(B, L, V, draft, ends);
   cut(V, B * ends[0] * (L && draft ? 2 : 1), 32, l.splits, l.chunk);
   cut(V, B, 128, l.pieces, l.piece);
+  // Few logits: 64-bit sums of all rows cost less than another launch (one stream's 16 tokens of 150144: 26 us, with
+  // total_kernel 30)
+  l.exact = L > 0 && l.ranges == 1 && B * (L + 1 + (draft ? L : 0)) * V <= kFew && l.chunk <= kHeld * 2048;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t r = at;
@@ -632,7 +713,7 @@ static void launch(Args a, hipStream_t st) {
       stats_kernel<DT><<<(unsigned)((int64_t)a.splits * (a.draft ? 2 : 1) * a.B * (a.t1 - a.t0)), 256, 0, st>>>(a);
     }
     --a.range;
-    total_kernel<DT><<<all, 256, 0, st>>>(a);
+    if (!a.exact) total_kernel<DT><<<all, 256, 0, st>>>(a);
   } else {
     sample_kernel<DT><<<all, 256, 0, st>>>(a);
   }
@@ -672,7 +753,7 @@ extern "C" int ksd_verify_draft(const void *target, const void *draft, int dtype
   spec::Args a{target, L ? draft : nullptr, target_b, target_t, draft_b, draft_t, tokens, uniforms, uniforms_wide, temperatures,
                temperature, lengths, out, accepted, (spec::Part *)(w + l.parts), (double *)(w + l.totals), (double *)(w + l.weights),
                (spec::Draw *)(w + l.draws), (int *)(w + l.refused), (int)B, (int)L, (int)V, l.splits,
-               l.chunk, l.pieces, l.piece, 0, 0, 0, 0};
+               l.chunk, l.pieces, l.piece, 0, 0, 0, 0, l.exact};
   hipStream_t st = (hipStream_t)stream;
   if (!grid_fits((int64_t)l.splits * 2 * B * (L + 1), 256) || !grid_fits(B * l.pieces, 256))
     return fail(KSD_EINVAL, "verify_draft: too many rows");

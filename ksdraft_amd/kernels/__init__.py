@@ -5,9 +5,13 @@ from .quant import GROUP_SIZE, SCALE_DTYPE, quantize_last_dim, dequantize_last_d
 from .linear import Int8Linear
 from .token_channel import TokenChannelLinear
 from .embedding import ScaledEmbedding
+from .adapters import adapter_linear
+from .dropout import Dropout
+from .speculate import sample_tokens, verify_draft
 
 __all__ = [
     "GROUP_SIZE", "SCALE_DTYPE",
     "quantize_last_dim", "dequantize_last_dim",
     "Int8Linear", "TokenChannelLinear", "ScaledEmbedding",
+    "adapter_linear", "Dropout", "sample_tokens", "verify_draft",
 ]

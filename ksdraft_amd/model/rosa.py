@@ -132,9 +132,10 @@ class RosaMixer(nn.Module):
     def _out(self, hard: torch.Tensor, residual: torch.Tensor | None) -> torch.Tensor:
         from ..kernels.linear import Int8Linear
         from ..kernels.token_channel import TokenChannelLinear
+        from .adapters import AdaptedLinear
         if residual is None:
             return self.out_proj(hard)
-        if isinstance(self.out_proj, (Int8Linear, TokenChannelLinear)):
+        if isinstance(self.out_proj, (Int8Linear, TokenChannelLinear, AdaptedLinear)):
             return self.out_proj(hard, residual=residual)
         return residual + self.out_proj(hard)
 
