@@ -133,6 +133,7 @@ struct PairArgs {
   int n, r, rows, cols;    // rows and columns (a multiple of 64) of a workgroup
   Mask mask;
   int mask_x, mask_y;
+  int odd_x, odd_y;        // 16-bit rows of x or a, of base or y, may begin on an odd half word
   const int32_t *order;    // tokens listed by adapter, and the pieces of the lists (NULL: rows as they lie)
   const Slot *slots;
   int tiles;               // workgroups of a piece
@@ -154,6 +155,52 @@ __device__ __forceinline__ typename Oct<DT>::V whole_oct(const typename Elem<DT>
   return ((const Any *)(row + c))->v;
 }
 
+// 8 values of 16 bits of a row that may begin on an odd half word: 16 bytes from the word that holds the first one, and
+// the word behind them, moved together once they are used. (A 16-byte load on an odd half word takes several times
+// as long: 2047 rows of 6869 columns 31.8 us in such loads and stores, of 6870 21.5.)
+template <int DT> struct Held {
+  typename Oct<DT>::V v;
+  uint32_t e;
+};
+template <int DT, bool ODD>
+__device__ __forceinline__ void hold(Held<DT> &h, const typename Elem<DT>::T *row, int64_t c) {
+  if constexpr (ODD && DT != KSD_F32) {
+    const uintptr_t at = (uintptr_t)(row + c), word = at & ~(uintptr_t)3;
+    h.v = *(const typename Oct<DT>::V __attribute__((aligned(4))) *)word;
+    h.e = *(const uint32_t *)(word + (at & 2 ? 16 : 12));
+  } else {
+    h.v = whole_oct<DT>(row, c);
+  }
+}
+template <int DT, bool ODD>
+__device__ __forceinline__ typename Oct<DT>::V held(const Held<DT> &h, const typename Elem<DT>::T *row, int64_t c) {
+  if constexpr (ODD && DT != KSD_F32) {
+    const uint32_t by = ((uintptr_t)(row + c) & 2) * 8;
+    const u32x4 w = __builtin_bit_cast(u32x4, h.v);
+    return __builtin_bit_cast(typename Oct<DT>::V, u32x4{__builtin_amdgcn_alignbit(w.y, w.x, by), __builtin_amdgcn_alignbit(w.z, w.y, by),
+                                                         __builtin_amdgcn_alignbit(w.w, w.z, by), __builtin_amdgcn_alignbit(h.e, w.w, by)});
+  } else {
+    return h.v;
+  }
+}
+template <int DT>
+__device__ __forceinline__ void put_oct(typename Elem<DT>::T *row, int64_t c, const typename Oct<DT>::V &v, bool odd) {
+  struct __attribute__((packed, aligned(sizeof(typename Elem<DT>::T)))) Any { typename Oct<DT>::V v; };
+  if constexpr (DT != KSD_F32) {
+    if (odd && ((uintptr_t)(row + c) & 2)) {
+      typedef uint32_t u32x3 __attribute__((ext_vector_type(3)));
+      struct __attribute__((packed, aligned(4))) Three { u32x3 v; };
+      const u32x4 w = __builtin_bit_cast(u32x4, v);
+      row[c] = (uint16_t)w.x;
+      ((Three *)(row + c + 1))->v = u32x3{__builtin_amdgcn_alignbit(w.y, w.x, 16), __builtin_amdgcn_alignbit(w.z, w.y, 16),
+                                          __builtin_amdgcn_alignbit(w.w, w.z, 16)};
+      row[c + 7] = (uint16_t)(w.w >> 16);
+      return;
+    }
+  }
+  ((Any *)(row + c))->v = v;
+}
+
 // The dropped ones of 8 values become 0; the kept ones stay as they are (fp32: are scaled). 16-bit values would be
 // rounded by the scale, which their sums take instead.
 template <int DT>
@@ -169,19 +216,39 @@ __device__ __forceinline__ void drop_oct(const Mask &m, uint4 bits, typename Oct
 
 // U steps of 32 columns of the narrow product. Rows of other adapters and ranks from r on are read from a
 // row that exists: their results are not used. `whole`: no step passes the row's end.
-template <int DT, int R16, int RT, int U, bool MASK>
+template <int DT, int R16, int RT, int U, bool MASK, bool ODD>
 __device__ __forceinline__ void narrow(const PairArgs &p, const typename Elem<DT>::T *const (&xr)[RT],
                                        const typename Elem<DT>::T *const (&ar)[R16], int64_t s, bool whole, MaskKey key,
                                        const int64_t (&row)[RT], int grp, f32x4 (&acc)[RT][R16]) {
   using V = typename Oct<DT>::V;
   V xv[U][RT], av[U][R16];
+  if (whole) {
+    Held<DT> xh[U][RT], ah[U][R16];
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int64_t k = (s + u) * 32 + grp * 8;
+    for (int u = 0; u < U; ++u) {
+      const int64_t k = (s + u) * 32 + grp * 8;
 #pragma unroll
-    for (int t = 0; t < RT; ++t) xv[u][t] = whole ? whole_oct<DT>(xr[t], k) : load_oct<DT>(xr[t], k, p.K);
+      for (int t = 0; t < RT; ++t) hold<DT, ODD>(xh[u][t], xr[t], k);
 #pragma unroll
-    for (int q = 0; q < R16; ++q) av[u][q] = whole ? whole_oct<DT>(ar[q], k) : load_oct<DT>(ar[q], k, p.K);
+      for (int q = 0; q < R16; ++q) hold<DT, ODD>(ah[u][q], ar[q], k);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t k = (s + u) * 32 + grp * 8;
+#pragma unroll
+      for (int t = 0; t < RT; ++t) xv[u][t] = held<DT, ODD>(xh[u][t], xr[t], k);
+#pragma unroll
+      for (int q = 0; q < R16; ++q) av[u][q] = held<DT, ODD>(ah[u][q], ar[q], k);
+    }
+  } else {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t k = (s + u) * 32 + grp * 8;
+#pragma unroll
+      for (int t = 0; t < RT; ++t) xv[u][t] = load_oct<DT>(xr[t], k, p.K);
+#pragma unroll
+      for (int q = 0; q < R16; ++q) av[u][q] = load_oct<DT>(ar[q], k, p.K);
+    }
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -225,13 +292,17 @@ __device__ __forceinline__ typename Oct<DT>::V bank_oct(const typename Elem<DT>:
   return w;
 }
 
-// R16: blocks of 16 ranks; RT: blocks of 16 rows.
-template <int DT, int R16, int RT, bool MASK, bool ALIGNED>
+// R16: blocks of 16 ranks; RT: blocks of 16 rows. KIND: kPlain; kOdd: 16-bit rows may begin on an odd half word; kAnyRank:
+// that, and a rank that is no multiple of a lane's. Each in registers of its own: with odd rows' code 8192 plain rows of 1536
+// take 21.6 us for 19.3.
+constexpr int kPlain = 0, kOdd = 1, kAnyRank = 2;
+template <int DT, int R16, int RT, bool MASK, int KIND>
 __global__ __launch_bounds__(64 * kWaves) void pair_kernel(const PairArgs p) {
   using T = typename Elem<DT>::T;
   using V = typename Oct<DT>::V;
   constexpr int R = 16 * R16, U = DT == KSD_F32 ? (R16 <= 1 ? 4 : R16 <= 2 ? 2 : 1) : (R16 <= 1 ? 6 : R16 <= 2 ? 4 : 2);
   constexpr int TB = R16 <= 2 ? 4 : R16 == 4 ? 2 : 1;  // products whose bank rows are loaded together
+  constexpr bool kMayBeOdd = DT != KSD_F32 && KIND != kPlain;
   constexpr bool kAhead = R16 == 1;  // the next bank rows are loaded during a block's products: more ranks, no registers for it
   constexpr int pitch = R + 4;  // floats: a row's four lanes of 16 bytes start 4 banks further than the last row's
   extern __shared__ float lds[];  // (kWaves, 16 RT, pitch): sums of a wave's columns; the first holds h
@@ -262,7 +333,7 @@ __global__ __launch_bounds__(64 * kWaves) void pair_kernel(const PairArgs p) {
 
   const int64_t n0 = (int64_t)blockIdx.y * p.cols, n1 = min(p.N, n0 + p.cols);
   // base of a block of 64 columns: 16 of them per lane
-  const auto load_base = [&](int64_t c, V (&v)[RT][2]) {
+  const auto load_base = [&](int64_t c, Held<DT> (&v)[RT][2]) {
     const bool whole = c + 64 <= p.N;
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
@@ -270,11 +341,13 @@ __global__ __launch_bounds__(64 * kWaves) void pair_kernel(const PairArgs p) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int64_t at = c + e * 32 + grp * 8;
-        v[t][e] = whole ? whole_oct<DT>(row, at) : load_oct<DT>(row, at, p.N);
+        if (!whole) v[t][e].v = load_oct<DT>(row, at, p.N);
+        else if (kMayBeOdd && p.odd_y) hold<DT, true>(v[t][e], row, at);
+        else hold<DT, false>(v[t][e], row, at);
       }
     }
   };
-  V bv[RT][2] = {};
+  Held<DT> bv[RT][2] = {};
   int64_t c = n0 + wave * 64;
   const bool wide = p.y && p.phase != 1, based = p.base && wide;
   if (based && c < n1) load_base(c, bv);
@@ -287,7 +360,7 @@ __global__ __launch_bounds__(64 * kWaves) void pair_kernel(const PairArgs p) {
     for (int t = 0; t < TB; ++t) {
       const int64_t n = c + (t0 + t) / 2 * 32 + (col >> 2) * 8 + (t0 + t) % 2 * 4 + (col & 3);
 #pragma unroll
-      for (int q = 0; q < R16; ++q) w[t][q] = bank_oct<DT, ALIGNED>(b + (whole ? n : min(n, p.N - 1)) * p.r, q, grp, p.r);
+      for (int q = 0; q < R16; ++q) w[t][q] = bank_oct<DT, KIND != kAnyRank>(b + (whole ? n : min(n, p.N - 1)) * p.r, q, grp, p.r);
     }
   };
   const auto lowest = [&](uint64_t rows) { return __shfl(mine, __builtin_ctzll(rows)); };
@@ -326,11 +399,16 @@ __global__ __launch_bounds__(64 * kWaves) void pair_kernel(const PairArgs p) {
       for (int q = 0; q < R16; ++q) ar[q] = a + (int64_t)min(q * 16 + col, p.r - 1) * p.K;
       f32x4 acc[RT][R16] = {};
       int64_t s = from;
-      for (; s + U <= upto; s += U) narrow<DT, R16, RT, U, MASK>(p, xr, ar, s, true, key, at_row, grp, acc);
-      if constexpr (U > 2) {
-        for (; s + 2 <= upto; s += 2) narrow<DT, R16, RT, 2, MASK>(p, xr, ar, s, true, key, at_row, grp, acc);
+      if (kMayBeOdd && p.odd_x) {
+        constexpr int O = U > 2 ? U / 2 : 1;
+        for (; s + O <= upto; s += O) narrow<DT, R16, RT, O, MASK, true>(p, xr, ar, s, true, key, at_row, grp, acc);
+      } else {
+        for (; s + U <= upto; s += U) narrow<DT, R16, RT, U, MASK, false>(p, xr, ar, s, true, key, at_row, grp, acc);
+        if constexpr (U > 2) {
+          for (; s + 2 <= upto; s += 2) narrow<DT, R16, RT, 2, MASK, false>(p, xr, ar, s, true, key, at_row, grp, acc);
+        }
       }
-      for (; s < to; ++s) narrow<DT, R16, RT, 1, MASK>(p, xr, ar, s, s < full, key, at_row, grp, acc);
+      for (; s < to; ++s) narrow<DT, R16, RT, 1, MASK, false>(p, xr, ar, s, s < full, key, at_row, grp, acc);
       float scale = p.scales ? p.scales[i] : 1.0f;
       if constexpr (MASK && DT != KSD_F32) scale *= p.mask_x ? p.mask.scale : 1.0f;
 #pragma unroll
@@ -416,7 +494,7 @@ __global__ __launch_bounds__(64 * kWaves) void pair_kernel(const PairArgs p) {
   }
   for (; c < n1; c += 64 * kWaves) {
     const bool whole = c + 64 <= p.N;
-    V next[RT][2] = {};
+    Held<DT> next[RT][2] = {};
     if (based && c + 64 * kWaves < n1) load_base(c + 64 * kWaves, next);
     f32x4 acc[RT][4] = {};
     for (uint64_t left = with; left;) {
@@ -472,17 +550,14 @@ __global__ __launch_bounds__(64 * kWaves) void pair_kernel(const PairArgs p) {
           if (p.mask_y) apply_mask(p.mask, mask_bits(p.mask, key, m, (uint32_t)(at >> 3)), f);
         }
         if (based) {
-          to_floats<DT>(bv[u][v], g);
+          const T *const row = (const T *)p.base + at_row[u] * p.base_stride;
+          to_floats<DT>(kMayBeOdd && p.odd_y && whole ? held<DT, true>(bv[u][v], row, at) : bv[u][v].v, g);
 #pragma unroll
           for (int j = 0; j < 8; ++j) f[j] = of[u] >= 0 ? f[j] + g[j] : g[j];
         }
         if (u * 16 + col < rows) {
-          if (whole) {
-            struct __attribute__((packed, aligned(sizeof(T)))) Any { V v; };
-            ((Any *)(out + at))->v = from_floats<DT>(f);
-          } else {
-            store_oct<DT>(out, at, p.N, f);
-          }
+          if (whole) put_oct<DT>(out, at, from_floats<DT>(f), kMayBeOdd && p.odd_y);
+          else store_oct<DT>(out, at, p.N, f);
         }
       }
     }
@@ -491,28 +566,37 @@ __global__ __launch_bounds__(64 * kWaves) void pair_kernel(const PairArgs p) {
   }
 }
 
-template <int DT, int R16, int RT, bool MASK, bool ALIGNED>
+static bool aligned_rank(int64_t r, int dtype) { return r % (dtype == KSD_F32 ? 4 : 8) == 0; }
+
+template <int DT, int R16, int RT, bool MASK, int KIND>
 static void launch_pair(const PairArgs &p, unsigned tiles, hipStream_t st) {
   const dim3 g(tiles, (unsigned)(p.phase == 1 ? p.splits : cdiv(p.N, p.cols)));
   constexpr int lds = kWaves * 16 * RT * (16 * R16 + 4) * 4;
   if constexpr (lds > 65536) {  // past HIP's default
-    static const hipError_t set = hipFuncSetAttribute((const void *)pair_kernel<DT, R16, RT, MASK, ALIGNED>,
+    static const hipError_t set = hipFuncSetAttribute((const void *)pair_kernel<DT, R16, RT, MASK, KIND>,
                                                       hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     (void)set;
   }
-  pair_kernel<DT, R16, RT, MASK, ALIGNED><<<g, 64 * kWaves, lds, st>>>(p);
+  pair_kernel<DT, R16, RT, MASK, KIND><<<g, 64 * kWaves, lds, st>>>(p);
 }
 template <int DT, int R16, int RT>
 static void launch_pair(const PairArgs &p, bool mask, unsigned tiles, hipStream_t st) {
   if constexpr (RT == 1) {
-    if (p.r % (DT == KSD_F32 ? 4 : 8)) {
-      if (mask) launch_pair<DT, R16, RT, true, false>(p, tiles, st);
-      else launch_pair<DT, R16, RT, false, false>(p, tiles, st);
+    if (!aligned_rank(p.r, DT)) {
+      if (mask) launch_pair<DT, R16, RT, true, kAnyRank>(p, tiles, st);
+      else launch_pair<DT, R16, RT, false, kAnyRank>(p, tiles, st);
       return;
     }
+    if constexpr (DT != KSD_F32) {
+      if (p.odd_x || p.odd_y) {
+        if (mask) launch_pair<DT, R16, RT, true, kOdd>(p, tiles, st);
+        else launch_pair<DT, R16, RT, false, kOdd>(p, tiles, st);
+        return;
+      }
+    }
   }
-  if (mask) launch_pair<DT, R16, RT, true, true>(p, tiles, st);
-  else launch_pair<DT, R16, RT, false, true>(p, tiles, st);
+  if (mask) launch_pair<DT, R16, RT, true, kPlain>(p, tiles, st);
+  else launch_pair<DT, R16, RT, false, kPlain>(p, tiles, st);
 }
 template <int DT>
 static void launch_pair(const PairArgs &p, bool mask, unsigned tiles, hipStream_t st) {
@@ -529,12 +613,13 @@ static void launch_pair(const PairArgs &p, bool mask, unsigned tiles, hipStream_
 // workgroups are left (8192 tokens: 18.6 us, with 16 rows 19.2; rank 64: 33 and 45). Columns are shared out where
 // fewer workgroups than CUs would run, each part forming h again: not where that is the longer product (2047 tokens,
 // 6869 to 1792: 43 us, in two parts 69; 1792 to 6869: 54 us, in 4 parts 47).
-static void shape(PairArgs &p, bool lists, bool aligned) {
+static void shape(PairArgs &p, bool lists, bool plain) {
   if (!lists && p.n > 1 && p.per < 16) p.rows = (int)std::max<int64_t>(1, std::min<int64_t>(16, cdiv(p.M, 1024)));
-  else p.rows = p.M <= 64 ? 1 : p.M <= 256 ? 4 : p.M <= 512 ? 8 : p.M >= 8192 && p.r <= 64 && aligned ? 32 : 16;
+  else p.rows = p.M <= 64 ? 1 : p.M <= 256 ? 4 : p.M <= 512 ? 8 : p.M >= 8192 && p.r <= 64 && plain ? 32 : 16;
   if (lists)
     while (kTile % p.rows) --p.rows;
   const int64_t tiles = std::max<int64_t>(1, cdiv(p.M, p.rows)), blocks = cdiv(p.N, 64);
+  // (the workspace is sized by splits, which `plain` leaves alone: from 8192 rows on there are none)
   // a long narrow product of few rows goes to several workgroups first (2047 tokens, 6869 to 1792: 44 us, so 34; one
   // token 24 and 13), whose sums the wide product's add
   p.splits = p.K >= 4096 && tiles < 256 ? 4 : 0;
@@ -674,10 +759,10 @@ __global__ __launch_bounds__(256) void grad_kernel(const GradArgs p) {
   const T *const z = (const T *)(of_a ? p.x : p.g);
   const float *const q = of_a ? p.gh : p.h;
   const int r0 = blockIdx.z * 64;
-  const bool masked = of_a && p.masked;
+  const bool masked = of_a && p.masked, odd = DT != KSD_F32 && ((uintptr_t)z & 3 || stride & 1);
   const MaskKey key = p.masked ? mask_key(p.mask) : MaskKey{};
   struct Step {
-    V z[4];
+    Held<DT> z[4];
     float p[4][RB];
     int m[4];
   };
@@ -687,8 +772,12 @@ __global__ __launch_bounds__(256) void grad_kernel(const GradArgs p) {
       const bool in = m0 + u * 4 + grp < s.to;
       const int64_t m = p.order[in ? m0 + u * 4 + grp : s.from];
       o.m[u] = (int)m;
-      o.z[u] = V{};
-      if (in) o.z[u] = whole ? whole_oct<DT>(z + m * stride, c) : load_oct<DT>(z + m * stride, c, width);
+      o.z[u] = Held<DT>{};
+      if (in) {
+        if (!whole) o.z[u].v = load_oct<DT>(z + m * stride, c, width);
+        else if (odd) hold<DT, true>(o.z[u], z + m * stride, c);
+        else hold<DT, false>(o.z[u], z + m * stride, c);
+      }
 #pragma unroll
       for (int b = 0; b < RB; ++b) {
         const int rank = r0 + b * 16 + col;
@@ -705,7 +794,7 @@ __global__ __launch_bounds__(256) void grad_kernel(const GradArgs p) {
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       float f[8];
-      to_floats<DT>(now.z[u], f);
+      to_floats<DT>(odd && whole ? held<DT, true>(now.z[u], z + now.m[u] * stride, c) : now.z[u].v, f);
       if (masked) apply_mask(p.mask, mask_bits(p.mask, key, now.m[u], (uint32_t)(c >> 3)), f);
 #pragma unroll
       for (int b = 0; b < RB; ++b)
@@ -796,7 +885,6 @@ static Groups groups(int64_t M, int64_t n) {
 static bool by_lists(int64_t M, int64_t K, int64_t N, int64_t r, int64_t n, int64_t per, int dtype) {
   return n > 1 && per < 16 && M > 64 && M * r * (K + N) * size_of(dtype) > (32 << 20);
 }
-static bool aligned_rank(int64_t r, int dtype) { return r % (dtype == KSD_F32 ? 4 : 8) == 0; }
 
 // The workspace of a forward pass: lists, then the narrow product's parts.
 struct Forward {
@@ -838,7 +926,11 @@ static bool fits(int64_t M, int64_t K, int64_t N, int64_t r, int64_t n) {
 
 static int run_pair(const PairArgs &args, int dtype, bool mask, hipStream_t st) {
   PairArgs p = args;
-  shape(p, p.slots != nullptr, aligned_rank(p.r, dtype));
+  if (dtype != KSD_F32) {
+    p.odd_x = (((uintptr_t)p.x | (uintptr_t)p.a) & 3) != 0 || ((p.x_stride | p.K) & 1);
+    p.odd_y = (((uintptr_t)p.base | (uintptr_t)p.y) & 3) != 0 || ((p.base_stride | p.N) & 1);
+  }
+  shape(p, p.slots != nullptr, aligned_rank(p.r, dtype) && !p.odd_x && !p.odd_y);
   int64_t tiles = cdiv(p.M, p.rows);
   if (p.slots) {
     p.tiles = kTile / p.rows;
@@ -906,7 +998,7 @@ extern "C" int ksd_adapter_linear(const void *x, int dtype, int64_t M, int64_t K
   hipStream_t st = (hipStream_t)stream;
   char *const w = (char *)workspace;
   PairArgs p{x, x_stride, M, K, N, a, b, index, index_wide, rows_per_index, scales, base, base_stride, y, hidden,
-             (int)n, (int)r, 0, 0, m, 1, 0, nullptr, nullptr, 1, 0, 0, (float *)(w + l.sums)};
+             (int)n, (int)r, 0, 0, m, 1, 0, 0, 0, nullptr, nullptr, 1, 0, 0, (float *)(w + l.sums)};
   if (l.lists) {
     const GroupArgs g = group_args(index, index_wide, rows_per_index, M, K, N, n, w);
     group_kernel<<<(unsigned)(n + 1), 1024, 0, st>>>(g);
@@ -965,7 +1057,7 @@ extern "C" int ksd_adapter_linear_backward(const void *g, int dtype, int64_t M, 
   if (dtype == KSD_F32) launch_prepare<uint32_t>(a, w + l.at, b, w + l.bt, n, r, K, N, !lists && da, ga, st);
   else launch_prepare<uint16_t>(a, w + l.at, b, w + l.bt, n, r, K, N, !lists && da, ga, st);
   PairArgs p{g, g_stride, M, N, K, w + l.bt, w + l.at, index, index_wide, rows_per_index, scales, base, base_stride, dx, gh,
-             (int)n, (int)r, 0, 0, m, 0, 1, nullptr, nullptr, 1, 0, 0, (float *)(w + l.sums)};
+             (int)n, (int)r, 0, 0, m, 0, 1, 0, 0, nullptr, nullptr, 1, 0, 0, (float *)(w + l.sums)};
   if (lists) p.order = ga.order, p.slots = ga.tiles;
   const int rc = run_pair(p, dtype, drop > 0, st);
   if (rc || !da) return rc;
