@@ -623,7 +623,10 @@ static void shape(PairArgs &p, bool lists, bool plain) {
   // a long narrow product of few rows goes to several workgroups first (2047 tokens, 6869 to 1792: 44 us, so 34; one
   // token 24 and 13), whose sums the wide product's add
   p.splits = p.K >= 4096 && tiles < 256 ? 4 : 0;
-  const int64_t parts = std::min({blocks / 6, cdiv(blocks < 64 ? 256 : 512, tiles), p.splits ? blocks : 4 * p.N / p.K});
+  // more parts where a row is long; not under a mask, which each part makes again (a train call of 2047 tokens of 1792 to
+  // 6869: 105 us with 256 workgroups, 107 with 512, 109 with 128)
+  const int64_t want = blocks < 64 || (p.mask_x && p.mask.drop) ? 256 : 512;
+  const int64_t parts = std::min({blocks / 6, cdiv(want, tiles), p.splits ? blocks : 4 * p.N / p.K});
   p.cols = (int)(cdiv(blocks, std::max<int64_t>(1, parts)) * 64);
 }
 
@@ -708,27 +711,36 @@ __device__ __forceinline__ void list_tokens(const GroupArgs &a, int i) {
 __global__ __launch_bounds__(1024) void group_kernel(const GroupArgs a) { list_tokens(a, blockIdx.x); }
 
 // ------------------------------------------------------------------------------- the adapters' gradients
-// out[i][c][r] = in[i][r][c] of 16- or 32-bit values, tiles of 32 x 32.
+// A bank the other way round: (r, width) to (width, r) or back, `cols` columns of all ranks at a time, whose (cols, r) side
+// is one run of memory. (48 adapters of rank 8, 1752 to 5504, fp32: 48 us in tiles of 32 x 32, three quarters of them empty.)
+constexpr int kTurn = 8192;  // values of a tile
+static int turn_cols(int64_t r) { return (int)std::min<int64_t>(4096, kTurn / r / 64 * 64); }
 template <typename T>
-__device__ __forceinline__ void turn(const T *__restrict__ in, T *__restrict__ out, int64_t rows, int64_t cols, unsigned block) {
-  __shared__ T tile[32][33];
-  const unsigned tr = (unsigned)((rows + 31) / 32), tc = (unsigned)((cols + 31) / 32);
-  const unsigned t = block % (tr * tc);
-  const int64_t i = block / (tr * tc), r0 = t / tc * 32, c0 = t % tc * 32;
-  const int y = threadIdx.x >> 5, x = threadIdx.x & 31;
-  in += i * rows * cols, out += i * rows * cols;
-  if (r0 + y < rows && c0 + x < cols) tile[y][x] = in[(r0 + y) * cols + c0 + x];
+__device__ __forceinline__ void turn(const T *__restrict__ in, T *__restrict__ out, int r, int64_t width, int cols, bool to_run,
+                                     unsigned block) {
+  __shared__ T tile[kTurn + 128];
+  const unsigned each = (unsigned)((width + cols - 1) / cols);
+  const int64_t i = block / each, c0 = (int64_t)(block % each) * cols;
+  const int n = (int)min((int64_t)cols, width - c0), pitch = cols + 1;
+  in += i * r * width, out += i * r * width;
+  for (int e = threadIdx.x; e < n * r; e += 1024) {
+    const int q = to_run ? e / n : e % r, c = to_run ? e % n : e / r;
+    tile[q * pitch + c] = in[to_run ? q * width + c0 + c : c0 * r + e];
+  }
   __syncthreads();
-  if (r0 + x < rows && c0 + y < cols) out[(c0 + y) * rows + r0 + x] = tile[x][y];
+  for (int e = threadIdx.x; e < n * r; e += 1024) {
+    const int q = to_run ? e % r : e / n, c = to_run ? e / r : e % n;
+    out[to_run ? c0 * r + e : q * width + c0 + c] = tile[q * pitch + c];
+  }
 }
 // What the backward pass starts with: both banks the other way round, and the lists where the forward made none.
 template <typename T>
 __global__ __launch_bounds__(1024) void prepare_kernel(const T *__restrict__ a, T *__restrict__ at, const T *__restrict__ b,
-                                                       T *__restrict__ bt, int64_t r, int64_t K, int64_t N, unsigned a_blocks,
-                                                       unsigned lists, const GroupArgs g) {
+                                                       T *__restrict__ bt, int r, int64_t K, int64_t N, int cols,
+                                                       unsigned a_blocks, unsigned lists, const GroupArgs g) {
   if (blockIdx.x < lists) list_tokens(g, blockIdx.x);
-  else if (blockIdx.x - lists < a_blocks) turn<T>(a, at, r, K, blockIdx.x - lists);
-  else turn<T>(b, bt, N, r, blockIdx.x - lists - a_blocks);
+  else if (blockIdx.x - lists < a_blocks) turn<T>(a, at, r, K, cols, true, blockIdx.x - lists);
+  else turn<T>(b, bt, r, N, cols, false, blockIdx.x - lists - a_blocks);
 }
 
 struct GradArgs {
@@ -849,6 +861,26 @@ __global__ __launch_bounds__(256) void join_kernel(const float *__restrict__ par
   else db[i * nb + e - na] = v;
 }
 
+// The same where an adapter has few slots: 1024 values a workgroup, slot after slot (48 adapters of 50 slots: 14 us in
+// the other form).
+__global__ __launch_bounds__(256) void join_few_kernel(const float *__restrict__ parts, const int2 *__restrict__ spans, int64_t na,
+                                                       int64_t nb, float *__restrict__ da, float *__restrict__ db) {
+  const int i = blockIdx.y;
+  const int2 s = spans[i];
+  const int64_t e0 = (int64_t)blockIdx.x * 1024 + threadIdx.x;
+  float v[4] = {};
+  for (int j = 0; j < s.y; ++j)
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (e0 + u * 256 < na + nb) v[u] += parts[(s.x + j) * (na + nb) + e0 + u * 256];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int64_t e = e0 + u * 256;
+    if (e < na) da[i * na + e] = v[u];
+    else if (e < na + nb) db[i * nb + e - na] = v[u];
+  }
+}
+
 static bool float_type(int t) { return t == KSD_F32 || t == KSD_BF16 || t == KSD_F16; }
 static int64_t size_of(int t) { return t == KSD_F32 ? 4 : 2; }
 
@@ -961,9 +993,18 @@ static void launch_grad(const GradArgs &q, dim3 grid, hipStream_t st) {
 template <typename T>
 static void launch_prepare(const void *a, void *at, const void *b, void *bt, int64_t n, int64_t r, int64_t K, int64_t N, bool lists,
                            const GroupArgs &g, hipStream_t st) {
-  const unsigned blocks = (unsigned)(n * cdiv(r, 32) * cdiv(K, 32)), lists_n = lists ? (unsigned)n + 1 : 0;
-  prepare_kernel<T><<<lists_n + blocks + (unsigned)(n * cdiv(r, 32) * cdiv(N, 32)), 1024, 0, st>>>(
-      (const T *)a, (T *)at, (const T *)b, (T *)bt, r, K, N, blocks, lists_n, g);
+  const int cols = turn_cols(r);
+  const unsigned blocks = (unsigned)(n * cdiv(K, cols)), lists_n = lists ? (unsigned)n + 1 : 0;
+  prepare_kernel<T><<<lists_n + blocks + (unsigned)(n * cdiv(N, cols)), 1024, 0, st>>>(
+      (const T *)a, (T *)at, (const T *)b, (T *)bt, (int)r, K, N, cols, blocks, lists_n, g);
+}
+static void launch_join(const float *parts, const int2 *spans, int64_t M, int64_t K, int64_t N, int64_t r, int64_t n, float *da,
+                        float *db, hipStream_t st) {
+  const int64_t each = r * (K + N);
+  if (M / piece_of(M, K, N) <= 4 * n)
+    join_few_kernel<<<dim3((unsigned)cdiv(each, 1024), (unsigned)n), 256, 0, st>>>(parts, spans, r * K, r * N, da, db);
+  else
+    join_kernel<<<dim3((unsigned)cdiv(each, 64), (unsigned)n), 256, 0, st>>>(parts, spans, r * K, r * N, da, db);
 }
 
 }  // namespace adp
@@ -1039,15 +1080,14 @@ extern "C" int ksd_adapter_linear_backward(const void *g, int dtype, int64_t M, 
     return fail(KSD_EINVAL, "adapter_linear_backward: short or misaligned workspace");
   const int64_t slots = M / piece_of(M, K, N) + n + 1, blocks_a = cdiv(K, 128), blocks_b = cdiv(N, 128), each = r * (K + N);
   if (slots > 65535 || !grid_fits(blocks_a + blocks_b, 256) || !grid_fits(cdiv(each, 64), 256) ||
-      !grid_fits(n * cdiv(r, 32) * (cdiv(K, 32) + cdiv(N, 32)) + n + 1, 1024))
+      !grid_fits(n * (cdiv(K, turn_cols(r)) + cdiv(N, turn_cols(r))) + n + 1, 1024))
     return fail(KSD_EINVAL, "adapter_linear_backward: too many tokens, columns or adapters");
   hipStream_t st = (hipStream_t)stream;
   char *const w = (char *)workspace;
   if (M == 0) {  // no slot has a token: zeros
     if (!da) return KSD_OK;
     group_kernel<<<(unsigned)(n + 1), 1024, 0, st>>>(group_args(index, index_wide, rows_per_index, M, K, N, n, w + l.groups));
-    join_kernel<<<dim3((unsigned)cdiv(each, 64), (unsigned)n), 256, 0, st>>>(
-        nullptr, (const int2 *)(w + l.groups + groups(M, n).spans), r * K, r * N, da, db);
+    launch_join(nullptr, (const int2 *)(w + l.groups + groups(M, n).spans), M, K, N, r, n, da, db, st);
     return check_launch("adapter_linear_backward");
   }
   const bool lists = f.lists;
@@ -1067,6 +1107,6 @@ extern "C" int ksd_adapter_linear_backward(const void *g, int dtype, int64_t M, 
   if (dtype == KSD_F32) launch_grad<KSD_F32>(q, grid, st);
   else if (dtype == KSD_BF16) launch_grad<KSD_BF16>(q, grid, st);
   else launch_grad<KSD_F16>(q, grid, st);
-  join_kernel<<<dim3((unsigned)cdiv(each, 64), (unsigned)n), 256, 0, st>>>(parts, ga.spans, r * K, r * N, da, db);
+  launch_join(parts, ga.spans, M, K, N, r, n, da, db, st);
   return check_launch("adapter_linear_backward");
 }
