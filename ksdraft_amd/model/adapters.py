@@ -102,7 +102,7 @@ class AdaptedLinear(nn.Module):
             return y + self._delta(x, a, b, index).to(y.dtype)
         if torch.is_grad_enabled() and (y.requires_grad or x.requires_grad or a.requires_grad or b.requires_grad):
             return self._delta(x, a, b, index, y)
-        return adapter_linear(x, a, b, index, self.adapter_scales, base=y, out=y if y.is_contiguous() else None)
+        return adapter_linear(x, a, b, index, self.adapter_scales, base=y)  # not into y: a hook of the base may hold it
 
     def _delta(self, x, a, b, index, base=None):
         p = self.dropout.p if self.training else 0.0

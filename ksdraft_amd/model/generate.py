@@ -53,5 +53,8 @@ def speculative_step(draft, target, tokens: torch.Tensor, length: int, uniforms:
     block, block_logits = draft_block(draft, tokens, length, first, temperatures, teacher_states)
     logits = target(torch.cat([tokens, block.to(tokens.dtype)], 1))
     logits = logits[0] if isinstance(logits, tuple) else logits
-    return verify_draft(logits[:, T - 1:], block, None if uniforms is None else uniforms[:, length:],
-                        draft_logits=block_logits.to(logits.dtype), temperatures=temperatures)
+    logits = logits[:, T - 1:]
+    if logits.dtype != block_logits.dtype:  # not one in the other's type: the block was drawn from its logits as they are
+        logits, block_logits = logits.float(), block_logits.float()
+    return verify_draft(logits, block, None if uniforms is None else uniforms[:, length:], draft_logits=block_logits,
+                        temperatures=temperatures)

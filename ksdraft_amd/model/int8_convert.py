@@ -28,10 +28,17 @@ from ..kernels.token_channel import TokenChannelLinear
 from .draft import KSDraftModel
 
 
+def _without_adapters(model: KSDraftModel) -> KSDraftModel:
+    from .adapters import adapted_layers
+    if adapted_layers(model):
+        raise ValueError("the model has adapters, which a conversion would drop: convert first, then add_adapters")
+    return model
+
+
 def to_int8(model: KSDraftModel, group: int = 128, nonlinear: str = "int8", *,
             trainable: bool = False, int8_embedding: bool = False,
             int8_injection: bool = False) -> KSDraftModel:
-    conv = copy.deepcopy(model)
+    conv = copy.deepcopy(_without_adapters(model))
     swapped = 0
     for block in conv.blocks:
         rosa = block.rosa
@@ -78,7 +85,7 @@ def to_token_channel(model: KSDraftModel, group: int = 128, nonlinear: str = "in
     groups of 128), the embedding a ScaledEmbedding on the head's weight (rows times
     embedding_scale), the FFNs trainable KS3Int8Cells as in ``to_int8``; norms, vectors and the
     injection stay float."""
-    conv = copy.deepcopy(model)
+    conv = copy.deepcopy(_without_adapters(model))
     swapped = 0
     for block in conv.blocks:
         for name in ("q_proj", "k_proj", "v_proj", "out_proj"):

@@ -7,7 +7,7 @@ import torch
 
 from ksdraft_amd.config import KSDraftConfig
 from ksdraft_amd.model import (AdaptedLinear, KSDraftModel, adapter_parameters, adapter_state_dict, add_adapters,
-                               select_adapters)
+                               select_adapters, to_int8, to_token_channel)
 from ksdraft_amd.model.adapters import AdapterSelection, adapted_layers
 from ksdraft_amd.train.adapter_step import AdapterTrainer
 
@@ -60,6 +60,9 @@ def test_refusals():
             add_adapters(m, **kwargs)
     with pytest.raises(ValueError):
         add_adapters(add_adapters(m, 1, 4), 1, 4)
+    for convert in (to_int8, to_token_channel):
+        with pytest.raises(ValueError):
+            convert(add_adapters(m, 1, 4))
     with pytest.raises(TypeError):
         AdaptedLinear(torch.nn.LayerNorm(8), 1, 4, AdapterSelection())
     with pytest.raises(ValueError):

@@ -181,6 +181,10 @@ def test_drafting():
     # the draft model verifies its own block whole: p = q
     again, all_in = verify_draft(rows_of(logits, rows), block, u[:, 4:], draft_logits=rows, temperatures=0.8)
     assert all_in.tolist() == [4, 4, 4] and torch.equal(again[:, :4], block)
+    # a target of another type: both as floats, q still what the block was drawn from
+    half = speculative_step(m, lambda s: base(s)[0].bfloat16(), t, 4, u, 0.8)
+    want = verify_draft(target.bfloat16().float(), block, u[:, 4:], draft_logits=rows, temperatures=0.8)
+    assert torch.equal(half[0], want[0]) and torch.equal(half[1], want[1])
     # greedily the tokens are the target's own, whatever is proposed
     with pytest.raises(ValueError):
         speculative_step(m, base, t[:1], 4, temperatures=0.0)  # three adapters, one sequence
