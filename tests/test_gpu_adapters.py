@@ -119,6 +119,49 @@ def test_sequences_and_many_rows(dtype):
     check_y(adapter_linear(*to(c, "x", "a", "b", "index", "scales", "base")), c)
 
 
+# tokens listed by adapter; a narrow product in parts; 32 rows a workgroup, with and without lists, at each block of ranks;
+# rows in parts of their columns; more adapters than tokens; odd widths of each
+FORMS = [(700, 300, 1000, 24, 5), (701, 301, 1001, 24, 5), (700, 301, 1000, 4, 200), (1500, 130, 515, 100, 3), (40, 4500, 130, 8, 2),
+         (300, 4097, 257, 16, 1), (130, 5000, 1793, 40, 3), (8200, 72, 136, 16, 1), (8200, 71, 135, 16, 1), (8200, 40, 72, 30, 1),
+         (8200, 40, 72, 64, 1), (9000, 130, 170, 16, 3), (9000, 131, 171, 33, 3), (70, 256, 1792, 16, 1), (100, 64, 6869, 7, 300),
+         (2, 5000, 3000, 16, 3)]
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("M,K,N,r,n", FORMS)
+def test_forms(M, K, N, r, n, dtype):
+    c = case(M, K, N, r, n, dtype, seed=M + r)
+    check_y(adapter_linear(*to(c, "x", "a", "b", "index", "scales", "base")), c)
+    backward_case(c, 0.2 if M % 2 else 0.0, seed=5, stream=M)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("offset", [1, 2, 3])
+def test_odd_addresses(dtype, offset):
+    """Tensors that begin on each half word, at even and odd widths."""
+    for K, N, r in ((64, 70, 8), (65, 71, 8), (64, 71, 3), (65, 70, 16)):
+        c = case(37, K, N, r, 3, dtype, seed=offset + K + N, none=True)
+        moved = {}
+        for k in ("x", "a", "b", "base"):
+            t = c[k]
+            room = torch.full((t.numel() + 8,), math.nan, dtype=t.dtype, device=DEV)
+            moved[k] = room[offset:offset + t.numel()].view(t.shape)
+            moved[k].copy_(t)
+        index, scales = to(c, "index", "scales")
+        room = torch.full((37 * N + 8,), 7.0, dtype=c["x"].dtype, device=DEV)
+        out = room[offset:offset + 37 * N].view(37, N)
+        check_y(adapter_linear(moved["x"], moved["a"], moved["b"], index, scales, moved["base"], out=out), c)
+        assert bool((room[:offset] == 7).all()) and bool((room[offset + 37 * N:] == 7).all())
+        y, saved = adapter_linear_train(moved["x"], moved["a"], moved["b"], index, scales, moved["base"])
+        check_y(y, c)
+        room = torch.full((37 * N + 8,), math.nan, dtype=c["x"].dtype, device=DEV)
+        dy = room[offset:offset + 37 * N].view(37, N)
+        dy.copy_(c["dy"])
+        plain = adapter_linear_backward(c["dy"].to(DEV), saved)
+        for p, q in zip(adapter_linear_backward(dy, saved), plain):
+            assert torch.equal(p, q)
+
+
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 def test_an_adapter_is_its_own(dtype):
     """NaN and inf in one adapter, or one token, reach nobody else's rows."""

@@ -127,7 +127,7 @@ def test_against_definition(B, L, V, with_draft, dtype):
     both(target, tokens, u.double(), d)
 
 
-@pytest.mark.parametrize("dtype,V", [("bf16", 150144), ("fp16", 32003), ("fp32", 150144)])
+@pytest.mark.parametrize("dtype,V", [("bf16", 150144), ("fp16", 32003), ("fp32", 150144), ("bf16", 600001)])
 def test_long_rows(dtype, V):
     target, draft, tokens, u, temps = make(2, 3, V, dtype, 5)
     for d in (draft, None):
