@@ -296,11 +296,15 @@ __device__ __forceinline__ typename Oct<DT>::V bank_oct(const typename Elem<DT>:
 // that, and a rank that is no multiple of a lane's. Each in registers of its own: with odd rows' code 8192 plain rows of 1536
 // take 21.6 us for 19.3.
 constexpr int kPlain = 0, kOdd = 1, kAnyRank = 2;
+// Masked 16-bit rows run two workgroups a CU (4000 tokens of 1536 with dropout: 24.2 us, in the registers of one 29.1);
+// the others' registers do not allow it.
+template <int DT, int R16, int RT, bool MASK>
+constexpr bool kTwo = MASK && DT != KSD_F32 && RT == 1 && R16 == 1;
 template <int DT, int R16, int RT, bool MASK, int KIND>
-__global__ __launch_bounds__(64 * kWaves) void pair_kernel(const PairArgs p) {
+__global__ __launch_bounds__(64 * kWaves, (kTwo<DT, R16, RT, MASK> ? 4 : 2)) void pair_kernel(const PairArgs p) {
   using T = typename Elem<DT>::T;
   using V = typename Oct<DT>::V;
-  constexpr int R = 16 * R16, U = DT == KSD_F32 ? (R16 <= 1 ? 4 : R16 <= 2 ? 2 : 1) : (R16 <= 1 ? 6 : R16 <= 2 ? 4 : 2);
+  constexpr int R = 16 * R16, U = DT == KSD_F32 ? (R16 <= 1 ? 4 : R16 <= 2 ? 2 : 1) : (kTwo<DT, R16, RT, MASK> ? 3 : R16 <= 1 ? 6 : R16 <= 2 ? 4 : 2);
   constexpr int TB = R16 <= 2 ? 4 : R16 == 4 ? 2 : 1;  // products whose bank rows are loaded together
   constexpr bool kMayBeOdd = DT != KSD_F32 && KIND != kPlain;
   constexpr bool kAhead = R16 == 1;  // the next bank rows are loaded during a block's products: more ranks, no registers for it
