@@ -654,9 +654,12 @@ struct Layout {
   int splits, chunk, pieces, piece, ranges, exact;
   int64_t parts, totals, weights, draws, refused, bytes;
 };
-// Pieces of whole 2048 tokens (256 threads, 16 or 32 bytes each), enough of them to occupy the device a few times over.
-static void cut(int64_t V, int64_t rows, int64_t most, int &n, int &size) {
-  const int64_t want = std::min<int64_t>(cdiv(V, 2048), std::max<int64_t>(1, std::min<int64_t>(most, cdiv(2048, rows))));
+// Pieces of whole 2048 tokens (256 threads, 16 or 32 bytes each), about so many workgroups of them. The statistics' hold 7
+// a CU: 6 leave a launch without a second turn (64 streams, 16 drafted tokens of 150144 with their logits: 143 us at 4
+// pieces a row, 150 at 5, 154 at 6, 148 at 3, 166 at 2; 158 at 11).
+constexpr int64_t kStats = 6 * 256, kDraws = 8 * 256;
+static void cut(int64_t V, int64_t rows, int64_t groups, int64_t most, int &n, int &size) {
+  const int64_t want = std::min<int64_t>(cdiv(V, 2048), std::max<int64_t>(1, std::min<int64_t>(most, cdiv(groups, rows))));
   size = (int)(cdiv(cdiv(V, want), 2048) * 2048);
   n = (int)cdiv(V, size);
 }
@@ -681,8 +684,8 @@ static Layout layout(int64_t B, int64_t L, int64_t V, int draft) {
   Layout l;
   int ends[kRanges];
   l.ranges = ranges_of(B, L, V, draft, ends);
-  cut(V, B * ends[0] * (L && draft ? 2 : 1), 32, l.splits, l.chunk);
-  cut(V, B, 128, l.pieces, l.piece);
+  cut(V, B * ends[0] * (L && draft ? 2 : 1), kStats, 32, l.splits, l.chunk);
+  cut(V, B, kDraws, 128, l.pieces, l.piece);
   // Few logits: 64-bit sums of all rows cost less than another launch (one stream's 16 tokens of 150144: 26 us, with
   // total_kernel 30)
   l.exact = L > 0 && l.ranges == 1 && B * (L + 1 + (draft ? L : 0)) * V <= kFew && l.chunk <= kHeld * 2048;
