@@ -166,7 +166,8 @@ template <int DT, bool ODD>
 __device__ __forceinline__ void hold(Held<DT> &h, const typename Elem<DT>::T *row, int64_t c) {
   if constexpr (ODD && DT != KSD_F32) {
     const uintptr_t at = (uintptr_t)(row + c), word = at & ~(uintptr_t)3;
-    h.v = *(const typename Oct<DT>::V __attribute__((aligned(4))) *)word;
+    struct __attribute__((packed, aligned(4))) Word { typename Oct<DT>::V v; };
+    h.v = ((const Word *)word)->v;
     h.e = *(const uint32_t *)(word + (at & 2 ? 16 : 12));
   } else {
     h.v = whole_oct<DT>(row, c);
@@ -717,8 +718,12 @@ __global__ __launch_bounds__(1024) void group_kernel(const GroupArgs a) { list_t
 // ------------------------------------------------------------------------------- the adapters' gradients
 // A bank the other way round: (r, width) to (width, r) or back, `cols` columns of all ranks at a time, whose (cols, r) side
 // is one run of memory. (48 adapters of rank 8, 1752 to 5504, fp32: 48 us in tiles of 32 x 32, three quarters of them empty.)
-constexpr int kTurn = 8192;  // values of a tile
-static int turn_cols(int64_t r) { return (int)std::min<int64_t>(4096, kTurn / r / 64 * 64); }
+// Smaller tiles where few of the largest would run: 3 adapters of rank 8, 1792 to 6869, 5.9 us in 27 workgroups, 4.0 in 204.
+constexpr int kTurn = 8192;  // the most values of a tile
+static int turn_cols(int64_t n, int64_t r, int64_t K, int64_t N) {
+  const int64_t values = std::min<int64_t>(kTurn, std::max<int64_t>(1024, n * r * (K + N) / 256));
+  return (int)std::max<int64_t>(64, std::min<int64_t>(4096, values / r / 64 * 64));
+}
 template <typename T>
 __device__ __forceinline__ void turn(const T *__restrict__ in, T *__restrict__ out, int r, int64_t width, int cols, bool to_run,
                                      unsigned block) {
@@ -997,7 +1002,7 @@ static void launch_grad(const GradArgs &q, dim3 grid, hipStream_t st) {
 template <typename T>
 static void launch_prepare(const void *a, void *at, const void *b, void *bt, int64_t n, int64_t r, int64_t K, int64_t N, bool lists,
                            const GroupArgs &g, hipStream_t st) {
-  const int cols = turn_cols(r);
+  const int cols = turn_cols(n, r, K, N);
   const unsigned blocks = (unsigned)(n * cdiv(K, cols)), lists_n = lists ? (unsigned)n + 1 : 0;
   prepare_kernel<T><<<lists_n + blocks + (unsigned)(n * cdiv(N, cols)), 1024, 0, st>>>(
       (const T *)a, (T *)at, (const T *)b, (T *)bt, (int)r, K, N, cols, blocks, lists_n, g);
@@ -1083,8 +1088,9 @@ extern "C" int ksd_adapter_linear_backward(const void *g, int dtype, int64_t M, 
       (M > 0 && f.lists && (!forward_workspace || forward_bytes < f.sums || (uintptr_t)forward_workspace % 16)))
     return fail(KSD_EINVAL, "adapter_linear_backward: short or misaligned workspace");
   const int64_t slots = M / piece_of(M, K, N) + n + 1, blocks_a = cdiv(K, 128), blocks_b = cdiv(N, 128), each = r * (K + N);
+  const int64_t cols = turn_cols(n, r, K, N);
   if (slots > 65535 || !grid_fits(blocks_a + blocks_b, 256) || !grid_fits(cdiv(each, 64), 256) ||
-      !grid_fits(n * (cdiv(K, turn_cols(r)) + cdiv(N, turn_cols(r))) + n + 1, 1024))
+      !grid_fits(n * (cdiv(K, cols) + cdiv(N, cols)) + n + 1, 1024))
     return fail(KSD_EINVAL, "adapter_linear_backward: too many tokens, columns or adapters");
   hipStream_t st = (hipStream_t)stream;
   char *const w = (char *)workspace;
