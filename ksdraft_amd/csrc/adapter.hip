@@ -628,9 +628,9 @@ static void shape(PairArgs &p, bool lists, bool plain) {
   // a long narrow product of few rows goes to several workgroups first (2047 tokens, 6869 to 1792: 44 us, so 34; one
   // token 24 and 13), whose sums the wide product's add
   p.splits = p.K >= 4096 && tiles < 256 ? 4 : 0;
-  // more parts where a row is long; not under a mask, which each part makes again (a train call of 2047 tokens of 1792 to
-  // 6869: 105 us with 256 workgroups, 107 with 512, 109 with 128)
-  const int64_t want = blocks < 64 || (p.mask_x && p.mask.drop) ? 256 : 512;
+  // more parts where a row is long (a train call with dropout of 2047 tokens of 1792 to 6869: 88.8 us with 256 workgroups,
+  // 86.6 with 512)
+  const int64_t want = blocks < 64 ? 256 : 512;
   const int64_t parts = std::min({blocks / 6, cdiv(want, tiles), p.splits ? blocks : 4 * p.N / p.K});
   p.cols = (int)(cdiv(blocks, std::max<int64_t>(1, parts)) * 64);
 }
