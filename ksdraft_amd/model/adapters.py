@@ -100,7 +100,8 @@ class AdaptedLinear(nn.Module):
         a, b = self.adapter_a.to(x.dtype), self.adapter_b.to(x.dtype)
         if y.dtype != x.dtype:  # a residual of another type
             return y + self._delta(x, a, b, index).to(y.dtype)
-        if torch.is_grad_enabled() and (y.requires_grad or x.requires_grad or a.requires_grad or b.requires_grad):
+        if (self.training and self.dropout.p) or (torch.is_grad_enabled() and (
+                y.requires_grad or x.requires_grad or a.requires_grad or b.requires_grad)):
             return self._delta(x, a, b, index, y)
         return adapter_linear(x, a, b, index, self.adapter_scales, base=y)  # not into y: a hook of the base may hold it
 

@@ -10,7 +10,7 @@ from ksdraft_amd.kernels.dropout import dropout
 from ksdraft_amd.kernels.speculate import verify_draft
 from ksdraft_amd.model import (KSDraftModel, add_adapters, draft_block, select_adapters, speculative_step, to_int8,
                                to_token_channel)
-from ksdraft_amd.model.adapters import adapted_layers, adapter_parameters
+from ksdraft_amd.model.adapters import AdaptedLinear, AdapterSelection, adapted_layers, adapter_parameters
 from ksdraft_amd.train.adapter_step import AdapterTrainer
 from tests.philox import mask
 
@@ -209,3 +209,26 @@ def test_drafting():
 def rows_of(logits, rows):
     """The target's rows where the draft is its own target: the rows that the block was drawn from, then the next."""
     return torch.cat([rows, logits[:, -1:]], 1)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_training_mode_without_gradients(dtype):
+    """A layer in training mode drops with and without gradients: the same streams, the same bits."""
+    torch.manual_seed(1)
+    base = torch.nn.Linear(96, 80, device=DEV, dtype=dtype)
+    layers = [AdaptedLinear(base, 2, 8, AdapterSelection(), dropout=0.5, seed=3) for _ in range(2)]
+    layers[1].load_state_dict(layers[0].state_dict())
+    x = torch.randn(3, 5, 96, device=DEV, dtype=dtype)
+    for layer in layers:
+        layer.selection.index = torch.tensor([1, -1, 0], device=DEV)
+        torch.nn.init.normal_(layer.adapter_b, generator=torch.Generator(DEV).manual_seed(5))
+    y = layers[0](x)
+    with torch.no_grad():
+        z = layers[1](x)
+        assert layers[1].dropout.calls == layers[0].dropout.calls == 1
+        assert torch.equal(y, z) and not z.requires_grad
+        layers[1].eval()
+        assert not torch.equal(y, layers[1](x))
+        layers[1].train()
+        layers[1].dropout.p = 1.0
+        assert torch.equal(layers[1](x), base(x))
