@@ -215,8 +215,18 @@ def capture_guard(dev: torch.device, *tensors):
     """Called in the forward of an autograd function; what it returns is kept in ctx. torch ends the process
     (in the capture's end) where a backward pass is captured while an eager graph of the same leaf made on another
     stream lives: the leaf's accumulation node belongs to that stream. Captured calls on such leaves raise
-    instead, as far as the eager graph is of a function that calls this too."""
-    leaves = {id(t) for t in tensors if t is not None and t.requires_grad and t.is_leaf}
+    instead, as far as the eager graph is of a function that calls this too. A leaf brought to another type counts as
+    itself."""
+    leaves = set()
+    for t in tensors:
+        if t is None or not t.requires_grad:
+            continue
+        if t.is_leaf:
+            leaves.add(id(t))
+        elif type(t.grad_fn).__name__ == "ToCopyBackward0":
+            leaf = getattr(t.grad_fn.next_functions[0][0], "variable", None)
+            if leaf is not None:
+                leaves.add(id(leaf))
     if not leaves:
         return None
     stream = stream_ptr(dev)

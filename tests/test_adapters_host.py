@@ -66,3 +66,36 @@ def test_capture_guard(monkeypatch):
     del kept
     gc.collect()
     assert _lib.capture_guard(dev, q, p) is None
+
+
+def test_capture_guard_sees_through_a_cast(monkeypatch):
+    """Adapters kept in fp32 and used in 16 bits: the leaf is the fp32 one."""
+    import pytest
+    import torch
+    dev = torch.device("cpu")
+    at = dict(stream=1, capturing=False)
+    monkeypatch.setattr(_lib, "stream_ptr", lambda d: at["stream"])
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: at["capturing"])
+    seen = []
+
+    class Guarded(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, t):
+            ctx.guard = _lib.capture_guard(dev, t)
+            seen.append(ctx.guard)
+            return t * 2
+
+        @staticmethod
+        def backward(ctx, g):
+            return g * 2
+
+    p, q = (torch.zeros(2, requires_grad=True) for _ in range(2))
+    y = Guarded.apply(p.to(torch.bfloat16))
+    assert seen[0] is not None and seen[0].leaves == {id(p)}
+    at.update(stream=2, capturing=True)
+    Guarded.apply(q.to(torch.bfloat16))
+    with pytest.raises(RuntimeError):
+        Guarded.apply(p.to(torch.float16))
+    del y
+    seen.clear()
+    Guarded.apply(p.to(torch.float16))
