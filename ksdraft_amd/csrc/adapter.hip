@@ -11,7 +11,9 @@
 // waves split the contraction of the narrow product, their sums join in LDS, and the same waves then split the
 // columns of the wide one. h is never rounded on its way: it is fp32 in LDS and enters the 16-bit matrix
 // instructions as a rounded value and the rounding's rest, side by side along the contraction, which a rank of 16
-// leaves half empty anyway. What bounds it is memory: x and base read once, y written once.
+// leaves half empty anyway. What bounds it is memory: x and base read once, y written once. 8192 tokens of 1536 to 1536,
+// rank 16: bf16 19 us for 76 MB (3.9 TB/s), fp32 43 us for 151 MB (3.5; the narrow product alone 17, the wide one 24). Few
+// tokens take a launch's latency: one token 5.4 us, 64 of as many adapters 6.7.
 #include "ksd_random.h"
 
 #include <algorithm>
@@ -647,7 +649,8 @@ struct GroupArgs {
 };
 
 // Workgroup i lists adapter i's tokens, workgroup n those without one: 8192 tokens at a time, whose indices are
-// loaded together.
+// loaded together. Each counts all indices instead of waiting for another one's sum. (1021 tokens of 5 adapters 6.4 us, 8192
+// of one 8.3 with the turned banks: two passes of latency.)
 __device__ __forceinline__ void list_tokens(const GroupArgs &a, int i) {
   constexpr int U = 8;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -765,7 +768,8 @@ struct GradArgs {
 
 // A slot's sums over its tokens for 128 columns of dA or dB and 16 RB ranks: D[rank][column] = p^T z in fp32 matrix
 // instructions of 4 tokens, which read both operands as they lie in memory. A wave takes 16 tokens at a time and has
-// the next 16 on the way.
+// the next 16 on the way. Memory bounds it where adapters have many tokens (fp32, 8192 of 1536 and 1536, rank 16: 28 us for
+// 101 MB, 3.6 TB/s); in short pieces it is the two steps' latency (bf16, 2047 of 1792 and 6869, rank 8, masked: 18 us for 35).
 template <int DT, int RB>
 __global__ __launch_bounds__(256) void grad_kernel(const GradArgs p) {
   using T = typename Elem<DT>::T;

@@ -8,7 +8,9 @@ namespace ksd {
 namespace drop {
 
 // One thread per counter (8 values of a row). chunk / nb by the product with ceil(2^64 / nb), exact for
-// chunks and nb below 2^32.
+// chunks and nb below 2^32. Memory bounds it, with the generator's 20 wide products a counter behind the loads: bf16 8192 x
+// 1536 with a residual 16.0 us (4.7 TB/s), without 12.3 (4.1), where a large copy reaches 5.1. A thread needs nothing of
+// another one, so small tensors take one launch's time (17 rows 3.0 us).
 template <int DT, bool RES>
 __global__ __launch_bounds__(256) void dropout_kernel(const void *__restrict__ x, int64_t stride, const void *__restrict__ res,
                                                       int64_t res_stride, void *__restrict__ out, int64_t row0, uint32_t chunks,

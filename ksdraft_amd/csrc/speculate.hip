@@ -241,7 +241,10 @@ __device__ __forceinline__ int refused_in(const Args &a, int b, int from, int to
 
 // ------------------------------------------------------------------------------- row statistics
 // The rows of the positions [t0, t1). A long batch goes through its positions in several launches: a stream's rows
-// behind a refused token need not be read, and a launch knows what its predecessors' rows refuse.
+// behind a refused token need not be read, and a launch knows what its predecessors' rows refuse (64 streams, 48 of them
+// drawn, 16 drafted tokens of 150144 with their logits, 93% of them accepted: a whole call 185 us with one launch, 147 with
+// three, by 6 pieces a row). What bounds it is memory and a workgroup's start and end: the three launches take 97 us at 4
+// pieces a row, the first one's 101 MB 28.5 us, 3.5 TB/s.
 template <int DT>
 __global__ __launch_bounds__(256) void stats_kernel(const Args a) {
   // blocks: split fastest, then target and draft, then requests, then positions
@@ -369,7 +372,8 @@ __device__ __forceinline__ void find_draw(const Args &a, int b, float T, Draw &d
   __syncthreads();
 }
 
-// Without a draft there is nothing to test: a piece's largest logit and sum of powers in 64 bits at once.
+// Without a draft there is nothing to test: a piece's largest logit and sum of powers in 64 bits at once (150144 fp32
+// logits: 3.9 us, the latency of a launch that reads once).
 template <int DT>
 __global__ __launch_bounds__(256) void sample_kernel(const Args a) {
   const int b = blockIdx.x / a.pieces, piece = blockIdx.x % a.pieces;
@@ -403,7 +407,9 @@ __global__ __launch_bounds__(256) void sample_kernel(const Args a) {
   }
 }
 
-// Sums of e^((z - m) / T) in 64 bits of a piece of the row that is drawn from, target and draft.
+// Sums of e^((z - m) / T) in 64 bits of a piece of the row that is drawn from, target and draft. Each workgroup finds the
+// row for itself, a read of its stream's few statistics. (64 streams of 150144 tokens: 24 us, by count about a third of them
+// 64-bit arithmetic.)
 template <int DT>
 __global__ __launch_bounds__(256) void total_kernel(const Args a) {
   const int b = blockIdx.x / a.pieces, piece = blockIdx.x % a.pieces;
@@ -478,7 +484,8 @@ __device__ __forceinline__ void weights_of(const Args &a, int b, const Draw &d, 
   }
 }
 
-// Sums of the weights of a piece, where a draft row is subtracted (elsewhere total_kernel's sums are the weights).
+// Sums of the weights of a piece, where a draft row is subtracted (elsewhere total_kernel's sums are the weights). 64
+// streams of 150144 tokens: 21 us, the arithmetic of total_kernel again; powers kept in memory would be 16 bytes a token.
 template <int DT>
 __global__ __launch_bounds__(256) void weight_kernel(const Args a) {
   const int b = blockIdx.x / a.pieces, piece = blockIdx.x % a.pieces, lane = threadIdx.x & 63;
@@ -514,7 +521,8 @@ __global__ __launch_bounds__(256) void weight_kernel(const Args a) {
 // A workgroup finds a stream's drawn token and writes its row of the result. The running sum goes by piece (each wave
 // for itself), then by 8192 tokens of the piece, by thread and by token. In a launch of its own: a stream's last
 // workgroup of weight_kernel could do it, but the fence that every workgroup then needs writes its XCD's L2 back
-// (64 streams of 150144 tokens: 97 us, as two launches 27).
+// (64 streams of 150144 tokens: 97 us, as two launches 27). Alone it takes 11 us for 64 streams and 7 for one, the latency
+// of its steps.
 template <int DT>
 __global__ __launch_bounds__(1024) void draw_kernel(const Args a) {
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
