@@ -17,6 +17,7 @@
 #include "ksd_random.h"
 
 #include <algorithm>
+#include <atomic>
 
 namespace ksd {
 namespace adp {
@@ -579,10 +580,15 @@ template <int DT, int R16, int RT, bool MASK, int KIND>
 static void launch_pair(const PairArgs &p, unsigned tiles, hipStream_t st) {
   const dim3 g(tiles, (unsigned)(p.phase == 1 ? p.splits : cdiv(p.N, p.cols)));
   constexpr int lds = kWaves * 16 * RT * (16 * R16 + 4) * 4;
-  if constexpr (lds > 65536) {  // past HIP's default
-    static const hipError_t set = hipFuncSetAttribute((const void *)pair_kernel<DT, R16, RT, MASK, KIND>,
-                                                      hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    (void)set;
+  if constexpr (lds > 65536) {  // past HIP's default, once on each device
+    static std::atomic<uint64_t> known{0};
+    int dev = 0;
+    (void)hipGetDevice(&dev);
+    const uint64_t bit = 1ull << (dev & 63);
+    if (!(known.load(std::memory_order_relaxed) & bit)) {
+      (void)hipFuncSetAttribute((const void *)pair_kernel<DT, R16, RT, MASK, KIND>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+      known.fetch_or(bit, std::memory_order_relaxed);
+    }
   }
   pair_kernel<DT, R16, RT, MASK, KIND><<<g, 64 * kWaves, lds, st>>>(p);
 }
@@ -704,6 +710,7 @@ __device__ __forceinline__ void list_tokens(const GroupArgs &a, int i) {
     __syncthreads();  // the other half of counts is read until the next round's
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      if (base + u * 1024 >= a.M) break;
       int at = done;
 #pragma unroll
       for (int w = 0; w < 16; ++w) {
