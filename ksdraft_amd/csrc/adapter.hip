@@ -396,7 +396,7 @@ __global__ __launch_bounds__(64 * kWaves, (kTwo<DT, R16, RT, MASK> ? 4 : 2)) voi
     for (int t = 0; t < RT; ++t) xr[t] = (const T *)p.x + at_row[t] * p.x_stride;
     const int64_t steps = (p.K + 31) / 32, full = p.K / 32;
     const int waves = p.phase ? kWaves * p.splits : kWaves, mark = p.phase ? blockIdx.y * kWaves + wave : wave;
-    const int64_t share = ((steps + waves - 1) / waves + 1) & ~1ll;
+    const int64_t share = (steps + waves - 1) / waves;
     const int64_t from = mark * share, to = min(steps, from + share), upto = min(to, full);
     for (uint64_t left = with; left;) {
       const int i = __shfl(mine, __builtin_ctzll(left));
@@ -408,7 +408,7 @@ __global__ __launch_bounds__(64 * kWaves, (kTwo<DT, R16, RT, MASK> ? 4 : 2)) voi
       f32x4 acc[RT][R16] = {};
       int64_t s = from;
       if (kMayBeOdd && p.odd_x) {
-        constexpr int O = U > 2 ? U / 2 : 1;
+        constexpr int O = R16 == 2 ? 3 : (U + 1) / 2;  // a step's loads take one more register per operand
         for (; s + O <= upto; s += O) narrow<DT, R16, RT, O, MASK, true>(p, xr, ar, s, true, key, at_row, grp, acc);
       } else {
         for (; s + U <= upto; s += U) narrow<DT, R16, RT, U, MASK, false>(p, xr, ar, s, true, key, at_row, grp, acc);
