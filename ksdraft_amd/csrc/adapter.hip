@@ -655,7 +655,7 @@ struct GroupArgs {
 };
 
 // Workgroup i lists adapter i's tokens, workgroup n those without one: 8192 tokens at a time, whose indices are
-// loaded together. Each counts all indices instead of waiting for another one's sum. (1021 tokens of 5 adapters 6.4 us, 8192
+// loaded together. Each counts all indices instead of waiting for another one's sum. (1021 tokens of 5 adapters 5.8 us, 8192
 // of one 8.3 with the turned banks: two passes of latency.)
 __device__ __forceinline__ void list_tokens(const GroupArgs &a, int i) {
   constexpr int U = 8;
