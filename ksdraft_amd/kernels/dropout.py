@@ -105,7 +105,9 @@ def dropout(x: torch.Tensor, p: float, seed: int | torch.Tensor, stream: int = 0
 class Dropout(nn.Module):
     """nn.Dropout on ``dropout``: the n-th training call of a module takes stream n of its seed (drawn from
     torch's CPU generator unless given), so a run is repeated by its seeds. Under graph capture the captured
-    stream is part of the graph: a captured step passes a device seed to ``dropout`` itself."""
+    stream is part of the graph: a captured step passes a device seed to ``dropout`` itself. A forward pass that is run
+    again for its backward (recomputed activations) would take the next stream's mask; it names seed and stream to
+    ``dropout`` too. ``calls`` counts the streams and may be set, to go on where a run ended."""
 
     def __init__(self, p: float = 0.1, seed: int | None = None):
         super().__init__()

@@ -232,3 +232,33 @@ def test_training_mode_without_gradients(dtype):
         layers[1].train()
         layers[1].dropout.p = 1.0
         assert torch.equal(layers[1](x), base(x))
+
+
+@pytest.mark.parametrize("kind", ["float", "token_channel"])
+def test_an_adapter_for_each_token(kind):
+    """Indices (B, T), out of range for none, on layers of (B, T, K) and of flattened inputs."""
+    base = make()
+    m = adapted(base if kind == "float" else to_token_channel(base)).eval()
+    index = torch.randint(-1, 4, (3, 33), generator=torch.Generator().manual_seed(8))
+    select_adapters(m, index.to(DEV))
+    seen = []
+    for layer in adapted_layers(m):
+        layer.base.register_forward_hook(lambda mod, a, out, l=layer: seen.append((l, a[0].clone(), out.clone())))
+        layer.register_forward_hook(lambda mod, a, k, out: seen.append((mod, out.clone(), k.get("residual"))), with_kwargs=True)
+    with torch.no_grad():
+        m(tokens())
+    assert len(seen) == 2 * len(adapted_layers(m))
+    at = index.reshape(-1).to(DEV)
+    for (layer, x, y), (same, out, res) in zip(seen[::2], seen[1::2]):
+        assert layer is same
+        K, N, r = layer.in_features, layer.out_features, 8
+        want, size = y.double().reshape(-1, N), y.double().abs().reshape(-1, N)
+        if kind == "float" and res is not None:
+            want, size = want + res.double().reshape(-1, N), size + res.double().abs().reshape(-1, N)
+        xs = x.double().reshape(-1, K)
+        for i in range(3):
+            a, b, of = layer.adapter_a[i].double(), layer.adapter_b[i].double(), at == i
+            want[of] += xs[of] @ a.t() @ b.t()
+            size[of] += xs[of].abs() @ a.abs().t() @ b.abs().t()
+        err = (out.double().reshape(want.shape) - want).abs()
+        assert bool((err <= 2 * (K + r + 6) * U * size).all())

@@ -417,3 +417,30 @@ def test_refusals():
         adapter_linear_backward(base, saved, base=base)
     with pytest.raises(RuntimeError):
         adapter_linear(x.cpu(), a, b, index)
+
+
+@pytest.mark.parametrize("M", [70, 900])  # rows one by one, and by lists
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_autograd_layouts(M, dtype):
+    """Strided inputs, a broadcast gradient and a graph that is kept: the dense tensors' bits, twice."""
+    c = case(M, 1200, 1300, 8, 3, dtype, seed=21)
+    c["x"] = c["x"].reshape(2, M // 2, 1200)
+    c["base"] = c["base"].reshape(2, M // 2, 1300)
+    c["index"] = c["index"].reshape(2, M // 2)
+    x, a, b, index, scales, base = to(c, "x", "a", "b", "index", "scales", "base")
+
+    def run(x, a, b, base, index, w):
+        x, a, b, base = (t.detach().requires_grad_() for t in (x, a, b, base))
+        y = adapt(x, a, b, index, scales, base, 0.25, 5, 2)
+        first = torch.autograd.grad(y, (x, a, b, base), w, retain_graph=True)
+        again = torch.autograd.grad(y, (x, a, b, base), w)
+        assert all(torch.equal(p, q) for p, q in zip(first, again))
+        return (y.detach(), *first)
+    w = torch.randn(1300, generator=torch.Generator().manual_seed(2)).to(x.dtype).to(DEV).expand(2, M // 2, 1300)
+    want = run(x, a, b, base, index, w.contiguous())
+    flip = [t.transpose(0, 1).contiguous().transpose(0, 1) for t in (x, base, index)]
+    turned = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in (a, b)]
+    got = run(flip[0], *turned, flip[1], flip[2], w)
+    for p, q in zip(want, got):
+        assert torch.equal(p, q)
+    assert torch.equal(got[4], w)
