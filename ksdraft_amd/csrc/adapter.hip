@@ -626,13 +626,18 @@ static void launch_pair(const PairArgs &p, bool mask, unsigned tiles, hipStream_
 // workgroups are left (8192 tokens: 18.6 us, with 16 rows 19.2; rank 64: 33 and 45). Columns are shared out where
 // fewer workgroups than CUs would run, each part forming h again: not where that is the longer product (2047 tokens,
 // 6869 to 1792: 43 us, in two parts 69; 1792 to 6869: 54 us, in 4 parts 47).
+// Every workgroup reads its adapter's banks: ranks past 16 take more rows (400 tokens, 1536 to 4096, fp32, rank 64: 24.6 us,
+// in fewer rows 40.5), and large banks 32 rows from 4096 tokens on (6110 tokens, 5974 to 6862, rank 32: 122 us and 168;
+// 6000 tokens, 4096 to 4096, rank 16: 57.5 and 48.5).
 static void shape(PairArgs &p, bool lists, bool plain) {
+  const int64_t few = p.M * cdiv(p.r, 16);
+  const bool tall = p.M >= 8192 || (p.M >= 4096 && p.r * (p.K + p.N) >= 1 << 18);
   if (!lists && p.n > 1 && p.per < 16) p.rows = (int)std::max<int64_t>(1, std::min<int64_t>(16, cdiv(p.M, 1024)));
-  else p.rows = p.M <= 64 ? 1 : p.M <= 256 ? 4 : p.M <= 512 ? 8 : p.M >= 8192 && p.r <= 64 && plain ? 32 : 16;
+  else p.rows = few <= 64 ? 1 : few <= 256 ? 4 : few <= 512 ? 8 : tall && p.r <= 64 && plain ? 32 : 16;
   if (lists)
     while (kTile % p.rows) --p.rows;
   const int64_t tiles = std::max<int64_t>(1, cdiv(p.M, p.rows)), blocks = cdiv(p.N, 64);
-  // (the workspace is sized by splits, which `plain` leaves alone: from 8192 rows on there are none)
+  // (the workspace is sized by the splits of a plain call, which are those of others or more)
   // a long narrow product of few rows goes to several workgroups first (2047 tokens, 6869 to 1792: 44 us, so 34; one
   // token 24 and 13), whose sums the wide product's add
   p.splits = p.K >= 4096 && tiles < 256 ? 4 : 0;

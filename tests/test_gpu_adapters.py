@@ -444,3 +444,20 @@ def test_autograd_layouts(M, dtype):
     for p, q in zip(want, got):
         assert torch.equal(p, q)
     assert torch.equal(got[4], w)
+
+
+@pytest.mark.parametrize("dtype,K,N,p", [("bf16", 4096, 4104, 0.0), ("fp32", 4104, 4160, 0.25), ("fp16", 4099, 4104, 0.0)])
+def test_large_banks(dtype, K, N, p):
+    """32 rows of one adapter and a narrow product in parts, both ways; 16 rows where they lie on odd half words."""
+    c = case(4200, K, N, 32, 2, dtype, seed=22, lead=(2, 2100))
+    c["index"] = torch.tensor([1, 0])
+    backward_case(c, p, seed=3)
+
+
+@pytest.mark.parametrize("M,K,N,r", [(40, 300, 200, 32), (130, 96, 1000, 64), (208, 1471, 650, 64), (70, 64, 600, 128)])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_ranks_choose_rows(M, K, N, r, dtype):
+    """A sequence's rows, more of them to a workgroup for larger ranks."""
+    c = case(M, K, N, r, 3, dtype, seed=23, lead=(2, M // 2))
+    c["index"] = torch.tensor([2, -1])
+    backward_case(c, 0.25, seed=4)
