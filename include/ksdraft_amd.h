@@ -867,7 +867,8 @@ int ksd_verify_draft(const void *target, const void *draft, int dtype, int64_t B
  * Low-rank adapters of many requests beside a shared projection (no reference counterpart):
  *   h[m] = scales[i] x~[m] A_i^T,  y[m] = base[m] + h[m] B_i^T,  i = index[m / rows_per_index]
  * x~ = x, or dropout(x) as ksd_dropout gives it (rows m, columns of K). Rows whose index lies outside [0, n) get
- * base alone. Sums are fp32, h is not rounded to fewer than 16 bits (fp32: 24), y is rounded once.
+ * base alone. Sums are fp32, h enters the second product with its 24 bits (fp16: 22 of the row's largest), y is rounded
+ * once. 16-bit types: an infinite value of b gives NaN where its product alone would be infinite.
  *   x (M, K), base (M, N) or NULL: row strides in elements; y (M, N) dense, may be base itself where that is
  *   dense; a (n, r, K), b (n, N, r) dense; all of dtype; r <= 128, n <= 65535
  *   index int64 (index_wide) or int32; scales (n,) fp32 or NULL (1); hidden (M, r) fp32 or NULL: h

@@ -9,9 +9,9 @@
 //
 // Both passes of a token's row are one launch of pair_kernel: a workgroup of 8 waves holds up to 32 rows; the
 // waves split the contraction of the narrow product, their sums join in LDS, and the same waves then split the
-// columns of the wide one. h is never rounded on its way: it is fp32 in LDS and enters the 16-bit matrix
+// columns of the wide one. h keeps its 24 bits on its way: it is fp32 in LDS and enters the 16-bit matrix
 // instructions as a rounded value and the rounding's rest, side by side along the contraction, which a rank of 16
-// leaves half empty anyway. What bounds it is memory: x and base read once, y written once. 8192 tokens of 1536 to 1536,
+// leaves half empty anyway (fp16: 11 bits each), and bf16, of 8 bits a part, as the rest's rest in another instruction. What bounds it is memory: x and base read once, y written once. 8192 tokens of 1536 to 1536,
 // rank 16: bf16 19 us for 76 MB (3.9 TB/s), fp32 43 us for 151 MB (3.5; the narrow product alone 17, the wide one 24). Few
 // tokens take a launch's latency: one token 5.4 us, 64 of as many adapters 6.7.
 #include "ksd_random.h"
@@ -304,16 +304,39 @@ constexpr int kPlain = 0, kOdd = 1, kAnyRank = 2;
 // the others' registers do not allow it.
 template <int DT, int R16, int RT, bool MASK>
 constexpr bool kTwo = MASK && DT != KSD_F32 && RT == 1 && R16 == 1;
+// Forms of rank up to 16 that stay within two workgroups' registers only if the bank's rows are loaded where they are used, 32
+// columns at a time (fp16, rank 7, 4000 tokens of 1536, a training call with dropout: 72.7 us, with rows ahead 80.9; bf16, rank
+// 16: 57 us and 59.5, in the spills that h's third part then makes).
+template <int DT, int R16, int RT, bool MASK, int KIND>
+constexpr bool kLean = kTwo<DT, R16, RT, MASK> || (DT == KSD_BF16 && RT == 1 && R16 == 1 && KIND == kOdd);
+// bf16 values of a row of h's third parts: 16 ranks, 16 zeros for the upper two groups, and so on; 16 bytes more spread rows
+// over the banks. (Two blocks' parts side by side in one instruction need the bank's rows side by side too: 8192 tokens of
+// 1536 to 1536, rank 64, 47 us for 34.)
+template <int R16>
+constexpr int kThirdPitch = 32 * R16 + 8;
 template <int DT, int R16, int RT, bool MASK, int KIND>
 __global__ __launch_bounds__(64 * kWaves, (kTwo<DT, R16, RT, MASK> ? 4 : 2)) void pair_kernel(const PairArgs p) {
   using T = typename Elem<DT>::T;
   using V = typename Oct<DT>::V;
   constexpr int R = 16 * R16, U = DT == KSD_F32 ? (R16 <= 1 ? 4 : R16 <= 2 ? 2 : 1) : (kTwo<DT, R16, RT, MASK> ? 3 : R16 <= 1 ? 6 : R16 <= 2 ? 4 : 2);
-  constexpr int TB = R16 <= 2 ? 4 : R16 == 4 ? 2 : 1;  // products whose bank rows are loaded together
+  constexpr int TB = kLean<DT, R16, RT, MASK, KIND> ? 2 : R16 <= 2 ? 4 : R16 == 4 ? 2 : 1;  // products whose bank rows are loaded together
   constexpr bool kMayBeOdd = DT != KSD_F32 && KIND != kPlain;
-  constexpr bool kAhead = R16 == 1;  // the next bank rows are loaded during a block's products: more ranks, no registers for it
+  constexpr bool kAhead = R16 == 1 && !kLean<DT, R16, RT, MASK, KIND>;  // the next bank rows are loaded during a block's products: more ranks, no registers for it
   constexpr int pitch = R + 4;  // floats: a row's four lanes of 16 bytes start 4 banks further than the last row's
+  constexpr bool kThird = DT == KSD_BF16;
   extern __shared__ float lds[];  // (kWaves, 16 RT, pitch): sums of a wave's columns; the first holds h
+  int16_t *const thirds = (int16_t *)(lds + kWaves * 16 * RT * pitch);  // (16 RT, kThirdPitch)
+  const auto put_third = [&](int t, int q, float v) {
+    float f[8] = {v}, g[8];
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
+      to_floats<DT>(from_floats<DT>(f), g);
+      f[0] = fabsf(g[0]) <= 3.0e38f ? f[0] - g[0] : 0.0f;
+    }
+    int16_t *const to = thirds + t * kThirdPitch<R16> + (q >> 4) * 32 + (q & 15);
+    to[0] = from_floats<DT>(f)[0];
+    to[16] = 0;  // the upper two groups' ranks
+  };
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, grp = lane >> 4;
   // lane l < rows: its token and the token's adapter
   int rows, mine = -1, token = 0;
@@ -387,6 +410,7 @@ __global__ __launch_bounds__(64 * kWaves, (kTwo<DT, R16, RT, MASK> ? 4 : 2)) voi
         for (int k = 0; k < p.splits; ++k) v += from[k * p.M * p.r];
       }
       lds[t * pitch + q] = v;
+      if constexpr (kThird) put_third(t, q, v);
     }
     __syncthreads();
   } else if (with) {
@@ -434,7 +458,9 @@ __global__ __launch_bounds__(64 * kWaves, (kTwo<DT, R16, RT, MASK> ? 4 : 2)) voi
         float v = lds[t * pitch + q];
 #pragma unroll
         for (int w = 1; w < kWaves; ++w) v += lds[(w * 16 * RT + t) * pitch + q];
-        lds[t * pitch + q] = q < p.r ? v : 0.0f;
+        v = q < p.r ? v : 0.0f;
+        lds[t * pitch + q] = v;
+        if constexpr (kThird) put_third(t, q, v);
       }
     }
     __syncthreads();
@@ -530,6 +556,9 @@ __global__ __launch_bounds__(64 * kWaves, (kTwo<DT, R16, RT, MASK> ? 4 : 2)) voi
                 for (int j = 0; j < 4; ++j) o = __builtin_amdgcn_mfma_f32_16x16x4f32(w[t][q][j], hv[u][q][j], o, 0, 0, 0);
               } else {
                 o = product<DT>(w[t][q], hv[u][q], o);
+                if constexpr (kThird) {
+                  o = product<DT>(w[t][q], *(const V *)(thirds + (u * 16 + col) * kThirdPitch<R16> + q * 32 + grp * 8), o);
+                }
               }
             }
         if constexpr (kAhead) {
@@ -574,12 +603,16 @@ __global__ __launch_bounds__(64 * kWaves, (kTwo<DT, R16, RT, MASK> ? 4 : 2)) voi
   }
 }
 
+// Bytes of LDS: the waves' sums, and bf16's third parts of h.
+template <int DT, int R16, int RT>
+constexpr int kLds = kWaves * 16 * RT * (16 * R16 + 4) * 4 + (DT == KSD_BF16 ? 16 * RT * kThirdPitch<R16> * 2 : 0);
+
 static bool aligned_rank(int64_t r, int dtype) { return r % (dtype == KSD_F32 ? 4 : 8) == 0; }
 
 template <int DT, int R16, int RT, bool MASK, int KIND>
 static void launch_pair(const PairArgs &p, unsigned tiles, hipStream_t st) {
   const dim3 g(tiles, (unsigned)(p.phase == 1 ? p.splits : cdiv(p.N, p.cols)));
-  constexpr int lds = kWaves * 16 * RT * (16 * R16 + 4) * 4;
+  constexpr int lds = kLds<DT, R16, RT>;
   if constexpr (lds > 65536) {  // past HIP's default, once on each device
     static std::atomic<uint64_t> known{0};
     int dev = 0;
