@@ -582,8 +582,8 @@ __global__ __launch_bounds__(1024) void draw_kernel(const Args a) {
       lo1 = piece_value(totals, lane, pieces, 1), hi1 = piece_value(totals, lane + 64, pieces, 1);
       if (a.L) {
         lo1 += lo, hi1 += hi;
-      } else {  // pieces with largest logits of their own
-        lo *= power(lo1, d.p), hi *= power(hi1, d.p);
+      } else {  // pieces with largest logits of their own; a lane without one has none, and 0 may lie far above the row's
+        lo *= power(lane < pieces ? lo1 : -FLT_MAX, d.p), hi *= power(lane + 64 < pieces ? hi1 : -FLT_MAX, d.p);
         lo1 = lo, hi1 = hi;
       }
     }
