@@ -201,7 +201,7 @@ class _AdapterFunction(torch.autograd.Function):
         # through save_for_backward, so that they are freed with the graph and writes into them are noticed
         device_seed = s.seed if isinstance(s.seed, torch.Tensor) else None
         ctx.save_for_backward(x, a, b, s.index, s.scales, s.hidden, s.work, device_seed)
-        ctx.args = (s.per, s.lead, s.mask)
+        ctx.args = (s.per, s.lead, (p, None if device_seed is not None else s.seed, stream))
         return y
 
     @staticmethod
@@ -209,9 +209,12 @@ class _AdapterFunction(torch.autograd.Function):
     def backward(ctx, grad):
         x, a, b, index, scales, hidden, work, seed = ctx.saved_tensors
         s = Saved()
-        s.per, s.lead, s.mask = ctx.args
+        s.per, s.lead, (p, number, stream) = ctx.args
         (s.x, _, s.pitch), s.a, s.b = _rows(x, x.shape[-1]), _dense(a), _dense(b)
-        s.index, s.scales, s.hidden, s.work, s.seed = index, scales, hidden, work, seed
+        s.index, s.scales, s.hidden, s.work = index, scales, hidden, work
+        # what was saved may come back elsewhere (hooks on saved tensors): the address of the seed as it is now
+        s.seed = number if seed is None else seed
+        s.mask = mask_arguments(p, s.seed, stream, x.device)
         need = ctx.needs_input_grad
         dx = da = db = None
         if need[0] or need[1] or need[2]:
