@@ -150,9 +150,13 @@ def adapter_linear_train(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, inde
     """The training forward: (y, saved), y as adapter_linear gives it on dropout(x) (``kernels.dropout`` with
     this probability, seed and stream; base is not touched by it)."""
     dev = _lib.require_gpu(x)
-    if isinstance(seed, torch.Tensor) and dropout:
-        seed = seed.clone()  # the caller may count it on before the backward pass
     mask = mask_arguments(dropout, seed, stream, dev)
+    if isinstance(seed, torch.Tensor):
+        if mask[0]:
+            seed = seed.clone()  # the caller may count it on before the backward pass
+            mask = mask_arguments(dropout, seed, stream, dev)
+        else:
+            seed, mask = 0, _NO_MASK  # nothing is dropped: the seed is not read
     s = Saved()
     s.mask, s.seed, s.lead = mask, seed, x.shape[:-1]
     y, (s.x, s.pitch, s.a, s.b, s.index, s.per, s.scales, s.hidden, s.work) = _forward(x, a, b, index, scales, base, None, mask, True)

@@ -46,3 +46,12 @@ def test_number_as_seed(calls):
     y = adapters.adapt(*inputs(), dropout=0.25, seed=1 << 40, stream=5)
     y.sum().backward()
     assert calls[0][1][FORWARD] == calls[1][1][BACKWARD] == (16384, 1 << 40, None, 5)
+
+
+def test_unused_seed_may_change(calls):
+    """At a probability of 0 nothing reads the seed: counting it on before the backward pass is no write into a saved tensor."""
+    seed = torch.tensor([77])
+    y = adapters.adapt(*inputs(), dropout=0.0, seed=seed)
+    seed += 1
+    y.sum().backward()
+    assert calls[1][1][BACKWARD][0] == 0
