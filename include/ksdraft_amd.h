@@ -871,7 +871,7 @@ int ksd_verify_draft(const void *target, const void *draft, int dtype, int64_t B
  * once. 16-bit types: an infinite value of b gives NaN where its product alone would be infinite.
  *   x (M, K), base (M, N) or NULL: row strides in elements; y (M, N) dense, may be base itself where that is
  *   dense; a (n, r, K), b (n, N, r) dense; all of dtype; r <= 128, n <= 65535
- *   index int64 (index_wide) or int32; scales (n,) fp32 or NULL (1); hidden (M, r) fp32 or NULL: h
+ *   index int64 (index_wide) or int32, rows_per_index from 1 to 2^31 - 1; scales (n,) fp32 or NULL (1); hidden (M, r) fp32 or NULL: h
  *   workspace: ksd_adapter_linear_workspace bytes, 16-byte aligned (NULL where that is 0)
  * The backward pass from g = dY and the forward's hidden and workspace, left as it was (tokens listed by adapter), g'[m] = scales[i] g[m] B_i:
  *   dx[m] = base[m] + mask(g'[m] A_i) (base (M, K): another branch's gradient, or NULL); NULL: not wanted

@@ -1014,6 +1014,9 @@ static bool fits(int64_t M, int64_t K, int64_t N, int64_t r, int64_t n) {
          K <= 0x7fffffff - 65536 && N <= 0x7fffffff - 65536;
 }
 
+// adapter_of divides by it in 32 bits.
+static bool per_fits(int64_t per) { return per >= 1 && per <= 0x7fffffff; }
+
 static int run_pair(const PairArgs &args, int dtype, bool mask, hipStream_t st) {
   PairArgs p = args;
   if (dtype != KSD_F32) {
@@ -1072,7 +1075,7 @@ using namespace ksd;
 
 extern "C" int ksd_adapter_linear_workspace(int64_t M, int64_t K, int64_t N, int64_t r, int64_t n, int64_t rows_per_index, int dtype,
                                             int64_t *bytes) {
-  if (!bytes || !adp::fits(M, K, N, r, n) || !adp::float_type(dtype) || rows_per_index < 1)
+  if (!bytes || !adp::fits(M, K, N, r, n) || !adp::float_type(dtype) || !adp::per_fits(rows_per_index))
     return fail(KSD_EINVAL, "adapter_linear_workspace: bad arguments");
   *bytes = adp::forward(M, K, N, r, n, rows_per_index, dtype).bytes;
   return KSD_OK;
@@ -1084,7 +1087,7 @@ extern "C" int ksd_adapter_linear(const void *x, int dtype, int64_t M, int64_t K
                                   const void *seed_from, int64_t stream_id, void *y, float *hidden, void *workspace,
                                   int64_t workspace_bytes, void *stream) {
   using namespace adp;
-  if (!fits(M, K, N, r, n) || rows_per_index < 1 || (M > 1 && (x_stride < K || (base && base_stride < N))))
+  if (!fits(M, K, N, r, n) || !per_fits(rows_per_index) || (M > 1 && (x_stride < K || (base && base_stride < N))))
     return fail(KSD_EINVAL, "adapter_linear: bad shape");
   if (!float_type(dtype)) return fail(KSD_ETYPE, "adapter_linear: unsupported element type");
   Mask m;
@@ -1108,7 +1111,7 @@ extern "C" int ksd_adapter_linear(const void *x, int dtype, int64_t M, int64_t K
 
 extern "C" int ksd_adapter_linear_backward_workspace(int64_t M, int64_t K, int64_t N, int64_t r, int64_t n, int64_t rows_per_index,
                                                      int dtype, int64_t *bytes) {
-  if (!bytes || !adp::fits(M, K, N, r, n) || !adp::float_type(dtype) || rows_per_index < 1)
+  if (!bytes || !adp::fits(M, K, N, r, n) || !adp::float_type(dtype) || !adp::per_fits(rows_per_index))
     return fail(KSD_EINVAL, "adapter_linear_backward_workspace: bad arguments");
   *bytes = adp::layout(M, K, N, r, n, rows_per_index, dtype).bytes;
   return KSD_OK;
@@ -1122,7 +1125,7 @@ extern "C" int ksd_adapter_linear_backward(const void *g, int dtype, int64_t M, 
                                            const void *seed_from, int64_t stream_id, void *dx, float *da, float *db,
                                            void *workspace, int64_t workspace_bytes, void *stream) {
   using namespace adp;
-  if (!fits(M, K, N, r, n) || rows_per_index < 1 ||
+  if (!fits(M, K, N, r, n) || !per_fits(rows_per_index) ||
       (M > 1 && (x_stride < K || g_stride < N || (base && base_stride < K))))
     return fail(KSD_EINVAL, "adapter_linear_backward: bad shape");
   if (!float_type(dtype)) return fail(KSD_ETYPE, "adapter_linear_backward: unsupported element type");
