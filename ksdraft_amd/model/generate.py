@@ -25,7 +25,7 @@ def draft_block(model, tokens: torch.Tensor, length: int, uniforms: torch.Tensor
         raise ValueError(f"a block has one token or more, got {length}")
     if uniforms is not None and uniforms.shape != (tokens.shape[0], length):
         raise ValueError(f"uniforms must be {(tokens.shape[0], length)}, got {tuple(uniforms.shape)}")
-    seen, drafted, rows = tokens, [], []
+    seen, drafted, rows = tokens, [], None
     for t in range(length):
         states = teacher_states
         if states is not None and t:
@@ -33,9 +33,12 @@ def draft_block(model, tokens: torch.Tensor, length: int, uniforms: torch.Tensor
         logits = model(seen, states)[0][:, -1] if states is not None else model(seen)[0][:, -1]
         token = sample_tokens(logits, None if uniforms is None else uniforms[:, t], temperatures)
         drafted.append(token)
-        rows.append(logits)
+        if rows is None:
+            rows = logits.new_empty(logits.shape[0], length, logits.shape[1])
+        rows[:, t] = logits  # a copy: a view would keep the logits of all positions
+        del logits
         seen = torch.cat([seen, token[:, None].to(seen.dtype)], 1)
-    return torch.stack(drafted, 1), torch.stack(rows, 1)
+    return torch.stack(drafted, 1), rows
 
 
 @torch.no_grad()
