@@ -14,13 +14,19 @@ import torch
 from ..kernels.speculate import sample_tokens, verify_draft
 
 
+def _fed(drawn: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """Drawn tokens as a model takes them: -1, of a row without a distribution, is no row of an embedding."""
+    return drawn.clamp(min=0).to(dtype)
+
+
 @torch.no_grad()
 def draft_block(model, tokens: torch.Tensor, length: int, uniforms: torch.Tensor | None = None, temperatures=None,
                 teacher_states: torch.Tensor | None = None):
     """(draft_tokens (B, length) int64, draft_logits (B, length, V)) behind tokens (B, T): token by token, each drawn
     from softmax(logits / T) by its number of uniforms (B, length). temperatures: (B,) float32, a number, or None
     (1); at the number 0 the largest logit is taken and uniforms may be None. teacher_states (B, T, teacher_dim):
-    positions behind T get the last one's."""
+    positions behind T get the last one's. A row without a distribution (NaN, or no finite logit) drafts -1, which
+    verification refuses; the model goes on from token 0 there."""
     if length < 1:
         raise ValueError(f"a block has one token or more, got {length}")
     if uniforms is not None and uniforms.shape != (tokens.shape[0], length):
@@ -37,7 +43,7 @@ def draft_block(model, tokens: torch.Tensor, length: int, uniforms: torch.Tensor
             rows = logits.new_empty(logits.shape[0], length, logits.shape[1])
         rows[:, t] = logits  # a copy: a view would keep the logits of all positions
         del logits
-        seen = torch.cat([seen, token[:, None].to(seen.dtype)], 1)
+        seen = torch.cat([seen, _fed(token[:, None], seen.dtype)], 1)
     return torch.stack(drafted, 1), rows
 
 
@@ -54,7 +60,7 @@ def speculative_step(draft, target, tokens: torch.Tensor, length: int, uniforms:
         raise ValueError(f"uniforms must be {(B, 2 * length + 1)}, got {tuple(uniforms.shape)}")
     first = None if uniforms is None else uniforms[:, :length]
     block, block_logits = draft_block(draft, tokens, length, first, temperatures, teacher_states)
-    logits = target(torch.cat([tokens, block.to(tokens.dtype)], 1))
+    logits = target(torch.cat([tokens, _fed(block, tokens.dtype)], 1))
     logits = logits[0] if isinstance(logits, tuple) else logits
     logits = logits[:, T - 1:]
     if logits.dtype != block_logits.dtype:  # not one in the other's type: the block was drawn from its logits as they are
