@@ -28,6 +28,13 @@ from .quant import (GROUP_SIZE, SCALE_DTYPE, dequantize_last_dim, quantize_dual,
                     quantize_transpose, requant_transpose)
 
 
+def dense_rows(x: torch.Tensor, weight: torch.Tensor) -> torch.Tensor:
+    """x as F.linear may take it with this weight. torch multiplies strided rows by a weight without gradient as a batch of
+    products whose right operand is a transposed view; in bfloat16 those have faulted GPUs of this kind, so such rows are made dense
+    first. Every other call takes x as it is."""
+    return x.contiguous() if x.dtype == torch.bfloat16 and not weight.requires_grad else x
+
+
 _OUT_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 

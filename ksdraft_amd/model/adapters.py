@@ -85,9 +85,7 @@ class AdaptedLinear(nn.Module):
         raise ValueError(f"the selected adapters {tuple(index.shape)} do not match an input {tuple(x.shape)}")
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
-        # dense rows for both products; torch multiplies strided ones with a frozen weight as a batch, whose
-        # bfloat16 products by a transposed operand have faulted this GPU
-        x = x.contiguous()
+        x = x.contiguous()  # dense rows for both products (kernels.linear.dense_rows, once)
         if residual is None:
             y = self.base(x)
         elif isinstance(self.base, nn.Linear):

@@ -14,6 +14,7 @@ import torch
 from torch import nn
 
 from ..config import KSDraftConfig
+from ..kernels.linear import dense_rows
 from .block import DraftBlock
 
 
@@ -49,7 +50,8 @@ class KSDraftModel(nn.Module):
         if teacher_states is not None:
             if self.teacher_proj is None:
                 raise ValueError("teacher_states passed but teacher_dim=0 at construction")
-            x = x + self.teacher_proj(teacher_states.to(self.teacher_proj.weight.dtype))
+            states = teacher_states.to(self.teacher_proj.weight.dtype)
+            x = x + self.teacher_proj(dense_rows(states, self.teacher_proj.weight))
         prev = None
         features = []
         for block in self.blocks:

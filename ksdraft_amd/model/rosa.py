@@ -130,9 +130,11 @@ class RosaMixer(nn.Module):
         return outs
 
     def _out(self, hard: torch.Tensor, residual: torch.Tensor | None) -> torch.Tensor:
-        from ..kernels.linear import Int8Linear
+        from ..kernels.linear import Int8Linear, dense_rows
         from ..kernels.token_channel import TokenChannelLinear
         from .adapters import AdaptedLinear
+        if isinstance(self.out_proj, nn.Linear):
+            hard = dense_rows(hard, self.out_proj.weight)
         if residual is None:
             return self.out_proj(hard)
         if isinstance(self.out_proj, (Int8Linear, TokenChannelLinear, AdaptedLinear)):

@@ -19,6 +19,8 @@ import torch
 from torch import nn
 import torch.nn.functional as F
 
+from ..kernels.linear import dense_rows
+
 
 class _LowRank(nn.Module):
     def __init__(self, width: int, rank: int):
@@ -88,6 +90,7 @@ class AdjacentInjection(nn.Module):
         if prev_layer_feature is not None:
             p_prev = torch.cat([prev_layer_feature[:, :1, :], p_prev[:, 1:, :]], dim=1)
         r2 = self.gate_p.down.out_features
+        p_prev = dense_rows(p_prev, self.gate_p.down.weight)
         pd = F.linear(p_prev, torch.cat([self.gate_p.down.weight, self.inject.down.weight]))
         pre = F.linear(torch.cat([zd[..., r1:], pd[..., :r2]], dim=-1),
                        torch.cat([self.gate_q.up.weight, self.gate_p.up.weight], dim=1),
