@@ -201,6 +201,8 @@ class _AdapterFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, a, b, index, scales, base, p, seed, stream):
         ctx.guard = _lib.capture_guard(_lib.require_gpu(x), x, a, b, base)
+        ctx.types = a.dtype, b.dtype
+        a, b = (t.to(x.dtype) if t.dtype == torch.float32 else t for t in (a, b))  # masters; their gradients stay fp32
         y, s = adapter_linear_train(x, a, b, index, scales, base, p, seed, stream)
         # through save_for_backward, so that they are freed with the graph and writes into them are noticed
         device_seed = s.seed if isinstance(s.seed, torch.Tensor) else None
@@ -223,13 +225,15 @@ class _AdapterFunction(torch.autograd.Function):
         dx = da = db = None
         if need[0] or need[1] or need[2]:
             dx, da, db = adapter_linear_backward(grad, s, None, need[0], need[1] or need[2])
-        return (dx, da.to(a.dtype) if need[1] else None, db.to(b.dtype) if need[2] else None, None, None,
+        type_a, type_b = ctx.types
+        return (dx, da.to(type_a) if need[1] else None, db.to(type_b) if need[2] else None, None, None,
                 grad if need[5] else None, None, None, None)
 
 
 def adapt(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, index: torch.Tensor, scales: torch.Tensor | None = None,
           base: torch.Tensor | None = None, dropout: float = 0.0, seed: int | torch.Tensor = 0,
           stream: int = 0) -> torch.Tensor:
-    """adapter_linear_train's y with gradients for x, a, b and base. A backward pass is captured only while no
+    """adapter_linear_train's y with gradients for x, a, b and base. a and b may also be fp32 where x is not: they are used
+    in x's type, and their gradients are the fp32 sums. A backward pass is captured only while no
     eager graph of the same leaves is alive (RuntimeError, where that graph is of this function)."""
     return _AdapterFunction.apply(x, a, b, index, scales, base, dropout, seed, stream)

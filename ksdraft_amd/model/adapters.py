@@ -38,7 +38,7 @@ class AdapterSelection:
 class AdaptedLinear(nn.Module):
     """base(x) + scales_i (dropout(x) A_i^T) B_i^T with the adapters that ``selection`` names. The base layer
     (nn.Linear, Int8Linear, TokenChannelLinear) is called as it is; A starts like an nn.Linear's weight, B at
-    zero. The adapters are kept in fp32 and used in x's type."""
+    zero. The adapters are kept in fp32 and used in x's type; their gradients are fp32."""
 
     def __init__(self, base: nn.Module, count: int, rank: int, selection: AdapterSelection, alpha: float | None = None,
                  dropout: float = 0.0, seed: int | None = None):
@@ -95,12 +95,13 @@ class AdaptedLinear(nn.Module):
         index = self._index(x)
         if index is None:
             return y
-        a, b = self.adapter_a.to(x.dtype), self.adapter_b.to(x.dtype)
+        a, b = self.adapter_a, self.adapter_b
         if y.dtype != x.dtype:  # a residual of another type
             return y + self._delta(x, a, b, index).to(y.dtype)
         if (self.training and self.dropout.p) or (torch.is_grad_enabled() and (
                 y.requires_grad or x.requires_grad or a.requires_grad or b.requires_grad)):
             return self._delta(x, a, b, index, y)
+        a, b = a.to(x.dtype), b.to(x.dtype)
         return adapter_linear(x, a, b, index, self.adapter_scales, base=y)  # not into y: a hook of the base may hold it
 
     def _delta(self, x, a, b, index, base=None):

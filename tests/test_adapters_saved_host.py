@@ -55,3 +55,32 @@ def test_unused_seed_may_change(calls):
     seed += 1
     y.sum().backward()
     assert calls[1][1][BACKWARD][0] == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_parameters_keep_their_gradients_bits(calls, monkeypatch, dtype):
+    """An adapted layer's fp32 parameters get the kernels' fp32 sums: what 16 bits would round, or not hold."""
+    from ksdraft_amd.model.adapters import AdaptedLinear, AdapterSelection
+    lin = AdaptedLinear(torch.nn.Linear(8, 5, dtype=dtype).requires_grad_(False), 2, 3, AdapterSelection())
+    lin.selection.index = torch.tensor([0, 1, -1, 0])
+    da, db = torch.randn(2, 3, 8) * 1e6, torch.randn(2, 5, 3) * 1e6 + 2.0 ** -10
+    monkeypatch.setattr(adapters, "adapter_linear_backward", lambda g, s, *a: (g.new_zeros(4, 8), da, db))
+    lin(torch.randn(4, 8, dtype=dtype)).sum().backward()
+    assert torch.equal(lin.adapter_a.grad, da) and torch.equal(lin.adapter_b.grad, db)
+    # what the kernels read is of x's type
+    assert calls[0][1][1] == _lib.dtype_code(dtype)
+
+
+def test_types_of_adapters(calls):
+    """Banks of x's type or fp32; the gradient is of the bank's type."""
+    x, a, b, index = inputs()
+    h = x.detach().half()
+    y = adapters.adapt(h, a.detach().half().requires_grad_(), b, index)
+    assert y.dtype == torch.float16 and y.requires_grad
+    y = adapters.adapt(h, a, b, index, base=torch.zeros(4, 5, dtype=torch.float16))
+    y.sum().backward()
+    assert a.grad.dtype == b.grad.dtype == torch.float32
+    with pytest.raises(TypeError):
+        adapters.adapt(h, a.bfloat16(), b, index)
+    with pytest.raises(TypeError):
+        adapters.adapt(x, a.half(), b, index)
