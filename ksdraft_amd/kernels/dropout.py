@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import torch
 from torch import nn
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
@@ -74,6 +75,7 @@ class _DropoutFunction(torch.autograd.Function):
         if isinstance(seed, torch.Tensor):  # the caller may count it on before the backward pass
             seed = seed.clone()
             ctx.save_for_backward(seed)
+            ctx.save_for_forward(seed)
             ctx.args = (p, None, stream)
         else:
             ctx.args = (p, seed, stream)
@@ -87,6 +89,21 @@ class _DropoutFunction(torch.autograd.Function):
         need = ctx.needs_input_grad
         return _dropout(grad, p, seed, stream, None) if need[0] else None, None, None, None, grad if need[4] else None
 
+    @staticmethod
+    def jvp(ctx, x, _p, _seed, _stream, residual):
+        if x is None:
+            return residual.clone()
+        p, seed, stream = ctx.args
+        return dropout(x, p, ctx.saved_tensors[0] if seed is None else seed, stream, residual)
+
+
+def _differentiated(*tensors) -> bool:
+    """Whether a derivative of a tensor is asked for, backwards or forwards."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return True
+    return forward_ad._current_level >= 0 and any(  # below 0 no tensor has a tangent
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
 
 def dropout(x: torch.Tensor, p: float, seed: int | torch.Tensor, stream: int = 0,
             residual: torch.Tensor | None = None) -> torch.Tensor:
@@ -96,8 +113,8 @@ def dropout(x: torch.Tensor, p: float, seed: int | torch.Tensor, stream: int = 0
 
     seed (64 bits) and stream (32 bits, a layer's number for instance) name the mask: the same ones on the
     same shape give the same mask. A seed on the device (one int64) is read by the kernel, so a graph replayed
-    after a change of it drops other values. The gradient goes through the same mask."""
-    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
+    after a change of it drops other values. The gradient, and a forward-mode tangent, go through the same mask."""
+    if _differentiated(x, residual):
         return _DropoutFunction.apply(x, p, seed, stream, residual)
     return _dropout(x, p, seed, stream, residual)
 
