@@ -123,8 +123,10 @@ class Dropout(nn.Module):
     """nn.Dropout on ``dropout``: the n-th training call of a module takes stream n of its seed (drawn from
     torch's CPU generator unless given), so a run is repeated by its seeds. Under graph capture the captured
     stream is part of the graph: a captured step passes a device seed to ``dropout`` itself. A forward pass that is run
-    again for its backward (recomputed activations) would take the next stream's mask; it names seed and stream to
-    ``dropout`` too. ``calls`` counts the streams and may be set, to go on where a run ended."""
+    again for its backward (recomputed activations) would take the next stream's mask, and raises RuntimeError, unless the
+    stream is named (``name_streams``). ``calls`` counts the streams and may be set, to go on where a run ended."""
+
+    stream = None  # the named one
 
     def __init__(self, p: float = 0.1, seed: int | None = None):
         super().__init__()
@@ -138,6 +140,10 @@ class Dropout(nn.Module):
         return f"p={self.p}"
 
     def next_stream(self) -> int:
+        if self.stream is not None:
+            return self.stream
+        if torch._C._current_graph_task_id() != -1:  # inside a backward pass
+            raise RuntimeError("a forward pass that is run again for its backward takes a named stream (name_streams)")
         n, self.calls = self.calls, (self.calls + 1) % (1 << 32)
         return n
 
@@ -145,3 +151,15 @@ class Dropout(nn.Module):
         if not self.training or self.p == 0:
             return x if residual is None else residual + x
         return dropout(x, self.p, self.seed, self.next_stream(), residual)
+
+
+def name_streams(module: nn.Module, stream: int | None) -> None:
+    """Every training call of module's ``Dropout`` layers (and those of its adapted layers) takes this stream of the layer's
+    seed, until another is named: a step's number for the step whose activations are recomputed. Layers have seeds of their
+    own, so one number names different masks; a layer called twice in a step drops the same places. None: streams are
+    counted again."""
+    if stream is not None and not 0 <= stream < 1 << 32:
+        raise ValueError(f"stream must lie in [0, 2**32), got {stream}")
+    for m in module.modules():
+        if isinstance(m, Dropout):
+            m.stream = stream
