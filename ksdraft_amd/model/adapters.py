@@ -11,7 +11,9 @@ frozen; ``train.adapter_step.AdapterTrainer`` trains the adapters.
 
 from __future__ import annotations
 
+import contextlib
 import copy
+import threading
 
 import torch
 from torch import nn
@@ -26,10 +28,19 @@ _ADAPTABLE = (nn.Linear, Int8Linear, TokenChannelLinear)
 
 
 class AdapterSelection:
-    """The index that a model's AdaptedLinear layers share; None: no adapter anywhere."""
+    """The index that a model's AdaptedLinear layers share; None: no adapter anywhere. ``lock`` is held where the index
+    belongs to one caller (``selected_adapters``)."""
 
     def __init__(self):
         self.index = None
+        self.lock = threading.RLock()
+
+    def __getstate__(self):
+        return {"index": self.index}
+
+    def __setstate__(self, state):
+        self.__init__()
+        self.index = state["index"]
 
     def __deepcopy__(self, memo):
         return AdapterSelection()  # a copied model selects for itself
@@ -125,14 +136,39 @@ def adapter_state_dict(model: nn.Module) -> dict:
 
 def select_adapters(model: nn.Module, index: torch.Tensor | None) -> None:
     """The adapters of the next calls: integers (B,) for each sequence, (B, T) for each token, values outside
-    [0, count) for none; None: no adapter anywhere. The tensor is read when a layer runs."""
+    [0, count) for none; None: no adapter anywhere. The tensor is read when a layer runs. A model has one selection:
+    threads that call it for different requests use ``selected_adapters``."""
+    for s in _selections(model, index):
+        s.index = index
+
+
+@contextlib.contextmanager
+def selected_adapters(model: nn.Module, index: torch.Tensor | None):
+    """``select_adapters`` for the calls of a with block, the selection before it again behind it. Blocks of other threads on
+    the same model wait (for the calls' launches, not for the GPU), so each sees its own adapters in every layer."""
+    with contextlib.ExitStack() as held:
+        selections = _selections(model, index)
+        if torch._C._current_graph_task_id() == -1:  # a backward pass runs again what its caller's block covers, in another thread
+            for s in selections:
+                held.enter_context(s.lock)
+        before = [s.index for s in selections]
+        try:
+            for s in selections:
+                s.index = index
+            yield
+        finally:
+            for s, i in zip(selections, before):
+                s.index = i
+
+
+def _selections(model: nn.Module, index: torch.Tensor | None) -> list:
+    """The model's selections (one, unless adapters were added twice) in the order in which they are locked."""
     layers = adapted_layers(model)
     if not layers:
         raise ValueError("the model has no adapters (add_adapters)")
     if index is not None and index.dtype not in (torch.int64, torch.int32):
         raise TypeError(f"index must be integers, got {index.dtype}")
-    for m in layers:
-        m.selection.index = index
+    return sorted({id(m.selection): m.selection for m in layers}.values(), key=id)
 
 
 def add_adapters(model: nn.Module, count: int, rank: int, *, targets=ROSA, alpha: float | None = None, dropout: float = 0.0,

@@ -13,7 +13,7 @@ import torch
 import torch.nn.functional as F
 
 from ..kernels.ks3_int8 import KS3Int8Cell
-from ..model.adapters import adapter_parameters, select_adapters
+from ..model.adapters import adapter_parameters, select_adapters, selected_adapters
 from . import IGNORE_INDEX, AdamWRequant
 from .clip import gradient_norm
 from .int8_step import Int8DraftTrainer, _check_loss_scale, transfer_space_loss
@@ -22,7 +22,8 @@ from .token_channel_step import check_targets
 
 class AdapterTrainer(Int8DraftTrainer):
     """Int8DraftTrainer's interface (``loss``, ``backward``, ``optimizer_step``, ``step``) for the adapters of a
-    model; ``index`` (B,) names each sequence's adapter. Every target must be a token."""
+    model; ``index`` (B,) names each sequence's adapter. Every target must be a token. ``loss`` leaves its batch's adapters
+    selected, which a backward pass with recomputed activations needs; ``step`` gives the selection before it back."""
 
     def __init__(self, model, lr: float = 3e-4, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.0,
                  grad_clip: float = 1.0, transfer_weight: float = 0.5, loss_scale: float = 1.0):
@@ -59,7 +60,8 @@ class AdapterTrainer(Int8DraftTrainer):
 
     def step(self, tokens: torch.Tensor, index: torch.Tensor, teacher_states: torch.Tensor | None = None):
         self.model.train()
-        loss, ce, ts = self.loss(tokens, index, teacher_states)
-        self.backward(loss)
+        with selected_adapters(self.model, index):
+            loss, ce, ts = self.loss(tokens, index, teacher_states)
+            self.backward(loss)
         self.optimizer_step()
         return loss.detach(), ce.detach(), ts.detach()
