@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import threading
 import weakref
 
 import torch
@@ -209,6 +210,7 @@ class _EagerGraph:
 
 
 _eager_graphs = weakref.WeakSet()  # of the living autograd graphs that ``capture_guard`` was called for
+_graphs_lock = threading.Lock()  # a set that another thread adds to cannot be walked through
 
 
 def capture_guard(dev: torch.device, *tensors):
@@ -231,14 +233,17 @@ def capture_guard(dev: torch.device, *tensors):
         return None
     stream = stream_ptr(dev)
     if torch.cuda.is_current_stream_capturing():
-        for g in list(_eager_graphs):
+        with _graphs_lock:
+            living = list(_eager_graphs)
+        for g in living:
             if g.stream != stream and not leaves.isdisjoint(g.leaves):
                 raise RuntimeError("an eager graph of the same leaf tensors is alive: drop it (its outputs and losses) "
                                    "before their backward pass is captured")
         return None
     g = _EagerGraph()
     g.leaves, g.stream = leaves, stream
-    _eager_graphs.add(g)
+    with _graphs_lock:
+        _eager_graphs.add(g)
     return g
 
 
