@@ -69,6 +69,14 @@ class AdaptedLinear(nn.Module):
         self.register_buffer("adapter_scales", torch.full((count,), float(scale), device=device))
         self.dropout = Dropout(dropout, seed)
 
+    def _apply(self, fn, *args, **kwargs):
+        adapters = {id(t) for p in (self.adapter_a, self.adapter_b, self.adapter_scales) for t in (p, p.grad)}
+
+        def move(t):  # a model's .bfloat16() and the like: the adapters move, and keep their type
+            out = fn(t)
+            return t.to(out.device) if id(t) in adapters and out.dtype != t.dtype else out
+        return super()._apply(move, *args, **kwargs)
+
     @property
     def in_features(self) -> int:
         return self.base.in_features
