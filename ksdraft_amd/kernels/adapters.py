@@ -97,8 +97,8 @@ def _forward(x, a, b, index, scales, base, out, mask, train):
     else:
         if out.shape != (*lead, N) or out.dtype != x.dtype or not out.is_contiguous():
             raise ValueError(f"out must be a contiguous {(*lead, N)} {x.dtype} tensor")
-        for name, t in (("x", x), ("a", a), ("b", b), ("index", index)):
-            if _shared(out, t):
+        for name, t in (("x", x), ("a", a), ("b", b), ("index", index), ("scales", scales)):
+            if t is not None and _shared(out, t):
                 raise ValueError(f"out shares memory with {name}")
         if base is not None and _shared(out, base) and (base_at != out.data_ptr() or base_pitch != N):
             raise ValueError("out shares memory with base and is not base itself")

@@ -84,3 +84,14 @@ def test_types_of_adapters(calls):
         adapters.adapt(h, a.bfloat16(), b, index)
     with pytest.raises(TypeError):
         adapters.adapt(x, a.half(), b, index)
+
+
+def test_out_over_an_operand(calls):
+    """The kernel reads the scales of every row while it writes out."""
+    x, a, b, index = (t.detach() for t in inputs())
+    room = torch.zeros(64)
+    out, scales = room[:20].view(4, 5), room[18:20]
+    with pytest.raises(ValueError, match="scales"):
+        adapters.adapter_linear(x, a, b, index, scales, out=out)
+    adapters.adapter_linear(x, a, b, index, room[20:22], out=out)
+    assert len(calls) == 1
