@@ -849,7 +849,7 @@ int ksd_dropout(const void *x, int dtype, int64_t rows, int64_t d, int64_t strid
  *   ones), which is drawn too
  * Uniforms lie in [0, 1). A draft token outside [0, V) is refused. A row without a finite logit, or with NaN or
  * +inf (greedy: NaN), has no distribution: a target's is refused and draws -1, a draft's with NaN or +inf refuses its
- * token and draws from p. Sums of the row that is drawn from are 64-bit, those of the tests 32-bit.
+ * token and draws from p, a draft's without a finite logit is q = 0. Sums of the row that is drawn from are 64-bit, those of the tests 32-bit.
  *   target (B, L + 1, V), draft (B, L, V) or NULL: dtype, last stride 1, the others in elements
  *   tokens (B, L) int64; uniforms (B, L + 1) fp32, or fp64 where uniforms_wide (NULL if all are greedy)
  *   temperatures (B,) fp32, or NULL: `temperature` for all

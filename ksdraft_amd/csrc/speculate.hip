@@ -7,11 +7,16 @@
 //   T = 0: accepted while the token is the row's largest logit (the lowest index of equal ones), which is drawn too
 //
 // One read of the rows gives each row's largest logit and sum of powers in 32 bits (stats_kernel): the tests
-// need p and q of one token a row, and an error of 2^-24 there moves one test in ten million. The drawn token is
+// need p and q of one token a row. A power's exponent y is rounded three times and the power once, and a sum of 150144 is
+// about 40 roundings deep: with |y| 17 on average at most (log2 of the vocabulary) a sum is off by less than 100 * 2^-24 =
+// 6e-6 of itself, by 1e-7 or so where the roundings are as random as they look. That moves one test in a hundred
+// thousand at the worst, whose u lies so near its border. The drawn token is
 // another matter: with 150144 tokens a running sum has as many borders, and sums in 32 bits would move about one draw in
 // a hundred across one. The one row of a stream that is drawn from is therefore read again with powers and sums in 64
-// bits (total_kernel, weight_kernel, draw_kernel). Logits of -inf have probability 0; a row without a finite logit, or with NaN or
-// +inf, has no distribution: a target's is refused and draws -1, a draft's refuses the token and draws from p.
+// bits (total_kernel, weight_kernel, draw_kernel). Logits of -inf have probability 0. A row with NaN or +inf has no
+// distribution (greedy: with NaN, +inf is a largest logit like any other), a target's without a finite logit neither: a
+// target's refuses its token and draws -1, a draft's refuses the token and draws from p. A draft's row of nothing but
+// -inf is q = 0: its token is accepted wherever p > 0.
 #include "ksd_common.h"
 
 #include <float.h>

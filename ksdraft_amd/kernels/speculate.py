@@ -73,7 +73,8 @@ def verify_draft(target_logits: torch.Tensor, draft_tokens: torch.Tensor, unifor
     (B,): drafted tokens of each stream (None: L); stream b's row lengths[b] is then the one behind the last.
 
     Logits of -inf have probability 0. A drafted token outside the vocabulary is refused. A target row
-    without a finite logit, or with NaN or +inf, refuses its token and draws -1."""
+    without a finite logit, or with NaN or +inf, refuses its token and draws -1 (greedily +inf is a largest logit like any
+    other). A draft row with NaN or +inf refuses its token, and the draw is from p; one of nothing but -inf is q = 0."""
     if draft_tokens is None:
         raise ValueError("draft_tokens are needed; sample_tokens draws without a draft")
     dev = _lib.require_gpu(target_logits, draft_tokens, uniforms, draft_logits, lengths,
