@@ -300,8 +300,9 @@ __device__ __forceinline__ typename Oct<DT>::V bank_oct(const typename Elem<DT>:
 // that, and a rank that is no multiple of a lane's. Each in registers of its own: with odd rows' code 8192 plain rows of 1536
 // take 21.6 us for 19.3.
 constexpr int kPlain = 0, kOdd = 1, kAnyRank = 2;
-// Masked 16-bit rows run two workgroups a CU (4000 tokens of 1536 with dropout: 24.2 us, in the registers of one 29.1);
-// the others' registers do not allow it.
+// Masked 16-bit rows of rank up to 16 are held to the registers of two workgroups a CU (4000 tokens of 1536 with dropout: 24.2
+// us, in the registers of one 29.1). Unmasked ones whose rank is a lane's multiple are that small by themselves (up to 128); the
+// other forms run one.
 template <int DT, int R16, int RT, bool MASK>
 constexpr bool kTwo = MASK && DT != KSD_F32 && RT == 1 && R16 == 1;
 // Forms of rank up to 16 that stay within two workgroups' registers only if the bank's rows are loaded where they are used, 32
@@ -675,7 +676,8 @@ static void shape(PairArgs &p, bool lists, bool plain) {
   // token 24 and 13), whose sums the wide product's add
   p.splits = p.K >= 4096 && tiles < 256 ? 4 : 0;
   // more parts where a row is long (a train call with dropout of 2047 tokens of 1792 to 6869: 88.8 us with 256 workgroups,
-  // 86.6 with 512)
+  // 86.6 with 512, which are resident together there: rank 8 in 16 bits, two a CU; measured in that form alone). The tiles that
+  // lists add at each adapter's end are not counted.
   const int64_t want = blocks < 64 ? 256 : 512;
   const int64_t parts = std::min({blocks / 6, cdiv(want, tiles), p.splits ? blocks : 4 * p.N / p.K});
   p.cols = (int)(cdiv(blocks, std::max<int64_t>(1, parts)) * 64);

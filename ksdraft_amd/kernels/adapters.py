@@ -20,20 +20,10 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from .dropout import mask_arguments
+from .dropout import _rows, mask_arguments
 
 _TYPES = (torch.float32, torch.bfloat16, torch.float16)
 _INDEX = (torch.int64, torch.int32)
-
-
-def _rows(t: torch.Tensor, width: int):
-    """(t or a copy, its rows, their pitch) of a tensor (..., width) as the kernels read it."""
-    if t.is_contiguous():
-        return t, t.numel() // width, width
-    t = t if t.dim() == 2 else t.reshape(-1, width)
-    if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < width):
-        t = t.contiguous()
-    return t, t.shape[0], t.stride(0) if t.shape[0] > 1 else width
 
 
 def _dense(t: torch.Tensor) -> torch.Tensor:

@@ -36,7 +36,7 @@ def mask_arguments(p: float, seed, stream: int, dev: torch.device):
 
 
 def _rows(t: torch.Tensor, d: int):
-    """(t or a copy, its rows, their pitch) of a tensor (..., d) as the kernel reads it."""
+    """(t or a copy, its rows, their pitch) of a tensor (..., d) as the kernels read it (``kernels.adapters``' too)."""
     if t.is_contiguous():
         return t, t.numel() // d, d
     t = t if t.dim() == 2 else t.reshape(-1, d)
