@@ -72,9 +72,15 @@ class RosaMixer(nn.Module):
         v_in = prev + (x - prev) * torch.sigmoid(self.time_mix_v)
         return q_in, k_in, v_in
 
+    @staticmethod
+    def _unadapted(layer: nn.Module) -> nn.Module:
+        """layer, or the base of an adapted one while no adapter is selected, which computes the same."""
+        from .adapters import AdaptedLinear
+        return layer.base if isinstance(layer, AdaptedLinear) and layer.selection.index is None else layer
+
     def _int8_projections(self) -> bool:
         from ..kernels.linear import Int8Linear
-        return all(isinstance(getattr(self, n), Int8Linear) for n in ("q_proj", "k_proj", "v_proj"))
+        return all(isinstance(self._unadapted(p), Int8Linear) for p in (self.q_proj, self.k_proj, self.v_proj))
 
     def _fused_training_projections(self, x: torch.Tensor):
         """Training with Int8Linear q/k/v: ShiftedInt8Projections, or None when its
@@ -82,7 +88,7 @@ class RosaMixer(nn.Module):
         from ..kernels.linear import Int8Linear
         projs = (self.q_proj, self.k_proj, self.v_proj)
         mixes = (self.time_mix_q, self.time_mix_k, self.time_mix_v)
-        if not (self.fused_shift and self._int8_projections()
+        if not (self.fused_shift and all(isinstance(p, Int8Linear) for p in projs)
                 and x.dtype in (torch.float32, torch.bfloat16, torch.float16)
                 and x.shape[-1] % 8 == 0 and all(m.dtype == torch.float32 for m in mixes)
                 and not any(p.ste_training for p in projs)):
@@ -105,7 +111,7 @@ class RosaMixer(nn.Module):
         """Eval with Int8Linear q/k/v: shift + quantize in one pass, then the W8A8 GEMMs
         (+ bias) exactly as Int8Linear.forward computes them (linear.py:62-73)."""
         from ..kernels.gemm import w8a8_gemm_out
-        projs = (self.q_proj, self.k_proj, self.v_proj)
+        projs = tuple(self._unadapted(p) for p in (self.q_proj, self.k_proj, self.v_proj))
         if not any(float(getattr(p, "_dither", 0.0)) > 0.0 or (p.training and p.weight.requires_grad)
                    for p in projs):
             out = R.shift_project(
@@ -170,7 +176,7 @@ class RosaMixer(nn.Module):
                                      vb.reshape(B * S, -1), T)
         from ..kernels.linear import Int8Linear
         types = (torch.float32, torch.bfloat16, torch.float16)
-        if (not torch.is_grad_enabled() and isinstance(self.out_proj, Int8Linear) and x.dtype in types
+        if (not torch.is_grad_enabled() and isinstance(self._unadapted(self.out_proj), Int8Linear) and x.dtype in types
                 and self.payload.dtype in types and R.hard_out_fits(B, S)):  # the products in one launch
             return self._out(R.hard_out(sign.reshape(B, S, T), self.payload, x.dtype), residual)
         out = self.payload[None, :, None] * sign.reshape(B, S, T).float()
