@@ -7,13 +7,14 @@
 // with x~ = dropout(x) where a mask is given (made from its counter, stored nowhere). A token without an adapter
 // keeps base. Adapters of other tokens never touch a token's row, whatever they hold.
 //
-// Both passes of a token's row are one launch of pair_kernel: a workgroup of 8 waves holds up to 32 rows; the
-// waves split the contraction of the narrow product, their sums join in LDS, and the same waves then split the
-// columns of the wide one. h keeps its 24 bits on its way: it is fp32 in LDS and enters the 16-bit matrix
-// instructions as a rounded value and the rounding's rest, side by side along the contraction, which a rank of 16
-// leaves half empty anyway (fp16: 11 bits each), and bf16, of 8 bits a part, as the rest's rest in another instruction. What bounds it is memory: x and base read once, y written once. 8192 tokens of 1536 to 1536,
-// rank 16: bf16 20 us for 76 MB (3.8 TB/s), fp32 43 us for 151 MB (3.5; the narrow product alone 17, the wide one 24). Few
-// tokens take a launch's latency: one token 5.4 us, 64 of as many adapters 6.7.
+// Both passes of a token's row are one launch of pair_kernel: a workgroup of 8 waves holds up to 32 rows; the waves
+// split the contraction of the narrow product, their sums join in LDS, and the same waves then split the columns of
+// the wide one. h keeps its 24 bits on its way: it is fp32 in LDS and enters the 16-bit matrix instructions as a
+// rounded value and the rounding's rest, side by side along the contraction, which a rank of 16 leaves half empty
+// anyway (fp16: 11 bits each), and bf16, of 8 bits a part, as the rest's rest in another instruction. What bounds it
+// is memory: x and base read once, y written once. 8192 tokens of 1536 to 1536, rank 16: bf16 20 us for 76 MB (3.8
+// TB/s), fp32 43 us for 151 MB (3.5; the narrow product alone 17, the wide one 24). Few tokens take a launch's
+// latency: one token 5.4 us, 64 of as many adapters 6.7.
 #include "ksd_random.h"
 
 #include <algorithm>
